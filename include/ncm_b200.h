@@ -415,6 +415,71 @@ int    ncmb_weights_import_safetensors(WeightStore *ws, const char *path, int co
  * -log(exp(l[next] - max) / sum exp(l - max) + 1e-30) in fp64. Logits never leave the device. */
 void   ncmb_lm_nll(NcmbLM *m, const int *ids, int B, int T, const int *lens, double *nll_out);
 
+/* ---- operators on long key/value caches ----
+ * A cache of the host program's own, in device memory: element (row b, kv head h, slot s, dim d) of the keys is
+ * k[b * row_stride + h * head_stride + s * token_stride + d], of the values likewise with v. So a cache that holds a
+ * token's keys and values side by side ([slot][2 * n_kv * hd], as the decode loops above do) and one laid out head by
+ * head are both stated by their strides. Slots [0, len[b]) of row b hold its cached tokens; keys are as attention uses
+ * them (rotated). Requirements: hd a multiple of 8, at most 128; k, v and every stride a multiple of 16 bytes.
+ * Lengths are read on the device; a length outside [0, capacity - new tokens] counts as the nearer end of that range.
+ * Slots that no token occupies may hold anything, infinities and NaN included.
+ * max_len (these four calls): an upper bound on the lengths that the host knows, by which the launch is sized; 0 =
+ * capacity. Results are right where it is exceeded, only slower.
+ * All four queue kernels on the library's stream and return 0, or print one line to stderr and return -1 for arguments
+ * they refuse (nothing is queued then). Rounding: scores, exponentials, sums and weights are fp32 whatever the cache's
+ * type. A call's scratch memory is kept for the next one and grows on demand. No counterpart in the reference. */
+enum { NCMB_F32 = 0, NCMB_BF16 = 1 };
+#define NCMB_MAX_NODES 256
+typedef struct {
+    void *k, *v;
+    int type;                        /* of keys and values: NCMB_F32 or NCMB_BF16 */
+    int rows, n_kv, hd, capacity;
+    int64_t row_stride, head_stride, token_stride;      /* in elements */
+    const int *len;                  /* device int[rows] */
+} NcmbCache;
+/* Attention of T new tokens of every row to the row's cache and to one another; their keys and values already stand in
+ * slots len[b] ... len[b] + T - 1. Query t of row b is at q + (b * T + t) * ldq, [n_head][hd], its result at out + (b * T
+ * + t) * ldo, both of type act_type (NCMB_BF16 with a bf16 cache only; ldq / ldo in elements, multiples of 16 bytes).
+ * parents NULL: the new tokens follow one another, token t sees the cache and new tokens 0 ... t (T = 1 is a decode
+ * step). Else device int[rows][T], a tree of drafted tokens: -1 for a token that follows the cache, 0 <= p < t for one
+ * that follows new token p; it sees the cache, itself and its ancestors. Any other entry is a place that holds no token:
+ * its result is zero and nothing sees it. scale 0 = 1 / sqrt(hd). T is 1 ... NCMB_MAX_NODES.
+ * weights: NULL, or device float[rows][n_kv][capacity] that receives each slot's attention probability, summed over the
+ * T tokens and the query heads that share the kv head: added to slots [0, len[b]), stored to the T new ones. */
+int ncmb_cache_attention(const NcmbCache *c, const void *q, int64_t ldq, void *out, int64_t ldo, int act_type, int n_head,
+                         int T, const int *parents, float scale, int max_len, float *weights);
+/* Holds every (row, kv head) of a cache to `budget` tokens: kept are the `recent` tokens latest in the text, then those
+ * with the largest weights, ties by the lower slot (a NaN weight ranks below all). With n = min(len[b], budget), kept
+ * tokens of slots below n keep their slot and the freed slots below n take the kept tokens from beyond, both ascending:
+ * attention does not depend on the order, and a step that is one token over budget moves one token.
+ * dst == src (same k and v): in place. Else dst is another cache that does not overlap src, of the same type, rows,
+ * n_kv and hd and of a capacity of budget (or of src's capacity, if less) at least; only its k, v and strides are used.
+ * weights [rows][n_kv][src->capacity], weights_dst [rows][n_kv][dst->capacity] (the same array in place).
+ * pos / pos_dst, int arrays of the same shapes: place in the text of each slot's token. Input pos is read for slots
+ * below known[b] only (device int[rows], NULL = 0: none); a slot beyond is the place seen[b] - len[b] + slot, that is,
+ * seen[b] (device int[rows]) tokens of the text have passed and the last ones stand in order. So known = the len_dst of
+ * the eviction before. len_dst: device int[rows], receives n; must not be src->len. len at most 393216. */
+int ncmb_cache_evict(const NcmbCache *src, const NcmbCache *dst, const float *weights, float *weights_dst, const int *pos,
+                     int *pos_dst, const int *known, const int *seen, int budget, int recent, int max_len, int *len_dst);
+/* Mean keys of blocks of `block` (16, 32, 64 or 128) slots in 8 bits, for the call below. Slots [0, len[b] + n_new) hold
+ * tokens; the blocks that hold a slot from first[b] on (device int[rows], NULL = 0) are formed anew, others stay.
+ * mean = sum of the block's n tokens / n in fp32 (the sum by halves of the block: slot i plus slot i + block/2, then the
+ * same of what is left, a slot without a token counting as zero), scale = max |mean| / 127, code = mean / scale rounded
+ * to the nearest (ties to even; 0 where scale is 0). codes: device int8 [rows][n_kv][nb][hd], scales: device
+ * float[rows][n_kv][nb], nb = ceil(capacity / block); codes 16-byte aligned. */
+int ncmb_block_summaries(const NcmbCache *c, int n_new, const int *first, int block, int max_len, signed char *codes,
+                         float *scales);
+/* Attention that reads a part of the cache. As ncmb_cache_attention without parents, but token t of row b, at place p =
+ * len[b] + t, sees of the slots 0 ... p those of at most n_sel blocks per kv head: the first n_first ones, the last n_last
+ * (>= 1) up to its own, and the blocks with the highest scores, ties to the lower block. Score: a head's query in 8
+ * bits (as the means: scale max |q| / 127), product with the block's codes as whole numbers, times the query's scale; the
+ * largest over the heads that share the kv head; times the block's scale. codes / scales must be up to date for all
+ * blocks that end before the row's last new token's n_last-th last block. n_first + n_last <= n_sel <= 1024.
+ * picks: NULL, or device int[rows][T][n_kv][n_sel], the blocks in ascending order, then -1. */
+int ncmb_block_attention(const NcmbCache *c, const void *q, int64_t ldq, void *out, int64_t ldo, int act_type, int n_head,
+                         int T, int block, const signed char *codes, const float *scales, int n_sel, int n_first,
+                         int n_last, float scale, int max_len, int *picks);
+
 #ifdef __cplusplus
 }
 #endif

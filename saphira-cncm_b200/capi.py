@@ -37,6 +37,29 @@ class Tensor(C.Structure):
     _fields_ = [("data", _P), ("shape", _I64 * 4), ("ndim", _I), ("n", _I64)]
 
 
+F32, BF16 = 0, 1              # NCMB_F32, NCMB_BF16
+
+
+class KVCache(C.Structure):
+    """NcmbCache: a key/value cache in device memory, stated by its strides."""
+    _fields_ = [("k", _P), ("v", _P), ("type", _I), ("rows", _I), ("n_kv", _I), ("hd", _I), ("capacity", _I),
+                ("row_stride", _I64), ("head_stride", _I64), ("token_stride", _I64), ("len", _P)]
+
+    @classmethod
+    def of(cls, k, v, length):
+        """From device arrays with ``data_ptr`` / ``stride`` / ``shape`` (torch tensors): k and v as views
+        [rows][n_kv][capacity][hd] of one layout, length int32[rows]. The caller keeps the arrays alive."""
+        if tuple(k.shape) != tuple(v.shape) or tuple(k.stride()) != tuple(v.stride()) or k.dtype != v.dtype:
+            raise ValueError("keys and values differ in shape, strides or type")
+        if k.stride(3) != 1 and k.shape[3] > 1:
+            raise ValueError("the head dim has to be contiguous")
+        kind = {4: F32, 2: BF16}[k.element_size()]
+        b, h, n, d = k.shape
+        c = cls(k.data_ptr(), v.data_ptr(), kind, b, h, d, n, k.stride(0), k.stride(1), k.stride(2), length.data_ptr())
+        c.held = (k, v, length)
+        return c
+
+
 # name -> (restype, argtypes); only the inference surface
 _SIGS = {
     # runtime (src/ncm.h:37-70,139,261)
@@ -158,6 +181,10 @@ _SIGS = {
     "ncmb_lm_logits": (None, [_P, _P, _I, _I, _P]),
     "ncmb_lm_nll": (None, [_P, _P, _I, _I, _P, _P]),
     "ncmb_weights_import_safetensors": (_I, [C.POINTER(WeightStore), C.c_char_p, _I]),
+    "ncmb_cache_attention": (_I, [C.POINTER(KVCache), _P, _I64, _P, _I64, _I, _I, _I, _P, _F, _I, _P]),
+    "ncmb_cache_evict": (_I, [C.POINTER(KVCache), C.POINTER(KVCache), _P, _P, _P, _P, _P, _P, _I, _I, _I, _P]),
+    "ncmb_block_summaries": (_I, [C.POINTER(KVCache), _I, _P, _I, _I, _P, _P]),
+    "ncmb_block_attention": (_I, [C.POINTER(KVCache), _P, _I64, _P, _I64, _I, _I, _I, _I, _P, _P, _I, _I, _I, _F, _I, _P]),
     "gpt2_cmd_ppl": (_I, [_P, C.c_char_p, C.c_char_p, C.c_char_p]),
     "gpt2_cmd_verify": (_I, [_P, C.c_char_p, C.c_char_p, C.c_char_p]),
     "qwen_cmd_ppl": (_I, [_P, C.c_char_p, C.c_char_p, C.c_char_p]),

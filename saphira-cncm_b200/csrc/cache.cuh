@@ -1,0 +1,114 @@
+// Shared by the operators on long key/value caches (cache_attention.cu, cache_evict.cu, cache_blocks.cu): the cache as
+// kernels see it, argument checks, and the scratch memory of a call.
+#pragma once
+#include "common.cuh"
+
+#include <cooperative_groups.h>
+#include <cuda_bf16.h>
+
+namespace ncmb {
+
+struct CacheDev {
+    const char *k, *v;               // bytes
+    int64_t rs, hs, ts;              // strides in bytes
+    int rows, nkv, hd, cap;
+    const int *len;
+};
+
+// One line to stderr and -1: what an entry point returns for arguments it refuses.
+int cache_refuse(const char *who, const char *fmt, ...);
+// 0 when the cache's description is one the kernels take (see ncm_b200.h), else -1 with a message
+int cache_check(const char *who, const NcmbCache *c, CacheDev &d);
+inline int cache_elem(const NcmbCache *c) { return c->type == NCMB_BF16 ? 2 : 4; }
+// Scratch of at least `bytes`, kept and grown; null with a message when the device has no room for it. Calls are ordered
+// by the library's stream, so all of them share it.
+void *cache_scratch(const char *who, size_t bytes);
+
+// order of floats as unsigned: larger is larger, -0 is 0, a NaN below everything
+__host__ __device__ __forceinline__ uint32_t float_key(float x) {
+    if (!(x == x)) return 0u;
+    if (x == 0.f) return 0x80000000u;
+    uint32_t u;
+#ifdef __CUDA_ARCH__
+    u = __float_as_uint(x);
+#else
+    memcpy(&u, &x, 4);
+#endif
+    return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+}
+
+#ifdef __CUDACC__
+__device__ __forceinline__ int cache_len(const CacheDev &c, int row, int n_new) {   // cached tokens, made to fit
+    return max(0, min(c.len[row], c.cap - n_new));
+}
+
+// ---- the k-th largest of many 32-bit keys, by a cluster of CTAs that each hold a part of them ----
+constexpr int SEL_BINS = 2048;
+struct SelShared {
+    uint32_t hist[3][SEL_BINS];      // one per pass, so that one cluster barrier a pass is enough
+    uint32_t wsum[32];
+    uint32_t bin, left;
+};
+// Digits of 11, 11 and 10 bits from the top: each pass counts the keys that agree with what is settled so far by their next
+// digit, adds the CTAs' counts up and settles the digit at which the count from above reaches k. key(i), i in [0, n): this
+// CTA's keys. Returns the k-th largest of all (1 <= k <= their number); `ties` of the keys equal to it are among the k
+// largest. All threads of all CTAs of the cluster call it; NT threads a CTA.
+template <int NT, class KEY>
+__device__ uint32_t select_kth(SelShared &s, int n, uint32_t k, uint32_t &ties, KEY key) {
+    namespace cg = cooperative_groups;
+    static_assert(SEL_BINS % NT == 0 && NT % 32 == 0, "whole bins a thread");
+    constexpr int BPT = SEL_BINS / NT;
+    cg::cluster_group cl = cg::this_cluster();
+    const int nc = (int)cl.num_blocks(), tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    for (int i = tid; i < 3 * SEL_BINS; i += NT) (&s.hist[0][0])[i] = 0;
+    __syncthreads();
+    uint32_t prefix = 0, settled = 0;            // settled: mask of the bits that prefix states
+    const int shifts[3] = {21, 10, 0};
+#pragma unroll
+    for (int pass = 0; pass < 3; pass++) {
+        const int sh = shifts[pass];
+        const uint32_t dm = pass == 2 ? 1023u : 2047u;
+        for (int i = tid; i < n; i += NT) {
+            const uint32_t u = key(i);
+            if ((u & settled) == prefix) atomicAdd(&s.hist[pass][(u >> sh) & dm], 1u);
+        }
+        if (nc > 1) cl.sync(); else __syncthreads();
+        uint32_t c[BPT], sum = 0;                // thread t has bins from 2047 - BPT t downwards
+#pragma unroll
+        for (int i = 0; i < BPT; i++) {
+            const int b = SEL_BINS - 1 - BPT * tid - i;
+            uint32_t v = 0;
+            for (int r = 0; r < nc; r++) v += nc > 1 ? cl.map_shared_rank(&s.hist[pass][0], r)[b] : s.hist[pass][b];
+            c[i] = v;
+            sum += v;
+        }
+        uint32_t inc = sum;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const uint32_t v = __shfl_up_sync(0xffffffffu, inc, o);
+            if (lane >= o) inc += v;
+        }
+        if (lane == 31) s.wsum[warp] = inc;
+        __syncthreads();
+        uint32_t above = inc - sum;
+        for (int w = 0; w < warp; w++) above += s.wsum[w];
+        if (above < k && above + sum >= k) {
+#pragma unroll
+            for (int i = 0; i < BPT; i++) {
+                if (above < k && above + c[i] >= k) { s.bin = SEL_BINS - 1 - BPT * tid - i; s.left = k - above; }
+                above += c[i];
+            }
+        }
+        __syncthreads();
+        prefix |= s.bin << sh;
+        settled |= dm << sh;
+        k = s.left;
+        __syncthreads();
+    }
+    if (nc > 1) cl.sync();                       // the others have read this CTA's counts
+    ties = k;
+    return prefix;
+}
+#endif
+
+} // namespace ncmb

@@ -1,0 +1,208 @@
+// A cache held to a budget of tokens by the attention each has received (ncmb_cache_evict, include/ncm_b200.h).
+//
+// Per (row, kv head) of n tokens, n2 = min(n, budget) are kept: key = the weight as an ordered integer, the `recent`
+// latest tokens above all; the n2-th largest key by three counting passes; of the tokens that tie with it those in the
+// lower slots. Kept tokens below slot n2 stay where they are and the others take the freed slots in order, so a step that
+// is one token over budget moves one token, and in place no source is a target.
+#include "cache.cuh"
+
+namespace ncmb {
+namespace {
+
+namespace cg = cooperative_groups;
+
+constexpr int EV_THREADS = 512, EV_WARPS = EV_THREADS / 32, EV_MAXC = 8;
+constexpr int EV_KEYS = 24576;       // keys a CTA holds in shared memory; beyond, they are read again
+constexpr int EV_MOST = 393216;      // slots of a row: a bit for each and EV_KEYS keys fit one CTA
+
+struct EvictArgs {
+    CacheDev c;
+    char *k2, *v2;
+    int64_t rs2, hs2, ts2;
+    int cap2, inplace, budget, recent, es, kcap;
+    const float *w; float *w2;
+    const int *pos; int *pos2;
+    const int *known, *seen;
+    int *len2;
+    int *from, *to;                  // scratch, [rows][nkv][min(budget, capacity)] each
+    int room;
+};
+
+__global__ void __launch_bounds__(EV_THREADS) k_cache_evict(EvictArgs a) {
+    extern __shared__ uint32_t dyn[];
+    __shared__ SelShared sel;
+    __shared__ int maxpos, wtie[EV_WARPS], wcount[EV_WARPS][3];
+    __shared__ int share[4];         // ties, freed slots, kept tokens from beyond, kept in place: of this CTA
+    cg::cluster_group cl = cg::this_cluster();
+    const int rank = (int)cl.block_rank(), nc = (int)cl.num_blocks();
+    const int kvh = blockIdx.y, b = blockIdx.z, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    uint32_t *keys = dyn, *kept = dyn + a.kcap;          // keys, then one bit a slot
+    const int n = cache_len(a.c, b, 0), n2 = min(n, a.budget);
+    const int64_t u = (int64_t)b * a.c.nkv + kvh;
+    const int seen = a.seen[b], known = a.known ? max(0, min(a.known[b], n)) : 0;
+    const float *w = a.w + u * a.c.cap;
+    const int *pos = a.pos + u * a.c.cap;
+    if (rank == 0 && kvh == 0 && tid == 0) a.len2[b] = n2;
+    if (n == 0) return;
+    // slots [lo, hi) are this CTA's; a warp's part of them is a whole number of 32
+    const int per_warp = ((n + nc * EV_WARPS - 1) / (nc * EV_WARPS) + 31) & ~31;
+    const int per = per_warp * EV_WARPS, lo = min(n, rank * per), hi = min(n, lo + per);
+    auto place = [&](int s) { return s < known ? pos[s] : seen - n + s; };
+    if (tid == 0) maxpos = INT_MIN;
+    __syncthreads();
+    int last = INT_MIN;
+    for (int s = lo + tid; s < hi; s += EV_THREADS) last = max(last, place(s));
+    last = __reduce_max_sync(0xffffffffu, last);
+    if (lane == 0) atomicMax(&maxpos, last);
+    if (nc > 1) cl.sync(); else __syncthreads();
+    for (int r = 0; r < nc; r++) last = max(last, nc > 1 ? *cl.map_shared_rank(&maxpos, r) : maxpos);
+    auto make_key = [&](int s) { return (int64_t)place(s) > (int64_t)last - a.recent ? 0xffffffffu : float_key(w[s]); };
+    for (int s = lo + tid; s < min(hi, lo + a.kcap); s += EV_THREADS) keys[s - lo] = make_key(s);
+    __syncthreads();
+    auto key = [&](int i) { return i < a.kcap ? keys[i] : make_key(lo + i); };
+    uint32_t bound = 0, ties = 0xffffffffu;              // all are kept where there is room for all
+    if (n2 < n) bound = select_kth<EV_THREADS>(sel, hi - lo, (uint32_t)n2, ties, key);
+
+    // ties before this warp's slots, so that the lower ones are kept
+    const int w0 = lo + warp * per_warp, w1 = min(hi, w0 + per_warp);
+    int mine = 0;
+    for (int s = w0; s < w1; s += 32) {
+        const bool tie = s + lane < w1 && key(s + lane - lo) == bound;
+        mine += __popc(__ballot_sync(0xffffffffu, tie));
+    }
+    if (lane == 0) wtie[warp] = mine;
+    __syncthreads();
+    if (tid == 0) { int t = 0; for (int i = 0; i < EV_WARPS; i++) t += wtie[i]; share[0] = t; }
+    if (nc > 1) cl.sync(); else __syncthreads();
+    uint32_t before = 0;
+    for (int r = 0; r < rank; r++) before += (uint32_t)*cl.map_shared_rank(&share[0], r);
+    for (int i = 0; i < warp; i++) before += (uint32_t)wtie[i];
+    int count[3] = {0, 0, 0};
+    for (int s = w0; s < w1; s += 32) {
+        const bool in = s + lane < w1;
+        const uint32_t x = in ? key(s + lane - lo) : 0;
+        const uint32_t tm = __ballot_sync(0xffffffffu, in && x == bound);
+        const bool keep = in && (x > bound || (x == bound && before + (uint32_t)__popc(tm & ((1u << lane) - 1)) < ties));
+        before += (uint32_t)__popc(tm);
+        const uint32_t km = __ballot_sync(0xffffffffu, keep);
+        const uint32_t below = n2 - s >= 32 ? 0xffffffffu : n2 > s ? (1u << (n2 - s)) - 1 : 0u;      // slots below n2
+        if (lane == 0) kept[(s - lo) >> 5] = km;
+        count[0] += __popc(~km & below);
+        count[1] += __popc(km & ~below);
+        count[2] += __popc(km & below);
+    }
+    if (lane < 3) wcount[warp][lane] = lane == 0 ? count[0] : lane == 1 ? count[1] : count[2];
+    __syncthreads();
+    if (tid < 3) { int t = 0; for (int i = 0; i < EV_WARPS; i++) t += wcount[i][tid]; share[1 + tid] = t; }
+    if (nc > 1) cl.sync(); else __syncthreads();
+    int at[3], moves = 0;
+#pragma unroll
+    for (int i = 0; i < 3; i++) {
+        at[i] = 0;
+        for (int r = 0; r < nc; r++) {
+            const int v = nc > 1 ? *cl.map_shared_rank(&share[1 + i], r) : share[1 + i];
+            if (r < rank) at[i] += v;
+            if (i == 0) moves += v;
+        }
+        for (int q = 0; q < warp; q++) at[i] += wcount[q][i];
+    }
+    // pairs (from, to): moves, then -- to another cache -- the tokens that keep their slot
+    int *from = a.from + u * a.room, *to = a.to + u * a.room;
+    for (int s = w0; s < w1; s += 32) {
+        const uint32_t km = kept[(s - lo) >> 5], lt = (1u << lane) - 1, me = 1u << lane;
+        const uint32_t below = n2 - s >= 32 ? 0xffffffffu : n2 > s ? (1u << (n2 - s)) - 1 : 0u;
+        if (~km & below & me) to[at[0] + __popc(~km & below & lt)] = s + lane;
+        if (km & ~below & me) from[at[1] + __popc(km & ~below & lt)] = s + lane;
+        if (km & below & me) {
+            if (!a.inplace) {
+                const int i = moves + at[2] + __popc(km & below & lt);
+                from[i] = to[i] = s + lane;
+            } else if (s + lane >= known) a.pos2[u * a.cap2 + s + lane] = seen - n + s + lane;
+        }
+        at[0] += __popc(~km & below);
+        at[1] += __popc(km & ~below);
+        at[2] += __popc(km & below);
+    }
+    if (nc > 1) cl.sync(); else __syncthreads();         // also: no key is read from w / pos any more
+    const int pairs = a.inplace ? moves : n2;
+    for (int i = rank * EV_THREADS + tid; i < pairs; i += nc * EV_THREADS) {
+        const int f = from[i], t = to[i];
+        a.w2[u * a.cap2 + t] = w[f];
+        a.pos2[u * a.cap2 + t] = place(f);
+    }
+    const char *k = a.c.k + b * a.c.rs + kvh * a.c.hs, *v = a.c.v + b * a.c.rs + kvh * a.c.hs;
+    char *k2 = a.k2 + b * a.rs2 + kvh * a.hs2, *v2 = a.v2 + b * a.rs2 + kvh * a.hs2;
+    const int units = a.c.hd * a.es / 16;                // of 16 bytes in a token's keys
+    const int64_t total = (int64_t)pairs * units;
+    for (int64_t i = rank * EV_THREADS + tid; i < total; i += nc * EV_THREADS) {
+        const int p = (int)(i / units), x = (int)(i % units) * 16;
+        const int64_t f = from[p], t = to[p];
+        const int4 kx = *(const int4 *)(k + f * a.c.ts + x), vx = *(const int4 *)(v + f * a.c.ts + x);
+        *(int4 *)(k2 + t * a.ts2 + x) = kx;
+        *(int4 *)(v2 + t * a.ts2 + x) = vx;
+    }
+}
+
+bool overlaps(const CacheDev &a, const CacheDev &b, int es) {
+    auto reach = [&](const CacheDev &c) { return (int64_t)(c.rows - 1) * c.rs + (int64_t)(c.nkv - 1) * c.hs + (int64_t)(c.cap - 1) * c.ts + (int64_t)c.hd * es; };
+    const int64_t ra = reach(a), rb = reach(b);
+    for (const char *x : {a.k, a.v})
+        for (const char *y : {b.k, b.v})
+            if (x < y + rb && y < x + ra) return true;
+    return false;
+}
+
+} // namespace
+} // namespace ncmb
+
+using namespace ncmb;
+
+extern "C" int ncmb_cache_evict(const NcmbCache *src, const NcmbCache *dst, const float *weights, float *weights_dst, const int *pos,
+                                int *pos_dst, const int *known, const int *seen, int budget, int recent, int max_len, int *len_dst) {
+    const char *who = "ncmb_cache_evict";
+    EvictArgs a;
+    CacheDev d;
+    if (cache_check(who, src, a.c) || cache_check(who, dst, d)) return -1;
+    if (src->type != dst->type || src->rows != dst->rows || src->n_kv != dst->n_kv || src->hd != dst->hd) return cache_refuse(who, "the two caches differ in type, rows, kv heads or head dim");
+    if (budget < 1 || recent < 0) return cache_refuse(who, "budget %d, recent %d", budget, recent);
+    if (src->capacity > EV_MOST) return cache_refuse(who, "capacity %d: at most %d slots", src->capacity, EV_MOST);
+    if (!weights || !weights_dst || !pos || !pos_dst || !seen || !len_dst) return cache_refuse(who, "a null pointer");
+    if (len_dst == src->len) return cache_refuse(who, "len_dst has to be another array than the lengths of the cache");
+    if (src->rows == 0) return 0;
+    a.inplace = src->k == dst->k && src->v == dst->v;
+    if (a.inplace && (src->capacity != dst->capacity || src->row_stride != dst->row_stride || src->head_stride != dst->head_stride || src->token_stride != dst->token_stride))
+        return cache_refuse(who, "one cache with two layouts");
+    if (a.inplace && (weights != weights_dst || pos != pos_dst)) return cache_refuse(who, "in place weights and places have to be in place too");
+    if (!a.inplace && (weights == weights_dst || pos == pos_dst)) return cache_refuse(who, "another cache needs weights and places of its own");
+    a.room = budget < src->capacity ? budget : src->capacity;
+    if (dst->capacity < a.room) return cache_refuse(who, "capacity %d for a budget of %d", dst->capacity, budget);
+    const int es = cache_elem(src);
+    if (!a.inplace && overlaps(a.c, d, es)) return cache_refuse(who, "the two caches overlap");
+    ensure_device();
+    a.k2 = (char *)dst->k; a.v2 = (char *)dst->v; a.rs2 = d.rs; a.hs2 = d.hs; a.ts2 = d.ts; a.cap2 = d.cap;
+    a.budget = budget; a.recent = recent; a.es = es;
+    a.w = weights; a.w2 = weights_dst; a.pos = pos; a.pos2 = pos_dst; a.known = known; a.seen = seen; a.len2 = len_dst;
+    if (max_len <= 0 || max_len > src->capacity) max_len = src->capacity;
+    const int64_t units = (int64_t)src->rows * src->n_kv;
+    a.from = (int *)cache_scratch(who, units * a.room * 8);
+    if (!a.from) return -1;
+    a.to = a.from + units * a.room;
+    // CTAs a (row, head): as many as keep the GPU busy, with 2048 slots each at least
+    int nc = 1;
+    while (nc < EV_MAXC && units * nc < ctx().sm_count && cdiv(max_len, nc) > 2048) nc *= 2;
+    // slots of a CTA when the row is as long as the cache can hold: bits for all, keys for as many as shared memory takes
+    const int64_t most = cdiv(cdiv(src->capacity, nc * EV_WARPS), 32) * 32 * EV_WARPS, hint = cdiv(cdiv(max_len, nc * EV_WARPS), 32) * 32 * EV_WARPS;
+    a.kcap = (int)(hint < EV_KEYS ? hint : EV_KEYS);
+    const size_t smem = (size_t)a.kcap * 4 + (size_t)most / 8;
+    CUDA_CHECK(cudaFuncSetAttribute(k_cache_evict, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(nc, src->n_kv, src->rows); cfg.blockDim = dim3(EV_THREADS); cfg.dynamicSmemBytes = smem; cfg.stream = stream();
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = nc; at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = 1;
+    cfg.attrs = at; cfg.numAttrs = 1;
+    cudaError_t e = cudaLaunchKernelEx(&cfg, k_cache_evict, a);
+    if (e != cudaSuccess) fatal("cache eviction: launch failed: %s", cudaGetErrorString(e));
+    ctx().launches++;
+    return 0;
+}

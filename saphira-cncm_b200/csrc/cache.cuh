@@ -21,8 +21,10 @@ int cache_refuse(const char *who, const char *fmt, ...);
 int cache_check(const char *who, const NcmbCache *c, CacheDev &d);
 inline int cache_elem(const NcmbCache *c) { return c->type == NCMB_BF16 ? 2 : 4; }
 // Scratch of at least `bytes`, kept and grown; null with a message when the device has no room for it. Calls are ordered
-// by the library's stream, so all of them share it.
-void *cache_scratch(const char *who, size_t bytes);
+// by the library's stream, so all of them share it; within a call, what one kernel leaves for another that has scratch of
+// its own stands in the other of the two areas.
+enum { SCRATCH_MAIN = 0, SCRATCH_PICKS = 1 };
+void *cache_scratch(const char *who, size_t bytes, int area = SCRATCH_MAIN);
 
 // order of floats as unsigned: larger is larger, -0 is 0, a NaN below everything
 __host__ __device__ __forceinline__ uint32_t float_key(float x) {

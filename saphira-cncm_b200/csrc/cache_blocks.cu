@@ -1,13 +1,11 @@
 // Attention over blocks of the cache that a cheap score picks for each query (ncmb_block_summaries and
 // ncmb_block_attention, include/ncm_b200.h).
-#include "cache.cuh"
+#include "cache_mma.cuh"
 
 namespace ncmb {
 namespace {
 
 template <class E> __device__ __forceinline__ float get(const char *p, int d) { return (float)((const E *)p)[d]; }
-__device__ __forceinline__ void put(float *p, float v) { *p = v; }
-__device__ __forceinline__ void put(__nv_bfloat16 *p, float v) { *p = __float2bfloat16(v); }
 
 // one warp per (row, kv head, block); a lane has the dims lane, lane + 32, ...
 template <class KE>
@@ -147,38 +145,6 @@ __global__ void __launch_bounds__(BP_THREADS) k_block_pick(BlockArgs a) {
     }
 }
 
-// one warp per (row, token, head), one key at a time
-template <class KE, class QE>
-__global__ void __launch_bounds__(128) k_block_attention_plain(BlockArgs a) {
-    const int lane = threadIdx.x & 31;
-    const int64_t w = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-    if (w >= (int64_t)a.c.rows * a.T * a.H) return;
-    const int h = (int)(w % a.H), t = (int)(w / a.H % a.T), b = (int)(w / a.H / a.T);
-    const int here = cache_len(a.c, b, a.T) + t;
-    const int *picks = a.picks + (((int64_t)b * a.T + t) * a.c.nkv + h / a.G) * a.n_sel;
-    QE *o = (QE *)(a.out + ((int64_t)b * a.T + t) * a.ldo) + (int64_t)h * a.c.hd;
-    const char *q = a.q + ((int64_t)b * a.T + t) * a.ldq + (int64_t)h * a.c.hd * sizeof(QE);
-    const char *k = a.c.k + b * a.c.rs + (h / a.G) * a.c.hs, *v = a.c.v + b * a.c.rs + (h / a.G) * a.c.hs;
-    float qr[4], acc[4] = {0.f, 0.f, 0.f, 0.f}, m = -INFINITY, l = 0.f;
-#pragma unroll
-    for (int i = 0; i < 4; i++) qr[i] = lane + 32 * i < a.c.hd ? get<QE>(q, lane + 32 * i) * a.scale : 0.f;
-    for (int p = 0; p < a.n_sel && picks[p] >= 0; p++)
-        for (int j = picks[p] * a.block; j < min((picks[p] + 1) * a.block, here + 1); j++) {
-            float s = 0.f;
-#pragma unroll
-            for (int i = 0; i < 4; i++) if (lane + 32 * i < a.c.hd) s = fmaf(qr[i], get<KE>(k + j * a.c.ts, lane + 32 * i), s);
-#pragma unroll
-            for (int x = 16; x; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
-            const float n = fmaxf(m, s), al = m == -INFINITY ? 0.f : expf(m - n), e = expf(s - n);
-            l = l * al + e;
-            m = n;
-#pragma unroll
-            for (int i = 0; i < 4; i++) if (lane + 32 * i < a.c.hd) acc[i] = acc[i] * al + e * get<KE>(v + j * a.c.ts, lane + 32 * i);
-        }
-#pragma unroll
-    for (int i = 0; i < 4; i++) if (lane + 32 * i < a.c.hd) put(o + lane + 32 * i, l > 0.f ? acc[i] / l : 0.f);
-}
-
 } // namespace
 } // namespace ncmb
 
@@ -225,15 +191,13 @@ extern "C" int ncmb_block_attention(const NcmbCache *c, const void *q, int64_t l
     a.scale = scale == 0.f ? 1.0f / sqrtf((float)c->hd) : scale;
     const int64_t units = (int64_t)c->rows * T * c->n_kv;
     const size_t need_picks = picks ? 0 : (size_t)units * n_sel * 4, need_keys = a.nb > BP_KEYS ? (size_t)units * a.nb * 4 : 0;
-    char *scratch = need_picks + need_keys ? (char *)cache_scratch(who, need_picks + need_keys) : nullptr;
+    char *scratch = need_picks + need_keys ? (char *)cache_scratch(who, need_picks + need_keys, SCRATCH_PICKS) : nullptr;
     if (need_picks + need_keys && !scratch) return -1;
     a.picks = picks ? picks : (int *)(scratch + need_keys);
     a.keys = need_keys ? (uint32_t *)scratch : nullptr;
     const size_t smem = (size_t)((a.G + 3) & ~3) * 4 + (((size_t)a.G * c->hd + 15) & ~(size_t)15) + (need_keys ? 0 : (size_t)a.nb * 4);
     if (smem > 150000) return cache_refuse(who, "%d query heads a kv head", a.G);
     const dim3 gp(T, c->n_kv, c->rows);
-    const unsigned ga = grid1d((int64_t)c->rows * T * n_head, 4);
-    (void)max_len;
     if (act_type == NCMB_F32) {
         CUDA_CHECK(cudaFuncSetAttribute(k_block_pick<float>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
         LAUNCH(k_block_pick<float>, gp, BP_THREADS, smem, a);
@@ -241,8 +205,12 @@ extern "C" int ncmb_block_attention(const NcmbCache *c, const void *q, int64_t l
         CUDA_CHECK(cudaFuncSetAttribute(k_block_pick<__nv_bfloat16>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
         LAUNCH(k_block_pick<__nv_bfloat16>, gp, BP_THREADS, smem, a);
     }
-    if (c->type == NCMB_F32) LAUNCH((k_block_attention_plain<float, float>), ga, 128, 0, a);
-    else if (act_type == NCMB_F32) LAUNCH((k_block_attention_plain<__nv_bfloat16, float>), ga, 128, 0, a);
-    else LAUNCH((k_block_attention_plain<__nv_bfloat16, __nv_bfloat16>), ga, 128, 0, a);
-    return 0;
+    CmArgs m = {};
+    m.c = a.c; m.q = a.q; m.out = a.out; m.ldq = a.ldq; m.ldo = a.ldo; m.H = a.H; m.G = a.G; m.T = T; m.M = a.G;
+    m.c2 = a.scale * 1.44269504f; m.block_log = block == 16 ? 4 : block == 32 ? 5 : block == 64 ? 6 : 7; m.n_sel = n_sel; m.picks = a.picks;
+    if (max_len <= 0 || max_len > c->capacity - T) max_len = c->capacity - T;
+    const int keys = (int)std::min<int64_t>(max_len + T, (int64_t)n_sel * block);
+    if (c->type == NCMB_F32) return cm_run<float, float, true>(who, m, keys);
+    if (act_type == NCMB_F32) return cm_run<__nv_bfloat16, float, true>(who, m, keys);
+    return cm_run<__nv_bfloat16, __nv_bfloat16, true>(who, m, keys);
 }

@@ -1,0 +1,738 @@
+// Attention of a few query rows to many cached keys on mma.sync tiles: what ncmb_cache_attention and
+// ncmb_block_attention share. The query rows of a kv head -- its G query heads times the tokens that share the keys --
+// are the 16-row tiles; a warp walks chunks of keys with a running maximum and sum a row.
+//
+// Products in fp32 grade whatever the types: a bf16 key meets an fp32 query as three bf16 terms (24 bits, exact products),
+// probabilities meet bf16 values as three terms (two where the result is bf16); fp32 keys and values as TF32 pairs, three
+// products. The leading term and the small ones have accumulators of their own, and a chunk's P V starts from zero and
+// is added to the running result in fp32 by the multiply-add that rescales it: the tensor core truncates its accumulator
+// after each product, which would bias a sum that runs over thousands of keys.
+#pragma once
+#include "cache.cuh"
+
+#include <algorithm>
+
+namespace ncmb {
+
+constexpr int CM_WARPS = 4, CM_THREADS = CM_WARPS * 32, CM_STAGES = 3, CM_STAGE = 8192;      // bytes of keys and values a stage
+
+template <class KE, class QE, int HDP_, int MT_> struct CmCfg {
+    static constexpr bool BF = sizeof(KE) == 2;
+    static constexpr int HDP = HDP_, MT = MT_, M = 16 * MT_;
+    static constexpr int ROW = HDP * (int)sizeof(KE);            // bytes of a key in shared memory
+    static constexpr int UPR = ROW / 16;
+    static constexpr int KC = CM_STAGE / (2 * ROW);              // keys a chunk: 32, 16, 16, 8
+    static constexpr int NT = KC / 8;                            // 8-key tiles a chunk
+    static constexpr int NQ = !BF ? 2 : sizeof(QE) == 4 ? 3 : 1; // terms of a query
+    static constexpr int NP = !BF ? 2 : sizeof(QE) == 4 ? 3 : 2; // terms of a probability
+    static constexpr int QBYTES = NQ * M * HDP * (BF ? 2 : 4);
+    static constexpr int RING = CM_WARPS * CM_STAGES * CM_STAGE;
+    static constexpr int SLOT = M * (HDP + 2);                   // floats of a partial result: maxima, sums, context
+};
+
+struct CmArgs {
+    CacheDev c;
+    const char *q; char *out;
+    int64_t ldq, ldo;                // bytes
+    int row0;                        // first row of this launch; items count from it
+    int H, G, T, M;                  // M: query rows of a kv head that share keys (T * G, or G)
+    int tiles;                       // tiles of CmCfg::M rows they make
+    int items;                       // rows, or rows * T where every token has keys of its own
+    const int *parents;
+    float c2;                        // scale * log2(e)
+    float *part;                     // partial results, one slot a (CTA + unit)
+    float *scores;                   // [row][kv head][M][pitch], or null
+    int64_t pitch;
+    float *weights;
+    // block attention
+    int block_log, n_sel;
+    const int *picks;
+};
+
+__device__ __forceinline__ uint32_t cm_smem(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void cm_cp16(uint32_t dst, const void *src, bool ok) {       // 16 bytes, zeros where not ok
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cm_ldm4(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void cm_ldm4t(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void cm_mma_bf16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void cm_mma_tf32(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void cm_tf32(float v, uint32_t &hi, uint32_t &lo) {
+    asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(hi) : "f"(v));
+    asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(lo) : "f"(v - __uint_as_float(hi)));
+}
+__device__ __forceinline__ float cm_exp2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ uint32_t cm_pack(float a, float b) {      // two bf16, a in the low half
+    const __nv_bfloat162 t = __floats2bfloat162_rn(a, b);
+    return *(const uint32_t *)&t;
+}
+__device__ __forceinline__ float2 cm_unpack(uint32_t u) { return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u)); }
+__device__ __forceinline__ void cm_put(float *p, float v) { *p = v; }
+__device__ __forceinline__ void cm_put(__nv_bfloat16 *p, float v) { *p = __float2bfloat16(v); }
+
+__device__ __forceinline__ bool cm_used(const int *par, int t) { return !par || (par[t] >= -1 && par[t] < t); }
+
+// keys that the queries of an item see
+template <bool BLOCKS> __device__ __forceinline__ int cm_keys(const CmArgs &a, int item) {
+    if (!BLOCKS) return cache_len(a.c, a.row0 + item, a.T) + a.T;
+    const int here = cache_len(a.c, a.row0 + item / a.T, a.T) + item % a.T, cur = here >> a.block_log;
+    return ((min(cur + 1, a.n_sel) - 1) << a.block_log) + (here & ((1 << a.block_log) - 1)) + 1;
+}
+
+// ---- how the chunks of all units are dealt to CTAs ----
+// The units (item, kv head, tile) in order, each with its chunks in order, are one sequence, of which every CTA takes an equal
+// run: rows of any lengths keep all SMs busy to the end. A unit is done by one CTA or by consecutive ones; CTA c's
+// partial result of unit u goes to slot c + u (along the sequence one of the two grows by one at a time).
+struct CmPlan { int64_t total, per; };
+__device__ __forceinline__ int64_t cm_block_sum(int64_t v, int64_t *sh) {      // over the CTA; all threads get it
+#pragma unroll
+    for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = v;
+    __syncthreads();
+    v = 0;
+#pragma unroll
+    for (int w = 0; w < CM_WARPS; w++) v += sh[w];
+    return v;
+}
+template <bool BLOCKS, int KC> __device__ __forceinline__ int64_t cm_chunks(const CmArgs &a, int item) {       // of all units of an item
+    return item < a.items ? (int64_t)((cm_keys<BLOCKS>(a, item) + KC - 1) / KC) * a.c.nkv * a.tiles : 0;
+}
+template <bool BLOCKS, int KC> __device__ CmPlan cm_plan(const CmArgs &a, int ctas, int64_t *sh) {
+    int64_t t = 0;
+    for (int i = threadIdx.x; i < a.items; i += CM_THREADS) t += cm_chunks<BLOCKS, KC>(a, i);
+    CmPlan p;
+    p.total = cm_block_sum(t, sh);
+    p.per = ((p.total + ctas - 1) / ctas + CM_WARPS - 1) / CM_WARPS * CM_WARPS;
+    return p;
+}
+// the item that holds place x of the sequence, and where that item begins; or, with item >= 0 given, where it begins
+template <bool BLOCKS, int KC> __device__ int cm_find(const CmArgs &a, int64_t x, int item, int64_t &start, int64_t *sh) {
+    __shared__ int found;
+    __shared__ int64_t at;
+    if (a.items == 1) { start = 0; return 0; }
+    int64_t before = 0;
+    for (int i0 = 0;; i0 += CM_THREADS) {
+        const int i = i0 + threadIdx.x, lane = threadIdx.x & 31;
+        const int64_t mine = cm_chunks<BLOCKS, KC>(a, i);
+        int64_t inc = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int64_t v = __shfl_up_sync(0xffffffffu, inc, o);
+            if (lane >= o) inc += v;
+        }
+        __syncthreads();
+        if (lane == 31) sh[threadIdx.x >> 5] = inc;
+        if (threadIdx.x == 0) found = -1;
+        __syncthreads();
+        int64_t lead = before;
+        for (int w = 0; w < (int)(threadIdx.x >> 5); w++) lead += sh[w];
+        const int64_t from = lead + inc - mine;
+        if (item >= 0 ? i == item : (i < a.items && x >= from && x < from + mine)) { found = i; at = from; }
+        for (int w = 0; w < CM_WARPS; w++) before += sh[w];
+        __syncthreads();
+        if (found >= 0 || i0 + CM_THREADS >= a.items) break;
+    }
+    start = at;
+    return found;
+}
+
+// ---- the attention kernel ----
+// Shared memory: the ring (per warp, CM_STAGES stages of keys then values), the terms of the queries, the masks of the nodes.
+// bf16 rows are swizzled by 16-byte units for ldmatrix (unit ^ row & 7); fp32 keys by (row & 1) << 2 and values by
+// ((row >> 1) & 3) << 1, for a lane's own 16-byte reads: a lane has the key n = lane / 4 of a score tile and of each 16 dims
+// the four from 4 (lane % 4) on, which are its elements of two k-steps; of a P V tile the keys 2 (lane % 4) and the next, and
+// of each 32 dims the four from 4 (lane / 4) on, which are its column of four tiles. Where a dim stands in a k-step and where a
+// column in a tile is free as long as both operands, or all who read the result, agree.
+template <class KE, class QE, int HDP, int MT, bool BLOCKS>
+__global__ void __launch_bounds__(CM_THREADS, 2) k_cache_attention(const __grid_constant__ CmArgs a) {
+    using F = CmCfg<KE, QE, HDP, MT>;
+    constexpr int KC = F::KC, NT = F::NT, NQ = F::NQ, NP = F::NP, ROW = F::ROW, UPR = F::UPR, M = F::M;
+    extern __shared__ __align__(128) char smem[];
+    char *ring = smem, *qs = smem + F::RING;
+    __shared__ int64_t sh[CM_WARPS];
+    __shared__ uint32_t node_bits[BLOCKS ? 1 : M][8];       // ancestors of the tile's nodes (from node m0 / G on)
+    __shared__ uint32_t used_bits[8];
+    __shared__ int spar[BLOCKS ? 1 : NCMB_MAX_NODES];
+    __shared__ int spicks[BLOCKS ? 1024 : 1];
+    __shared__ float wm[CM_WARPS][M], wl[CM_WARPS][M];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c4 = lane & 3;
+    const int hd = a.c.hd, G = a.G;
+    pdl_launch_dependents();
+    pdl_wait();
+    const CmPlan plan = cm_plan<BLOCKS, KC>(a, gridDim.x, sh);
+    int64_t at = (int64_t)blockIdx.x * plan.per;
+    const int64_t end = min(plan.total, at + plan.per);
+    if (at >= end) return;
+    int64_t item_at;
+    int item = cm_find<BLOCKS, KC>(a, at, -1, item_at, sh);
+    char *my = ring + warp * (CM_STAGES * CM_STAGE);
+    while (at < end) {
+        const int n = cm_keys<BLOCKS>(a, item), nch = (n + KC - 1) / KC;
+        const int64_t into = at - item_at;
+        const int sub = (int)(into / nch), kvh = sub / a.tiles, tile = sub % a.tiles;
+        const int first = (int)(into % nch), stop = (int)min((int64_t)nch, first + (end - at));
+        const int64_t unit = (int64_t)item * a.c.nkv * a.tiles + sub;
+        const int m0 = tile * M;
+        const int row = a.row0 + (BLOCKS ? item / a.T : item), tok = BLOCKS ? item % a.T : 0, len = BLOCKS ? n : n - a.T;
+        const bool tail = !BLOCKS && stop * KC > len;            // this run has keys of the new tokens
+        const int *par = a.parents ? a.parents + (int64_t)row * a.T : nullptr;
+        __syncthreads();
+        if (BLOCKS) {
+            const int np = ((n - 1) >> a.block_log) + 1;
+            const int *picks = a.picks + ((int64_t)(a.row0 * a.T + item) * a.c.nkv + kvh) * a.n_sel;
+            for (int i = tid; i < np; i += CM_THREADS) spicks[i] = picks[i];
+        } else if (par) {
+            for (int i = tid; i < a.T; i += CM_THREADS) spar[i] = par[i];
+        }
+        __syncthreads();
+        if (!BLOCKS && par) {
+            for (int w = warp; w < 8; w += CM_WARPS) {
+                const int t = w * 32 + lane;
+                const uint32_t u = __ballot_sync(0xffffffffu, t < a.T && spar[t] >= -1 && spar[t] < t);
+                if (lane == 0) used_bits[w] = u;
+            }
+            __syncthreads();
+        }
+        auto used = [&](int t) { return !par || ((used_bits[t >> 5] >> (t & 31)) & 1u); };
+        // loads run CM_STAGES - 1 chunks ahead of the arithmetic
+        const char *kb = a.c.k + row * a.c.rs + kvh * a.c.hs, *vb = a.c.v + row * a.c.rs + kvh * a.c.hs;
+        const int lu = lane % UPR, lr = lane / UPR;
+        constexpr int RPI = 32 / UPR;                            // rows that the warp's lanes cover at once
+        const bool lane_in = lu * 16 < hd * (int)sizeof(KE);
+        auto load = [&](int ch, int stage) {
+            const uint32_t ks = cm_smem(my + stage * CM_STAGE), vs = ks + CM_STAGE / 2;
+#pragma unroll
+            for (int i = 0; i < KC / RPI; i++) {
+                const int r = lr + i * RPI, pos = ch * KC + r;
+                bool ok = lane_in && pos < n;
+                int64_t slot = pos;
+                if (BLOCKS) slot = ok ? ((int64_t)spicks[pos >> a.block_log] << a.block_log) + (pos & ((1 << a.block_log) - 1)) : 0;
+                else if (tail && ok && pos >= len) ok = used(pos - len);
+                const int64_t off = ok ? slot * a.c.ts + lu * 16 : 0;
+                const int ku = F::BF ? lu ^ (r & 7) : lu ^ ((r & 1) << 2), vu = F::BF ? ku : lu ^ (((r >> 1) & 3) << 1);
+                cm_cp16(ks + r * ROW + ku * 16, kb + off, ok);
+                cm_cp16(vs + r * ROW + vu * 16, vb + off, ok);
+            }
+        };
+        int next = first + warp;
+#pragma unroll
+        for (int s = 0; s < CM_STAGES - 1; s++) {
+            if (next < stop) load(next, s);
+            asm volatile("cp.async.commit_group;" ::: "memory");
+            next += CM_WARPS;
+        }
+        // the tile's queries as terms, zero where no query stands
+        for (int i = tid; i < M * HDP / 8; i += CM_THREADS) {
+            const int m = i / (HDP / 8), d0 = i % (HDP / 8) * 8, mm = m0 + m;
+            float x[8];
+#pragma unroll
+            for (int e = 0; e < 8; e++) x[e] = 0.f;
+            if (mm < a.M && d0 < hd) {
+                const int t = BLOCKS ? tok : mm / G, h = kvh * G + mm % G;
+                if (BLOCKS || used(t)) {
+                    const char *p = a.q + ((int64_t)row * a.T + t) * a.ldq + ((int64_t)h * hd + d0) * sizeof(QE);
+                    if (sizeof(QE) == 4) {
+                        *(float4 *)&x[0] = *(const float4 *)p;
+                        *(float4 *)&x[4] = *(const float4 *)(p + 16);
+                    } else {
+                        const uint4 u = *(const uint4 *)p;
+                        const uint32_t uu[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+                        for (int e = 0; e < 4; e++) { const float2 f = cm_unpack(uu[e]); x[2 * e] = f.x; x[2 * e + 1] = f.y; }
+                    }
+                }
+            }
+            if constexpr (F::BF) {
+#pragma unroll
+                for (int k = 0; k < NQ; k++) {
+                    uint32_t u[4];
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        u[e] = cm_pack(x[2 * e], x[2 * e + 1]);
+                        const float2 f = cm_unpack(u[e]);
+                        x[2 * e] -= f.x; x[2 * e + 1] -= f.y;
+                    }
+                    *(uint4 *)(qs + (k * M + m) * ROW + (((d0 / 8) ^ (m & 7)) * 16)) = make_uint4(u[0], u[1], u[2], u[3]);
+                }
+            } else {
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    uint32_t hi[4], lo[4];
+#pragma unroll
+                    for (int e = 0; e < 4; e++) cm_tf32(x[4 * h + e], hi[e], lo[e]);
+                    const int u = (d0 / 4 + h) ^ ((m & 1) << 2);
+                    *(uint4 *)(qs + m * ROW + u * 16) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                    *(uint4 *)(qs + (M + m) * ROW + u * 16) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                }
+            }
+        }
+        if (tail) {
+            const int t0 = m0 / G, nt = (min(a.M, m0 + M) + G - 1) / G - t0;       // nodes of this tile
+            for (int i = tid; i < nt; i += CM_THREADS) {
+                const int t = t0 + i;
+                uint32_t b[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+                if (!par) {
+#pragma unroll
+                    for (int w = 0; w < 8; w++) b[w] = t >= 32 * w + 31 ? 0xffffffffu : t >= 32 * w ? (2u << (t - 32 * w)) - 1 : 0u;
+                } else {
+                    for (int x = t; x >= 0 && used(x); x = spar[x]) {
+#pragma unroll
+                        for (int w = 0; w < 8; w++) if ((x >> 5) == w) b[w] |= 1u << (x & 31);
+                    }
+                }
+#pragma unroll
+                for (int w = 0; w < 8; w++) node_bits[i][w] = b[w];
+            }
+        }
+        __syncthreads();
+        float O[MT][HDP / 8][4], mx[MT][2], ls[MT][2];
+#pragma unroll
+        for (int mt = 0; mt < MT; mt++) {
+#pragma unroll
+            for (int j = 0; j < HDP / 8; j++) { O[mt][j][0] = O[mt][j][1] = O[mt][j][2] = O[mt][j][3] = 0.f; }
+            mx[mt][0] = mx[mt][1] = -INFINITY;
+            ls[mt][0] = ls[mt][1] = 0.f;
+        }
+        int stage = 0;
+        for (int ch = first + warp; ch < stop; ch += CM_WARPS) {
+            asm volatile("cp.async.wait_group %0;" ::"n"(CM_STAGES - 2) : "memory");
+            __syncwarp();
+            {
+                int s = stage + CM_STAGES - 1;
+                if (s >= CM_STAGES) s -= CM_STAGES;
+                if (next < stop) load(next, s);
+                asm volatile("cp.async.commit_group;" ::: "memory");
+                next += CM_WARPS;
+            }
+            const char *kt = my + stage * CM_STAGE, *vt = kt + CM_STAGE / 2;
+            const bool masked = (ch + 1) * KC > len;
+#pragma unroll
+            for (int mt = 0; mt < MT; mt++) {
+                if (MT > 1 && m0 + 16 * mt >= a.M) break;
+                float S[NT][4], L[NT][4];
+#pragma unroll
+                for (int j = 0; j < NT; j++) { S[j][0] = S[j][1] = S[j][2] = S[j][3] = 0.f; L[j][0] = L[j][1] = L[j][2] = L[j][3] = 0.f; }
+                if constexpr (F::BF) {
+#pragma unroll
+                    for (int kp = 0; kp < HDP / 32; kp++) {              // two k-steps at a time
+                        uint32_t kf[NT][4];
+#pragma unroll
+                        for (int j = 0; j < NT; j++)
+                            cm_ldm4(kf[j], cm_smem(kt) + (8 * j + (lane & 7)) * ROW + (((4 * kp + (lane >> 3)) ^ (lane & 7)) * 16));
+#pragma unroll
+                        for (int e = 0; e < 2; e++) {
+                            const int qr = 16 * mt + (lane & 15), qu = 4 * kp + 2 * e + (lane >> 4);
+#pragma unroll
+                            for (int k = NQ - 1; k >= 0; k--) {
+                                uint32_t qf[4];
+                                cm_ldm4(qf, cm_smem(qs) + (k * M + qr) * ROW + ((qu ^ (qr & 7)) * 16));
+#pragma unroll
+                                for (int j = 0; j < NT; j++) cm_mma_bf16(k ? L[j] : S[j], qf, kf[j][2 * e], kf[j][2 * e + 1]);
+                            }
+                        }
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < HDP / 16; i++) {                 // two k-steps at a time
+                        const int r0 = 16 * mt + g, u0 = (4 * i + c4) ^ ((r0 & 1) << 2);       // r0 and r0 + 8: the same parity
+                        const uint4 h0 = *(const uint4 *)(qs + r0 * ROW + u0 * 16), h1 = *(const uint4 *)(qs + (r0 + 8) * ROW + u0 * 16);
+                        const uint4 l0 = *(const uint4 *)(qs + (M + r0) * ROW + u0 * 16), l1 = *(const uint4 *)(qs + (M + r0 + 8) * ROW + u0 * 16);
+                        const uint32_t ah[2][4] = {{h0.x, h1.x, h0.y, h1.y}, {h0.z, h1.z, h0.w, h1.w}};
+                        const uint32_t al[2][4] = {{l0.x, l1.x, l0.y, l1.y}, {l0.z, l1.z, l0.w, l1.w}};
+#pragma unroll
+                        for (int j = 0; j < NT; j++) {
+                            const float4 kx = *(const float4 *)(kt + (8 * j + g) * ROW + (((4 * i + c4) ^ ((g & 1) << 2)) * 16));
+                            const float kv[4] = {kx.x, kx.y, kx.z, kx.w};
+#pragma unroll
+                            for (int e = 0; e < 2; e++) {
+                                uint32_t bh[2], bl[2];
+                                cm_tf32(kv[2 * e], bh[0], bl[0]);
+                                cm_tf32(kv[2 * e + 1], bh[1], bl[1]);
+                                cm_mma_tf32(L[j], al[e], bh[0], bh[1]);
+                                cm_mma_tf32(L[j], ah[e], bl[0], bl[1]);
+                                cm_mma_tf32(S[j], ah[e], bh[0], bh[1]);
+                            }
+                        }
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < NT; j++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) S[j][e] = (S[j][e] + L[j][e]) * a.c2;
+                if (masked) {
+#pragma unroll
+                    for (int hh = 0; hh < 2; hh++) {
+                        const int mm = min(m0 + 16 * mt + g + 8 * hh, a.M - 1);
+                        const uint32_t *bits = node_bits[BLOCKS ? 0 : mm / G - m0 / G];
+#pragma unroll
+                        for (int j = 0; j < NT; j++)
+#pragma unroll
+                            for (int e = 0; e < 2; e++) {
+                                const int pos = ch * KC + 8 * j + 2 * c4 + e;
+                                bool see = pos < len;
+                                if (!BLOCKS && !see && pos < n) see = (bits[(pos - len) >> 5] >> ((pos - len) & 31)) & 1u;
+                                if (!see) S[j][2 * hh + e] = -INFINITY;
+                            }
+                    }
+                }
+                if (!BLOCKS && a.scores) {
+                    float *sp = a.scores + ((int64_t)item * a.c.nkv + kvh) * a.M * a.pitch + ch * KC + 2 * c4;
+#pragma unroll
+                    for (int hh = 0; hh < 2; hh++) {
+                        const int mm = m0 + 16 * mt + g + 8 * hh;
+                        if (mm < a.M) {
+#pragma unroll
+                            for (int j = 0; j < NT; j++) *(float2 *)(sp + mm * a.pitch + 8 * j) = make_float2(S[j][2 * hh], S[j][2 * hh + 1]);
+                        }
+                    }
+                }
+                float al[2];
+#pragma unroll
+                for (int hh = 0; hh < 2; hh++) {
+                    float t = -INFINITY;
+#pragma unroll
+                    for (int j = 0; j < NT; j++) t = fmaxf(t, fmaxf(S[j][2 * hh], S[j][2 * hh + 1]));
+                    t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 1));
+                    t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 2));
+                    t = fmaxf(t, mx[mt][hh]);
+                    const float base = t == -INFINITY ? 0.f : t;
+                    al[hh] = cm_exp2(mx[mt][hh] - base);
+                    mx[mt][hh] = t;
+                    float sum = 0.f;
+#pragma unroll
+                    for (int j = 0; j < NT; j++)
+#pragma unroll
+                        for (int e = 0; e < 2; e++) { S[j][2 * hh + e] = cm_exp2(S[j][2 * hh + e] - base); sum += S[j][2 * hh + e]; }
+                    ls[mt][hh] = ls[mt][hh] * al[hh] + sum;
+                }
+                bool odd = false;                                        // an infinity or NaN among values that not every row sees
+                if (masked && !BLOCKS) {
+                    for (int i = lane; i < KC * HDP; i += 32) {
+                        const float x = (float)((const KE *)vt)[i];
+                        odd |= !(fabsf(x) < INFINITY);
+                    }
+                    odd = __any_sync(0xffffffffu, odd);
+                }
+                if (odd) {
+                    // rows that do not see such a value must not multiply it by zero: one key at a time
+#pragma unroll
+                    for (int j = 0; j < HDP / 8; j++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) O[mt][j][e] *= al[e >> 1];
+#pragma unroll
+                    for (int jj = 0; jj < NT; jj++)
+                        for (int r = 0; r < 8; r++) {
+                            const int src = (lane & ~3) | (r >> 1);
+                            const float p0 = __shfl_sync(0xffffffffu, (r & 1) ? S[jj][1] : S[jj][0], src), p1 = __shfl_sync(0xffffffffu, (r & 1) ? S[jj][3] : S[jj][2], src);
+                            const int kr = 8 * jj + r;
+#pragma unroll
+                            for (int j = 0; j < HDP / 8; j++)
+#pragma unroll
+                                for (int e = 0; e < 2; e++) {
+                                    const int d = F::BF ? 8 * j + 2 * c4 + e : 32 * (j / 4) + 8 * c4 + 4 * e + j % 4;
+                                    const int u = d * (int)sizeof(KE) / 16, us = F::BF ? u ^ (kr & 7) : u ^ (((kr >> 1) & 3) << 1);
+                                    const float x = (float)*(const KE *)(vt + kr * ROW + us * 16 + d * sizeof(KE) % 16);
+                                    if (p0 != 0.f) O[mt][j][e] = fmaf(p0, x, O[mt][j][e]);
+                                    if (p1 != 0.f) O[mt][j][2 + e] = fmaf(p1, x, O[mt][j][2 + e]);
+                                }
+                        }
+                    continue;
+                }
+                if constexpr (F::BF) {
+                    uint32_t pf[NP][KC / 16][4];
+#pragma unroll
+                    for (int k2 = 0; k2 < KC / 16; k2++)
+#pragma unroll
+                        for (int k = 0; k < NP; k++)
+#pragma unroll
+                            for (int e = 0; e < 4; e++) {
+                                float *s = &S[2 * k2 + (e >> 1)][2 * (e & 1)];
+                                pf[k][k2][e] = cm_pack(s[0], s[1]);
+                                const float2 f = cm_unpack(pf[k][k2][e]);
+                                s[0] -= f.x; s[1] -= f.y;
+                            }
+#pragma unroll
+                    for (int jp = 0; jp < HDP / 16; jp++) {              // two tiles of 8 dims at a time
+                        float c0[4] = {0.f, 0.f, 0.f, 0.f}, c1[4] = {0.f, 0.f, 0.f, 0.f}, d0[4] = {0.f, 0.f, 0.f, 0.f}, d1[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                        for (int k2 = 0; k2 < KC / 16; k2++) {
+                            uint32_t vf[4];
+                            const int vr = 16 * k2 + (lane & 15);
+                            cm_ldm4t(vf, cm_smem(vt) + vr * ROW + (((2 * jp + (lane >> 4)) ^ (vr & 7)) * 16));
+#pragma unroll
+                            for (int k = NP - 1; k >= 1; k--) { cm_mma_bf16(d0, pf[k][k2], vf[0], vf[1]); cm_mma_bf16(d1, pf[k][k2], vf[2], vf[3]); }
+                            cm_mma_bf16(c0, pf[0][k2], vf[0], vf[1]);
+                            cm_mma_bf16(c1, pf[0][k2], vf[2], vf[3]);
+                        }
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            O[mt][2 * jp][e] = fmaf(O[mt][2 * jp][e], al[e >> 1], c0[e] + d0[e]);
+                            O[mt][2 * jp + 1][e] = fmaf(O[mt][2 * jp + 1][e], al[e >> 1], c1[e] + d1[e]);
+                        }
+                    }
+                } else {
+                    uint32_t ph[NT][4], pl[NT][4];
+#pragma unroll
+                    for (int j = 0; j < NT; j++) {                       // k position c: key 2 c, position c + 4: key 2 c + 1
+                        cm_tf32(S[j][0], ph[j][0], pl[j][0]); cm_tf32(S[j][2], ph[j][1], pl[j][1]);
+                        cm_tf32(S[j][1], ph[j][2], pl[j][2]); cm_tf32(S[j][3], ph[j][3], pl[j][3]);
+                    }
+#pragma unroll
+                    for (int jj = 0; jj < HDP / 32; jj++) {              // four tiles of 8 dims at a time
+                        float cc[4][4], dd[4][4];
+#pragma unroll
+                        for (int x = 0; x < 4; x++)
+#pragma unroll
+                            for (int e = 0; e < 4; e++) cc[x][e] = dd[x][e] = 0.f;
+#pragma unroll
+                        for (int j = 0; j < NT; j++) {
+                            const int r0 = 8 * j + 2 * c4, u = (8 * jj + g) ^ (c4 << 1);        // (row >> 1) & 3 = c4 for both rows
+                            const float4 v0 = *(const float4 *)(vt + r0 * ROW + u * 16), v1 = *(const float4 *)(vt + (r0 + 1) * ROW + u * 16);
+                            const float va[4] = {v0.x, v0.y, v0.z, v0.w}, vv[4] = {v1.x, v1.y, v1.z, v1.w};
+#pragma unroll
+                            for (int x = 0; x < 4; x++) {
+                                uint32_t bh[2], bl[2];
+                                cm_tf32(va[x], bh[0], bl[0]);
+                                cm_tf32(vv[x], bh[1], bl[1]);
+                                cm_mma_tf32(dd[x], pl[j], bh[0], bh[1]);
+                                cm_mma_tf32(dd[x], ph[j], bl[0], bl[1]);
+                                cm_mma_tf32(cc[x], ph[j], bh[0], bh[1]);
+                            }
+                        }
+#pragma unroll
+                        for (int x = 0; x < 4; x++)
+#pragma unroll
+                            for (int e = 0; e < 4; e++) O[mt][4 * jj + x][e] = fmaf(O[mt][4 * jj + x][e], al[e >> 1], cc[x][e] + dd[x][e]);
+                    }
+                }
+            }
+            if (++stage == CM_STAGES) stage = 0;
+        }
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+        // the warps' results meet in shared memory: every warp's maxima first, then scaled contexts where the ring was
+#pragma unroll
+        for (int mt = 0; mt < MT; mt++)
+#pragma unroll
+            for (int hh = 0; hh < 2; hh++) {
+                float l = ls[mt][hh];
+                l += __shfl_xor_sync(0xffffffffu, l, 1);
+                l += __shfl_xor_sync(0xffffffffu, l, 2);
+                if (c4 == 0) { wm[warp][16 * mt + g + 8 * hh] = mx[mt][hh]; wl[warp][16 * mt + g + 8 * hh] = l; }
+            }
+        __syncthreads();
+        float *ctx_sh = (float *)ring;                           // [warp][M][HDP]
+        static_assert(CM_WARPS * M * HDP * 4 <= F::RING, "contexts of the warps fit the ring");
+#pragma unroll
+        for (int mt = 0; mt < MT; mt++)
+#pragma unroll
+            for (int hh = 0; hh < 2; hh++) {
+                const int m = 16 * mt + g + 8 * hh;
+                float top = wm[0][m];
+#pragma unroll
+                for (int w = 1; w < CM_WARPS; w++) top = fmaxf(top, wm[w][m]);
+                const float f = mx[mt][hh] == -INFINITY ? 0.f : cm_exp2(mx[mt][hh] - top);
+                float *o = ctx_sh + (warp * M + m) * HDP;
+#pragma unroll
+                for (int j = 0; j < HDP / 8; j++)
+#pragma unroll
+                    for (int e = 0; e < 2; e++) {
+                        const int d = F::BF ? 8 * j + 2 * c4 + e : 32 * (j / 4) + 8 * c4 + 4 * e + j % 4;
+                        o[d] = O[mt][j][2 * hh + e] * f;
+                    }
+            }
+        __syncthreads();
+        const bool whole = first == 0 && stop == nch;
+        float *slot = a.part + ((int64_t)blockIdx.x + unit) * F::SLOT;
+        for (int m = tid; m < M; m += CM_THREADS) {
+            float top = wm[0][m], l = 0.f;
+#pragma unroll
+            for (int w = 1; w < CM_WARPS; w++) top = fmaxf(top, wm[w][m]);
+#pragma unroll
+            for (int w = 0; w < CM_WARPS; w++) l += wm[w][m] == -INFINITY ? 0.f : wl[w][m] * cm_exp2(wm[w][m] - top);
+            slot[m] = top;
+            slot[M + m] = l;
+            wl[0][m] = l;                                        // read by the owner of this m alone until the barrier
+        }
+        __syncthreads();
+        for (int i = tid; i < M * HDP; i += CM_THREADS) {
+            const int m = i / HDP, d = i % HDP, mm = m0 + m;
+            if (mm >= a.M) break;
+            if (d >= hd) continue;
+            float o = 0.f;
+#pragma unroll
+            for (int w = 0; w < CM_WARPS; w++) o += ctx_sh[(w * M + m) * HDP + d];
+            if (!whole) { slot[2 * M + i] = o; continue; }
+            const int t = BLOCKS ? tok : mm / G, h = kvh * G + mm % G;
+            const float l = wl[0][m];
+            const bool ok = l > 0.f && (BLOCKS || used(t));
+            cm_put((QE *)(a.out + ((int64_t)row * a.T + t) * a.ldo) + (int64_t)h * hd + d, ok ? o / l : 0.f);
+        }
+        at += stop - first;
+        if (at == item_at + (int64_t)nch * a.c.nkv * a.tiles) { item_at = at; item++; }
+    }
+}
+
+// ---- units that several CTAs share are joined; weights are added up ----
+// CTAs [0, units): one unit each. The others: 512 slots of one (row, kv head) each, from the scores that the kernel above left.
+constexpr int CM_WKEYS = 512;
+template <class KE, class QE, int HDP, int MT, bool BLOCKS>
+__global__ void __launch_bounds__(CM_THREADS) k_cache_join(const __grid_constant__ CmArgs a, int ctas, int units) {
+    using F = CmCfg<KE, QE, HDP, MT>;
+    constexpr int M = F::M, KC = F::KC;
+    __shared__ int64_t sh[CM_WARPS];
+    __shared__ float lse[NCMB_MAX_NODES];
+    const int tid = threadIdx.x, G = a.G, hd = a.c.hd;
+    pdl_launch_dependents();
+    pdl_wait();
+    const CmPlan plan = cm_plan<BLOCKS, KC>(a, ctas, sh);
+    const bool join = (int)blockIdx.x < units;
+    const int per_item = a.c.nkv * a.tiles;
+    int item, sub, key0 = 0;
+    if (join) { item = blockIdx.x / per_item; sub = blockIdx.x % per_item; }
+    else {
+        const int span = (int)((a.pitch + CM_WKEYS - 1) / CM_WKEYS), x = blockIdx.x - units;
+        key0 = x % span * CM_WKEYS;
+        sub = x / span % a.c.nkv * a.tiles;
+        item = x / span / a.c.nkv;
+    }
+    const int n = cm_keys<BLOCKS>(a, item), nch = (n + KC - 1) / KC;
+    if (!join && key0 >= n) return;
+    int64_t start;
+    cm_find<BLOCKS, KC>(a, 0, item, start, sh);
+    const int row = a.row0 + (BLOCKS ? item / a.T : item);
+    const int *par = a.parents ? a.parents + (int64_t)row * a.T : nullptr;
+    // CTAs that have a part of a unit
+    auto parts = [&](int s, int &c0, int &c1) {
+        const int64_t from = start + (int64_t)s * nch;
+        c0 = (int)(from / plan.per);
+        c1 = (int)((from + nch - 1) / plan.per);
+    };
+    int c0, c1;
+    if (join) {
+        parts(sub, c0, c1);
+        if (c0 == c1) return;                                    // written already
+        const float *slot = a.part + (int64_t)(c0 + blockIdx.x) * F::SLOT;
+        const int kvh = sub / a.tiles, m0 = sub % a.tiles * M, nm = min(M, a.M - m0);
+        for (int i = tid; i < nm * (HDP / 4); i += CM_THREADS) {
+            const int m = i / (HDP / 4), d = i % (HDP / 4) * 4, mm = m0 + m;
+            if (d >= hd) continue;
+            float top = -INFINITY, l = 0.f;
+            float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+            for (int c = 0; c <= c1 - c0; c++) top = fmaxf(top, slot[c * F::SLOT + m]);
+            for (int c = 0; c <= c1 - c0; c++) {
+                const float x = slot[c * F::SLOT + m], f = x == -INFINITY ? 0.f : cm_exp2(x - top);
+                const float4 p = *(const float4 *)(slot + c * F::SLOT + 2 * M + m * HDP + d);
+                l = fmaf(slot[c * F::SLOT + M + m], f, l);
+                o.x = fmaf(p.x, f, o.x); o.y = fmaf(p.y, f, o.y); o.z = fmaf(p.z, f, o.z); o.w = fmaf(p.w, f, o.w);
+            }
+            const int t = BLOCKS ? item % a.T : mm / G, h = kvh * G + mm % G;
+            const float r = l > 0.f && (BLOCKS || cm_used(par, t)) ? 1.f / l : 0.f;
+            QE *out = (QE *)(a.out + ((int64_t)row * a.T + t) * a.ldo) + (int64_t)h * hd + d;
+            cm_put(out, o.x * r); cm_put(out + 1, o.y * r); cm_put(out + 2, o.z * r); cm_put(out + 3, o.w * r);
+        }
+        return;
+    }
+    const int kvh = sub / a.tiles, len = n - a.T;
+    float w[CM_WKEYS / CM_THREADS];
+#pragma unroll
+    for (int x = 0; x < CM_WKEYS / CM_THREADS; x++) w[x] = 0.f;
+    const float *sc = a.scores + ((int64_t)item * a.c.nkv + kvh) * a.M * a.pitch + key0 + tid;
+    for (int mb = 0; mb < a.M; mb += NCMB_MAX_NODES) {
+        const int nm = min(NCMB_MAX_NODES, a.M - mb);
+        __syncthreads();
+        for (int i = tid; i < nm; i += CM_THREADS) {
+            const int mm = mb + i, s = sub + mm / M, m = mm % M;
+            parts(s, c0, c1);
+            const float *slot = a.part + ((int64_t)c0 + (int64_t)item * per_item + s) * F::SLOT;
+            float top = -INFINITY, l = 0.f;
+            for (int c = 0; c <= c1 - c0; c++) top = fmaxf(top, slot[c * F::SLOT + m]);
+            for (int c = 0; c <= c1 - c0; c++) {
+                const float x = slot[c * F::SLOT + m];
+                if (x != -INFINITY) l = fmaf(slot[c * F::SLOT + M + m], cm_exp2(x - top), l);
+            }
+            lse[i] = l > 0.f && cm_used(par, mm / G) ? top + log2f(l) : INFINITY;
+        }
+        __syncthreads();
+        for (int i = 0; i < nm; i++) {
+            const float e = lse[i];
+#pragma unroll
+            for (int x = 0; x < CM_WKEYS / CM_THREADS; x++)
+                if (key0 + tid + x * CM_THREADS < n) w[x] += cm_exp2(sc[(int64_t)(mb + i) * a.pitch + x * CM_THREADS] - e);
+        }
+    }
+    float *wp = a.weights + ((int64_t)row * a.c.nkv + kvh) * a.c.cap;
+#pragma unroll
+    for (int x = 0; x < CM_WKEYS / CM_THREADS; x++) {
+        const int key = key0 + tid + x * CM_THREADS;
+        if (key < len) wp[key] += w[x];
+        else if (key < n) wp[key] = w[x];
+    }
+}
+
+// ---- launches ----
+template <class KE, class QE, int HDP, int MT, bool BLOCKS>
+int cm_run_as(const char *who, CmArgs a, int max_keys) {
+    using F = CmCfg<KE, QE, HDP, MT>;
+    a.tiles = (int)cdiv(a.M, F::M);
+    const int smem = F::RING + F::QBYTES;
+    static bool set = false;
+    if (!set) {
+        CUDA_CHECK(cudaFuncSetAttribute(k_cache_attention<KE, QE, HDP, MT, BLOCKS>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+        set = true;
+    }
+    // rows of a launch: as many as leave the scores some GB at most
+    const int rows = a.c.rows, per_row = BLOCKS ? a.T : 1;
+    int step = rows;
+    if (a.weights) {
+        a.pitch = cdiv((int64_t)a.c.cap, CM_WKEYS) * CM_WKEYS;
+        const int64_t row_bytes = (int64_t)a.c.nkv * a.M * a.pitch * 4;
+        step = (int)std::max<int64_t>(1, std::min<int64_t>(rows, ((int64_t)2 << 30) / row_bytes));
+    }
+    const int64_t units = (int64_t)step * per_row * a.c.nkv * a.tiles;
+    const int64_t spans = a.weights ? cdiv(a.pitch, CM_WKEYS) * step * a.c.nkv : 0;
+    if (units + spans > 0x7fffffff) return cache_refuse(who, "%lld query tiles", (long long)units);
+    const int64_t est = units * cdiv(max_keys, F::KC);
+    const int ctas = (int)std::max<int64_t>(1, std::min<int64_t>(2 * ctx().sm_count, cdiv(est, CM_WARPS)));
+    const size_t part = (size_t)(units + ctas) * F::SLOT * 4, sc = a.weights ? (size_t)step * a.c.nkv * a.M * a.pitch * 4 : 0;
+    char *scratch = (char *)cache_scratch(who, part + sc);
+    if (!scratch) return -1;
+    a.scores = a.weights ? (float *)scratch : nullptr;
+    a.part = (float *)(scratch + sc);
+    for (int r = 0; r < rows; r += step) {
+        const int nr = std::min(step, rows - r);
+        a.row0 = r;
+        a.items = nr * per_row;
+        const int u = a.items * a.c.nkv * a.tiles;
+        LAUNCH_PDL((k_cache_attention<KE, QE, HDP, MT, BLOCKS>), ctas, CM_THREADS, smem, a);
+        LAUNCH_PDL((k_cache_join<KE, QE, HDP, MT, BLOCKS>), (unsigned)(u + spans / step * nr), CM_THREADS, 0, a, ctas, u);
+    }
+    return 0;
+}
+// tiles of 16, 32 or (head dim 64) 64 query rows
+template <class KE, class QE, bool BLOCKS>
+int cm_run(const char *who, const CmArgs &a, int max_keys) {
+    if (a.c.hd <= 64) {
+        if (a.M <= 16) return cm_run_as<KE, QE, 64, 1, BLOCKS>(who, a, max_keys);
+        if (a.M <= 32) return cm_run_as<KE, QE, 64, 2, BLOCKS>(who, a, max_keys);
+        return cm_run_as<KE, QE, 64, 4, BLOCKS>(who, a, max_keys);
+    }
+    if (a.M <= 16) return cm_run_as<KE, QE, 128, 1, BLOCKS>(who, a, max_keys);
+    return cm_run_as<KE, QE, 128, 2, BLOCKS>(who, a, max_keys);
+}
+
+} // namespace ncmb

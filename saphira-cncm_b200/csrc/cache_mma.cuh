@@ -14,18 +14,30 @@
 
 namespace ncmb {
 
-constexpr int CM_WARPS = 4, CM_THREADS = CM_WARPS * 32, CM_STAGES = 3, CM_STAGE = 8192;      // bytes of keys and values a stage
+constexpr int CM_WARPS = 4, CM_THREADS = CM_WARPS * 32;
+#ifndef CM_SB
+#define CM_SB 8192
+#define CM_ST 2
+#define CM_CTAS 3
+#endif
+constexpr int CM_STAGES = CM_ST, CM_STAGE = CM_SB;      // stages of a warp's ring, and bytes of keys and values in one
 
-template <class KE, class QE, int HDP_, int MT_> struct CmCfg {
+// R: query rows of a tile, 16 or 8. A tile of 8 has two terms of its queries (or probabilities) stacked in the 16 rows of the
+// tensor-core tile; a lane holds rows lane / 4 and lane / 4 + 8 of a result, so it adds the two terms' products up itself.
+template <class KE, class QE, int HDP_, int R_> struct CmCfg {
     static constexpr bool BF = sizeof(KE) == 2;
-    static constexpr int HDP = HDP_, MT = MT_, M = 16 * MT_;
+    static constexpr int HDP = HDP_, M = R_;
+    static constexpr bool R8 = R_ == 8;
+    static constexpr int NH = R8 ? 1 : 2;                        // rows a lane has
     static constexpr int ROW = HDP * (int)sizeof(KE);            // bytes of a key in shared memory
     static constexpr int UPR = ROW / 16;
-    static constexpr int KC = CM_STAGE / (2 * ROW);              // keys a chunk: 32, 16, 16, 8
+    static constexpr int KC = CM_STAGE / (2 * ROW);              // keys a chunk
     static constexpr int NT = KC / 8;                            // 8-key tiles a chunk
     static constexpr int NQ = !BF ? 2 : sizeof(QE) == 4 ? 3 : 1; // terms of a query
     static constexpr int NP = !BF ? 2 : sizeof(QE) == 4 ? 3 : 2; // terms of a probability
-    static constexpr int QBYTES = NQ * M * HDP * (BF ? 2 : 4);
+    static constexpr int QT = !BF ? 2 : R8 ? (NQ + 1) / 2 : NQ;  // tiles of 16 rows the queries take; fp32: of M rows
+    static constexpr int QROWS = BF ? 16 : M;
+    static constexpr int QBYTES = QT * QROWS * HDP * (BF ? 2 : 4);
     static constexpr int RING = CM_WARPS * CM_STAGES * CM_STAGE;
     static constexpr int SLOT = M * (HDP + 2);                   // floats of a partial result: maxima, sums, context
 };
@@ -158,10 +170,11 @@ template <bool BLOCKS, int KC> __device__ int cm_find(const CmArgs &a, int64_t x
 // the four from 4 (lane % 4) on, which are its elements of two k-steps; of a P V tile the keys 2 (lane % 4) and the next, and
 // of each 32 dims the four from 4 (lane / 4) on, which are its column of four tiles. Where a dim stands in a k-step and where a
 // column in a tile is free as long as both operands, or all who read the result, agree.
-template <class KE, class QE, int HDP, int MT, bool BLOCKS>
-__global__ void __launch_bounds__(CM_THREADS, 2) k_cache_attention(const __grid_constant__ CmArgs a) {
-    using F = CmCfg<KE, QE, HDP, MT>;
-    constexpr int KC = F::KC, NT = F::NT, NQ = F::NQ, NP = F::NP, ROW = F::ROW, UPR = F::UPR, M = F::M;
+template <class KE, class QE, int HDP, int R, bool BLOCKS>
+__global__ void __launch_bounds__(CM_THREADS, CM_CTAS) k_cache_attention(const __grid_constant__ CmArgs a) {
+    using F = CmCfg<KE, QE, HDP, R>;
+    constexpr int KC = F::KC, NT = F::NT, NQ = F::NQ, NP = F::NP, ROW = F::ROW, UPR = F::UPR, M = F::M, NH = F::NH;
+    constexpr bool R8 = F::R8;
     extern __shared__ __align__(128) char smem[];
     char *ring = smem, *qs = smem + F::RING;
     __shared__ int64_t sh[CM_WARPS];
@@ -259,15 +272,16 @@ __global__ void __launch_bounds__(CM_THREADS, 2) k_cache_attention(const __grid_
             }
             if constexpr (F::BF) {
 #pragma unroll
-                for (int k = 0; k < NQ; k++) {
-                    uint32_t u[4];
+                for (int k = 0; k < (R8 ? 2 * F::QT : NQ); k++) {
+                    uint32_t u[4] = {0, 0, 0, 0};
 #pragma unroll
-                    for (int e = 0; e < 4; e++) {
+                    for (int e = 0; k < NQ && e < 4; e++) {
                         u[e] = cm_pack(x[2 * e], x[2 * e + 1]);
                         const float2 f = cm_unpack(u[e]);
                         x[2 * e] -= f.x; x[2 * e + 1] -= f.y;
                     }
-                    *(uint4 *)(qs + (k * M + m) * ROW + (((d0 / 8) ^ (m & 7)) * 16)) = make_uint4(u[0], u[1], u[2], u[3]);
+                    const int r = k * M + m;                     // 8 rows: terms 0 and 1 are one tile of 16, then 2 and zeros
+                    *(uint4 *)(qs + r * ROW + (((d0 / 8) ^ (r & 7)) * 16)) = make_uint4(u[0], u[1], u[2], u[3]);
                 }
             } else {
 #pragma unroll
@@ -300,14 +314,13 @@ __global__ void __launch_bounds__(CM_THREADS, 2) k_cache_attention(const __grid_
             }
         }
         __syncthreads();
-        float O[MT][HDP / 8][4], mx[MT][2], ls[MT][2];
+        float O[HDP / 8][2 * NH], mx[NH], ls[NH];                // context, maximum and sum of the lane's rows
 #pragma unroll
-        for (int mt = 0; mt < MT; mt++) {
+        for (int j = 0; j < HDP / 8; j++)
 #pragma unroll
-            for (int j = 0; j < HDP / 8; j++) { O[mt][j][0] = O[mt][j][1] = O[mt][j][2] = O[mt][j][3] = 0.f; }
-            mx[mt][0] = mx[mt][1] = -INFINITY;
-            ls[mt][0] = ls[mt][1] = 0.f;
-        }
+            for (int e = 0; e < 2 * NH; e++) O[j][e] = 0.f;
+#pragma unroll
+        for (int hh = 0; hh < NH; hh++) { mx[hh] = -INFINITY; ls[hh] = 0.f; }
         int stage = 0;
         for (int ch = first + warp; ch < stop; ch += CM_WARPS) {
             asm volatile("cp.async.wait_group %0;" ::"n"(CM_STAGES - 2) : "memory");
@@ -321,240 +334,269 @@ __global__ void __launch_bounds__(CM_THREADS, 2) k_cache_attention(const __grid_
             }
             const char *kt = my + stage * CM_STAGE, *vt = kt + CM_STAGE / 2;
             const bool masked = (ch + 1) * KC > len;
+            float S[NT][4];
 #pragma unroll
-            for (int mt = 0; mt < MT; mt++) {
-                if (MT > 1 && m0 + 16 * mt >= a.M) break;
-                float S[NT][4], L[NT][4];
+            for (int j = 0; j < NT; j++) S[j][0] = S[j][1] = S[j][2] = S[j][3] = 0.f;
+            if constexpr (F::BF) {
+                float L[NT][4];                                  // 16 rows: the smaller terms
 #pragma unroll
-                for (int j = 0; j < NT; j++) { S[j][0] = S[j][1] = S[j][2] = S[j][3] = 0.f; L[j][0] = L[j][1] = L[j][2] = L[j][3] = 0.f; }
-                if constexpr (F::BF) {
+                for (int j = 0; j < NT; j++) L[j][0] = L[j][1] = L[j][2] = L[j][3] = 0.f;
 #pragma unroll
-                    for (int kp = 0; kp < HDP / 32; kp++) {              // two k-steps at a time
-                        uint32_t kf[NT][4];
+                for (int kp = 0; kp < HDP / 32; kp++) {          // two k-steps at a time
+                    uint32_t kf[NT][4];
 #pragma unroll
-                        for (int j = 0; j < NT; j++)
-                            cm_ldm4(kf[j], cm_smem(kt) + (8 * j + (lane & 7)) * ROW + (((4 * kp + (lane >> 3)) ^ (lane & 7)) * 16));
+                    for (int j = 0; j < NT; j++)
+                        cm_ldm4(kf[j], cm_smem(kt) + (8 * j + (lane & 7)) * ROW + (((4 * kp + (lane >> 3)) ^ (lane & 7)) * 16));
 #pragma unroll
-                        for (int e = 0; e < 2; e++) {
-                            const int qr = 16 * mt + (lane & 15), qu = 4 * kp + 2 * e + (lane >> 4);
+                    for (int e = 0; e < 2; e++) {
+                        const int qr = lane & 15, qu = 4 * kp + 2 * e + (lane >> 4);
 #pragma unroll
-                            for (int k = NQ - 1; k >= 0; k--) {
-                                uint32_t qf[4];
-                                cm_ldm4(qf, cm_smem(qs) + (k * M + qr) * ROW + ((qu ^ (qr & 7)) * 16));
+                        for (int k = F::QT - 1; k >= 0; k--) {
+                            uint32_t qf[4];
+                            cm_ldm4(qf, cm_smem(qs) + (16 * k + qr) * ROW + ((qu ^ (qr & 7)) * 16));
 #pragma unroll
-                                for (int j = 0; j < NT; j++) cm_mma_bf16(k ? L[j] : S[j], qf, kf[j][2 * e], kf[j][2 * e + 1]);
-                            }
-                        }
-                    }
-                } else {
-#pragma unroll
-                    for (int i = 0; i < HDP / 16; i++) {                 // two k-steps at a time
-                        const int r0 = 16 * mt + g, u0 = (4 * i + c4) ^ ((r0 & 1) << 2);       // r0 and r0 + 8: the same parity
-                        const uint4 h0 = *(const uint4 *)(qs + r0 * ROW + u0 * 16), h1 = *(const uint4 *)(qs + (r0 + 8) * ROW + u0 * 16);
-                        const uint4 l0 = *(const uint4 *)(qs + (M + r0) * ROW + u0 * 16), l1 = *(const uint4 *)(qs + (M + r0 + 8) * ROW + u0 * 16);
-                        const uint32_t ah[2][4] = {{h0.x, h1.x, h0.y, h1.y}, {h0.z, h1.z, h0.w, h1.w}};
-                        const uint32_t al[2][4] = {{l0.x, l1.x, l0.y, l1.y}, {l0.z, l1.z, l0.w, l1.w}};
-#pragma unroll
-                        for (int j = 0; j < NT; j++) {
-                            const float4 kx = *(const float4 *)(kt + (8 * j + g) * ROW + (((4 * i + c4) ^ ((g & 1) << 2)) * 16));
-                            const float kv[4] = {kx.x, kx.y, kx.z, kx.w};
-#pragma unroll
-                            for (int e = 0; e < 2; e++) {
-                                uint32_t bh[2], bl[2];
-                                cm_tf32(kv[2 * e], bh[0], bl[0]);
-                                cm_tf32(kv[2 * e + 1], bh[1], bl[1]);
-                                cm_mma_tf32(L[j], al[e], bh[0], bh[1]);
-                                cm_mma_tf32(L[j], ah[e], bl[0], bl[1]);
-                                cm_mma_tf32(S[j], ah[e], bh[0], bh[1]);
-                            }
+                            for (int j = 0; j < NT; j++) cm_mma_bf16(k && !R8 ? L[j] : S[j], qf, kf[j][2 * e], kf[j][2 * e + 1]);
                         }
                     }
                 }
 #pragma unroll
                 for (int j = 0; j < NT; j++)
 #pragma unroll
-                    for (int e = 0; e < 4; e++) S[j][e] = (S[j][e] + L[j][e]) * a.c2;
-                if (masked) {
+                    for (int e = 0; e < 4; e++) S[j][e] += L[j][e];
+            } else {
+                float L[NT][4];
 #pragma unroll
-                    for (int hh = 0; hh < 2; hh++) {
-                        const int mm = min(m0 + 16 * mt + g + 8 * hh, a.M - 1);
-                        const uint32_t *bits = node_bits[BLOCKS ? 0 : mm / G - m0 / G];
+                for (int j = 0; j < NT; j++) L[j][0] = L[j][1] = L[j][2] = L[j][3] = 0.f;
 #pragma unroll
-                        for (int j = 0; j < NT; j++)
-#pragma unroll
-                            for (int e = 0; e < 2; e++) {
-                                const int pos = ch * KC + 8 * j + 2 * c4 + e;
-                                bool see = pos < len;
-                                if (!BLOCKS && !see && pos < n) see = (bits[(pos - len) >> 5] >> ((pos - len) & 31)) & 1u;
-                                if (!see) S[j][2 * hh + e] = -INFINITY;
-                            }
+                for (int i = 0; i < HDP / 16; i++) {             // two k-steps at a time
+                    const int u0 = (4 * i + c4) ^ ((g & 1) << 2);       // rows g and g + 8: the same parity
+                    uint32_t ah[2][4], al[2][4];
+                    {
+                        const uint4 h0 = *(const uint4 *)(qs + g * ROW + u0 * 16), l0 = *(const uint4 *)(qs + (M + g) * ROW + u0 * 16);
+                        if constexpr (R8) {                      // leading terms in rows 0 ... 7, remainders in 8 ... 15
+                            ah[0][0] = h0.x; ah[0][1] = l0.x; ah[0][2] = h0.y; ah[0][3] = l0.y;
+                            ah[1][0] = h0.z; ah[1][1] = l0.z; ah[1][2] = h0.w; ah[1][3] = l0.w;
+                        } else {
+                            const uint4 h1 = *(const uint4 *)(qs + (g + 8) * ROW + u0 * 16), l1 = *(const uint4 *)(qs + (M + g + 8) * ROW + u0 * 16);
+                            ah[0][0] = h0.x; ah[0][1] = h1.x; ah[0][2] = h0.y; ah[0][3] = h1.y;
+                            ah[1][0] = h0.z; ah[1][1] = h1.z; ah[1][2] = h0.w; ah[1][3] = h1.w;
+                            al[0][0] = l0.x; al[0][1] = l1.x; al[0][2] = l0.y; al[0][3] = l1.y;
+                            al[1][0] = l0.z; al[1][1] = l1.z; al[1][2] = l0.w; al[1][3] = l1.w;
+                        }
                     }
-                }
-                if (!BLOCKS && a.scores) {
-                    float *sp = a.scores + ((int64_t)item * a.c.nkv + kvh) * a.M * a.pitch + ch * KC + 2 * c4;
 #pragma unroll
-                    for (int hh = 0; hh < 2; hh++) {
-                        const int mm = m0 + 16 * mt + g + 8 * hh;
-                        if (mm < a.M) {
+                    for (int j = 0; j < NT; j++) {
+                        const float4 kx = *(const float4 *)(kt + (8 * j + g) * ROW + u0 * 16);
+                        const float kv[4] = {kx.x, kx.y, kx.z, kx.w};
 #pragma unroll
-                            for (int j = 0; j < NT; j++) *(float2 *)(sp + mm * a.pitch + 8 * j) = make_float2(S[j][2 * hh], S[j][2 * hh + 1]);
+                        for (int e = 0; e < 2; e++) {
+                            uint32_t bh[2], bl[2];
+                            cm_tf32(kv[2 * e], bh[0], bl[0]);
+                            cm_tf32(kv[2 * e + 1], bh[1], bl[1]);
+                            if constexpr (!R8) cm_mma_tf32(L[j], al[e], bh[0], bh[1]);
+                            cm_mma_tf32(L[j], ah[e], bl[0], bl[1]);
+                            cm_mma_tf32(S[j], ah[e], bh[0], bh[1]);
                         }
                     }
                 }
-                float al[2];
 #pragma unroll
-                for (int hh = 0; hh < 2; hh++) {
-                    float t = -INFINITY;
+                for (int j = 0; j < NT; j++)
 #pragma unroll
-                    for (int j = 0; j < NT; j++) t = fmaxf(t, fmaxf(S[j][2 * hh], S[j][2 * hh + 1]));
-                    t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 1));
-                    t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 2));
-                    t = fmaxf(t, mx[mt][hh]);
-                    const float base = t == -INFINITY ? 0.f : t;
-                    al[hh] = cm_exp2(mx[mt][hh] - base);
-                    mx[mt][hh] = t;
-                    float sum = 0.f;
+                    for (int e = 0; e < 4; e++) S[j][e] += L[j][e];
+            }
+#pragma unroll
+            for (int j = 0; j < NT; j++)
+#pragma unroll
+                for (int e = 0; e < 2 * NH; e++) S[j][e] = (R8 ? S[j][e] + S[j][2 + e] : S[j][e]) * a.c2;
+            if (masked) {
+#pragma unroll
+                for (int hh = 0; hh < NH; hh++) {
+                    const int mm = min(m0 + g + 8 * hh, a.M - 1);
+                    const uint32_t *bits = node_bits[BLOCKS ? 0 : mm / G - m0 / G];
 #pragma unroll
                     for (int j = 0; j < NT; j++)
 #pragma unroll
-                        for (int e = 0; e < 2; e++) { S[j][2 * hh + e] = cm_exp2(S[j][2 * hh + e] - base); sum += S[j][2 * hh + e]; }
-                    ls[mt][hh] = ls[mt][hh] * al[hh] + sum;
+                        for (int e = 0; e < 2; e++) {
+                            const int pos = ch * KC + 8 * j + 2 * c4 + e;
+                            bool see = pos < len;
+                            if (!BLOCKS && !see && pos < n) see = (bits[(pos - len) >> 5] >> ((pos - len) & 31)) & 1u;
+                            if (!see) S[j][2 * hh + e] = -INFINITY;
+                        }
                 }
-                bool odd = false;                                        // an infinity or NaN among values that not every row sees
-                if (masked && !BLOCKS) {
-                    for (int i = lane; i < KC * HDP; i += 32) {
-                        const float x = (float)((const KE *)vt)[i];
-                        odd |= !(fabsf(x) < INFINITY);
-                    }
-                    odd = __any_sync(0xffffffffu, odd);
-                }
-                if (odd) {
-                    // rows that do not see such a value must not multiply it by zero: one key at a time
+            }
+            if (!BLOCKS && a.scores) {
+                float *sp = a.scores + ((int64_t)item * a.c.nkv + kvh) * a.M * a.pitch + ch * KC + 2 * c4;
 #pragma unroll
-                    for (int j = 0; j < HDP / 8; j++)
+                for (int hh = 0; hh < NH; hh++) {
+                    const int mm = m0 + g + 8 * hh;
+                    if (mm < a.M) {
 #pragma unroll
-                        for (int e = 0; e < 4; e++) O[mt][j][e] *= al[e >> 1];
-#pragma unroll
-                    for (int jj = 0; jj < NT; jj++)
-                        for (int r = 0; r < 8; r++) {
-                            const int src = (lane & ~3) | (r >> 1);
-                            const float p0 = __shfl_sync(0xffffffffu, (r & 1) ? S[jj][1] : S[jj][0], src), p1 = __shfl_sync(0xffffffffu, (r & 1) ? S[jj][3] : S[jj][2], src);
-                            const int kr = 8 * jj + r;
-#pragma unroll
-                            for (int j = 0; j < HDP / 8; j++)
-#pragma unroll
-                                for (int e = 0; e < 2; e++) {
-                                    const int d = F::BF ? 8 * j + 2 * c4 + e : 32 * (j / 4) + 8 * c4 + 4 * e + j % 4;
-                                    const int u = d * (int)sizeof(KE) / 16, us = F::BF ? u ^ (kr & 7) : u ^ (((kr >> 1) & 3) << 1);
-                                    const float x = (float)*(const KE *)(vt + kr * ROW + us * 16 + d * sizeof(KE) % 16);
-                                    if (p0 != 0.f) O[mt][j][e] = fmaf(p0, x, O[mt][j][e]);
-                                    if (p1 != 0.f) O[mt][j][2 + e] = fmaf(p1, x, O[mt][j][2 + e]);
-                                }
-                        }
-                    continue;
-                }
-                if constexpr (F::BF) {
-                    uint32_t pf[NP][KC / 16][4];
-#pragma unroll
-                    for (int k2 = 0; k2 < KC / 16; k2++)
-#pragma unroll
-                        for (int k = 0; k < NP; k++)
-#pragma unroll
-                            for (int e = 0; e < 4; e++) {
-                                float *s = &S[2 * k2 + (e >> 1)][2 * (e & 1)];
-                                pf[k][k2][e] = cm_pack(s[0], s[1]);
-                                const float2 f = cm_unpack(pf[k][k2][e]);
-                                s[0] -= f.x; s[1] -= f.y;
-                            }
-#pragma unroll
-                    for (int jp = 0; jp < HDP / 16; jp++) {              // two tiles of 8 dims at a time
-                        float c0[4] = {0.f, 0.f, 0.f, 0.f}, c1[4] = {0.f, 0.f, 0.f, 0.f}, d0[4] = {0.f, 0.f, 0.f, 0.f}, d1[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                        for (int k2 = 0; k2 < KC / 16; k2++) {
-                            uint32_t vf[4];
-                            const int vr = 16 * k2 + (lane & 15);
-                            cm_ldm4t(vf, cm_smem(vt) + vr * ROW + (((2 * jp + (lane >> 4)) ^ (vr & 7)) * 16));
-#pragma unroll
-                            for (int k = NP - 1; k >= 1; k--) { cm_mma_bf16(d0, pf[k][k2], vf[0], vf[1]); cm_mma_bf16(d1, pf[k][k2], vf[2], vf[3]); }
-                            cm_mma_bf16(c0, pf[0][k2], vf[0], vf[1]);
-                            cm_mma_bf16(c1, pf[0][k2], vf[2], vf[3]);
-                        }
-#pragma unroll
-                        for (int e = 0; e < 4; e++) {
-                            O[mt][2 * jp][e] = fmaf(O[mt][2 * jp][e], al[e >> 1], c0[e] + d0[e]);
-                            O[mt][2 * jp + 1][e] = fmaf(O[mt][2 * jp + 1][e], al[e >> 1], c1[e] + d1[e]);
-                        }
-                    }
-                } else {
-                    uint32_t ph[NT][4], pl[NT][4];
-#pragma unroll
-                    for (int j = 0; j < NT; j++) {                       // k position c: key 2 c, position c + 4: key 2 c + 1
-                        cm_tf32(S[j][0], ph[j][0], pl[j][0]); cm_tf32(S[j][2], ph[j][1], pl[j][1]);
-                        cm_tf32(S[j][1], ph[j][2], pl[j][2]); cm_tf32(S[j][3], ph[j][3], pl[j][3]);
-                    }
-#pragma unroll
-                    for (int jj = 0; jj < HDP / 32; jj++) {              // four tiles of 8 dims at a time
-                        float cc[4][4], dd[4][4];
-#pragma unroll
-                        for (int x = 0; x < 4; x++)
-#pragma unroll
-                            for (int e = 0; e < 4; e++) cc[x][e] = dd[x][e] = 0.f;
-#pragma unroll
-                        for (int j = 0; j < NT; j++) {
-                            const int r0 = 8 * j + 2 * c4, u = (8 * jj + g) ^ (c4 << 1);        // (row >> 1) & 3 = c4 for both rows
-                            const float4 v0 = *(const float4 *)(vt + r0 * ROW + u * 16), v1 = *(const float4 *)(vt + (r0 + 1) * ROW + u * 16);
-                            const float va[4] = {v0.x, v0.y, v0.z, v0.w}, vv[4] = {v1.x, v1.y, v1.z, v1.w};
-#pragma unroll
-                            for (int x = 0; x < 4; x++) {
-                                uint32_t bh[2], bl[2];
-                                cm_tf32(va[x], bh[0], bl[0]);
-                                cm_tf32(vv[x], bh[1], bl[1]);
-                                cm_mma_tf32(dd[x], pl[j], bh[0], bh[1]);
-                                cm_mma_tf32(dd[x], ph[j], bl[0], bl[1]);
-                                cm_mma_tf32(cc[x], ph[j], bh[0], bh[1]);
-                            }
-                        }
-#pragma unroll
-                        for (int x = 0; x < 4; x++)
-#pragma unroll
-                            for (int e = 0; e < 4; e++) O[mt][4 * jj + x][e] = fmaf(O[mt][4 * jj + x][e], al[e >> 1], cc[x][e] + dd[x][e]);
+                        for (int j = 0; j < NT; j++) *(float2 *)(sp + mm * a.pitch + 8 * j) = make_float2(S[j][2 * hh], S[j][2 * hh + 1]);
                     }
                 }
             }
+            float al[NH];
+#pragma unroll
+            for (int hh = 0; hh < NH; hh++) {
+                float t = mx[hh];
+#pragma unroll
+                for (int j = 0; j < NT; j++) t = fmaxf(t, fmaxf(S[j][2 * hh], S[j][2 * hh + 1]));
+                t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 1));
+                t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 2));
+                const float base = t == -INFINITY ? 0.f : t;
+                al[hh] = cm_exp2(mx[hh] - base);
+                mx[hh] = t;
+                float sum = 0.f;
+#pragma unroll
+                for (int j = 0; j < NT; j++)
+#pragma unroll
+                    for (int e = 0; e < 2; e++) { S[j][2 * hh + e] = cm_exp2(S[j][2 * hh + e] - base); sum += S[j][2 * hh + e]; }
+                ls[hh] = ls[hh] * al[hh] + sum;
+            }
             if (++stage == CM_STAGES) stage = 0;
+            bool odd = false;                                    // an infinity or NaN among values that not every row sees
+            if (masked && !BLOCKS) {
+                for (int i = lane; i < KC * HDP; i += 32) {
+                    const float x = (float)((const KE *)vt)[i];
+                    odd |= !(fabsf(x) < INFINITY);
+                }
+                odd = __any_sync(0xffffffffu, odd);
+            }
+            if (odd) {
+                // rows that do not see such a value must not multiply it by zero: one key at a time
+#pragma unroll
+                for (int j = 0; j < HDP / 8; j++)
+#pragma unroll
+                    for (int e = 0; e < 2 * NH; e++) O[j][e] *= al[e >> 1];
+#pragma unroll
+                for (int jj = 0; jj < NT; jj++)
+                    for (int r = 0; r < 8; r++) {
+                        const int src = (lane & ~3) | (r >> 1), kr = 8 * jj + r;
+                        float p[NH];
+#pragma unroll
+                        for (int hh = 0; hh < NH; hh++) p[hh] = __shfl_sync(0xffffffffu, (r & 1) ? S[jj][2 * hh + 1] : S[jj][2 * hh], src);
+#pragma unroll
+                        for (int j = 0; j < HDP / 8; j++)
+#pragma unroll
+                            for (int e = 0; e < 2; e++) {
+                                const int d = F::BF ? 8 * j + 2 * c4 + e : 32 * (j / 4) + 8 * c4 + 4 * e + j % 4;
+                                const int u = d * (int)sizeof(KE) / 16, us = F::BF ? u ^ (kr & 7) : u ^ (((kr >> 1) & 3) << 1);
+                                const float x = (float)*(const KE *)(vt + kr * ROW + us * 16 + d * sizeof(KE) % 16);
+#pragma unroll
+                                for (int hh = 0; hh < NH; hh++) if (p[hh] != 0.f) O[j][2 * hh + e] = fmaf(p[hh], x, O[j][2 * hh + e]);
+                            }
+                    }
+                continue;
+            }
+            auto add = [&](int j, const float (&c)[4]) {         // a chunk's part of tile j
+#pragma unroll
+                for (int e = 0; e < 2 * NH; e++) O[j][e] = fmaf(O[j][e], al[e >> 1], R8 ? c[e] + c[(2 + e) & 3] : c[e]);
+            };
+            if constexpr (F::BF) {
+                constexpr int PT = R8 ? (NP + 1) / 2 : NP;       // tiles the probabilities take
+                uint32_t pf[KC / 16][PT][4];
+#pragma unroll
+                for (int k2 = 0; k2 < KC / 16; k2++)
+#pragma unroll
+                    for (int e = 0; e < 2 * NH; e++) {           // 16 rows: e & 1 is the row, e >> 1 the half of the keys; 8: e the half
+                        float *s = R8 ? &S[2 * k2 + e][0] : &S[2 * k2 + (e >> 1)][2 * (e & 1)];
+#pragma unroll
+                        for (int k = 0; k < (R8 ? 2 * PT : NP); k++) {
+                            uint32_t u = 0;
+                            if (k < NP) {
+                                u = cm_pack(s[0], s[1]);
+                                const float2 f = cm_unpack(u);
+                                s[0] -= f.x; s[1] -= f.y;
+                            }
+                            if (R8) pf[k2][k / 2][2 * e + (k & 1)] = u; else pf[k2][k][e] = u;
+                        }
+                    }
+#pragma unroll
+                for (int jp = 0; jp < HDP / 16; jp++) {          // two tiles of 8 dims at a time
+                    float c0[4] = {0.f, 0.f, 0.f, 0.f}, c1[4] = {0.f, 0.f, 0.f, 0.f};
+                    uint32_t vf[KC / 16][4];
+#pragma unroll
+                    for (int k2 = 0; k2 < KC / 16; k2++) {
+                        const int vr = 16 * k2 + (lane & 15);
+                        cm_ldm4t(vf[k2], cm_smem(vt) + vr * ROW + (((2 * jp + (lane >> 4)) ^ (vr & 7)) * 16));
+                    }
+#pragma unroll
+                    for (int k = PT - 1; k >= 0; k--)            // small terms first
+#pragma unroll
+                        for (int k2 = 0; k2 < KC / 16; k2++) {
+                            cm_mma_bf16(c0, pf[k2][k], vf[k2][0], vf[k2][1]);
+                            cm_mma_bf16(c1, pf[k2][k], vf[k2][2], vf[k2][3]);
+                        }
+                    add(2 * jp, c0);
+                    add(2 * jp + 1, c1);
+                }
+            } else {
+                uint32_t ph[NT][4], pl[NT][4];
+#pragma unroll
+                for (int j = 0; j < NT; j++) {                   // k position c: key 2 c, position c + 4: key 2 c + 1
+                    if constexpr (R8) {
+                        cm_tf32(S[j][0], ph[j][0], ph[j][1]);
+                        cm_tf32(S[j][1], ph[j][2], ph[j][3]);
+                    } else {
+                        cm_tf32(S[j][0], ph[j][0], pl[j][0]); cm_tf32(S[j][2], ph[j][1], pl[j][1]);
+                        cm_tf32(S[j][1], ph[j][2], pl[j][2]); cm_tf32(S[j][3], ph[j][3], pl[j][3]);
+                    }
+                }
+#pragma unroll
+                for (int jj = 0; jj < HDP / 32; jj++) {          // four tiles of 8 dims at a time
+                    float cc[4][4];
+#pragma unroll
+                    for (int x = 0; x < 4; x++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) cc[x][e] = 0.f;
+#pragma unroll
+                    for (int j = 0; j < NT; j++) {
+                        const int r0 = 8 * j + 2 * c4, u = (8 * jj + g) ^ (c4 << 1);        // (row >> 1) & 3 = c4 for both rows
+                        const float4 v0 = *(const float4 *)(vt + r0 * ROW + u * 16), v1 = *(const float4 *)(vt + (r0 + 1) * ROW + u * 16);
+                        const float va[4] = {v0.x, v0.y, v0.z, v0.w}, vv[4] = {v1.x, v1.y, v1.z, v1.w};
+#pragma unroll
+                        for (int x = 0; x < 4; x++) {
+                            uint32_t bh[2], bl[2];
+                            cm_tf32(va[x], bh[0], bl[0]);
+                            cm_tf32(vv[x], bh[1], bl[1]);
+                            if constexpr (!R8) cm_mma_tf32(cc[x], pl[j], bh[0], bh[1]);
+                            cm_mma_tf32(cc[x], ph[j], bl[0], bl[1]);
+                            cm_mma_tf32(cc[x], ph[j], bh[0], bh[1]);
+                        }
+                    }
+#pragma unroll
+                    for (int x = 0; x < 4; x++) add(4 * jj + x, cc[x]);
+                }
+            }
         }
         asm volatile("cp.async.wait_group 0;" ::: "memory");
         // the warps' results meet in shared memory: every warp's maxima first, then scaled contexts where the ring was
 #pragma unroll
-        for (int mt = 0; mt < MT; mt++)
-#pragma unroll
-            for (int hh = 0; hh < 2; hh++) {
-                float l = ls[mt][hh];
-                l += __shfl_xor_sync(0xffffffffu, l, 1);
-                l += __shfl_xor_sync(0xffffffffu, l, 2);
-                if (c4 == 0) { wm[warp][16 * mt + g + 8 * hh] = mx[mt][hh]; wl[warp][16 * mt + g + 8 * hh] = l; }
-            }
+        for (int hh = 0; hh < NH; hh++) {
+            float l = ls[hh];
+            l += __shfl_xor_sync(0xffffffffu, l, 1);
+            l += __shfl_xor_sync(0xffffffffu, l, 2);
+            if (c4 == 0) { wm[warp][g + 8 * hh] = mx[hh]; wl[warp][g + 8 * hh] = l; }
+        }
         __syncthreads();
         float *ctx_sh = (float *)ring;                           // [warp][M][HDP]
         static_assert(CM_WARPS * M * HDP * 4 <= F::RING, "contexts of the warps fit the ring");
 #pragma unroll
-        for (int mt = 0; mt < MT; mt++)
+        for (int hh = 0; hh < NH; hh++) {
+            const int m = g + 8 * hh;
+            float top = wm[0][m];
 #pragma unroll
-            for (int hh = 0; hh < 2; hh++) {
-                const int m = 16 * mt + g + 8 * hh;
-                float top = wm[0][m];
+            for (int w = 1; w < CM_WARPS; w++) top = fmaxf(top, wm[w][m]);
+            const float f = mx[hh] == -INFINITY ? 0.f : cm_exp2(mx[hh] - top);
+            float *o = ctx_sh + (warp * M + m) * HDP;
 #pragma unroll
-                for (int w = 1; w < CM_WARPS; w++) top = fmaxf(top, wm[w][m]);
-                const float f = mx[mt][hh] == -INFINITY ? 0.f : cm_exp2(mx[mt][hh] - top);
-                float *o = ctx_sh + (warp * M + m) * HDP;
+            for (int j = 0; j < HDP / 8; j++)
 #pragma unroll
-                for (int j = 0; j < HDP / 8; j++)
-#pragma unroll
-                    for (int e = 0; e < 2; e++) {
-                        const int d = F::BF ? 8 * j + 2 * c4 + e : 32 * (j / 4) + 8 * c4 + 4 * e + j % 4;
-                        o[d] = O[mt][j][2 * hh + e] * f;
-                    }
-            }
+                for (int e = 0; e < 2; e++) {
+                    const int d = F::BF ? 8 * j + 2 * c4 + e : 32 * (j / 4) + 8 * c4 + 4 * e + j % 4;
+                    o[d] = O[j][2 * hh + e] * f;
+                }
+        }
         __syncthreads();
         const bool whole = first == 0 && stop == nch;
         float *slot = a.part + ((int64_t)blockIdx.x + unit) * F::SLOT;
@@ -588,24 +630,28 @@ __global__ void __launch_bounds__(CM_THREADS, 2) k_cache_attention(const __grid_
 }
 
 // ---- units that several CTAs share are joined; weights are added up ----
-// CTAs [0, units): one unit each. The others: 512 slots of one (row, kv head) each, from the scores that the kernel above left.
+// CTAs [0, joins): rows of one unit each. A thread has four dims of a row; of the CTA's groups of HDP / 4 threads either each
+// has a row, or (`split`: few units, each in many parts) all have the same row and every one a share of its parts.
+// The others: 512 slots of one (row, kv head) each, from the scores that the kernel above left.
 constexpr int CM_WKEYS = 512;
-template <class KE, class QE, int HDP, int MT, bool BLOCKS>
-__global__ void __launch_bounds__(CM_THREADS) k_cache_join(const __grid_constant__ CmArgs a, int ctas, int units) {
-    using F = CmCfg<KE, QE, HDP, MT>;
-    constexpr int M = F::M, KC = F::KC;
+template <class KE, class QE, int HDP, int R, bool BLOCKS>
+__global__ void __launch_bounds__(CM_THREADS) k_cache_join(const __grid_constant__ CmArgs a, int ctas, int joins, int split) {
+    using F = CmCfg<KE, QE, HDP, R>;
+    constexpr int M = F::M, KC = F::KC, D4 = HDP / 4, GROUPS = CM_THREADS / D4;
     __shared__ int64_t sh[CM_WARPS];
     __shared__ float lse[NCMB_MAX_NODES];
+    __shared__ float gm[GROUPS], gl[GROUPS];
+    __shared__ float4 go[GROUPS][D4];
     const int tid = threadIdx.x, G = a.G, hd = a.c.hd;
     pdl_launch_dependents();
     pdl_wait();
     const CmPlan plan = cm_plan<BLOCKS, KC>(a, ctas, sh);
-    const bool join = (int)blockIdx.x < units;
-    const int per_item = a.c.nkv * a.tiles;
+    const bool join = (int)blockIdx.x < joins;
+    const int per_item = a.c.nkv * a.tiles, rows = split ? 1 : GROUPS, steps = M / rows;      // rows a CTA, CTAs a unit
     int item, sub, key0 = 0;
-    if (join) { item = blockIdx.x / per_item; sub = blockIdx.x % per_item; }
+    if (join) { item = blockIdx.x / steps / per_item; sub = blockIdx.x / steps % per_item; }
     else {
-        const int span = (int)((a.pitch + CM_WKEYS - 1) / CM_WKEYS), x = blockIdx.x - units;
+        const int span = (int)((a.pitch + CM_WKEYS - 1) / CM_WKEYS), x = blockIdx.x - joins;
         key0 = x % span * CM_WKEYS;
         sub = x / span % a.c.nkv * a.tiles;
         item = x / span / a.c.nkv;
@@ -626,25 +672,46 @@ __global__ void __launch_bounds__(CM_THREADS) k_cache_join(const __grid_constant
     if (join) {
         parts(sub, c0, c1);
         if (c0 == c1) return;                                    // written already
-        const float *slot = a.part + (int64_t)(c0 + blockIdx.x) * F::SLOT;
-        const int kvh = sub / a.tiles, m0 = sub % a.tiles * M, nm = min(M, a.M - m0);
-        for (int i = tid; i < nm * (HDP / 4); i += CM_THREADS) {
-            const int m = i / (HDP / 4), d = i % (HDP / 4) * 4, mm = m0 + m;
-            if (d >= hd) continue;
-            float top = -INFINITY, l = 0.f;
-            float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-            for (int c = 0; c <= c1 - c0; c++) top = fmaxf(top, slot[c * F::SLOT + m]);
-            for (int c = 0; c <= c1 - c0; c++) {
-                const float x = slot[c * F::SLOT + m], f = x == -INFINITY ? 0.f : cm_exp2(x - top);
-                const float4 p = *(const float4 *)(slot + c * F::SLOT + 2 * M + m * HDP + d);
-                l = fmaf(slot[c * F::SLOT + M + m], f, l);
+        const float *slot = a.part + ((int64_t)c0 + (int64_t)item * per_item + sub) * F::SLOT;
+        const int grp = tid / D4, d = tid % D4 * 4, kvh = sub / a.tiles;
+        const int m = (int)(blockIdx.x % steps) * rows + (split ? 0 : grp), mm = sub % a.tiles * M + m;
+        if (split && mm >= a.M) return;
+        float top = -INFINITY, l = 0.f;
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (mm < a.M) {
+#pragma unroll 4
+            for (int c = split ? grp : 0; c <= c1 - c0; c += split ? GROUPS : 1) {
+                const float *s = slot + (int64_t)c * F::SLOT;
+                const float x = s[m], xl = s[M + m];
+                const float4 p = *(const float4 *)(s + 2 * M + m * HDP + d);
+                const float t = fmaxf(top, x), base = t == -INFINITY ? 0.f : t, fo = cm_exp2(top - base), fp = cm_exp2(x - base);
+                top = t;
+                l = l * fo + xl * fp;
+                o.x = o.x * fo + p.x * fp; o.y = o.y * fo + p.y * fp; o.z = o.z * fo + p.z * fp; o.w = o.w * fo + p.w * fp;
+            }
+        }
+        if (split) {
+            if (d == 0) { gm[grp] = top; gl[grp] = l; }
+            go[grp][d / 4] = o;
+            __syncthreads();
+            if (grp > 0) return;
+            for (int q = 0; q < GROUPS; q++) top = fmaxf(top, gm[q]);
+            const float base = top == -INFINITY ? 0.f : top;
+            l = 0.f;
+            o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int q = 0; q < GROUPS; q++) {
+                const float f = cm_exp2(gm[q] - base);
+                const float4 p = go[q][d / 4];
+                l = fmaf(gl[q], f, l);
                 o.x = fmaf(p.x, f, o.x); o.y = fmaf(p.y, f, o.y); o.z = fmaf(p.z, f, o.z); o.w = fmaf(p.w, f, o.w);
             }
-            const int t = BLOCKS ? item % a.T : mm / G, h = kvh * G + mm % G;
-            const float r = l > 0.f && (BLOCKS || cm_used(par, t)) ? 1.f / l : 0.f;
-            QE *out = (QE *)(a.out + ((int64_t)row * a.T + t) * a.ldo) + (int64_t)h * hd + d;
-            cm_put(out, o.x * r); cm_put(out + 1, o.y * r); cm_put(out + 2, o.z * r); cm_put(out + 3, o.w * r);
         }
+        if (mm >= a.M || d >= hd) return;
+        const int t = BLOCKS ? item % a.T : mm / G, h = kvh * G + mm % G;
+        const float r = l > 0.f && (BLOCKS || cm_used(par, t)) ? 1.f / l : 0.f;
+        QE *out = (QE *)(a.out + ((int64_t)row * a.T + t) * a.ldo) + (int64_t)h * hd + d;
+        cm_put(out, o.x * r); cm_put(out + 1, o.y * r); cm_put(out + 2, o.z * r); cm_put(out + 3, o.w * r);
         return;
     }
     const int kvh = sub / a.tiles, len = n - a.T;
@@ -685,14 +752,14 @@ __global__ void __launch_bounds__(CM_THREADS) k_cache_join(const __grid_constant
 }
 
 // ---- launches ----
-template <class KE, class QE, int HDP, int MT, bool BLOCKS>
+template <class KE, class QE, int HDP, int R, bool BLOCKS>
 int cm_run_as(const char *who, CmArgs a, int max_keys) {
-    using F = CmCfg<KE, QE, HDP, MT>;
+    using F = CmCfg<KE, QE, HDP, R>;
     a.tiles = (int)cdiv(a.M, F::M);
     const int smem = F::RING + F::QBYTES;
     static bool set = false;
     if (!set) {
-        CUDA_CHECK(cudaFuncSetAttribute(k_cache_attention<KE, QE, HDP, MT, BLOCKS>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+        CUDA_CHECK(cudaFuncSetAttribute(k_cache_attention<KE, QE, HDP, R, BLOCKS>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
         set = true;
     }
     // rows of a launch: as many as leave the scores some GB at most
@@ -705,34 +772,29 @@ int cm_run_as(const char *who, CmArgs a, int max_keys) {
     }
     const int64_t units = (int64_t)step * per_row * a.c.nkv * a.tiles;
     const int64_t spans = a.weights ? cdiv(a.pitch, CM_WKEYS) * step * a.c.nkv : 0;
-    if (units + spans > 0x7fffffff) return cache_refuse(who, "%lld query tiles", (long long)units);
+    if (units * F::M + spans > 0x7fffffff) return cache_refuse(who, "%lld query tiles", (long long)units);
     const int64_t est = units * cdiv(max_keys, F::KC);
-    const int ctas = (int)std::max<int64_t>(1, std::min<int64_t>(2 * ctx().sm_count, cdiv(est, CM_WARPS)));
+    const int ctas = (int)std::max<int64_t>(1, std::min<int64_t>(CM_CTAS * ctx().sm_count, cdiv(est, CM_WARPS)));
     const size_t part = (size_t)(units + ctas) * F::SLOT * 4, sc = a.weights ? (size_t)step * a.c.nkv * a.M * a.pitch * 4 : 0;
     char *scratch = (char *)cache_scratch(who, part + sc);
     if (!scratch) return -1;
     a.scores = a.weights ? (float *)scratch : nullptr;
     a.part = (float *)(scratch + sc);
+    const int split = ctas > 4 * units;                          // many parts a unit
     for (int r = 0; r < rows; r += step) {
         const int nr = std::min(step, rows - r);
         a.row0 = r;
         a.items = nr * per_row;
-        const int u = a.items * a.c.nkv * a.tiles;
-        LAUNCH_PDL((k_cache_attention<KE, QE, HDP, MT, BLOCKS>), ctas, CM_THREADS, smem, a);
-        LAUNCH_PDL((k_cache_join<KE, QE, HDP, MT, BLOCKS>), (unsigned)(u + spans / step * nr), CM_THREADS, 0, a, ctas, u);
+        const int64_t u = (int64_t)a.items * a.c.nkv * a.tiles, joins = u * (F::M / (split ? 1 : CM_THREADS / (HDP / 4)));
+        LAUNCH_PDL((k_cache_attention<KE, QE, HDP, R, BLOCKS>), ctas, CM_THREADS, smem, a);
+        LAUNCH_PDL((k_cache_join<KE, QE, HDP, R, BLOCKS>), (unsigned)(joins + spans / step * nr), CM_THREADS, 0, a, ctas, (int)joins, split);
     }
     return 0;
 }
-// tiles of 16, 32 or (head dim 64) 64 query rows
 template <class KE, class QE, bool BLOCKS>
 int cm_run(const char *who, const CmArgs &a, int max_keys) {
-    if (a.c.hd <= 64) {
-        if (a.M <= 16) return cm_run_as<KE, QE, 64, 1, BLOCKS>(who, a, max_keys);
-        if (a.M <= 32) return cm_run_as<KE, QE, 64, 2, BLOCKS>(who, a, max_keys);
-        return cm_run_as<KE, QE, 64, 4, BLOCKS>(who, a, max_keys);
-    }
-    if (a.M <= 16) return cm_run_as<KE, QE, 128, 1, BLOCKS>(who, a, max_keys);
-    return cm_run_as<KE, QE, 128, 2, BLOCKS>(who, a, max_keys);
+    if (a.c.hd <= 64) return a.M <= 8 ? cm_run_as<KE, QE, 64, 8, BLOCKS>(who, a, max_keys) : cm_run_as<KE, QE, 64, 16, BLOCKS>(who, a, max_keys);
+    return a.M <= 8 ? cm_run_as<KE, QE, 128, 8, BLOCKS>(who, a, max_keys) : cm_run_as<KE, QE, 128, 16, BLOCKS>(who, a, max_keys);
 }
 
 } // namespace ncmb

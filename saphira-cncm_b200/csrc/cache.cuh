@@ -44,6 +44,22 @@ __device__ __forceinline__ int cache_len(const CacheDev &c, int row, int n_new) 
     return max(0, min(c.len[row], c.cap - n_new));
 }
 
+// a launch in clusters of nc CTAs along x, started under its predecessor
+template <typename... KArgs, typename... Args>
+void cache_launch(void (*kernel)(KArgs...), dim3 grid, int threads, size_t smem, int nc, Args... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid; cfg.blockDim = dim3(threads); cfg.dynamicSmemBytes = smem; cfg.stream = stream();
+    cudaLaunchAttribute at[2];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim.x = nc; at[1].val.clusterDim.y = 1; at[1].val.clusterDim.z = 1;
+    cfg.attrs = at; cfg.numAttrs = nc > 1 ? 2 : 1;
+    cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, KArgs(args)...);
+    if (e != cudaSuccess) fatal("cache operators: launch failed: %s", cudaGetErrorString(e));
+    ctx().launches++;
+}
+
 // ---- the k-th largest of many 32-bit keys, by a cluster of CTAs that each hold a part of them ----
 constexpr int SEL_BINS = 2048;
 struct SelShared {

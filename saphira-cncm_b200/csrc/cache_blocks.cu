@@ -7,46 +7,101 @@ namespace {
 
 template <class E> __device__ __forceinline__ float get(const char *p, int d) { return (float)((const E *)p)[d]; }
 
-// one warp per (row, kv head, block); a lane has the dims lane, lane + 32, ...
-template <class KE>
-__global__ void __launch_bounds__(128) k_block_summaries(CacheDev c, int n_new, const int *first, int block, int nb, signed char *codes, float *scales) {
-    const int lane = threadIdx.x & 31, i = blockIdx.x * 4 + (threadIdx.x >> 5), kvh = blockIdx.y, b = blockIdx.z;
-    const int n = cache_len(c, b, n_new) + n_new, f = first ? first[b] : 0;
-    if (i >= nb || i * (int64_t)block >= n || (i + 1) * (int64_t)block <= f) return;
-    const int s0 = i * block, cnt = min(block, n - s0);
-    const char *k = c.k + b * c.rs + kvh * c.hs + s0 * c.ts;
-    float mean[4], top = 0.f;
+// ---- mean keys ----
+// One warp a block. A lane has 16 bytes of the dims of every R-th slot (R: rows of slots that the warp's lanes cover), CNT
+// slots in all; sums by halves of the block are sums by halves of a lane's own slots first, then of the lanes' rows.
+// Bound by reading the keys: 8 loads of 16 bytes a lane are in flight, with no more registers than let the SM hold half its
+// warps.
+template <class KE> struct BsVec { static constexpr int N = 16 / sizeof(KE); };
+template <class KE, int CNT>
+__device__ __forceinline__ void bs_sum(float (&r)[16 / sizeof(KE)], const char *p, int64_t ts, int i, int step, int cnt) {
+    constexpr int VE = BsVec<KE>::N;
+    if constexpr (CNT <= 8) {
+        uint4 raw[CNT];
 #pragma unroll
-    for (int x = 0; x < 4; x++) {
-        const int d = lane + 32 * x;
-        mean[x] = 0.f;
-        if (d >= c.hd) continue;
-        // by halves: slot j of what is left plus slot j + half. In the order of a binary counter over bit-reversed slots, so
-        // that one partial sum a level is enough.
-        float part[8];
-        const int bits = 31 - __clz(block);
-        for (int j = 0; j < block; j++) {
-            const int s = (int)(__brev((unsigned)j) >> (32 - bits));
-            float v = s < cnt ? get<KE>(k + s * c.ts, d) : 0.f;
-            int lev = 0;
-            for (int jj = j; jj & 1; jj >>= 1, lev++) v = __fadd_rn(part[lev], v);
-            part[lev] = v;
+        for (int j = 0; j < CNT; j++) raw[j] = i + step * j < cnt ? *(const uint4 *)(p + (i + step * j) * ts) : make_uint4(0, 0, 0, 0);
+        float x[CNT][VE];
+#pragma unroll
+        for (int j = 0; j < CNT; j++) {
+            const uint32_t u[4] = {raw[j].x, raw[j].y, raw[j].z, raw[j].w};
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                if constexpr (VE == 4) x[j][e] = __uint_as_float(u[e]);
+                else { x[j][2 * e] = __uint_as_float(u[e] << 16); x[j][2 * e + 1] = __uint_as_float(u[e] & 0xffff0000u); }
+            }
         }
-        mean[x] = __fdiv_rn(part[bits], (float)cnt);
-        top = fmaxf(top, fabsf(mean[x]));
-    }
 #pragma unroll
-    for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    const float sc = __fdiv_rn(top, 127.f);
-    const int64_t at = ((int64_t)b * c.nkv + kvh) * nb + i;
+        for (int h = CNT / 2; h > 0; h >>= 1)
 #pragma unroll
-    for (int x = 0; x < 4; x++) {
-        const int d = lane + 32 * x;
-        if (d < c.hd) codes[at * c.hd + d] = sc > 0.f ? (signed char)(int)rintf(__fdiv_rn(mean[x], sc)) : 0;
+            for (int j = 0; j < h; j++)
+#pragma unroll
+                for (int e = 0; e < VE; e++) x[j][e] = __fadd_rn(x[j][e], x[j + h][e]);
+#pragma unroll
+        for (int e = 0; e < VE; e++) r[e] = x[0][e];
+    } else {
+        float b[VE];
+        bs_sum<KE, CNT / 2>(r, p, ts, i, 2 * step, cnt);
+        bs_sum<KE, CNT / 2>(b, p, ts, i + step, 2 * step, cnt);
+#pragma unroll
+        for (int e = 0; e < VE; e++) r[e] = __fadd_rn(r[e], b[e]);
     }
-    if (lane == 0) scales[at] = sc;
 }
 
+template <class KE, int CNT>
+__global__ void __launch_bounds__(256) k_block_summaries(CacheDev c, int n_new, const int *first, int block, int nb, int upr_log, signed char *codes, float *scales) {
+    constexpr int VE = BsVec<KE>::N;
+    const int lane = threadIdx.x & 31, kvh = blockIdx.y, b = blockIdx.z;
+    const int u = lane & ((1 << upr_log) - 1), tr = lane >> upr_log, R = block / CNT;
+    pdl_launch_dependents();
+    pdl_wait();
+    const int n = cache_len(c, b, n_new) + n_new, f = first ? max(0, first[b]) : 0;
+    const bool in = u * VE < c.hd && tr < R;
+    const char *kb = c.k + b * c.rs + kvh * c.hs + u * 16;
+    for (int64_t i = f / block + (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); i * block < n; i += (int64_t)gridDim.x * 8) {
+        const int s0 = (int)i * block, cnt = min(block, n - s0);
+        float m[VE];
+        bs_sum<KE, CNT>(m, kb + s0 * c.ts, c.ts, tr, R, in ? cnt : 0);
+        for (int o = (R >> 1) << upr_log; o >= (1 << upr_log); o >>= 1)
+#pragma unroll
+            for (int e = 0; e < VE; e++) m[e] = __fadd_rn(m[e], __shfl_xor_sync(0xffffffffu, m[e], o));
+        float top = 0.f;
+#pragma unroll
+        for (int e = 0; e < VE; e++) { m[e] = __fdiv_rn(m[e], (float)cnt); top = fmaxf(top, fabsf(m[e])); }
+        if (!in) top = 0.f;
+        for (int o = 1; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        const float sc = __fdiv_rn(top, 127.f);
+        const int64_t at = ((int64_t)b * c.nkv + kvh) * nb + i;
+        if (in && tr == 0) {
+            uint32_t w[VE / 4];
+#pragma unroll
+            for (int x = 0; x < VE / 4; x++) {
+                w[x] = 0;
+#pragma unroll
+                for (int e = 0; e < 4; e++) w[x] |= (sc > 0.f ? (uint32_t)(int)rintf(__fdiv_rn(m[4 * x + e], sc)) & 255u : 0u) << (8 * e);
+            }
+            uint32_t *p = (uint32_t *)(codes + at * c.hd + u * VE);
+#pragma unroll
+            for (int x = 0; x < VE / 4; x++) p[x] = w[x];
+        }
+        if (lane == 0) scales[at] = sc;
+    }
+}
+
+template <class KE>
+void run_summaries(const CacheDev &d, int n_new, const int *first, int block, int nb, int hint, signed char *codes, float *scales) {
+    const int units = d.hd * (int)sizeof(KE) / 16;
+    int ul = 0;
+    while ((1 << ul) < units) ul++;
+    const int rows = 32 >> ul, cnt = block / (rows < block ? rows : block);
+    const dim3 grid((unsigned)std::max<int64_t>(1, cdiv(hint, 8)), d.nkv, d.rows);
+    switch (cnt) {
+#define BS_CASE(N) case N: LAUNCH_PDL((k_block_summaries<KE, N>), grid, 256, 0, d, n_new, first, block, nb, ul, codes, scales); break
+        BS_CASE(1); BS_CASE(2); BS_CASE(4); BS_CASE(8); BS_CASE(16); BS_CASE(32); BS_CASE(64); BS_CASE(128);
+#undef BS_CASE
+    }
+}
+
+// ---- picks ----
 struct BlockArgs {
     CacheDev c;
     const char *q; char *out;
@@ -58,70 +113,123 @@ struct BlockArgs {
     uint32_t *keys;                  // scratch [rows][T][nkv][nb] when they do not fit shared memory, else null
 };
 
-constexpr int BP_THREADS = 256;
-constexpr int BP_KEYS = 16384;       // keys a CTA holds in shared memory
+constexpr int BP_THREADS = 512, BP_WARPS = BP_THREADS / 32, BP_MAXC = 8;
+constexpr int BP_KEYS = 32768;       // keys a CTA holds in shared memory
 
-// picks of one (row, token, kv head)
+__device__ __forceinline__ void mma_s8(int (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// Picks of one (row, token, kv head), by a cluster of CTAs that each score a part of the blocks. Scores are integer products on
+// m16n8k32 tiles -- 16 heads of the group against 8 blocks -- with the dims of a tile's k positions chosen so that a lane's
+// codes are 8 bytes in a row (any order of the dims gives the same whole numbers). Bound by latency: the codes of 128K
+// tokens in blocks of 64 are 128 KB a kv head.
 template <class QE>
 __global__ void __launch_bounds__(BP_THREADS) k_block_pick(BlockArgs a) {
+    namespace cg = cooperative_groups;
     extern __shared__ __align__(16) char dyn[];
     __shared__ SelShared sel;
-    __shared__ int wtie[BP_THREADS / 32], wkeep[BP_THREADS / 32];
-    const int t = blockIdx.x, kvh = blockIdx.y, b = blockIdx.z, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, hd = a.c.hd;
+    __shared__ int wtie[BP_WARPS], wkeep[BP_WARPS], share[2];
+    cg::cluster_group cl = cg::this_cluster();
+    const int rank = (int)cl.block_rank(), nc = (int)cl.num_blocks();
+    const int t = blockIdx.x / nc, kvh = blockIdx.y, b = blockIdx.z, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, hd = a.c.hd;
+    pdl_launch_dependents();
+    pdl_wait();
     const int cur = (cache_len(a.c, b, a.T) + t) / a.block, n = cur + 1, k = min(n, a.n_sel);
     const int64_t u = ((int64_t)b * a.T + t) * a.c.nkv + kvh;
     int *picks = a.picks + u * a.n_sel;
-    for (int i = k + tid; i < a.n_sel; i += BP_THREADS) picks[i] = -1;
+    if (rank == 0) for (int i = k + tid; i < a.n_sel; i += BP_THREADS) picks[i] = -1;
     if (n <= a.n_sel) {
-        for (int i = tid; i < n; i += BP_THREADS) picks[i] = i;
-        return;
+        if (rank == 0) for (int i = tid; i < n; i += BP_THREADS) picks[i] = i;
+        return;                                                              // all CTAs of the cluster
     }
-    float *qs = (float *)dyn;                                                // [G]
-    signed char *q8 = (signed char *)(qs + ((a.G + 3) & ~3));                // [G][hd]
-    uint32_t *keys = a.keys ? a.keys + u * a.nb : (uint32_t *)(q8 + ((a.G * hd + 15) & ~15));
-    for (int g = warp; g < a.G; g += BP_THREADS / 32) {
+    // queries in 8 bits, heads in whole tiles of 16, dims in whole 32
+    const int gt = (a.G + 15) / 16, hp = (hd + 31) & ~31;
+    float *qs = (float *)dyn;                                                // [16 gt]
+    signed char *q8 = (signed char *)(qs + 16 * gt);                         // [16 gt][hp + 8]: rows 8 bytes apart in banks
+    const int qrow = hp + 8;
+    for (int g = warp; g < 16 * gt; g += BP_WARPS) {
         const char *q = a.q + ((int64_t)b * a.T + t) * a.ldq + (int64_t)(kvh * a.G + g) * hd * sizeof(QE);
         float v[4], top = 0.f;
 #pragma unroll
-        for (int x = 0; x < 4; x++) { v[x] = lane + 32 * x < hd ? get<QE>(q, lane + 32 * x) : 0.f; top = fmaxf(top, fabsf(v[x])); }
+        for (int x = 0; x < 4; x++) { v[x] = g < a.G && lane + 32 * x < hd ? get<QE>(q, lane + 32 * x) : 0.f; top = fmaxf(top, fabsf(v[x])); }
 #pragma unroll
         for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
         const float sc = __fdiv_rn(top, 127.f);
         if (lane == 0) qs[g] = sc;
 #pragma unroll
         for (int x = 0; x < 4; x++)
-            if (lane + 32 * x < hd) q8[g * hd + lane + 32 * x] = sc > 0.f ? (signed char)(int)rintf(__fdiv_rn(v[x], sc)) : 0;
+            if (32 * x < hp) q8[g * qrow + lane + 32 * x] = sc > 0.f ? (signed char)(int)rintf(__fdiv_rn(v[x], sc)) : 0;
     }
     __syncthreads();
+    const int per = ((n + nc - 1) / nc + 31) & ~31, lo = min(n, rank * per), hi = min(n, lo + per);
+    uint32_t *keys = a.keys ? a.keys + u * a.nb + lo : (uint32_t *)(q8 + 16 * gt * qrow);
     const signed char *codes = a.codes + ((int64_t)b * a.c.nkv + kvh) * a.nb * hd;
     const float *scales = a.scales + ((int64_t)b * a.c.nkv + kvh) * a.nb;
-    for (int i = tid; i < n; i += BP_THREADS) {
-        uint32_t key = 0xffffffffu;
-        if (i >= a.n_first && i <= cur - a.n_last) {
-            int2 c[16];                                                      // up to 128 codes
+    const int g4 = lane >> 2, c4 = lane & 3;
+    constexpr int UN = 4;                                                    // tiles of 8 blocks a warp has in flight
+    for (int i0 = lo + warp * 8 * UN; i0 < hi; i0 += BP_WARPS * 8 * UN) {
+        int2 cd[UN][4];
 #pragma unroll
-            for (int x = 0; x < 16; x++) if (x * 8 < hd) c[x] = *(const int2 *)(codes + (int64_t)i * hd + x * 8);
-            float best = -INFINITY;
-            for (int g = 0; g < a.G; g++) {
-                int dot = 0;
+        for (int x = 0; x < UN; x++) {
+            const int i = i0 + 8 * x + g4;
 #pragma unroll
-                for (int x = 0; x < 16; x++)
-                    if (x * 8 < hd) {
-                        const int2 q = *(const int2 *)(q8 + g * hd + x * 8);
-                        dot = __dp4a(c[x].x, q.x, dot);
-                        dot = __dp4a(c[x].y, q.y, dot);
-                    }
-                const float s = __fmul_rn((float)dot, qs[g]);
-                best = s > best || !(s == s) ? s : best;
+            for (int s = 0; s < 4; s++) {
+                cd[x][s] = make_int2(0, 0);
+                if (32 * s + 8 * c4 < hd && i < hi) cd[x][s] = *(const int2 *)(codes + (int64_t)i * hd + 32 * s + 8 * c4);
             }
-            key = float_key(__fmul_rn(best, scales[i]));
         }
-        keys[i] = key;
+        float best[UN][2];
+#pragma unroll
+        for (int x = 0; x < UN; x++) best[x][0] = best[x][1] = -INFINITY;
+        for (int tt = 0; tt < gt; tt++) {
+            int dot[UN][4];
+#pragma unroll
+            for (int x = 0; x < UN; x++) dot[x][0] = dot[x][1] = dot[x][2] = dot[x][3] = 0;
+#pragma unroll
+            for (int s = 0; s < 4; s++) {
+                if (32 * s >= hd) continue;
+                const signed char *q = q8 + (16 * tt + g4) * qrow + 32 * s + 8 * c4;
+                const uint2 q0 = *(const uint2 *)q, q1 = *(const uint2 *)(q + 8 * qrow);
+                const uint32_t qa[4] = {q0.x, q1.x, q0.y, q1.y};
+#pragma unroll
+                for (int x = 0; x < UN; x++) mma_s8(dot[x], qa, (uint32_t)cd[x][s].x, (uint32_t)cd[x][s].y);
+            }
+#pragma unroll
+            for (int hh = 0; hh < 2; hh++) {
+                const int g = 16 * tt + g4 + 8 * hh;
+                const float sc = qs[g];
+#pragma unroll
+                for (int x = 0; x < UN; x++)
+#pragma unroll
+                    for (int e = 0; e < 2; e++) {
+                        const float v = __fmul_rn((float)dot[x][2 * hh + e], sc);
+                        if (g < a.G && (v > best[x][e] || !(v == v))) best[x][e] = v;
+                    }
+            }
+        }
+#pragma unroll
+        for (int x = 0; x < UN; x++)
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                float v = best[x][e];
+#pragma unroll
+                for (int o = 4; o < 32; o <<= 1) {
+                    const float w = __shfl_xor_sync(0xffffffffu, v, o);
+                    v = w > v || !(w == w) ? w : v;
+                }
+                const int i = i0 + 8 * x + 2 * c4 + e;
+                if (g4 == 0 && i < hi) {
+                    const bool always = i < a.n_first || i > cur - a.n_last;
+                    keys[i - lo] = always ? 0xffffffffu : float_key(__fmul_rn(v, scales[i]));
+                }
+            }
     }
     __syncthreads();
     uint32_t ties;
-    const uint32_t bound = select_kth<BP_THREADS>(sel, n, (uint32_t)k, ties, [&](int i) { return keys[i]; });
-    const int per = ((n + BP_THREADS - 1) / BP_THREADS) * 32, w0 = min(n, warp * per), w1 = min(n, w0 + per);
+    const uint32_t bound = select_kth<BP_THREADS>(sel, hi - lo, (uint32_t)k, ties, [&](int i) { return keys[i]; });
+    const int part = ((hi - lo + BP_THREADS - 1) / BP_THREADS) * 32, w0 = min(hi - lo, warp * part), w1 = min(hi - lo, w0 + part);
     int nt = 0, above = 0;
     for (int s = w0; s < w1; s += 32) {
         const uint32_t x = s + lane < w1 ? keys[s + lane] : 0;
@@ -130,7 +238,10 @@ __global__ void __launch_bounds__(BP_THREADS) k_block_pick(BlockArgs a) {
     }
     if (lane == 0) { wtie[warp] = nt; wkeep[warp] = above; }
     __syncthreads();
+    if (tid == 0) { int x = 0, y = 0; for (int i = 0; i < BP_WARPS; i++) { x += wtie[i]; y += wkeep[i]; } share[0] = x; share[1] = y; }
+    if (nc > 1) cl.sync();
     int tb = 0, at = 0;                          // ties before this warp; picks before it
+    for (int r = 0; r < rank; r++) { tb += *cl.map_shared_rank(&share[0], r); at += *cl.map_shared_rank(&share[1], r); }
     for (int i = 0; i < warp; i++) { at += wkeep[i]; tb += wtie[i]; }
     at += min(tb, (int)ties);
     for (int s = w0; s < w1; s += 32) {
@@ -139,10 +250,17 @@ __global__ void __launch_bounds__(BP_THREADS) k_block_pick(BlockArgs a) {
         const uint32_t tm = __ballot_sync(0xffffffffu, in && x == bound);
         const bool keep = in && (x > bound || (x == bound && tb + __popc(tm & lt) < (int)ties));
         const uint32_t km = __ballot_sync(0xffffffffu, keep);
-        if (keep) picks[at + __popc(km & lt)] = s + lane;
+        if (keep) picks[at + __popc(km & lt)] = lo + s + lane;
         at += __popc(km);
         tb += __popc(tm);
     }
+    if (nc > 1) cl.sync();                       // the others have read this CTA's counts
+}
+
+template <class QE>
+void run_pick(const BlockArgs &a, int nc, size_t smem) {
+    CUDA_CHECK(cudaFuncSetAttribute(k_block_pick<QE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    cache_launch(k_block_pick<QE>, dim3(a.T * nc, a.c.nkv, a.c.rows), BP_THREADS, smem, nc, a);
 }
 
 } // namespace
@@ -160,10 +278,10 @@ extern "C" int ncmb_block_summaries(const NcmbCache *c, int n_new, const int *fi
     if (c->rows == 0) return 0;
     ensure_device();
     const int nb = (int)cdiv(c->capacity, block);
-    const dim3 grid((unsigned)cdiv(nb, 4), c->n_kv, c->rows);
-    if (c->type == NCMB_F32) LAUNCH(k_block_summaries<float>, grid, 128, 0, d, n_new, first, block, nb, codes, scales);
-    else LAUNCH(k_block_summaries<__nv_bfloat16>, grid, 128, 0, d, n_new, first, block, nb, codes, scales);
-    (void)max_len;
+    if (max_len <= 0 || max_len > c->capacity - n_new) max_len = c->capacity - n_new;
+    const int hint = (int)cdiv((int64_t)max_len + n_new, block);
+    if (c->type == NCMB_F32) run_summaries<float>(d, n_new, first, block, nb, hint, codes, scales);
+    else run_summaries<__nv_bfloat16>(d, n_new, first, block, nb, hint, codes, scales);
     return 0;
 }
 
@@ -190,25 +308,24 @@ extern "C" int ncmb_block_attention(const NcmbCache *c, const void *q, int64_t l
     a.n_sel = n_sel; a.n_first = n_first; a.n_last = n_last; a.codes = codes; a.scales = scales;
     a.scale = scale == 0.f ? 1.0f / sqrtf((float)c->hd) : scale;
     const int64_t units = (int64_t)c->rows * T * c->n_kv;
-    const size_t need_picks = picks ? 0 : (size_t)units * n_sel * 4, need_keys = a.nb > BP_KEYS ? (size_t)units * a.nb * 4 : 0;
+    if (max_len <= 0 || max_len > c->capacity - T) max_len = c->capacity - T;
+    // CTAs a (row, token, head): as many as keep the GPU busy, with 256 blocks each at least
+    int nc = 1;
+    while (nc < BP_MAXC && units * nc * 2 <= ctx().sm_count && cdiv(cdiv(max_len, block), nc) > 256) nc *= 2;
+    const int64_t per = (cdiv(a.nb, nc) + 31) & ~31;
+    const size_t need_picks = picks ? 0 : (size_t)units * n_sel * 4, need_keys = per > BP_KEYS ? (size_t)units * a.nb * 4 : 0;
     char *scratch = need_picks + need_keys ? (char *)cache_scratch(who, need_picks + need_keys, SCRATCH_PICKS) : nullptr;
     if (need_picks + need_keys && !scratch) return -1;
     a.picks = picks ? picks : (int *)(scratch + need_keys);
     a.keys = need_keys ? (uint32_t *)scratch : nullptr;
-    const size_t smem = (size_t)((a.G + 3) & ~3) * 4 + (((size_t)a.G * c->hd + 15) & ~(size_t)15) + (need_keys ? 0 : (size_t)a.nb * 4);
-    if (smem > 150000) return cache_refuse(who, "%d query heads a kv head", a.G);
-    const dim3 gp(T, c->n_kv, c->rows);
-    if (act_type == NCMB_F32) {
-        CUDA_CHECK(cudaFuncSetAttribute(k_block_pick<float>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-        LAUNCH(k_block_pick<float>, gp, BP_THREADS, smem, a);
-    } else {
-        CUDA_CHECK(cudaFuncSetAttribute(k_block_pick<__nv_bfloat16>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-        LAUNCH(k_block_pick<__nv_bfloat16>, gp, BP_THREADS, smem, a);
-    }
+    const int gt = (a.G + 15) / 16;
+    const size_t smem = (size_t)gt * 16 * (4 + ((c->hd + 31) & ~31) + 8) + (need_keys ? 0 : (size_t)per * 4);
+    if (smem > 190000) return cache_refuse(who, "%d query heads a kv head", a.G);
+    if (act_type == NCMB_F32) run_pick<float>(a, nc, smem);
+    else run_pick<__nv_bfloat16>(a, nc, smem);
     CmArgs m = {};
     m.c = a.c; m.q = a.q; m.out = a.out; m.ldq = a.ldq; m.ldo = a.ldo; m.H = a.H; m.G = a.G; m.T = T; m.M = a.G;
     m.c2 = a.scale * 1.44269504f; m.block_log = block == 16 ? 4 : block == 32 ? 5 : block == 64 ? 6 : 7; m.n_sel = n_sel; m.picks = a.picks;
-    if (max_len <= 0 || max_len > c->capacity - T) max_len = c->capacity - T;
     const int keys = (int)std::min<int64_t>(max_len + T, (int64_t)n_sel * block);
     if (c->type == NCMB_F32) return cm_run<float, float, true>(who, m, keys);
     if (act_type == NCMB_F32) return cm_run<__nv_bfloat16, float, true>(who, m, keys);

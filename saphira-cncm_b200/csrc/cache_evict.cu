@@ -25,7 +25,9 @@ struct EvictArgs {
     const int *known, *seen;
     int *len2;
     int *from, *to;                  // scratch, [rows][nkv][min(budget, capacity)] each
+    int *pairs;                      // scratch, [rows][nkv]: how many of them
     int room;
+    int move_here;                   // few tokens move: the kernel that picks moves them too
 };
 
 __global__ void __launch_bounds__(EV_THREADS) k_cache_evict(EvictArgs a) {
@@ -37,27 +39,34 @@ __global__ void __launch_bounds__(EV_THREADS) k_cache_evict(EvictArgs a) {
     const int rank = (int)cl.block_rank(), nc = (int)cl.num_blocks();
     const int kvh = blockIdx.y, b = blockIdx.z, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     uint32_t *keys = dyn, *kept = dyn + a.kcap;          // keys, then one bit a slot
+    pdl_launch_dependents();
+    pdl_wait();
     const int n = cache_len(a.c, b, 0), n2 = min(n, a.budget);
     const int64_t u = (int64_t)b * a.c.nkv + kvh;
     const int seen = a.seen[b], known = a.known ? max(0, min(a.known[b], n)) : 0;
     const float *w = a.w + u * a.c.cap;
     const int *pos = a.pos + u * a.c.cap;
     if (rank == 0 && kvh == 0 && tid == 0) a.len2[b] = n2;
-    if (n == 0) return;
+    if (n == 0) {
+        if (rank == 0 && tid == 0) a.pairs[u] = 0;
+        return;
+    }
     // slots [lo, hi) are this CTA's; a warp's part of them is a whole number of 32
     const int per_warp = ((n + nc * EV_WARPS - 1) / (nc * EV_WARPS) + 31) & ~31;
     const int per = per_warp * EV_WARPS, lo = min(n, rank * per), hi = min(n, lo + per);
     auto place = [&](int s) { return s < known ? pos[s] : seen - n + s; };
     if (tid == 0) maxpos = INT_MIN;
     __syncthreads();
-    int last = INT_MIN;
-    for (int s = lo + tid; s < hi; s += EV_THREADS) last = max(last, place(s));
+    int last = known < n ? seen - 1 : INT_MIN;
+    for (int s = lo + tid; s < min(hi, lo + a.kcap); s += EV_THREADS) keys[s - lo] = float_key(w[s]);
+    for (int s = lo + tid; s < min(hi, known); s += EV_THREADS) last = max(last, pos[s]);
     last = __reduce_max_sync(0xffffffffu, last);
     if (lane == 0) atomicMax(&maxpos, last);
     if (nc > 1) cl.sync(); else __syncthreads();
     for (int r = 0; r < nc; r++) last = max(last, nc > 1 ? *cl.map_shared_rank(&maxpos, r) : maxpos);
     auto make_key = [&](int s) { return (int64_t)place(s) > (int64_t)last - a.recent ? 0xffffffffu : float_key(w[s]); };
-    for (int s = lo + tid; s < min(hi, lo + a.kcap); s += EV_THREADS) keys[s - lo] = make_key(s);
+    for (int s = lo + tid; s < min(hi, lo + a.kcap); s += EV_THREADS)
+        if ((int64_t)place(s) > (int64_t)last - a.recent) keys[s - lo] = 0xffffffffu;
     __syncthreads();
     auto key = [&](int i) { return i < a.kcap ? keys[i] : make_key(lo + i); };
     uint32_t bound = 0, ties = 0xffffffffu;              // all are kept where there is room for all
@@ -130,6 +139,8 @@ __global__ void __launch_bounds__(EV_THREADS) k_cache_evict(EvictArgs a) {
         a.w2[u * a.cap2 + t] = w[f];
         a.pos2[u * a.cap2 + t] = place(f);
     }
+    if (rank == 0 && tid == 0) a.pairs[u] = pairs;
+    if (!a.move_here) return;
     const char *k = a.c.k + b * a.c.rs + kvh * a.c.hs, *v = a.c.v + b * a.c.rs + kvh * a.c.hs;
     char *k2 = a.k2 + b * a.rs2 + kvh * a.hs2, *v2 = a.v2 + b * a.rs2 + kvh * a.hs2;
     const int units = a.c.hd * a.es / 16;                // of 16 bytes in a token's keys
@@ -141,6 +152,31 @@ __global__ void __launch_bounds__(EV_THREADS) k_cache_evict(EvictArgs a) {
         *(int4 *)(k2 + t * a.ts2 + x) = kx;
         *(int4 *)(v2 + t * a.ts2 + x) = vx;
     }
+}
+
+// The tokens that move, over the whole GPU. A thread has 16 bytes of a token's keys or values, of EV_AHEAD tokens.
+constexpr int EV_MTHREADS = 256, EV_AHEAD = 4;
+__global__ void __launch_bounds__(EV_MTHREADS) k_cache_move(EvictArgs a, int ul) {
+    const int kvh = blockIdx.y, b = blockIdx.z, tid = threadIdx.x;
+    const int x = tid & ((1 << ul) - 1), is_v = (tid >> ul) & 1, tok = tid >> (ul + 1), tpc = EV_MTHREADS >> (ul + 1);
+    const int64_t u = (int64_t)b * a.c.nkv + kvh;
+    pdl_launch_dependents();
+    pdl_wait();
+    const int pairs = a.pairs[u], p0 = (int)blockIdx.x * tpc * EV_AHEAD + tok;
+    if (x * 16 >= a.c.hd * a.es) return;
+    const int *from = a.from + u * a.room, *to = a.to + u * a.room;
+    const char *src = (is_v ? a.c.v : a.c.k) + b * a.c.rs + kvh * a.c.hs + x * 16;
+    char *dst = (is_v ? a.v2 : a.k2) + b * a.rs2 + kvh * a.hs2 + x * 16;
+    int4 r[EV_AHEAD];
+    int64_t t[EV_AHEAD];
+#pragma unroll
+    for (int i = 0; i < EV_AHEAD; i++) {
+        const int p = p0 + i * tpc;
+        t[i] = p < pairs ? to[p] : -1;
+        if (t[i] >= 0) r[i] = *(const int4 *)(src + from[p] * a.c.ts);
+    }
+#pragma unroll
+    for (int i = 0; i < EV_AHEAD; i++) if (t[i] >= 0) *(int4 *)(dst + t[i] * a.ts2) = r[i];
 }
 
 bool overlaps(const CacheDev &a, const CacheDev &b, int es) {
@@ -184,25 +220,25 @@ extern "C" int ncmb_cache_evict(const NcmbCache *src, const NcmbCache *dst, cons
     a.w = weights; a.w2 = weights_dst; a.pos = pos; a.pos2 = pos_dst; a.known = known; a.seen = seen; a.len2 = len_dst;
     if (max_len <= 0 || max_len > src->capacity) max_len = src->capacity;
     const int64_t units = (int64_t)src->rows * src->n_kv;
-    a.from = (int *)cache_scratch(who, units * a.room * 8);
+    a.from = (int *)cache_scratch(who, units * a.room * 8 + units * 4);
     if (!a.from) return -1;
     a.to = a.from + units * a.room;
-    // CTAs a (row, head): as many as keep the GPU busy, with 2048 slots each at least
+    a.pairs = a.to + units * a.room;
+    // CTAs a (row, head): as many as keep the GPU busy, with 4096 slots each at least
     int nc = 1;
-    while (nc < EV_MAXC && units * nc < ctx().sm_count && cdiv(max_len, nc) > 2048) nc *= 2;
+    while (nc < EV_MAXC && units * nc * 2 <= ctx().sm_count && cdiv(max_len, nc) > 4096) nc *= 2;
+    a.move_here = a.inplace && max_len - a.room <= 64;   // that many tokens move at most, by what the host knows
     // slots of a CTA when the row is as long as the cache can hold: bits for all, keys for as many as shared memory takes
     const int64_t most = cdiv(cdiv(src->capacity, nc * EV_WARPS), 32) * 32 * EV_WARPS, hint = cdiv(cdiv(max_len, nc * EV_WARPS), 32) * 32 * EV_WARPS;
     a.kcap = (int)(hint < EV_KEYS ? hint : EV_KEYS);
     const size_t smem = (size_t)a.kcap * 4 + (size_t)most / 8;
     CUDA_CHECK(cudaFuncSetAttribute(k_cache_evict, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(nc, src->n_kv, src->rows); cfg.blockDim = dim3(EV_THREADS); cfg.dynamicSmemBytes = smem; cfg.stream = stream();
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = nc; at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = 1;
-    cfg.attrs = at; cfg.numAttrs = 1;
-    cudaError_t e = cudaLaunchKernelEx(&cfg, k_cache_evict, a);
-    if (e != cudaSuccess) fatal("cache eviction: launch failed: %s", cudaGetErrorString(e));
-    ctx().launches++;
+    cache_launch(k_cache_evict, dim3(nc, src->n_kv, src->rows), EV_THREADS, smem, nc, a);
+    if (!a.move_here) {
+        int ul = 0;
+        while ((16 << ul) < src->hd * es) ul++;
+        const int per = (EV_MTHREADS >> (ul + 1)) * EV_AHEAD;
+        cache_launch(k_cache_move, dim3((unsigned)cdiv(a.room, per), src->n_kv, src->rows), EV_MTHREADS, 0, 1, a, ul);
+    }
     return 0;
 }

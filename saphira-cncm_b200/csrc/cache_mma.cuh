@@ -20,8 +20,6 @@ constexpr int CM_WARPS = 4, CM_THREADS = CM_WARPS * 32;
 #define CM_ST 2
 #define CM_CTAS 3
 #endif
-constexpr int CM_STAGES = CM_ST, CM_STAGE = CM_SB;      // stages of a warp's ring, and bytes of keys and values in one
-
 // R: query rows of a tile, 16 or 8. A tile of 8 has two terms of its queries (or probabilities) stacked in the 16 rows of the
 // tensor-core tile; a lane holds rows lane / 4 and lane / 4 + 8 of a result, so it adds the two terms' products up itself.
 template <class KE, class QE, int HDP_, int R_> struct CmCfg {
@@ -31,6 +29,8 @@ template <class KE, class QE, int HDP_, int R_> struct CmCfg {
     static constexpr int NH = R8 ? 1 : 2;                        // rows a lane has
     static constexpr int ROW = HDP * (int)sizeof(KE);            // bytes of a key in shared memory
     static constexpr int UPR = ROW / 16;
+    static constexpr int CM_STAGE = HDP == 64 ? CM_SB : 8192;    // bytes of keys and values in a stage of a warp's ring
+    static constexpr int CM_STAGES = HDP == 64 ? CM_ST : 2, CTAS = HDP == 64 ? CM_CTAS : 3;      // stages, CTAs an SM
     static constexpr int KC = CM_STAGE / (2 * ROW);              // keys a chunk
     static constexpr int NT = KC / 8;                            // 8-key tiles a chunk
     static constexpr int NQ = !BF ? 2 : sizeof(QE) == 4 ? 3 : 1; // terms of a query
@@ -53,6 +53,7 @@ struct CmArgs {
     const int *parents;
     float c2;                        // scale * log2(e)
     float *part;                     // partial results, one slot a (CTA + unit)
+    int2 *range;                     // first and last CTA of each unit
     float *scores;                   // [row][kv head][M][pitch], or null
     int64_t pitch;
     float *weights;
@@ -171,10 +172,11 @@ template <bool BLOCKS, int KC> __device__ int cm_find(const CmArgs &a, int64_t x
 // of each 32 dims the four from 4 (lane / 4) on, which are its column of four tiles. Where a dim stands in a k-step and where a
 // column in a tile is free as long as both operands, or all who read the result, agree.
 template <class KE, class QE, int HDP, int R, bool BLOCKS>
-__global__ void __launch_bounds__(CM_THREADS, CM_CTAS) k_cache_attention(const __grid_constant__ CmArgs a) {
+__global__ void __launch_bounds__(CM_THREADS, CmCfg<KE, QE, HDP, R>::CTAS) k_cache_attention(const __grid_constant__ CmArgs a) {
     using F = CmCfg<KE, QE, HDP, R>;
     constexpr int KC = F::KC, NT = F::NT, NQ = F::NQ, NP = F::NP, ROW = F::ROW, UPR = F::UPR, M = F::M, NH = F::NH;
     constexpr bool R8 = F::R8;
+    constexpr int CM_STAGE = F::CM_STAGE, CM_STAGES = F::CM_STAGES;
     extern __shared__ __align__(128) char smem[];
     char *ring = smem, *qs = smem + F::RING;
     __shared__ int64_t sh[CM_WARPS];
@@ -599,6 +601,8 @@ __global__ void __launch_bounds__(CM_THREADS, CM_CTAS) k_cache_attention(const _
         }
         __syncthreads();
         const bool whole = first == 0 && stop == nch;
+        if (tid == 0 && first == 0) a.range[unit].x = blockIdx.x;
+        if (tid == 0 && stop == nch) a.range[unit].y = blockIdx.x;
         float *slot = a.part + ((int64_t)blockIdx.x + unit) * F::SLOT;
         for (int m = tid; m < M; m += CM_THREADS) {
             float top = wm[0][m], l = 0.f;
@@ -635,17 +639,15 @@ __global__ void __launch_bounds__(CM_THREADS, CM_CTAS) k_cache_attention(const _
 // The others: 512 slots of one (row, kv head) each, from the scores that the kernel above left.
 constexpr int CM_WKEYS = 512;
 template <class KE, class QE, int HDP, int R, bool BLOCKS>
-__global__ void __launch_bounds__(CM_THREADS) k_cache_join(const __grid_constant__ CmArgs a, int ctas, int joins, int split) {
+__global__ void __launch_bounds__(CM_THREADS) k_cache_join(const __grid_constant__ CmArgs a, int joins, int split) {
     using F = CmCfg<KE, QE, HDP, R>;
-    constexpr int M = F::M, KC = F::KC, D4 = HDP / 4, GROUPS = CM_THREADS / D4;
-    __shared__ int64_t sh[CM_WARPS];
+    constexpr int M = F::M, D4 = HDP / 4, GROUPS = CM_THREADS / D4;
     __shared__ float lse[NCMB_MAX_NODES];
     __shared__ float gm[GROUPS], gl[GROUPS];
     __shared__ float4 go[GROUPS][D4];
     const int tid = threadIdx.x, G = a.G, hd = a.c.hd;
     pdl_launch_dependents();
     pdl_wait();
-    const CmPlan plan = cm_plan<BLOCKS, KC>(a, ctas, sh);
     const bool join = (int)blockIdx.x < joins;
     const int per_item = a.c.nkv * a.tiles, rows = split ? 1 : GROUPS, steps = M / rows;      // rows a CTA, CTAs a unit
     int item, sub, key0 = 0;
@@ -656,21 +658,12 @@ __global__ void __launch_bounds__(CM_THREADS) k_cache_join(const __grid_constant
         sub = x / span % a.c.nkv * a.tiles;
         item = x / span / a.c.nkv;
     }
-    const int n = cm_keys<BLOCKS>(a, item), nch = (n + KC - 1) / KC;
-    if (!join && key0 >= n) return;
-    int64_t start;
-    cm_find<BLOCKS, KC>(a, 0, item, start, sh);
     const int row = a.row0 + (BLOCKS ? item / a.T : item);
     const int *par = a.parents ? a.parents + (int64_t)row * a.T : nullptr;
-    // CTAs that have a part of a unit
-    auto parts = [&](int s, int &c0, int &c1) {
-        const int64_t from = start + (int64_t)s * nch;
-        c0 = (int)(from / plan.per);
-        c1 = (int)((from + nch - 1) / plan.per);
-    };
-    int c0, c1;
+    const int64_t unit0 = (int64_t)item * per_item + sub;
     if (join) {
-        parts(sub, c0, c1);
+        const int2 cr = a.range[unit0];                          // CTAs that have a part of it
+        const int c0 = cr.x, c1 = cr.y;
         if (c0 == c1) return;                                    // written already
         const float *slot = a.part + ((int64_t)c0 + (int64_t)item * per_item + sub) * F::SLOT;
         const int grp = tid / D4, d = tid % D4 * 4, kvh = sub / a.tiles;
@@ -714,7 +707,8 @@ __global__ void __launch_bounds__(CM_THREADS) k_cache_join(const __grid_constant
         cm_put(out, o.x * r); cm_put(out + 1, o.y * r); cm_put(out + 2, o.z * r); cm_put(out + 3, o.w * r);
         return;
     }
-    const int kvh = sub / a.tiles, len = n - a.T;
+    const int kvh = sub / a.tiles, n = cm_keys<BLOCKS>(a, item), len = n - a.T;
+    if (key0 >= n) return;
     float w[CM_WKEYS / CM_THREADS];
 #pragma unroll
     for (int x = 0; x < CM_WKEYS / CM_THREADS; x++) w[x] = 0.f;
@@ -723,14 +717,17 @@ __global__ void __launch_bounds__(CM_THREADS) k_cache_join(const __grid_constant
         const int nm = min(NCMB_MAX_NODES, a.M - mb);
         __syncthreads();
         for (int i = tid; i < nm; i += CM_THREADS) {
-            const int mm = mb + i, s = sub + mm / M, m = mm % M;
-            parts(s, c0, c1);
-            const float *slot = a.part + ((int64_t)c0 + (int64_t)item * per_item + s) * F::SLOT;
+            const int mm = mb + i, m = mm % M;
+            const int64_t u = unit0 + mm / M;
+            const int2 cr = a.range[u];
+            const float *slot = a.part + (cr.x + u) * F::SLOT;
             float top = -INFINITY, l = 0.f;
-            for (int c = 0; c <= c1 - c0; c++) top = fmaxf(top, slot[c * F::SLOT + m]);
-            for (int c = 0; c <= c1 - c0; c++) {
-                const float x = slot[c * F::SLOT + m];
-                if (x != -INFINITY) l = fmaf(slot[c * F::SLOT + M + m], cm_exp2(x - top), l);
+#pragma unroll 4
+            for (int c = 0; c <= cr.y - cr.x; c++) {
+                const float x = slot[c * F::SLOT + m], xl = slot[c * F::SLOT + M + m];
+                const float t = fmaxf(top, x), base = t == -INFINITY ? 0.f : t;
+                l = l * cm_exp2(top - base) + xl * cm_exp2(x - base);
+                top = t;
             }
             lse[i] = l > 0.f && cm_used(par, mm / G) ? top + log2f(l) : INFINITY;
         }
@@ -774,12 +771,13 @@ int cm_run_as(const char *who, CmArgs a, int max_keys) {
     const int64_t spans = a.weights ? cdiv(a.pitch, CM_WKEYS) * step * a.c.nkv : 0;
     if (units * F::M + spans > 0x7fffffff) return cache_refuse(who, "%lld query tiles", (long long)units);
     const int64_t est = units * cdiv(max_keys, F::KC);
-    const int ctas = (int)std::max<int64_t>(1, std::min<int64_t>(CM_CTAS * ctx().sm_count, cdiv(est, CM_WARPS)));
-    const size_t part = (size_t)(units + ctas) * F::SLOT * 4, sc = a.weights ? (size_t)step * a.c.nkv * a.M * a.pitch * 4 : 0;
+    const int ctas = (int)std::max<int64_t>(1, std::min<int64_t>(F::CTAS * ctx().sm_count, cdiv(est, CM_WARPS)));
+    const size_t ranges = ((size_t)units * 8 + 255) & ~(size_t)255, part = (size_t)(units + ctas) * F::SLOT * 4 + ranges, sc = a.weights ? (size_t)step * a.c.nkv * a.M * a.pitch * 4 : 0;
     char *scratch = (char *)cache_scratch(who, part + sc);
     if (!scratch) return -1;
     a.scores = a.weights ? (float *)scratch : nullptr;
-    a.part = (float *)(scratch + sc);
+    a.range = (int2 *)(scratch + sc);
+    a.part = (float *)(scratch + sc + ranges);
     const int split = ctas > 4 * units;                          // many parts a unit
     for (int r = 0; r < rows; r += step) {
         const int nr = std::min(step, rows - r);
@@ -787,7 +785,7 @@ int cm_run_as(const char *who, CmArgs a, int max_keys) {
         a.items = nr * per_row;
         const int64_t u = (int64_t)a.items * a.c.nkv * a.tiles, joins = u * (F::M / (split ? 1 : CM_THREADS / (HDP / 4)));
         LAUNCH_PDL((k_cache_attention<KE, QE, HDP, R, BLOCKS>), ctas, CM_THREADS, smem, a);
-        LAUNCH_PDL((k_cache_join<KE, QE, HDP, R, BLOCKS>), (unsigned)(joins + spans / step * nr), CM_THREADS, 0, a, ctas, (int)joins, split);
+        LAUNCH_PDL((k_cache_join<KE, QE, HDP, R, BLOCKS>), (unsigned)(joins + spans / step * nr), CM_THREADS, 0, a, (int)joins, split);
     }
     return 0;
 }

@@ -63,67 +63,73 @@ void cache_launch(void (*kernel)(KArgs...), dim3 grid, int threads, size_t smem,
 // ---- the k-th largest of many 32-bit keys, by a cluster of CTAs that each hold a part of them ----
 constexpr int SEL_BINS = 2048;
 struct SelShared {
-    uint32_t hist[3][SEL_BINS];      // one per pass, so that one cluster barrier a pass is enough
+    alignas(16) uint32_t hist[3][SEL_BINS];      // one per pass, so that one cluster barrier a pass is enough
     uint32_t wsum[32];
     uint32_t bin, left;
 };
 // Digits of 11, 11 and 10 bits from the top: each pass counts the keys that agree with what is settled so far by their next
 // digit, adds the CTAs' counts up and settles the digit at which the count from above reaches k. key(i), i in [0, n): this
 // CTA's keys. Returns the k-th largest of all (1 <= k <= their number); `ties` of the keys equal to it are among the k
-// largest. All threads of all CTAs of the cluster call it; NT threads a CTA.
-template <int NT, class KEY>
+// largest. All threads of all CTAs of the cluster call it; NT threads a CTA, CL: more than one CTA. Nothing is unrolled on
+// purpose: code that runs once a call is paced by instruction fetches (unrolled, a pass took 5000 cycles).
+template <int NT, bool CL, class KEY>
 __device__ uint32_t select_kth(SelShared &s, int n, uint32_t k, uint32_t &ties, KEY key) {
     namespace cg = cooperative_groups;
-    static_assert(SEL_BINS % NT == 0 && NT % 32 == 0, "whole bins a thread");
+    static_assert(SEL_BINS % (4 * NT) == 0 && NT % 32 == 0, "whole groups of four bins a thread");
     constexpr int BPT = SEL_BINS / NT;
-    cg::cluster_group cl = cg::this_cluster();
-    const int nc = (int)cl.num_blocks(), tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    for (int i = tid; i < 3 * SEL_BINS; i += NT) (&s.hist[0][0])[i] = 0;
+    static_assert(BPT == 4, "a thread has four bins");
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    for (int i = tid; i < 3 * SEL_BINS / 4; i += NT) ((uint4 *)&s.hist[0][0])[i] = make_uint4(0, 0, 0, 0);
     __syncthreads();
     uint32_t prefix = 0, settled = 0;            // settled: mask of the bits that prefix states
-    const int shifts[3] = {21, 10, 0};
-#pragma unroll
+#pragma unroll 1
     for (int pass = 0; pass < 3; pass++) {
-        const int sh = shifts[pass];
+        const int sh = pass == 0 ? 21 : pass == 1 ? 10 : 0;
         const uint32_t dm = pass == 2 ? 1023u : 2047u;
+        uint32_t *hist = s.hist[pass];
+#pragma unroll 1
         for (int i = tid; i < n; i += NT) {
             const uint32_t u = key(i);
-            if ((u & settled) == prefix) atomicAdd(&s.hist[pass][(u >> sh) & dm], 1u);
+            if ((u & settled) == prefix) atomicAdd(&hist[(u >> sh) & dm], 1u);
         }
-        if (nc > 1) cl.sync(); else __syncthreads();
-        uint32_t c[BPT], sum = 0;                // thread t has bins from 2047 - BPT t downwards
-#pragma unroll
-        for (int i = 0; i < BPT; i++) {
-            const int b = SEL_BINS - 1 - BPT * tid - i;
-            uint32_t v = 0;
-            for (int r = 0; r < nc; r++) v += nc > 1 ? cl.map_shared_rank(&s.hist[pass][0], r)[b] : s.hist[pass][b];
-            c[i] = v;
-            sum += v;
+        const int b = SEL_BINS - 4 - 4 * tid;    // thread t has bins b + 3 ... b
+        uint4 c;
+        if constexpr (CL) {
+            cg::cluster_group cl = cg::this_cluster();
+            cl.sync();
+            c = make_uint4(0, 0, 0, 0);
+#pragma unroll 1
+            for (int r = 0; r < (int)cl.num_blocks(); r++) {
+                const uint4 v = *(const uint4 *)(cl.map_shared_rank(hist, r) + b);
+                c.x += v.x; c.y += v.y; c.z += v.z; c.w += v.w;
+            }
+        } else {
+            __syncthreads();
+            c = *(const uint4 *)(hist + b);
         }
+        const uint32_t sum = c.x + c.y + c.z + c.w;
         uint32_t inc = sum;
-#pragma unroll
+#pragma unroll 1
         for (int o = 1; o < 32; o <<= 1) {
             const uint32_t v = __shfl_up_sync(0xffffffffu, inc, o);
             if (lane >= o) inc += v;
         }
         if (lane == 31) s.wsum[warp] = inc;
         __syncthreads();
-        uint32_t above = inc - sum;
-        for (int w = 0; w < warp; w++) above += s.wsum[w];
+        const uint32_t others = __reduce_add_sync(0xffffffffu, lane < warp ? s.wsum[lane] : 0u);
+        uint32_t above = others + inc - sum;
         if (above < k && above + sum >= k) {
-#pragma unroll
-            for (int i = 0; i < BPT; i++) {
-                if (above < k && above + c[i] >= k) { s.bin = SEL_BINS - 1 - BPT * tid - i; s.left = k - above; }
-                above += c[i];
-            }
+            uint32_t bin = b + 3;
+            if (above + c.w < k) { above += c.w; bin--; if (above + c.z < k) { above += c.z; bin--; if (above + c.y < k) { above += c.y; bin--; } } }
+            s.bin = bin;
+            s.left = k - above;
         }
         __syncthreads();
         prefix |= s.bin << sh;
         settled |= dm << sh;
         k = s.left;
-        __syncthreads();
     }
-    if (nc > 1) cl.sync();                       // the others have read this CTA's counts
+    if constexpr (CL) cg::this_cluster().sync();     // the others have read this CTA's counts
     ties = k;
     return prefix;
 }

@@ -125,14 +125,14 @@ __device__ __forceinline__ void mma_s8(int (&c)[4], const uint32_t (&a)[4], uint
 // m16n8k32 tiles -- 16 heads of the group against 8 blocks -- with the dims of a tile's k positions chosen so that a lane's
 // codes are 8 bytes in a row (any order of the dims gives the same whole numbers). Bound by latency: the codes of 128K
 // tokens in blocks of 64 are 128 KB a kv head.
-template <class QE>
+template <class QE, bool CL>
 __global__ void __launch_bounds__(BP_THREADS) k_block_pick(BlockArgs a) {
     namespace cg = cooperative_groups;
     extern __shared__ __align__(16) char dyn[];
     __shared__ SelShared sel;
     __shared__ int wtie[BP_WARPS], wkeep[BP_WARPS], share[2];
     cg::cluster_group cl = cg::this_cluster();
-    const int rank = (int)cl.block_rank(), nc = (int)cl.num_blocks();
+    const int rank = CL ? (int)cl.block_rank() : 0, nc = CL ? (int)cl.num_blocks() : 1;
     const int t = blockIdx.x / nc, kvh = blockIdx.y, b = blockIdx.z, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, hd = a.c.hd;
     pdl_launch_dependents();
     pdl_wait();
@@ -228,9 +228,10 @@ __global__ void __launch_bounds__(BP_THREADS) k_block_pick(BlockArgs a) {
     }
     __syncthreads();
     uint32_t ties;
-    const uint32_t bound = select_kth<BP_THREADS>(sel, hi - lo, (uint32_t)k, ties, [&](int i) { return keys[i]; });
+    const uint32_t bound = select_kth<BP_THREADS, CL>(sel, hi - lo, (uint32_t)k, ties, [&](int i) { return keys[i]; });
     const int part = ((hi - lo + BP_THREADS - 1) / BP_THREADS) * 32, w0 = min(hi - lo, warp * part), w1 = min(hi - lo, w0 + part);
     int nt = 0, above = 0;
+#pragma unroll 1
     for (int s = w0; s < w1; s += 32) {
         const uint32_t x = s + lane < w1 ? keys[s + lane] : 0;
         nt += __popc(__ballot_sync(0xffffffffu, s + lane < w1 && x == bound));
@@ -238,12 +239,19 @@ __global__ void __launch_bounds__(BP_THREADS) k_block_pick(BlockArgs a) {
     }
     if (lane == 0) { wtie[warp] = nt; wkeep[warp] = above; }
     __syncthreads();
-    if (tid == 0) { int x = 0, y = 0; for (int i = 0; i < BP_WARPS; i++) { x += wtie[i]; y += wkeep[i]; } share[0] = x; share[1] = y; }
-    if (nc > 1) cl.sync();
-    int tb = 0, at = 0;                          // ties before this warp; picks before it
-    for (int r = 0; r < rank; r++) { tb += *cl.map_shared_rank(&share[0], r); at += *cl.map_shared_rank(&share[1], r); }
-    for (int i = 0; i < warp; i++) { at += wkeep[i]; tb += wtie[i]; }
-    at += min(tb, (int)ties);
+    const int vt = lane < BP_WARPS ? wtie[lane] : 0, vk = lane < BP_WARPS ? wkeep[lane] : 0;
+    int tb = __reduce_add_sync(0xffffffffu, lane < warp ? vt : 0), at = __reduce_add_sync(0xffffffffu, lane < warp ? vk : 0);
+    if constexpr (CL) {
+        if (warp == 0) {
+            const int x = __reduce_add_sync(0xffffffffu, vt), y = __reduce_add_sync(0xffffffffu, vk);
+            if (lane == 0) { share[0] = x; share[1] = y; }
+        }
+        cl.sync();
+        tb += __reduce_add_sync(0xffffffffu, lane < rank ? *cl.map_shared_rank(&share[0], lane) : 0);
+        at += __reduce_add_sync(0xffffffffu, lane < rank ? *cl.map_shared_rank(&share[1], lane) : 0);
+    }
+    at += min(tb, (int)ties);                    // ties before this warp: tb; picks before it: at
+#pragma unroll 1
     for (int s = w0; s < w1; s += 32) {
         const bool in = s + lane < w1;
         const uint32_t x = in ? keys[s + lane] : 0, lt = (1u << lane) - 1;
@@ -254,13 +262,14 @@ __global__ void __launch_bounds__(BP_THREADS) k_block_pick(BlockArgs a) {
         at += __popc(km);
         tb += __popc(tm);
     }
-    if (nc > 1) cl.sync();                       // the others have read this CTA's counts
+    if constexpr (CL) cl.sync();                 // the others have read this CTA's counts
 }
 
 template <class QE>
 void run_pick(const BlockArgs &a, int nc, size_t smem) {
-    CUDA_CHECK(cudaFuncSetAttribute(k_block_pick<QE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-    cache_launch(k_block_pick<QE>, dim3(a.T * nc, a.c.nkv, a.c.rows), BP_THREADS, smem, nc, a);
+    auto kernel = nc > 1 ? k_block_pick<QE, true> : k_block_pick<QE, false>;
+    if (smem > 20000) CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    cache_launch(kernel, dim3(a.T * nc, a.c.nkv, a.c.rows), BP_THREADS, smem, nc, a);
 }
 
 } // namespace

@@ -30,13 +30,16 @@ struct EvictArgs {
     int move_here;                   // few tokens move: the kernel that picks moves them too
 };
 
+// CL: a cluster of CTAs a (row, kv head), each with a part of the slots; else one CTA.
+template <bool CL>
 __global__ void __launch_bounds__(EV_THREADS) k_cache_evict(EvictArgs a) {
     extern __shared__ uint32_t dyn[];
     __shared__ SelShared sel;
-    __shared__ int maxpos, wtie[EV_WARPS], wcount[EV_WARPS][3];
+    __shared__ int maxpos, wcount[4][EV_WARPS];
     __shared__ int share[4];         // ties, freed slots, kept tokens from beyond, kept in place: of this CTA
     cg::cluster_group cl = cg::this_cluster();
-    const int rank = (int)cl.block_rank(), nc = (int)cl.num_blocks();
+    const int rank = CL ? (int)cl.block_rank() : 0, nc = CL ? (int)cl.num_blocks() : 1;
+    auto sync = [&] { if constexpr (CL) cl.sync(); else __syncthreads(); };
     const int kvh = blockIdx.y, b = blockIdx.z, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     uint32_t *keys = dyn, *kept = dyn + a.kcap;          // keys, then one bit a slot
     pdl_launch_dependents();
@@ -62,77 +65,77 @@ __global__ void __launch_bounds__(EV_THREADS) k_cache_evict(EvictArgs a) {
     for (int s = lo + tid; s < min(hi, known); s += EV_THREADS) last = max(last, pos[s]);
     last = __reduce_max_sync(0xffffffffu, last);
     if (lane == 0) atomicMax(&maxpos, last);
-    if (nc > 1) cl.sync(); else __syncthreads();
-    for (int r = 0; r < nc; r++) last = max(last, nc > 1 ? *cl.map_shared_rank(&maxpos, r) : maxpos);
-    auto make_key = [&](int s) { return (int64_t)place(s) > (int64_t)last - a.recent ? 0xffffffffu : float_key(w[s]); };
-    for (int s = lo + tid; s < min(hi, lo + a.kcap); s += EV_THREADS)
-        if ((int64_t)place(s) > (int64_t)last - a.recent) keys[s - lo] = 0xffffffffu;
+    sync();
+    if constexpr (CL) { for (int r = 0; r < nc; r++) last = max(last, *cl.map_shared_rank(&maxpos, r)); }
+    else last = maxpos;
+    auto latest = [&](int s) { return (int64_t)place(s) > (int64_t)last - a.recent; };
+#pragma unroll 1
+    for (int s = lo + tid; s < min(hi, lo + a.kcap); s += EV_THREADS) if (latest(s)) keys[s - lo] = 0xffffffffu;
     __syncthreads();
-    auto key = [&](int i) { return i < a.kcap ? keys[i] : make_key(lo + i); };
+    auto key = [&](int i) { return i < a.kcap ? keys[i] : latest(lo + i) ? 0xffffffffu : float_key(w[lo + i]); };
     uint32_t bound = 0, ties = 0xffffffffu;              // all are kept where there is room for all
-    if (n2 < n) bound = select_kth<EV_THREADS>(sel, hi - lo, (uint32_t)n2, ties, key);
+    if (n2 < n) bound = select_kth<EV_THREADS, CL>(sel, hi - lo, (uint32_t)n2, ties, key);
 
-    // ties before this warp's slots, so that the lower ones are kept
+    // how many of something the slots before this warp's hold, given its own count; total: all CTAs'
     const int w0 = lo + warp * per_warp, w1 = min(hi, w0 + per_warp);
-    int mine = 0;
-    for (int s = w0; s < w1; s += 32) {
-        const bool tie = s + lane < w1 && key(s + lane - lo) == bound;
-        mine += __popc(__ballot_sync(0xffffffffu, tie));
-    }
-    if (lane == 0) wtie[warp] = mine;
-    __syncthreads();
-    if (tid == 0) { int t = 0; for (int i = 0; i < EV_WARPS; i++) t += wtie[i]; share[0] = t; }
-    if (nc > 1) cl.sync(); else __syncthreads();
-    uint32_t before = 0;
-    for (int r = 0; r < rank; r++) before += (uint32_t)*cl.map_shared_rank(&share[0], r);
-    for (int i = 0; i < warp; i++) before += (uint32_t)wtie[i];
-    int count[3] = {0, 0, 0};
+    auto before = [&](int which, int mine, int &total) {
+        if (lane == 0) wcount[which][warp] = mine;
+        __syncthreads();
+        const int v = lane < EV_WARPS ? wcount[which][lane] : 0;
+        int lead = __reduce_add_sync(0xffffffffu, lane < warp ? v : 0);
+        total = __reduce_add_sync(0xffffffffu, v);
+        if constexpr (CL) {
+            if (tid == 0) share[which] = total;
+            cl.sync();
+            const int o = lane < nc ? *cl.map_shared_rank(&share[which], lane) : 0;
+            lead += __reduce_add_sync(0xffffffffu, lane < rank ? o : 0);
+            total = __reduce_add_sync(0xffffffffu, o);
+        }
+        return lead;
+    };
+    int mine = 0, all;
+#pragma unroll 1
+    for (int s = w0; s < w1; s += 32) mine += __popc(__ballot_sync(0xffffffffu, s + lane < w1 && key(s + lane - lo) == bound));
+    uint32_t tied = (uint32_t)before(0, mine, all);      // the lower ones are kept
+    int freed = 0, beyond = 0, stay = 0;
+#pragma unroll 1
     for (int s = w0; s < w1; s += 32) {
         const bool in = s + lane < w1;
         const uint32_t x = in ? key(s + lane - lo) : 0;
         const uint32_t tm = __ballot_sync(0xffffffffu, in && x == bound);
-        const bool keep = in && (x > bound || (x == bound && before + (uint32_t)__popc(tm & ((1u << lane) - 1)) < ties));
-        before += (uint32_t)__popc(tm);
+        const bool keep = in && (x > bound || (x == bound && tied + (uint32_t)__popc(tm & ((1u << lane) - 1)) < ties));
+        tied += (uint32_t)__popc(tm);
         const uint32_t km = __ballot_sync(0xffffffffu, keep);
         const uint32_t below = n2 - s >= 32 ? 0xffffffffu : n2 > s ? (1u << (n2 - s)) - 1 : 0u;      // slots below n2
         if (lane == 0) kept[(s - lo) >> 5] = km;
-        count[0] += __popc(~km & below);
-        count[1] += __popc(km & ~below);
-        count[2] += __popc(km & below);
+        freed += __popc(~km & below);
+        beyond += __popc(km & ~below);
+        stay += __popc(km & below);
     }
-    if (lane < 3) wcount[warp][lane] = lane == 0 ? count[0] : lane == 1 ? count[1] : count[2];
-    __syncthreads();
-    if (tid < 3) { int t = 0; for (int i = 0; i < EV_WARPS; i++) t += wcount[i][tid]; share[1 + tid] = t; }
-    if (nc > 1) cl.sync(); else __syncthreads();
-    int at[3], moves = 0;
-#pragma unroll
-    for (int i = 0; i < 3; i++) {
-        at[i] = 0;
-        for (int r = 0; r < nc; r++) {
-            const int v = nc > 1 ? *cl.map_shared_rank(&share[1 + i], r) : share[1 + i];
-            if (r < rank) at[i] += v;
-            if (i == 0) moves += v;
-        }
-        for (int q = 0; q < warp; q++) at[i] += wcount[q][i];
-    }
+    int moves;
+    freed = before(1, freed, moves);
+    beyond = before(2, beyond, all);
+    if (!a.inplace) stay = moves + before(3, stay, all);
     // pairs (from, to): moves, then -- to another cache -- the tokens that keep their slot
     int *from = a.from + u * a.room, *to = a.to + u * a.room;
+    __syncwarp();
+#pragma unroll 1
     for (int s = w0; s < w1; s += 32) {
         const uint32_t km = kept[(s - lo) >> 5], lt = (1u << lane) - 1, me = 1u << lane;
         const uint32_t below = n2 - s >= 32 ? 0xffffffffu : n2 > s ? (1u << (n2 - s)) - 1 : 0u;
-        if (~km & below & me) to[at[0] + __popc(~km & below & lt)] = s + lane;
-        if (km & ~below & me) from[at[1] + __popc(km & ~below & lt)] = s + lane;
+        if (~km & below & me) to[freed + __popc(~km & below & lt)] = s + lane;
+        if (km & ~below & me) from[beyond + __popc(km & ~below & lt)] = s + lane;
         if (km & below & me) {
             if (!a.inplace) {
-                const int i = moves + at[2] + __popc(km & below & lt);
+                const int i = stay + __popc(km & below & lt);
                 from[i] = to[i] = s + lane;
             } else if (s + lane >= known) a.pos2[u * a.cap2 + s + lane] = seen - n + s + lane;
         }
-        at[0] += __popc(~km & below);
-        at[1] += __popc(km & ~below);
-        at[2] += __popc(km & below);
+        freed += __popc(~km & below);
+        beyond += __popc(km & ~below);
+        stay += __popc(km & below);
     }
-    if (nc > 1) cl.sync(); else __syncthreads();         // also: no key is read from w / pos any more
+    sync();                                              // also: no key is read from w / pos any more
     const int pairs = a.inplace ? moves : n2;
     for (int i = rank * EV_THREADS + tid; i < pairs; i += nc * EV_THREADS) {
         const int f = from[i], t = to[i];
@@ -144,13 +147,13 @@ __global__ void __launch_bounds__(EV_THREADS) k_cache_evict(EvictArgs a) {
     const char *k = a.c.k + b * a.c.rs + kvh * a.c.hs, *v = a.c.v + b * a.c.rs + kvh * a.c.hs;
     char *k2 = a.k2 + b * a.rs2 + kvh * a.hs2, *v2 = a.v2 + b * a.rs2 + kvh * a.hs2;
     const int units = a.c.hd * a.es / 16;                // of 16 bytes in a token's keys
-    const int64_t total = (int64_t)pairs * units;
-    for (int64_t i = rank * EV_THREADS + tid; i < total; i += nc * EV_THREADS) {
-        const int p = (int)(i / units), x = (int)(i % units) * 16;
+    for (int p = rank * EV_WARPS + warp; p < pairs; p += nc * EV_WARPS) {
         const int64_t f = from[p], t = to[p];
-        const int4 kx = *(const int4 *)(k + f * a.c.ts + x), vx = *(const int4 *)(v + f * a.c.ts + x);
-        *(int4 *)(k2 + t * a.ts2 + x) = kx;
-        *(int4 *)(v2 + t * a.ts2 + x) = vx;
+        if (lane < units) {
+            const int4 kx = *(const int4 *)(k + f * a.c.ts + lane * 16), vx = *(const int4 *)(v + f * a.c.ts + lane * 16);
+            *(int4 *)(k2 + t * a.ts2 + lane * 16) = kx;
+            *(int4 *)(v2 + t * a.ts2 + lane * 16) = vx;
+        }
     }
 }
 
@@ -232,8 +235,9 @@ extern "C" int ncmb_cache_evict(const NcmbCache *src, const NcmbCache *dst, cons
     const int64_t most = cdiv(cdiv(src->capacity, nc * EV_WARPS), 32) * 32 * EV_WARPS, hint = cdiv(cdiv(max_len, nc * EV_WARPS), 32) * 32 * EV_WARPS;
     a.kcap = (int)(hint < EV_KEYS ? hint : EV_KEYS);
     const size_t smem = (size_t)a.kcap * 4 + (size_t)most / 8;
-    CUDA_CHECK(cudaFuncSetAttribute(k_cache_evict, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-    cache_launch(k_cache_evict, dim3(nc, src->n_kv, src->rows), EV_THREADS, smem, nc, a);
+    auto kernel = nc > 1 ? k_cache_evict<true> : k_cache_evict<false>;
+    if (smem > 20000) CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    cache_launch(kernel, dim3(nc, src->n_kv, src->rows), EV_THREADS, smem, nc, a);
     if (!a.move_here) {
         int ul = 0;
         while ((16 << ul) < src->hd * es) ul++;

@@ -22,8 +22,9 @@ int cache_check(const char *who, const NcmbCache *c, CacheDev &d);
 inline int cache_elem(const NcmbCache *c) { return c->type == NCMB_BF16 ? 2 : 4; }
 // Scratch of at least `bytes`, kept and grown; null with a message when the device has no room for it. Calls are ordered
 // by the library's stream, so all of them share it; within a call, what one kernel leaves for another that has scratch of
-// its own stands in the other of the two areas.
-enum { SCRATCH_MAIN = 0, SCRATCH_PICKS = 1 };
+// its own stands in another area.
+// SCRATCH_DONE holds zeros when it is given out, and whoever uses it leaves zeros.
+enum { SCRATCH_MAIN = 0, SCRATCH_PICKS = 1, SCRATCH_DONE = 2, SCRATCH_AREAS = 3 };
 void *cache_scratch(const char *who, size_t bytes, int area = SCRATCH_MAIN);
 
 // order of floats as unsigned: larger is larger, -0 is 0, a NaN below everything
@@ -69,9 +70,11 @@ struct SelShared {
 };
 // Digits of 11, 11 and 10 bits from the top: each pass counts the keys that agree with what is settled so far by their next
 // digit, adds the CTAs' counts up and settles the digit at which the count from above reaches k. key(i), i in [0, n): this
-// CTA's keys. Returns the k-th largest of all (1 <= k <= their number); `ties` of the keys equal to it are among the k
-// largest. All threads of all CTAs of the cluster call it; NT threads a CTA, CL: more than one CTA. Nothing is unrolled on
+// CTA's keys. Returns a bound: the keys above it and `ties` of the keys equal to it are the k largest (1 <= k <= their
+// number). Where all keys with the digits settled so far are among them, the rest is left open: the bound is the smallest
+// key with these digits, and ties says all. All threads of all CTAs of the cluster call it; NT threads a CTA, CL: more than one CTA. Nothing is unrolled on
 // purpose: code that runs once a call is paced by instruction fetches (unrolled, a pass took 5000 cycles).
+__device__ __forceinline__ uint32_t hist_of(const uint4 &c, uint32_t i) { return i & 2u ? (i & 1u ? c.w : c.z) : (i & 1u ? c.y : c.x); }
 template <int NT, bool CL, class KEY>
 __device__ uint32_t select_kth(SelShared &s, int n, uint32_t k, uint32_t &ties, KEY key) {
     namespace cg = cooperative_groups;
@@ -88,9 +91,15 @@ __device__ uint32_t select_kth(SelShared &s, int n, uint32_t k, uint32_t &ties, 
         const uint32_t dm = pass == 2 ? 1023u : 2047u;
         uint32_t *hist = s.hist[pass];
 #pragma unroll 1
-        for (int i = tid; i < n; i += NT) {
-            const uint32_t u = key(i);
-            if ((u & settled) == prefix) atomicAdd(&hist[(u >> sh) & dm], 1u);
+        for (int i0 = 0; i0 < n; i0 += NT) {     // lanes that agree with the first of their warp add once: equal keys are common
+            const int i = i0 + tid;
+            const uint32_t u = i < n ? key(i) : 0u;
+            const bool in = i < n && (u & settled) == prefix;
+            const uint32_t d = (u >> sh) & dm, m = __ballot_sync(0xffffffffu, in);
+            if (m == 0) continue;
+            const int lead = __ffs(m) - 1;
+            const uint32_t d0 = __shfl_sync(0xffffffffu, d, lead), same = __ballot_sync(0xffffffffu, in && d == d0);
+            if (in && (d != d0 || lane == lead)) atomicAdd(&hist[d], d == d0 ? (uint32_t)__popc(same) : 1u);
         }
         const int b = SEL_BINS - 4 - 4 * tid;    // thread t has bins b + 3 ... b
         uint4 c;
@@ -122,12 +131,13 @@ __device__ uint32_t select_kth(SelShared &s, int n, uint32_t k, uint32_t &ties, 
             uint32_t bin = b + 3;
             if (above + c.w < k) { above += c.w; bin--; if (above + c.z < k) { above += c.z; bin--; if (above + c.y < k) { above += c.y; bin--; } } }
             s.bin = bin;
-            s.left = k - above;
+            s.left = k - above == hist_of(c, bin & 3u) ? 0xffffffffu : k - above;
         }
         __syncthreads();
         prefix |= s.bin << sh;
         settled |= dm << sh;
         k = s.left;
+        if (k == 0xffffffffu) break;             // all of them
     }
     if constexpr (CL) cg::this_cluster().sync();     // the others have read this CTA's counts
     ties = k;

@@ -37,8 +37,8 @@ int cache_check(const char *who, const NcmbCache *c, CacheDev &d) {
 }
 
 void *cache_scratch(const char *who, size_t bytes, int area) {
-    static void *bases[2] = {nullptr, nullptr};
-    static size_t caps[2] = {0, 0};
+    static void *bases[SCRATCH_AREAS] = {};
+    static size_t caps[SCRATCH_AREAS] = {};
     void *&base = bases[area];
     size_t &cap = caps[area];
     if (bytes <= cap) return base;
@@ -50,7 +50,11 @@ void *cache_scratch(const char *who, size_t bytes, int area) {
     }
     const size_t want = (bytes + (bytes >> 2) + ((size_t)1 << 20)) & ~(size_t)255;
     for (size_t b : {want, (bytes + 255) & ~(size_t)255}) {
-        if (cudaMalloc(&base, b) == cudaSuccess) { cap = b; return base; }
+        if (cudaMalloc(&base, b) == cudaSuccess) {
+            if (area == SCRATCH_DONE) CUDA_CHECK(cudaMemsetAsync(base, 0, b, stream()));
+            cap = b;
+            return base;
+        }
         (void)cudaGetLastError();
         base = nullptr;
     }

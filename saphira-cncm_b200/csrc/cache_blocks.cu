@@ -52,8 +52,8 @@ __global__ void __launch_bounds__(256) k_block_summaries(CacheDev c, int n_new, 
     constexpr int VE = BsVec<KE>::N;
     const int lane = threadIdx.x & 31, kvh = blockIdx.y, b = blockIdx.z;
     const int u = lane & ((1 << upr_log) - 1), tr = lane >> upr_log, R = block / CNT;
-    pdl_launch_dependents();
     pdl_wait();
+    pdl_launch_dependents();
     const int n = cache_len(c, b, n_new) + n_new, f = first ? max(0, first[b]) : 0;
     const bool in = u * VE < c.hd && tr < R;
     const char *kb = c.k + b * c.rs + kvh * c.hs + u * 16;
@@ -134,8 +134,8 @@ __global__ void __launch_bounds__(BP_THREADS) k_block_pick(BlockArgs a) {
     cg::cluster_group cl = cg::this_cluster();
     const int rank = CL ? (int)cl.block_rank() : 0, nc = CL ? (int)cl.num_blocks() : 1;
     const int t = blockIdx.x / nc, kvh = blockIdx.y, b = blockIdx.z, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, hd = a.c.hd;
-    pdl_launch_dependents();
     pdl_wait();
+    pdl_launch_dependents();
     const int cur = (cache_len(a.c, b, a.T) + t) / a.block, n = cur + 1, k = min(n, a.n_sel);
     const int64_t u = ((int64_t)b * a.T + t) * a.c.nkv + kvh;
     int *picks = a.picks + u * a.n_sel;
@@ -250,13 +250,13 @@ __global__ void __launch_bounds__(BP_THREADS) k_block_pick(BlockArgs a) {
         tb += __reduce_add_sync(0xffffffffu, lane < rank ? *cl.map_shared_rank(&share[0], lane) : 0);
         at += __reduce_add_sync(0xffffffffu, lane < rank ? *cl.map_shared_rank(&share[1], lane) : 0);
     }
-    at += min(tb, (int)ties);                    // ties before this warp: tb; picks before it: at
+    at += (int)min((uint32_t)tb, ties);          // ties before this warp: tb; picks before it: at
 #pragma unroll 1
     for (int s = w0; s < w1; s += 32) {
         const bool in = s + lane < w1;
         const uint32_t x = in ? keys[s + lane] : 0, lt = (1u << lane) - 1;
         const uint32_t tm = __ballot_sync(0xffffffffu, in && x == bound);
-        const bool keep = in && (x > bound || (x == bound && tb + __popc(tm & lt) < (int)ties));
+        const bool keep = in && (x > bound || (x == bound && (uint32_t)(tb + __popc(tm & lt)) < ties));
         const uint32_t km = __ballot_sync(0xffffffffu, keep);
         if (keep) picks[at + __popc(km & lt)] = lo + s + lane;
         at += __popc(km);

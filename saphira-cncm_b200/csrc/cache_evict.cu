@@ -42,8 +42,8 @@ __global__ void __launch_bounds__(EV_THREADS) k_cache_evict(EvictArgs a) {
     auto sync = [&] { if constexpr (CL) cl.sync(); else __syncthreads(); };
     const int kvh = blockIdx.y, b = blockIdx.z, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     uint32_t *keys = dyn, *kept = dyn + a.kcap;          // keys, then one bit a slot
-    pdl_launch_dependents();
     pdl_wait();
+    pdl_launch_dependents();
     const int n = cache_len(a.c, b, 0), n2 = min(n, a.budget);
     const int64_t u = (int64_t)b * a.c.nkv + kvh;
     const int seen = a.seen[b], known = a.known ? max(0, min(a.known[b], n)) : 0;
@@ -93,10 +93,14 @@ __global__ void __launch_bounds__(EV_THREADS) k_cache_evict(EvictArgs a) {
         }
         return lead;
     };
-    int mine = 0, all;
+    int all;
+    uint32_t tied = 0;                                   // ties before, of which the lower ones are kept
+    if (ties != 0xffffffffu) {
+        int mine = 0;
 #pragma unroll 1
-    for (int s = w0; s < w1; s += 32) mine += __popc(__ballot_sync(0xffffffffu, s + lane < w1 && key(s + lane - lo) == bound));
-    uint32_t tied = (uint32_t)before(0, mine, all);      // the lower ones are kept
+        for (int s = w0; s < w1; s += 32) mine += __popc(__ballot_sync(0xffffffffu, s + lane < w1 && key(s + lane - lo) == bound));
+        tied = (uint32_t)before(0, mine, all);
+    }
     int freed = 0, beyond = 0, stay = 0;
 #pragma unroll 1
     for (int s = w0; s < w1; s += 32) {
@@ -163,8 +167,8 @@ __global__ void __launch_bounds__(EV_MTHREADS) k_cache_move(EvictArgs a, int ul)
     const int kvh = blockIdx.y, b = blockIdx.z, tid = threadIdx.x;
     const int x = tid & ((1 << ul) - 1), is_v = (tid >> ul) & 1, tok = tid >> (ul + 1), tpc = EV_MTHREADS >> (ul + 1);
     const int64_t u = (int64_t)b * a.c.nkv + kvh;
-    pdl_launch_dependents();
     pdl_wait();
+    pdl_launch_dependents();
     const int pairs = a.pairs[u], p0 = (int)blockIdx.x * tpc * EV_AHEAD + tok;
     if (x * 16 >= a.c.hd * a.es) return;
     const int *from = a.from + u * a.room, *to = a.to + u * a.room;

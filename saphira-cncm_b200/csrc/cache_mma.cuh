@@ -54,6 +54,7 @@ struct CmArgs {
     float c2;                        // scale * log2(e)
     float *part;                     // partial results, one slot a (CTA + unit)
     int2 *range;                     // first and last CTA of each unit
+    int *done;                       // chunks of each unit that are in `part`, zero between calls; null: k_cache_join joins
     float *scores;                   // [row][kv head][M][pitch], or null
     int64_t pitch;
     float *weights;
@@ -99,6 +100,8 @@ __device__ __forceinline__ void cm_put(__nv_bfloat16 *p, float v) { *p = __float
 
 __device__ __forceinline__ bool cm_used(const int *par, int t) { return !par || (par[t] >= -1 && par[t] < t); }
 
+static __device__ __noinline__ unsigned cm_div(unsigned x, unsigned d) { return x / d; }       // one copy of the code
+
 // keys that the queries of an item see
 template <bool BLOCKS> __device__ __forceinline__ int cm_keys(const CmArgs &a, int item) {
     if (!BLOCKS) return cache_len(a.c, a.row0 + item, a.T) + a.T;
@@ -110,58 +113,49 @@ template <bool BLOCKS> __device__ __forceinline__ int cm_keys(const CmArgs &a, i
 // The units (item, kv head, tile) in order, each with its chunks in order, are one sequence, of which every CTA takes an equal
 // run: rows of any lengths keep all SMs busy to the end. A unit is done by one CTA or by consecutive ones; CTA c's
 // partial result of unit u goes to slot c + u (along the sequence one of the two grows by one at a time).
-struct CmPlan { int64_t total, per; };
-__device__ __forceinline__ int64_t cm_block_sum(int64_t v, int64_t *sh) {      // over the CTA; all threads get it
-#pragma unroll
-    for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = v;
-    __syncthreads();
-    v = 0;
-#pragma unroll
-    for (int w = 0; w < CM_WARPS; w++) v += sh[w];
-    return v;
+// (Counts are 32-bit: the host limits the rows of a launch. Nothing here is unrolled: code that runs once is paced by
+// instruction fetches, about 150 cycles for 8 instructions.)
+struct CmPlan { int total, per; };
+template <bool BLOCKS, int KC> __device__ __forceinline__ int cm_chunks(const CmArgs &a, int item) {           // of all units of an item
+    return item < a.items ? ((cm_keys<BLOCKS>(a, item) + KC - 1) / KC) * a.c.nkv * a.tiles : 0;
 }
-template <bool BLOCKS, int KC> __device__ __forceinline__ int64_t cm_chunks(const CmArgs &a, int item) {       // of all units of an item
-    return item < a.items ? (int64_t)((cm_keys<BLOCKS>(a, item) + KC - 1) / KC) * a.c.nkv * a.tiles : 0;
-}
-template <bool BLOCKS, int KC> __device__ CmPlan cm_plan(const CmArgs &a, int ctas, int64_t *sh) {
-    int64_t t = 0;
+template <bool BLOCKS, int KC> __device__ CmPlan cm_plan(const CmArgs &a, int ctas, int *sh) {
+    int t = 0;
+#pragma unroll 1
     for (int i = threadIdx.x; i < a.items; i += CM_THREADS) t += cm_chunks<BLOCKS, KC>(a, i);
+    t = __reduce_add_sync(0xffffffffu, t);
+    if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = t;
+    __syncthreads();
     CmPlan p;
-    p.total = cm_block_sum(t, sh);
-    p.per = ((p.total + ctas - 1) / ctas + CM_WARPS - 1) / CM_WARPS * CM_WARPS;
+    p.total = sh[0] + sh[1] + sh[2] + sh[3];
+    p.per = ((unsigned)(p.total + ctas - 1) / (unsigned)ctas + CM_WARPS - 1) & ~(CM_WARPS - 1);
     return p;
 }
-// the item that holds place x of the sequence, and where that item begins; or, with item >= 0 given, where it begins
-template <bool BLOCKS, int KC> __device__ int cm_find(const CmArgs &a, int64_t x, int item, int64_t &start, int64_t *sh) {
-    __shared__ int found;
-    __shared__ int64_t at;
-    if (a.items == 1) { start = 0; return 0; }
-    int64_t before = 0;
+// the item that holds place x of the sequence, and where that item begins
+template <bool BLOCKS, int KC> __device__ int cm_find(const CmArgs &a, int x, int &start, int *sh) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    int before = 0;
+#pragma unroll 1
     for (int i0 = 0;; i0 += CM_THREADS) {
-        const int i = i0 + threadIdx.x, lane = threadIdx.x & 31;
-        const int64_t mine = cm_chunks<BLOCKS, KC>(a, i);
-        int64_t inc = mine;
-#pragma unroll
+        const int i = i0 + threadIdx.x, mine = cm_chunks<BLOCKS, KC>(a, i);
+        int inc = mine;
+#pragma unroll 1
         for (int o = 1; o < 32; o <<= 1) {
-            const int64_t v = __shfl_up_sync(0xffffffffu, inc, o);
+            const int v = __shfl_up_sync(0xffffffffu, inc, o);
             if (lane >= o) inc += v;
         }
         __syncthreads();
-        if (lane == 31) sh[threadIdx.x >> 5] = inc;
-        if (threadIdx.x == 0) found = -1;
+        if (lane == 31) sh[warp] = inc;
         __syncthreads();
-        int64_t lead = before;
-        for (int w = 0; w < (int)(threadIdx.x >> 5); w++) lead += sh[w];
-        const int64_t from = lead + inc - mine;
-        if (item >= 0 ? i == item : (i < a.items && x >= from && x < from + mine)) { found = i; at = from; }
-        for (int w = 0; w < CM_WARPS; w++) before += sh[w];
-        __syncthreads();
-        if (found >= 0 || i0 + CM_THREADS >= a.items) break;
+        const int v = lane < CM_WARPS ? sh[lane] : 0;
+        const int from = before + __reduce_add_sync(0xffffffffu, lane < warp ? v : 0) + inc - mine;
+        if (x >= from && x < from + mine) { sh[CM_WARPS] = i; sh[CM_WARPS + 1] = from; }
+        before += __reduce_add_sync(0xffffffffu, v);
+        if (x < before || i0 + CM_THREADS >= a.items) break;
     }
-    start = at;
-    return found;
+    __syncthreads();
+    start = sh[CM_WARPS + 1];
+    return sh[CM_WARPS];
 }
 
 // ---- the attention kernel ----
@@ -179,7 +173,7 @@ __global__ void __launch_bounds__(CM_THREADS, CmCfg<KE, QE, HDP, R>::CTAS) k_cac
     constexpr int CM_STAGE = F::CM_STAGE, CM_STAGES = F::CM_STAGES;
     extern __shared__ __align__(128) char smem[];
     char *ring = smem, *qs = smem + F::RING;
-    __shared__ int64_t sh[CM_WARPS];
+    __shared__ int sh[CM_WARPS + 2], joined;
     __shared__ uint32_t node_bits[BLOCKS ? 1 : M][8];       // ancestors of the tile's nodes (from node m0 / G on)
     __shared__ uint32_t used_bits[8];
     __shared__ int spar[BLOCKS ? 1 : NCMB_MAX_NODES];
@@ -187,21 +181,19 @@ __global__ void __launch_bounds__(CM_THREADS, CmCfg<KE, QE, HDP, R>::CTAS) k_cac
     __shared__ float wm[CM_WARPS][M], wl[CM_WARPS][M];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c4 = lane & 3;
     const int hd = a.c.hd, G = a.G;
-    pdl_launch_dependents();
     pdl_wait();
+    pdl_launch_dependents();           // after the wait: one kernel ahead, not a queue of them that takes the SMs' room
     const CmPlan plan = cm_plan<BLOCKS, KC>(a, gridDim.x, sh);
-    int64_t at = (int64_t)blockIdx.x * plan.per;
-    const int64_t end = min(plan.total, at + plan.per);
+    int at = min((int64_t)blockIdx.x * plan.per, (int64_t)plan.total);
+    const int end = min((int64_t)plan.total, (int64_t)at + plan.per);
     if (at >= end) return;
-    int64_t item_at;
-    int item = cm_find<BLOCKS, KC>(a, at, -1, item_at, sh);
+    int item_at = 0, item = a.items == 1 ? 0 : cm_find<BLOCKS, KC>(a, at, item_at, sh);
     char *my = ring + warp * (CM_STAGES * CM_STAGE);
     while (at < end) {
         const int n = cm_keys<BLOCKS>(a, item), nch = (n + KC - 1) / KC;
-        const int64_t into = at - item_at;
-        const int sub = (int)(into / nch), kvh = sub / a.tiles, tile = sub % a.tiles;
-        const int first = (int)(into % nch), stop = (int)min((int64_t)nch, first + (end - at));
-        const int64_t unit = (int64_t)item * a.c.nkv * a.tiles + sub;
+        const int sub = cm_div(at - item_at, nch), kvh = a.tiles == 1 ? sub : cm_div(sub, a.tiles), tile = sub - kvh * a.tiles;
+        const int from = item_at + sub * nch, first = at - from, stop = min(nch, first + (end - at));
+        const int unit = item * a.c.nkv * a.tiles + sub;
         const int m0 = tile * M;
         const int row = a.row0 + (BLOCKS ? item / a.T : item), tok = BLOCKS ? item % a.T : 0, len = BLOCKS ? n : n - a.T;
         const bool tail = !BLOCKS && stop * KC > len;            // this run has keys of the new tokens
@@ -224,14 +216,13 @@ __global__ void __launch_bounds__(CM_THREADS, CmCfg<KE, QE, HDP, R>::CTAS) k_cac
             __syncthreads();
         }
         auto used = [&](int t) { return !par || ((used_bits[t >> 5] >> (t & 31)) & 1u); };
-        // loads run CM_STAGES - 1 chunks ahead of the arithmetic
         const char *kb = a.c.k + row * a.c.rs + kvh * a.c.hs, *vb = a.c.v + row * a.c.rs + kvh * a.c.hs;
         const int lu = lane % UPR, lr = lane / UPR;
         constexpr int RPI = 32 / UPR;                            // rows that the warp's lanes cover at once
         const bool lane_in = lu * 16 < hd * (int)sizeof(KE);
         auto load = [&](int ch, int stage) {
             const uint32_t ks = cm_smem(my + stage * CM_STAGE), vs = ks + CM_STAGE / 2;
-#pragma unroll
+#pragma unroll 2
             for (int i = 0; i < KC / RPI; i++) {
                 const int r = lr + i * RPI, pos = ch * KC + r;
                 bool ok = lane_in && pos < n;
@@ -244,78 +235,66 @@ __global__ void __launch_bounds__(CM_THREADS, CmCfg<KE, QE, HDP, R>::CTAS) k_cac
                 cm_cp16(vs + r * ROW + vu * 16, vb + off, ok);
             }
         };
-        int next = first + warp;
+        // the tile's queries as terms, zero where no query stands, and what each of its nodes sees; under the first loads
+        auto prepare = [&] {
+#pragma unroll 1
+            for (int i = tid; i < M * HDP / 8; i += CM_THREADS) {
+                const int m = i / (HDP / 8), d0 = i % (HDP / 8) * 8, mm = m0 + m;
+                float x[8];
 #pragma unroll
-        for (int s = 0; s < CM_STAGES - 1; s++) {
-            if (next < stop) load(next, s);
-            asm volatile("cp.async.commit_group;" ::: "memory");
-            next += CM_WARPS;
-        }
-        // the tile's queries as terms, zero where no query stands
-        for (int i = tid; i < M * HDP / 8; i += CM_THREADS) {
-            const int m = i / (HDP / 8), d0 = i % (HDP / 8) * 8, mm = m0 + m;
-            float x[8];
+                for (int e = 0; e < 8; e++) x[e] = 0.f;
+                if (mm < a.M && d0 < hd) {
+                    const int t = BLOCKS ? tok : mm / G, h = kvh * G + mm % G;
+                    if (BLOCKS || used(t)) {
+                        const char *p = a.q + ((int64_t)row * a.T + t) * a.ldq + ((int64_t)h * hd + d0) * sizeof(QE);
+                        if (sizeof(QE) == 4) {
+                            *(float4 *)&x[0] = *(const float4 *)p;
+                            *(float4 *)&x[4] = *(const float4 *)(p + 16);
+                        } else {
+                            const uint4 u = *(const uint4 *)p;
+                            const uint32_t uu[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
-            for (int e = 0; e < 8; e++) x[e] = 0.f;
-            if (mm < a.M && d0 < hd) {
-                const int t = BLOCKS ? tok : mm / G, h = kvh * G + mm % G;
-                if (BLOCKS || used(t)) {
-                    const char *p = a.q + ((int64_t)row * a.T + t) * a.ldq + ((int64_t)h * hd + d0) * sizeof(QE);
-                    if (sizeof(QE) == 4) {
-                        *(float4 *)&x[0] = *(const float4 *)p;
-                        *(float4 *)&x[4] = *(const float4 *)(p + 16);
-                    } else {
-                        const uint4 u = *(const uint4 *)p;
-                        const uint32_t uu[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-                        for (int e = 0; e < 4; e++) { const float2 f = cm_unpack(uu[e]); x[2 * e] = f.x; x[2 * e + 1] = f.y; }
+                            for (int e = 0; e < 4; e++) { const float2 f = cm_unpack(uu[e]); x[2 * e] = f.x; x[2 * e + 1] = f.y; }
+                        }
                     }
                 }
-            }
-            if constexpr (F::BF) {
+                if constexpr (F::BF) {
 #pragma unroll
-                for (int k = 0; k < (R8 ? 2 * F::QT : NQ); k++) {
-                    uint32_t u[4] = {0, 0, 0, 0};
+                    for (int k = 0; k < (R8 ? 2 * F::QT : NQ); k++) {
+                        uint32_t u[4] = {0, 0, 0, 0};
 #pragma unroll
-                    for (int e = 0; k < NQ && e < 4; e++) {
-                        u[e] = cm_pack(x[2 * e], x[2 * e + 1]);
-                        const float2 f = cm_unpack(u[e]);
-                        x[2 * e] -= f.x; x[2 * e + 1] -= f.y;
+                        for (int e = 0; k < NQ && e < 4; e++) {
+                            u[e] = cm_pack(x[2 * e], x[2 * e + 1]);
+                            const float2 f = cm_unpack(u[e]);
+                            x[2 * e] -= f.x; x[2 * e + 1] -= f.y;
+                        }
+                        const int r = k * M + m;                     // 8 rows: terms 0 and 1 are one tile of 16, then 2 and zeros
+                        *(uint4 *)(qs + r * ROW + (((d0 / 8) ^ (r & 7)) * 16)) = make_uint4(u[0], u[1], u[2], u[3]);
                     }
-                    const int r = k * M + m;                     // 8 rows: terms 0 and 1 are one tile of 16, then 2 and zeros
-                    *(uint4 *)(qs + r * ROW + (((d0 / 8) ^ (r & 7)) * 16)) = make_uint4(u[0], u[1], u[2], u[3]);
-                }
-            } else {
-#pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    uint32_t hi[4], lo[4];
-#pragma unroll
-                    for (int e = 0; e < 4; e++) cm_tf32(x[4 * h + e], hi[e], lo[e]);
-                    const int u = (d0 / 4 + h) ^ ((m & 1) << 2);
-                    *(uint4 *)(qs + m * ROW + u * 16) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-                    *(uint4 *)(qs + (M + m) * ROW + u * 16) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-                }
-            }
-        }
-        if (tail) {
-            const int t0 = m0 / G, nt = (min(a.M, m0 + M) + G - 1) / G - t0;       // nodes of this tile
-            for (int i = tid; i < nt; i += CM_THREADS) {
-                const int t = t0 + i;
-                uint32_t b[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-                if (!par) {
-#pragma unroll
-                    for (int w = 0; w < 8; w++) b[w] = t >= 32 * w + 31 ? 0xffffffffu : t >= 32 * w ? (2u << (t - 32 * w)) - 1 : 0u;
                 } else {
-                    for (int x = t; x >= 0 && used(x); x = spar[x]) {
 #pragma unroll
-                        for (int w = 0; w < 8; w++) if ((x >> 5) == w) b[w] |= 1u << (x & 31);
+                    for (int h = 0; h < 2; h++) {
+                        uint32_t hi[4], lo[4];
+#pragma unroll
+                        for (int e = 0; e < 4; e++) cm_tf32(x[4 * h + e], hi[e], lo[e]);
+                        const int u = (d0 / 4 + h) ^ ((m & 1) << 2);
+                        *(uint4 *)(qs + m * ROW + u * 16) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                        *(uint4 *)(qs + (M + m) * ROW + u * 16) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
                     }
                 }
-#pragma unroll
-                for (int w = 0; w < 8; w++) node_bits[i][w] = b[w];
             }
-        }
-        __syncthreads();
+            if (tail) {
+                const int t0 = m0 / G, nt = (min(a.M, m0 + M) + G - 1) / G - t0;   // nodes of this tile
+                for (int i = tid; i < nt; i += CM_THREADS) {
+                    const int t = t0 + i;
+#pragma unroll 1
+                    for (int w = 0; w < 8; w++) node_bits[i][w] = par ? 0u : t >= 32 * w + 31 ? 0xffffffffu : t >= 32 * w ? (2u << (t - 32 * w)) - 1 : 0u;
+#pragma unroll 1
+                    for (int x = par ? t : -1; x >= 0 && used(x); x = spar[x]) node_bits[i][x >> 5] |= 1u << (x & 31);
+                }
+            }
+            __syncthreads();
+        };
         float O[HDP / 8][2 * NH], mx[NH], ls[NH];                // context, maximum and sum of the lane's rows
 #pragma unroll
         for (int j = 0; j < HDP / 8; j++)
@@ -324,16 +303,19 @@ __global__ void __launch_bounds__(CM_THREADS, CmCfg<KE, QE, HDP, R>::CTAS) k_cac
 #pragma unroll
         for (int hh = 0; hh < NH; hh++) { mx[hh] = -INFINITY; ls[hh] = 0.f; }
         int stage = 0;
-        for (int ch = first + warp; ch < stop; ch += CM_WARPS) {
-            asm volatile("cp.async.wait_group %0;" ::"n"(CM_STAGES - 2) : "memory");
-            __syncwarp();
-            {
-                int s = stage + CM_STAGES - 1;
-                if (s >= CM_STAGES) s -= CM_STAGES;
-                if (next < stop) load(next, s);
-                asm volatile("cp.async.commit_group;" ::: "memory");
-                next += CM_WARPS;
+        // loads run CM_STAGES - 1 chunks ahead of the arithmetic
+        for (int ch = first + warp - (CM_STAGES - 1) * CM_WARPS, ahead = 0; ch < stop; ch += CM_WARPS) {
+            const int next = ch + (CM_STAGES - 1) * CM_WARPS;
+            __syncwarp();                                        // the stage it goes to has been read
+            if (next < stop) load(next, ahead);
+            asm volatile("cp.async.commit_group;" ::: "memory");
+            if (++ahead == CM_STAGES) ahead = 0;
+            if (ch < first) {
+                if (next == first + warp) prepare();
+                continue;
             }
+            asm volatile("cp.async.wait_group %0;" ::"n"(CM_STAGES - 1) : "memory");
+            __syncwarp();
             const char *kt = my + stage * CM_STAGE, *vt = kt + CM_STAGE / 2;
             const bool masked = (ch + 1) * KC > len;
             float S[NT][4];
@@ -343,7 +325,7 @@ __global__ void __launch_bounds__(CM_THREADS, CmCfg<KE, QE, HDP, R>::CTAS) k_cac
                 float L[NT][4];                                  // 16 rows: the smaller terms
 #pragma unroll
                 for (int j = 0; j < NT; j++) L[j][0] = L[j][1] = L[j][2] = L[j][3] = 0.f;
-#pragma unroll
+#pragma unroll 1
                 for (int kp = 0; kp < HDP / 32; kp++) {          // two k-steps at a time
                     uint32_t kf[NT][4];
 #pragma unroll
@@ -369,7 +351,7 @@ __global__ void __launch_bounds__(CM_THREADS, CmCfg<KE, QE, HDP, R>::CTAS) k_cac
                 float L[NT][4];
 #pragma unroll
                 for (int j = 0; j < NT; j++) L[j][0] = L[j][1] = L[j][2] = L[j][3] = 0.f;
-#pragma unroll
+#pragma unroll 1
                 for (int i = 0; i < HDP / 16; i++) {             // two k-steps at a time
                     const int u0 = (4 * i + c4) ^ ((g & 1) << 2);       // rows g and g + 8: the same parity
                     uint32_t ah[2][4], al[2][4];
@@ -472,6 +454,7 @@ __global__ void __launch_bounds__(CM_THREADS, CmCfg<KE, QE, HDP, R>::CTAS) k_cac
                     for (int e = 0; e < 2 * NH; e++) O[j][e] *= al[e >> 1];
 #pragma unroll
                 for (int jj = 0; jj < NT; jj++)
+#pragma unroll 1
                     for (int r = 0; r < 8; r++) {
                         const int src = (lane & ~3) | (r >> 1), kr = 8 * jj + r;
                         float p[NH];
@@ -601,10 +584,11 @@ __global__ void __launch_bounds__(CM_THREADS, CmCfg<KE, QE, HDP, R>::CTAS) k_cac
         }
         __syncthreads();
         const bool whole = first == 0 && stop == nch;
+        float *slot = a.part + ((int64_t)blockIdx.x + unit) * F::SLOT;
         if (tid == 0 && first == 0) a.range[unit].x = blockIdx.x;
         if (tid == 0 && stop == nch) a.range[unit].y = blockIdx.x;
-        float *slot = a.part + ((int64_t)blockIdx.x + unit) * F::SLOT;
-        for (int m = tid; m < M; m += CM_THREADS) {
+        if (tid < M) {
+            const int m = tid;
             float top = wm[0][m], l = 0.f;
 #pragma unroll
             for (int w = 1; w < CM_WARPS; w++) top = fmaxf(top, wm[w][m]);
@@ -615,21 +599,72 @@ __global__ void __launch_bounds__(CM_THREADS, CmCfg<KE, QE, HDP, R>::CTAS) k_cac
             wl[0][m] = l;                                        // read by the owner of this m alone until the barrier
         }
         __syncthreads();
-        for (int i = tid; i < M * HDP; i += CM_THREADS) {
-            const int m = i / HDP, d = i % HDP, mm = m0 + m;
-            if (mm >= a.M) break;
+        const int nm = min(M, a.M - m0);                         // rows that hold a query
+        auto write = [&](int m, int d, float4 o, float l) {      // a result, four dims of a row
+            const int mm = m0 + m, t = BLOCKS ? tok : mm / G, h = kvh * G + mm % G;
+            const float r = l > 0.f && (BLOCKS || used(t)) ? 1.f / l : 0.f;
+            QE *p = (QE *)(a.out + ((int64_t)row * a.T + t) * a.ldo) + (int64_t)h * hd + d;
+            if constexpr (sizeof(QE) == 4) *(float4 *)p = make_float4(o.x * r, o.y * r, o.z * r, o.w * r);
+            else *(uint2 *)p = make_uint2(cm_pack(o.x * r, o.y * r), cm_pack(o.z * r, o.w * r));
+        };
+#pragma unroll 1
+        for (int i = tid; i < nm * (HDP / 4); i += CM_THREADS) {
+            const int m = i / (HDP / 4), d = i % (HDP / 4) * 4;
             if (d >= hd) continue;
-            float o = 0.f;
+            float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-            for (int w = 0; w < CM_WARPS; w++) o += ctx_sh[(w * M + m) * HDP + d];
-            if (!whole) { slot[2 * M + i] = o; continue; }
-            const int t = BLOCKS ? tok : mm / G, h = kvh * G + mm % G;
-            const float l = wl[0][m];
-            const bool ok = l > 0.f && (BLOCKS || used(t));
-            cm_put((QE *)(a.out + ((int64_t)row * a.T + t) * a.ldo) + (int64_t)h * hd + d, ok ? o / l : 0.f);
+            for (int w = 0; w < CM_WARPS; w++) {
+                const float4 x = *(const float4 *)(ctx_sh + (w * M + m) * HDP + d);
+                o.x += x.x; o.y += x.y; o.z += x.z; o.w += x.w;
+            }
+            if (whole) write(m, d, o, wl[0][m]);
+            else *(float4 *)(slot + 2 * M + m * HDP + d) = o;
+        }
+        if (a.done && !whole) {
+            // the CTA that brings the unit's last chunks joins its parts
+            __threadfence();
+            __syncthreads();
+            if (tid == 0) joined = atomicAdd(&a.done[unit], stop - first) + stop - first;
+            __syncthreads();
+            if (joined == nch) {
+                if (tid == 0) a.done[unit] = 0;                  // for the next call
+                __threadfence();
+                const int c0 = from / plan.per, parts = (from + nch - 1) / plan.per - c0 + 1;
+                const float *p0 = a.part + ((int64_t)c0 + unit) * F::SLOT;
+                constexpr int D4 = HDP / 4;
+                int ways = 1;                                    // threads that share the parts of four dims of a row
+                while (ways * 2 * nm * D4 <= CM_THREADS) ways *= 2;
+                const int way = tid & (ways - 1);
+#pragma unroll 1
+                for (int i0 = 0; i0 < nm * D4; i0 += CM_THREADS / ways) {
+                    const int i = i0 + tid / ways, m = min(i / D4, nm - 1), d = i % D4 * 4;
+                    float top = -INFINITY, l = 0.f;
+                    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+                    auto add = [&](float x, float xl, float4 p) {
+                        const float t = fmaxf(top, x), base = t == -INFINITY ? 0.f : t, fo = cm_exp2(top - base), fp = cm_exp2(x - base);
+                        top = t;
+                        l = l * fo + xl * fp;
+                        o.x = o.x * fo + p.x * fp; o.y = o.y * fo + p.y * fp; o.z = o.z * fo + p.z * fp; o.w = o.w * fo + p.w * fp;
+                    };
+#pragma unroll 4
+                    for (int c = way; c < parts; c += ways) {
+                        const float *s = p0 + (int64_t)c * F::SLOT;
+                        add(__ldcg(s + m), __ldcg(s + M + m), __ldcg((const float4 *)(s + 2 * M + m * HDP + d)));
+                    }
+#pragma unroll 1
+                    for (int w = 1; w < ways; w <<= 1) {
+                        const float x = __shfl_xor_sync(0xffffffffu, top, w), xl = __shfl_xor_sync(0xffffffffu, l, w);
+                        float4 p;
+                        p.x = __shfl_xor_sync(0xffffffffu, o.x, w); p.y = __shfl_xor_sync(0xffffffffu, o.y, w);
+                        p.z = __shfl_xor_sync(0xffffffffu, o.z, w); p.w = __shfl_xor_sync(0xffffffffu, o.w, w);
+                        add(x, xl, p);
+                    }
+                    if (way == 0 && i < nm * D4 && d < hd) write(m, d, o, l);
+                }
+            }
         }
         at += stop - first;
-        if (at == item_at + (int64_t)nch * a.c.nkv * a.tiles) { item_at = at; item++; }
+        if (at == item_at + nch * a.c.nkv * a.tiles) { item_at = at; item++; }
     }
 }
 
@@ -646,8 +681,8 @@ __global__ void __launch_bounds__(CM_THREADS) k_cache_join(const __grid_constant
     __shared__ float gm[GROUPS], gl[GROUPS];
     __shared__ float4 go[GROUPS][D4];
     const int tid = threadIdx.x, G = a.G, hd = a.c.hd;
-    pdl_launch_dependents();
     pdl_wait();
+    pdl_launch_dependents();           // after the wait: one kernel ahead, not a queue of them that takes the SMs' room
     const bool join = (int)blockIdx.x < joins;
     const int per_item = a.c.nkv * a.tiles, rows = split ? 1 : GROUPS, steps = M / rows;      // rows a CTA, CTAs a unit
     int item, sub, key0 = 0;
@@ -749,6 +784,9 @@ __global__ void __launch_bounds__(CM_THREADS) k_cache_join(const __grid_constant
 }
 
 // ---- launches ----
+#ifndef CM_FUSED
+#define CM_FUSED 24
+#endif
 template <class KE, class QE, int HDP, int R, bool BLOCKS>
 int cm_run_as(const char *who, CmArgs a, int max_keys) {
     using F = CmCfg<KE, QE, HDP, R>;
@@ -759,32 +797,39 @@ int cm_run_as(const char *who, CmArgs a, int max_keys) {
         CUDA_CHECK(cudaFuncSetAttribute(k_cache_attention<KE, QE, HDP, R, BLOCKS>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
         set = true;
     }
-    // rows of a launch: as many as leave the scores some GB at most
+    // rows of a launch: as many as leave the scores some GB at most, and the count of chunks in 31 bits
     const int rows = a.c.rows, per_row = BLOCKS ? a.T : 1;
-    int step = rows;
+    const int64_t row_units = (int64_t)per_row * a.c.nkv * a.tiles;
+    const int64_t row_chunks = row_units * cdiv(BLOCKS ? (int64_t)a.n_sel << a.block_log : a.c.cap, F::KC);
+    int64_t most = 0x70000000 / row_chunks;
     if (a.weights) {
         a.pitch = cdiv((int64_t)a.c.cap, CM_WKEYS) * CM_WKEYS;
-        const int64_t row_bytes = (int64_t)a.c.nkv * a.M * a.pitch * 4;
-        step = (int)std::max<int64_t>(1, std::min<int64_t>(rows, ((int64_t)2 << 30) / row_bytes));
+        most = std::min(most, std::max<int64_t>(1, ((int64_t)2 << 30) / (a.c.nkv * a.M * a.pitch * 4)));
     }
-    const int64_t units = (int64_t)step * per_row * a.c.nkv * a.tiles;
-    const int64_t spans = a.weights ? cdiv(a.pitch, CM_WKEYS) * step * a.c.nkv : 0;
+    if (most < 1) return cache_refuse(who, "%lld pieces of keys in a row", (long long)row_chunks);
+    const int step = (int)std::min<int64_t>(rows, most);
+    const int64_t units = step * row_units, spans = a.weights ? cdiv(a.pitch, CM_WKEYS) * step * a.c.nkv : 0;
     if (units * F::M + spans > 0x7fffffff) return cache_refuse(who, "%lld query tiles", (long long)units);
-    const int64_t est = units * cdiv(max_keys, F::KC);
-    const int ctas = (int)std::max<int64_t>(1, std::min<int64_t>(F::CTAS * ctx().sm_count, cdiv(est, CM_WARPS)));
-    const size_t ranges = ((size_t)units * 8 + 255) & ~(size_t)255, part = (size_t)(units + ctas) * F::SLOT * 4 + ranges, sc = a.weights ? (size_t)step * a.c.nkv * a.M * a.pitch * 4 : 0;
-    char *scratch = (char *)cache_scratch(who, part + sc);
+    const int ctas = (int)std::max<int64_t>(1, std::min<int64_t>(F::CTAS * ctx().sm_count, cdiv(units * cdiv(max_keys, F::KC), CM_WARPS)));
+    const size_t ranges = ((size_t)units * 8 + 255) & ~(size_t)255, part = (size_t)(units + ctas) * F::SLOT * 4;
+    const size_t sc = a.weights ? (size_t)step * a.c.nkv * a.M * a.pitch * 4 : 0;
+    char *scratch = (char *)cache_scratch(who, sc + ranges + part);
     if (!scratch) return -1;
     a.scores = a.weights ? (float *)scratch : nullptr;
     a.range = (int2 *)(scratch + sc);
     a.part = (float *)(scratch + sc + ranges);
-    const int split = ctas > 4 * units;                          // many parts a unit
+    // Few parts a unit: the CTA that finishes it joins them. Many: a kernel of its own, which has a CTA for each row of a
+    // unit; it also adds up weights.
+    const bool fused = !a.weights && ctas <= CM_FUSED * units;
+    if (fused && !(a.done = (int *)cache_scratch(who, (size_t)units * 4, SCRATCH_DONE))) return -1;
+    const int split = ctas > 4 * units;
     for (int r = 0; r < rows; r += step) {
         const int nr = std::min(step, rows - r);
         a.row0 = r;
         a.items = nr * per_row;
-        const int64_t u = (int64_t)a.items * a.c.nkv * a.tiles, joins = u * (F::M / (split ? 1 : CM_THREADS / (HDP / 4)));
         LAUNCH_PDL((k_cache_attention<KE, QE, HDP, R, BLOCKS>), ctas, CM_THREADS, smem, a);
+        if (fused) continue;
+        const int64_t joins = nr * row_units * (F::M / (split ? 1 : CM_THREADS / (HDP / 4)));
         LAUNCH_PDL((k_cache_join<KE, QE, HDP, R, BLOCKS>), (unsigned)(joins + spans / step * nr), CM_THREADS, 0, a, (int)joins, split);
     }
     return 0;

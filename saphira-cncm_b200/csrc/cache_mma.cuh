@@ -165,7 +165,9 @@ template <bool BLOCKS, int KC> __device__ int cm_find(const CmArgs &a, int x, in
 // the four from 4 (lane % 4) on, which are its elements of two k-steps; of a P V tile the keys 2 (lane % 4) and the next, and
 // of each 32 dims the four from 4 (lane / 4) on, which are its column of four tiles. Where a dim stands in a k-step and where a
 // column in a tile is free as long as both operands, or all who read the result, agree.
-template <class KE, class QE, int HDP, int R, bool BLOCKS>
+// CL: a cluster of CTAs does a unit, each an equal run of its chunks, and their results meet in distributed shared memory: for
+// calls that are all latency. Else the units' chunks are dealt out as above.
+template <class KE, class QE, int HDP, int R, bool BLOCKS, bool CL>
 __global__ void __launch_bounds__(CM_THREADS, CmCfg<KE, QE, HDP, R>::CTAS) k_cache_attention(const __grid_constant__ CmArgs a) {
     using F = CmCfg<KE, QE, HDP, R>;
     constexpr int KC = F::KC, NT = F::NT, NQ = F::NQ, NP = F::NP, ROW = F::ROW, UPR = F::UPR, M = F::M, NH = F::NH;
@@ -178,21 +180,33 @@ __global__ void __launch_bounds__(CM_THREADS, CmCfg<KE, QE, HDP, R>::CTAS) k_cac
     __shared__ uint32_t used_bits[8];
     __shared__ int spar[BLOCKS ? 1 : NCMB_MAX_NODES];
     __shared__ int spicks[BLOCKS ? 1024 : 1];
-    __shared__ float wm[CM_WARPS][M], wl[CM_WARPS][M];
+    __shared__ float wm[CM_WARPS][M], wl[CM_WARPS][M], cmax[M];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c4 = lane & 3;
     const int hd = a.c.hd, G = a.G;
     pdl_wait();
     pdl_launch_dependents();           // after the wait: one kernel ahead, not a queue of them that takes the SMs' room
-    const CmPlan plan = cm_plan<BLOCKS, KC>(a, gridDim.x, sh);
+    namespace cg = cooperative_groups;
+    cg::cluster_group cl = cg::this_cluster();
+    const int rank = CL ? (int)cl.block_rank() : 0, nc = CL ? (int)cl.num_blocks() : 1;
+    CmPlan plan = {};
+    if constexpr (!CL) plan = cm_plan<BLOCKS, KC>(a, gridDim.x, sh);
     int at = min((int64_t)blockIdx.x * plan.per, (int64_t)plan.total);
     const int end = min((int64_t)plan.total, (int64_t)at + plan.per);
-    if (at >= end) return;
-    int item_at = 0, item = a.items == 1 ? 0 : cm_find<BLOCKS, KC>(a, at, item_at, sh);
+    if (!CL && at >= end) return;
+    int item_at = 0, item = CL ? blockIdx.z : 0;
+    if constexpr (!CL) { if (a.items > 1) item = cm_find<BLOCKS, KC>(a, at, item_at, sh); }
     char *my = ring + warp * (CM_STAGES * CM_STAGE);
-    while (at < end) {
+    do {
         const int n = cm_keys<BLOCKS>(a, item), nch = (n + KC - 1) / KC;
-        const int sub = cm_div(at - item_at, nch), kvh = a.tiles == 1 ? sub : cm_div(sub, a.tiles), tile = sub - kvh * a.tiles;
-        const int from = item_at + sub * nch, first = at - from, stop = min(nch, first + (end - at));
+        int sub, kvh, tile, first, stop;
+        if constexpr (CL) {
+            const int share = ((nch + nc - 1) / nc + CM_WARPS - 1) & ~(CM_WARPS - 1);
+            kvh = blockIdx.y; tile = a.tiles == 1 ? 0 : blockIdx.x / nc; sub = kvh * a.tiles + tile;
+            first = min(nch, rank * share); stop = min(nch, first + share);
+        } else {
+            sub = cm_div(at - item_at, nch); kvh = a.tiles == 1 ? sub : cm_div(sub, a.tiles); tile = sub - kvh * a.tiles;
+            first = at - item_at - sub * nch; stop = min(nch, first + (end - at));
+        }
         const int unit = item * a.c.nkv * a.tiles + sub;
         const int m0 = tile * M;
         const int row = a.row0 + (BLOCKS ? item / a.T : item), tok = BLOCKS ? item % a.T : 0, len = BLOCKS ? n : n - a.T;
@@ -584,9 +598,11 @@ __global__ void __launch_bounds__(CM_THREADS, CmCfg<KE, QE, HDP, R>::CTAS) k_cac
         }
         __syncthreads();
         const bool whole = first == 0 && stop == nch;
-        float *slot = a.part + ((int64_t)blockIdx.x + unit) * F::SLOT;
-        if (tid == 0 && first == 0) a.range[unit].x = blockIdx.x;
-        if (tid == 0 && stop == nch) a.range[unit].y = blockIdx.x;
+        float *slot = CL ? nullptr : a.part + ((int64_t)blockIdx.x + unit) * F::SLOT;
+        if constexpr (!CL) {
+            if (tid == 0 && first == 0) a.range[unit].x = blockIdx.x;
+            if (tid == 0 && stop == nch) a.range[unit].y = blockIdx.x;
+        }
         if (tid < M) {
             const int m = tid;
             float top = wm[0][m], l = 0.f;
@@ -594,11 +610,11 @@ __global__ void __launch_bounds__(CM_THREADS, CmCfg<KE, QE, HDP, R>::CTAS) k_cac
             for (int w = 1; w < CM_WARPS; w++) top = fmaxf(top, wm[w][m]);
 #pragma unroll
             for (int w = 0; w < CM_WARPS; w++) l += wm[w][m] == -INFINITY ? 0.f : wl[w][m] * cm_exp2(wm[w][m] - top);
-            slot[m] = top;
-            slot[M + m] = l;
+            if constexpr (CL) cmax[m] = top;
+            else { slot[m] = top; slot[M + m] = l; }
             wl[0][m] = l;                                        // read by the owner of this m alone until the barrier
         }
-        __syncthreads();
+        if constexpr (!CL) __syncthreads();
         const int nm = min(M, a.M - m0);                         // rows that hold a query
         auto write = [&](int m, int d, float4 o, float l) {      // a result, four dims of a row
             const int mm = m0 + m, t = BLOCKS ? tok : mm / G, h = kvh * G + mm % G;
@@ -607,8 +623,53 @@ __global__ void __launch_bounds__(CM_THREADS, CmCfg<KE, QE, HDP, R>::CTAS) k_cac
             if constexpr (sizeof(QE) == 4) *(float4 *)p = make_float4(o.x * r, o.y * r, o.z * r, o.w * r);
             else *(uint2 *)p = make_uint2(cm_pack(o.x * r, o.y * r), cm_pack(o.z * r, o.w * r));
         };
+        if constexpr (CL) {
+            // a thread has the same four dims of a row in every CTA; row m's factors: every CTA's maximum against the cluster's
+            cl.sync();
 #pragma unroll 1
-        for (int i = tid; i < nm * (HDP / 4); i += CM_THREADS) {
+            for (int i = rank * CM_THREADS + tid; i < nm * (HDP / 4); i += nc * CM_THREADS) {
+                const int m = i / (HDP / 4), d = i % (HDP / 4) * 4;
+                float top = -INFINITY, l = 0.f;
+                float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
+                for (int r = 0; r < nc; r++) top = fmaxf(top, *cl.map_shared_rank(&cmax[m], r));
+                const float base = top == -INFINITY ? 0.f : top;
+#pragma unroll 1
+                for (int r = 0; r < nc; r++) {
+                    const float f = cm_exp2(*cl.map_shared_rank(&cmax[m], r) - base);
+                    const float *cs = cl.map_shared_rank(ctx_sh, r) + m * HDP + d;
+                    l = fmaf(*cl.map_shared_rank(&wl[0][m], r), f, l);
+#pragma unroll
+                    for (int w = 0; w < CM_WARPS; w++) {
+                        const float4 x = *(const float4 *)(cs + w * M * HDP);
+                        o.x = fmaf(x.x, f, o.x); o.y = fmaf(x.y, f, o.y); o.z = fmaf(x.z, f, o.z); o.w = fmaf(x.w, f, o.w);
+                    }
+                }
+                if (d < hd) write(m, d, o, l);
+            }
+            if (!BLOCKS && a.weights) {                          // one tile a kv head: this CTA's slots, from its own scores
+                if (tid < M) {
+                    float top = -INFINITY, l = 0.f;
+                    for (int r = 0; r < nc; r++) top = fmaxf(top, *cl.map_shared_rank(&cmax[tid], r));
+                    const float base = top == -INFINITY ? 0.f : top;
+                    for (int r = 0; r < nc; r++) l = fmaf(*cl.map_shared_rank(&wl[0][tid], r), cm_exp2(*cl.map_shared_rank(&cmax[tid], r) - base), l);
+                    wm[0][tid] = tid < a.M && l > 0.f && used(tid / G) ? top + log2f(l) : INFINITY;
+                }
+                __syncthreads();
+                const float *sp = a.scores + ((int64_t)item * a.c.nkv + kvh) * a.M * a.pitch;
+                float *wp = a.weights + ((int64_t)row * a.c.nkv + kvh) * a.c.cap;
+#pragma unroll 1
+                for (int key = first * KC + tid; key < min(n, stop * KC); key += CM_THREADS) {
+                    float w = 0.f;
+#pragma unroll 4
+                    for (int m = 0; m < a.M; m++) w += cm_exp2(sp[m * a.pitch + key] - wm[0][m]);
+                    wp[key] = key < len ? wp[key] + w : w;
+                }
+            }
+            cl.sync();                                           // the others have read this CTA's results
+        }
+#pragma unroll 1
+        for (int i = tid; !CL && i < nm * (HDP / 4); i += CM_THREADS) {
             const int m = i / (HDP / 4), d = i % (HDP / 4) * 4;
             if (d >= hd) continue;
             float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -620,7 +681,7 @@ __global__ void __launch_bounds__(CM_THREADS, CmCfg<KE, QE, HDP, R>::CTAS) k_cac
             if (whole) write(m, d, o, wl[0][m]);
             else *(float4 *)(slot + 2 * M + m * HDP + d) = o;
         }
-        if (a.done && !whole) {
+        if (!CL && a.done && !whole) {
             // the CTA that brings the unit's last chunks joins its parts
             __threadfence();
             __syncthreads();
@@ -629,7 +690,7 @@ __global__ void __launch_bounds__(CM_THREADS, CmCfg<KE, QE, HDP, R>::CTAS) k_cac
             if (joined == nch) {
                 if (tid == 0) a.done[unit] = 0;                  // for the next call
                 __threadfence();
-                const int c0 = from / plan.per, parts = (from + nch - 1) / plan.per - c0 + 1;
+                const int from = at - first, c0 = from / plan.per, parts = (from + nch - 1) / plan.per - c0 + 1;
                 const float *p0 = a.part + ((int64_t)c0 + unit) * F::SLOT;
                 constexpr int D4 = HDP / 4;
                 int ways = 1;                                    // threads that share the parts of four dims of a row
@@ -663,9 +724,10 @@ __global__ void __launch_bounds__(CM_THREADS, CmCfg<KE, QE, HDP, R>::CTAS) k_cac
                 }
             }
         }
+        if (CL) break;
         at += stop - first;
         if (at == item_at + nch * a.c.nkv * a.tiles) { item_at = at; item++; }
-    }
+    } while (at < end);
 }
 
 // ---- units that several CTAs share are joined; weights are added up ----
@@ -784,6 +846,10 @@ __global__ void __launch_bounds__(CM_THREADS) k_cache_join(const __grid_constant
 }
 
 // ---- launches ----
+#ifndef CM_MAXC
+#define CM_MAXC 8
+#define CM_ROUNDS 8
+#endif
 #ifndef CM_FUSED
 #define CM_FUSED 24
 #endif
@@ -794,7 +860,8 @@ int cm_run_as(const char *who, CmArgs a, int max_keys) {
     const int smem = F::RING + F::QBYTES;
     static bool set = false;
     if (!set) {
-        CUDA_CHECK(cudaFuncSetAttribute(k_cache_attention<KE, QE, HDP, R, BLOCKS>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+        CUDA_CHECK(cudaFuncSetAttribute(k_cache_attention<KE, QE, HDP, R, BLOCKS, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+        CUDA_CHECK(cudaFuncSetAttribute(k_cache_attention<KE, QE, HDP, R, BLOCKS, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
         set = true;
     }
     // rows of a launch: as many as leave the scores some GB at most, and the count of chunks in 31 bits
@@ -810,6 +877,15 @@ int cm_run_as(const char *who, CmArgs a, int max_keys) {
     const int step = (int)std::min<int64_t>(rows, most);
     const int64_t units = step * row_units, spans = a.weights ? cdiv(a.pitch, CM_WKEYS) * step * a.c.nkv : 0;
     if (units * F::M + spans > 0x7fffffff) return cache_refuse(who, "%lld query tiles", (long long)units);
+    // Clusters: where one, of as many CTAs as give a warp two chunks, does a unit in a few rounds and all of them fit the GPU
+    int nc = 1;
+    while (nc < CM_MAXC && nc * 2 * CM_WARPS <= cdiv(max_keys, F::KC) && units * nc * 2 <= F::CTAS * ctx().sm_count) nc *= 2;
+    if (step == rows && units * nc <= F::CTAS * ctx().sm_count && cdiv(max_keys, F::KC) <= (int64_t)CM_ROUNDS * nc * CM_WARPS && (!a.weights || a.tiles == 1)) {
+        if (a.weights && !(a.scores = (float *)cache_scratch(who, (size_t)rows * a.c.nkv * a.M * a.pitch * 4))) return -1;
+        a.items = rows * per_row;
+        cache_launch(k_cache_attention<KE, QE, HDP, R, BLOCKS, true>, dim3(nc * a.tiles, a.c.nkv, a.items), CM_THREADS, smem, nc, a);
+        return 0;
+    }
     const int ctas = (int)std::max<int64_t>(1, std::min<int64_t>(F::CTAS * ctx().sm_count, cdiv(units * cdiv(max_keys, F::KC), CM_WARPS)));
     const size_t ranges = ((size_t)units * 8 + 255) & ~(size_t)255, part = (size_t)(units + ctas) * F::SLOT * 4;
     const size_t sc = a.weights ? (size_t)step * a.c.nkv * a.M * a.pitch * 4 : 0;
@@ -827,7 +903,7 @@ int cm_run_as(const char *who, CmArgs a, int max_keys) {
         const int nr = std::min(step, rows - r);
         a.row0 = r;
         a.items = nr * per_row;
-        LAUNCH_PDL((k_cache_attention<KE, QE, HDP, R, BLOCKS>), ctas, CM_THREADS, smem, a);
+        LAUNCH_PDL((k_cache_attention<KE, QE, HDP, R, BLOCKS, false>), ctas, CM_THREADS, smem, a);
         if (fused) continue;
         const int64_t joins = nr * row_units * (F::M / (split ? 1 : CM_THREADS / (HDP / 4)));
         LAUNCH_PDL((k_cache_join<KE, QE, HDP, R, BLOCKS>), (unsigned)(joins + spans / step * nr), CM_THREADS, 0, a, (int)joins, split);

@@ -3,7 +3,7 @@
 //
 // For query head h of kv head h / G and node t:  s_j = scale q.k_j over the slots j that t sees, p_j = exp(s_j - max s) /
 // sum, out = sum p_j v_j; weights_j (+)= sum over the G heads and the T nodes of p_j.
-#include "cache_mma.cuh"
+#include "cache_tc.cuh"
 
 #include <stdarg.h>
 
@@ -62,6 +62,20 @@ void *cache_scratch(const char *who, size_t bytes, int area) {
     return nullptr;
 }
 
+namespace {
+
+template <class KE, class QE>
+int run_attention(const char *who, const CmArgs &a, int max_keys) {
+    static const int dev = getenv("NCM_CT") ? atoi(getenv("NCM_CT")) : 1;
+    if (a.c.hd <= 64) {
+        if (dev && a.M > 16) return ct_run_as<KE, QE, 64>(who, a, max_keys);
+        return a.M <= 8 ? cm_run_as<KE, QE, 64, 8, false>(who, a, max_keys) : cm_run_as<KE, QE, 64, 16, false>(who, a, max_keys);
+    }
+    if constexpr (sizeof(KE) == 2) { if (dev && a.M > 16) return ct_run_as<KE, QE, 128>(who, a, max_keys); }
+    return a.M <= 8 ? cm_run_as<KE, QE, 128, 8, false>(who, a, max_keys) : cm_run_as<KE, QE, 128, 16, false>(who, a, max_keys);
+}
+
+} // namespace
 } // namespace ncmb
 
 using namespace ncmb;
@@ -84,7 +98,7 @@ extern "C" int ncmb_cache_attention(const NcmbCache *c, const void *q, int64_t l
     a.H = n_head; a.G = n_head / c->n_kv; a.T = T; a.M = T * a.G; a.parents = parents; a.weights = weights;
     a.c2 = (scale == 0.f ? 1.0f / sqrtf((float)c->hd) : scale) * 1.44269504f;
     if (max_len <= 0 || max_len > c->capacity - T) max_len = c->capacity - T;
-    if (c->type == NCMB_F32) return cm_run<float, float, false>(who, a, max_len + T);
-    if (act_type == NCMB_F32) return cm_run<__nv_bfloat16, float, false>(who, a, max_len + T);
-    return cm_run<__nv_bfloat16, __nv_bfloat16, false>(who, a, max_len + T);
+    if (c->type == NCMB_F32) return run_attention<float, float>(who, a, max_len + T);
+    if (act_type == NCMB_F32) return run_attention<__nv_bfloat16, float>(who, a, max_len + T);
+    return run_attention<__nv_bfloat16, __nv_bfloat16>(who, a, max_len + T);
 }

@@ -910,10 +910,5 @@ int cm_run_as(const char *who, CmArgs a, int max_keys) {
     }
     return 0;
 }
-template <class KE, class QE, bool BLOCKS>
-int cm_run(const char *who, const CmArgs &a, int max_keys) {
-    if (a.c.hd <= 64) return a.M <= 8 ? cm_run_as<KE, QE, 64, 8, BLOCKS>(who, a, max_keys) : cm_run_as<KE, QE, 64, 16, BLOCKS>(who, a, max_keys);
-    return a.M <= 8 ? cm_run_as<KE, QE, 128, 8, BLOCKS>(who, a, max_keys) : cm_run_as<KE, QE, 128, 16, BLOCKS>(who, a, max_keys);
-}
 
 } // namespace ncmb

@@ -62,6 +62,25 @@ void *cache_scratch(const char *who, size_t bytes, int area) {
     return nullptr;
 }
 
+int ct_map(const char *who, const CacheDev &c, const char *p, int kt, CUtensorMap &m) {
+    using Encode = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *, const cuuint32_t *,
+                                const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+    static Encode encode = nullptr;
+    if (!encode) {
+        cudaDriverEntryPointQueryResult found;
+        void *f = nullptr;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &found) != cudaSuccess || !f) return cache_refuse(who, "the driver has no tensor maps");
+        encode = (Encode)f;
+    }
+    // a dim of one element has a stride that is not used: any valid one
+    const cuuint64_t dims[4] = {(cuuint64_t)c.hd, (cuuint64_t)c.cap, (cuuint64_t)c.nkv, (cuuint64_t)c.rows};
+    const cuuint64_t strides[3] = {(cuuint64_t)(c.cap > 1 ? c.ts : 256), (cuuint64_t)(c.nkv > 1 ? c.hs : 256), (cuuint64_t)(c.rows > 1 ? c.rs : 256)};
+    const cuuint32_t box[4] = {64, (cuuint32_t)kt, 1, 1}, one[4] = {1, 1, 1, 1};
+    const CUresult r = encode(&m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<char *>(p), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? 0 : cache_refuse(who, "tensor map: %d (strides of 2^40 bytes or more?)", (int)r);
+}
+
 namespace {
 
 template <class KE, class QE>

@@ -1,15 +1,17 @@
 // Attention of many query rows (trees, runs of tokens, several heads a kv head) to cached keys on tcgen05 tiles: the wide
 // variant of cache_mma.cuh, for ncmb_cache_attention.
 //
-// A CTA has 128 query rows of a kv head and walks tiles of 64 keys: S = Q K^T into tensor memory, softmax with a running
-// maximum by 256 threads (two a row, 32 keys each), O = P V of the tile into tensor memory, added to the running result
-// in registers in fp32. Operands are bf16 terms, as in cache_mma.cuh: a query is 3 (bf16 activations: 1), a probability 3
-// (2), a bf16 key or value 1, an fp32 one 3, of whose nine products the six largest are taken (2^-24 and more). Roles:
-// warps 0 - 7 softmax (they also turn the queries into terms and write the results), warp 8 issues the MMAs, the others load
-// keys and values -- bf16 by cp.async, fp32 through registers, where the terms are formed.
+// A CTA has 128 query rows of a kv head and walks tiles of 128 keys: S = Q K^T into tensor memory, softmax with a running
+// maximum by 256 threads (two a row, 64 keys each), the probabilities back into tensor memory as the next product's operand,
+// O = P V of the tile into tensor memory, added to the running result in registers in fp32. Operands are bf16 terms, as in
+// cache_mma.cuh: a query is 3 (bf16 activations: 1), a probability 3 (2), a bf16 key or value 1, an fp32 one 3, of whose nine
+// products the six largest are taken (2^-24 and more). Roles: warps 0 - 7 softmax (they also turn the queries into terms and
+// write the results), warp 8 issues the MMAs, the others load: keys of the next tile, values of this one, in turn through
+// one ring -- bf16 by cp.async, fp32 through registers, where the terms are formed.
 //
-// Bound by operand fetch from shared memory: an MMA of 128 x 64 x 16 reads 6 KB in about 48 cycles where its arithmetic
-// takes 16; with one product that is below the time the keys take from HBM at 128 rows and head dim 128.
+// Tiles are 128 keys wide because MMAs are paced by operand fetch: 128 x 64 x 16 takes about 100 cycles, as long as
+// 128 x 128 x 16, and probabilities in shared memory would be fetched again by every MMA (64-key tiles with probabilities
+// in shared memory: 2.5 times the time of this one).
 #pragma once
 #include "cache_mma.cuh"
 #include "tc_common.cuh"
@@ -18,14 +20,15 @@ namespace ncmb {
 
 template <class KE, class QE, int HDP_> struct CtCfg {
     static constexpr bool BF = sizeof(KE) == 2;
-    static constexpr int HDP = HDP_, ATOMS = HDP / 64, M = 128, KT = 64;
+    static constexpr int HDP = HDP_, ATOMS = HDP / 64, M = 128, KT = 128;
     static constexpr int NQ = sizeof(QE) == 4 ? 3 : 1, NP = sizeof(QE) == 4 ? 3 : 2, NK = BF ? 1 : 3;
     static constexpr int KATOM = KT * 128, QATOM = M * 128;          // bytes of 64 dims of the keys, of the queries
-    static constexpr int STAGE = 2 * NK * ATOMS * KATOM, QB = NQ * ATOMS * QATOM, PB = NP * QATOM;
-    static constexpr int FIT = (221 * 1024 - QB - PB) / STAGE, NST = FIT < 6 ? FIT : 6;
+    static constexpr int STAGE = NK * ATOMS * KATOM, QB = NQ * ATOMS * QATOM;        // a stage: a tile's keys or its values
+    static constexpr int FIT = (217 * 1024 - QB) / STAGE, NST = FIT < 8 ? FIT : 8;
     static constexpr int PW = BF ? 3 : 7, SW = 8, THREADS = 32 * (SW + 1 + PW);      // whole warps a scheduler: registers
-    static constexpr int SMEM = QB + PB + NST * STAGE + 1024;
-    static constexpr int TMEM = HDP == 64 ? 256 : 256;               // columns: two score tiles of 64, the tile's context
+    static constexpr int SMEM = QB + NST * STAGE + 1024;
+    // columns of tensor memory: probabilities (two to a column), context, one or two score tiles
+    static constexpr int PCOL = 0, OCOL = NP * 64, SCOL = OCOL + HDP, NSB = SCOL + 256 <= 512 ? 2 : 1;
 };
 
 __host__ __device__ constexpr uint32_t umma_idesc_bf16(int M, int N) {
@@ -37,21 +40,38 @@ struct CtWait {
         if (!dead && !mbar_wait(bar, parity, err, code)) dead = true;
     }
 };
-__device__ __forceinline__ bool ct_try(uint32_t bar, uint32_t parity) {
-    uint32_t ok;
-    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
-    return ok != 0;
+// the same MMA with A in tensor memory (16-bit elements, two to a column)
+__device__ __forceinline__ void umma_f16_ta(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+                 ::"r"(tmem_d), "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&w)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+                 ::"r"(taddr), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7]) : "memory");
+}
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+                 "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];\n\ttcgen05.wait::ld.sync.aligned;"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+                   "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+                 : "r"(taddr) : "memory");
+}
+__device__ __forceinline__ void ct_tma(uint32_t dst, const CUtensorMap *m, int d, int slot, int head, int row, uint32_t bar) {
+    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
+                 ::"r"(dst), "l"(m), "r"(d), "r"(slot), "r"(head), "r"(row), "r"(bar) : "memory");
 }
 __device__ __forceinline__ void ct_fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
 template <class KE, class QE, int HDP>
-__global__ void __launch_bounds__(CtCfg<KE, QE, HDP>::THREADS, 1) k_cache_attention_tc(const __grid_constant__ CmArgs a, int *err) {
+__global__ void __launch_bounds__(CtCfg<KE, QE, HDP>::THREADS, 1) k_cache_attention_tc(const __grid_constant__ CmArgs a, const __grid_constant__ CUtensorMap mk,
+                                                                                        const __grid_constant__ CUtensorMap mv, int *err) {
     using F = CtCfg<KE, QE, HDP>;
     constexpr int M = F::M, KT = F::KT, NST = F::NST, ATOMS = F::ATOMS, SLOT = M * (HDP + 2);
     extern __shared__ char smem_raw[];
     char *smem = (char *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-    char *qs = smem, *ps = qs + F::QB, *ring = ps + F::PB;
-    __shared__ uint64_t bars[2 * 8 + 8];
+    char *qs = smem, *ring = qs + F::QB;
+    __shared__ uint64_t bars[2 * 8 + 8];                             // stages full, stages free, see below
     __shared__ uint32_t tmem_at;
     __shared__ int plan[4];                                          // total, per, item, where it begins
     __shared__ float xm[2][2][M], xl[2][M];
@@ -60,13 +80,14 @@ __global__ void __launch_bounds__(CtCfg<KE, QE, HDP>::THREADS, 1) k_cache_attent
     auto full = [&](int s) { return cm_smem(&bars[s]); };
     auto empty = [&](int s) { return cm_smem(&bars[8 + s]); };
     const uint32_t bar_q = cm_smem(&bars[16]), bar_s = cm_smem(&bars[17]), bar_p = cm_smem(&bars[19]), bar_pv = cm_smem(&bars[20]);
+    const uint32_t bar_sf = cm_smem(&bars[21]);                      // queries ready, scores ready (2), probabilities ready, context ready, scores read
     pdl_wait();
     pdl_launch_dependents();
     __shared__ int s_abort;
     if (tid == 0) {
         s_abort = *(volatile int *)err;                              // a wait ran out earlier: nothing more is started
         for (int s = 0; s < NST; s++) { mbar_init(full(s), F::PW); mbar_init(empty(s), 1); }
-        mbar_init(bar_q, F::SW); mbar_init(bar_s, 1); mbar_init(bar_s + 8, 1); mbar_init(bar_p, F::SW); mbar_init(bar_pv, 1);
+        mbar_init(bar_q, F::SW); mbar_init(bar_s, 1); mbar_init(bar_s + 8, 1); mbar_init(bar_p, F::SW); mbar_init(bar_pv, 1); mbar_init(bar_sf, F::SW);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 0) {
@@ -93,7 +114,7 @@ __global__ void __launch_bounds__(CtCfg<KE, QE, HDP>::THREADS, 1) k_cache_attent
     __syncthreads();
     if (s_abort || (int64_t)blockIdx.x * plan[1] >= plan[0]) return;
     if (warp == F::SW) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(cm_smem(&tmem_at)), "r"(F::TMEM) : "memory");
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(cm_smem(&tmem_at)), "r"(512) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
     tc_fence_before();
@@ -118,13 +139,14 @@ __global__ void __launch_bounds__(CtCfg<KE, QE, HDP>::THREADS, 1) k_cache_attent
         return true;
     };
     Unit u;
-    uint32_t it = 0, un = 0;                                         // tiles and units so far
+    uint32_t it = 0, un = 0, items = 0;                              // tiles, units, stages (two a tile) so far
 
     if (warp < F::SW) {
-        // ================= softmax: row r of the tile, keys 32 hf ... of a key tile, half hf of the dims =================
+        // ================= softmax: row r of the tile, keys 64 hf ... of a key tile, half hf of the dims =================
         const int r = (warp & 3) * 32 + lane, hf = warp >> 2;
         const uint32_t tl = tmem + ((uint32_t)(warp & 3) << 21);     // this warp's 32 lanes of tensor memory
         constexpr int HC = HDP / 2;
+        const float c2 = fabsf(a.c2);                                // a negative scale goes into the queries
         auto group_sync = [] { asm volatile("bar.sync 1, %0;" ::"n"(F::SW * 32) : "memory"); };
         while (next_unit(u)) {
             const int *par = a.parents ? a.parents + (int64_t)u.row * a.T : nullptr;
@@ -150,6 +172,10 @@ __global__ void __launch_bounds__(CtCfg<KE, QE, HDP>::THREADS, 1) k_cache_attent
                         }
                     }
                 }
+                if (a.c2 < 0.f) {
+#pragma unroll
+                    for (int e = 0; e < 8; e++) x[e] = -x[e];
+                }
 #pragma unroll
                 for (int k = 0; k < F::NQ; k++) {
                     uint32_t w[4];
@@ -164,6 +190,8 @@ __global__ void __launch_bounds__(CtCfg<KE, QE, HDP>::THREADS, 1) k_cache_attent
             }
             const int mm = u.m0 + r, node = min(mm, a.M - 1) / G;
             const bool row_used = mm < a.M && cm_used(par, node);
+            const bool busy = u.m0 + (warp & 3) * 32 < a.M;          // the warp has rows: else it only keeps the others' time
+            const int tiles = u.stop - u.first;
             if (u.stop * KT > u.len && hf == 0) {                    // what the row's node sees of the new tokens
 #pragma unroll 1
                 for (int w = 0; w < 8; w++) node_bits[r][w] = par ? 0u : node >= 32 * w + 31 ? 0xffffffffu : node >= 32 * w ? (2u << (node - 32 * w)) - 1 : 0u;
@@ -180,84 +208,110 @@ __global__ void __launch_bounds__(CtCfg<KE, QE, HDP>::THREADS, 1) k_cache_attent
             auto add_context = [&]() {                               // of the tile before
                 wait(bar_pv, (it - 1) & 1u, 41);
                 tc_fence_after();
-                if (skip) { skip = false; return; }
+                if (skip || !busy) { skip = false; return; }
 #pragma unroll
                 for (int x = 0; x < HC; x += 32) {
                     uint32_t o[32];
-                    tmem_ld32(tl + 128u + (uint32_t)(hf * HC + x), o);
+                    tmem_ld32(tl + (uint32_t)(F::OCOL + hf * HC + x), o);
 #pragma unroll
                     for (int d = 0; d < 32; d++) O[x + d] = fmaf(O[x + d], al_prev, __uint_as_float(o[d]));
                 }
             };
             for (int t = u.first; t < u.stop; t++, it++) {
-                wait(bar_s + 8 * (it & 1u), (it >> 1) & 1u, 42);
+                const uint32_t sb = F::NSB == 2 ? it & 1u : 0u, scol = tl + (uint32_t)F::SCOL + sb * 128u + (uint32_t)hf * 64u;
+                wait(bar_s + 8 * sb, F::NSB == 2 ? (it >> 1) & 1u : it & 1u, 42);
                 tc_fence_after();
-                uint32_t sr[32];
-                tmem_ld32(tl + (it & 1u) * 64u + (uint32_t)hf * 32u, sr);
-                float s[32];
-                const int p0 = t * KT + 32 * hf;
+                const int p0 = t * KT + 64 * hf;
                 const bool masked = (t + 1) * KT > u.len;
-                uint32_t see = 0xffffffffu;
-                if (masked) {
-                    // bit j: the row sees slot p0 + j
-                    const int rel = p0 - u.len;                      // node of the first slot
+                auto sees = [&](int from) {                          // bit j: the row sees slot from + j
+                    uint32_t see = 0xffffffffu;
+                    const int rel = from - u.len;                    // node of the first slot
                     if (rel > -32) {
                         uint32_t lo = 0, hi = 0;
-                        const int w = rel < 0 ? -1 : rel >> 5, sh = rel & 31;
+                        const int w = rel < 0 ? -1 : rel >> 5;
                         if (w >= 0 && w < 8) lo = node_bits[r][w];
                         if (w < 0) lo = 0xffffffffu;                 // slots of the cache
                         if (w + 1 < 8) hi = node_bits[r][w + 1];
-                        see = __funnelshift_r(lo, hi, sh);
+                        see = __funnelshift_r(lo, hi, rel & 31);
                     }
-                    if (u.n - p0 < 32) see &= u.n > p0 ? (1u << (u.n - p0)) - 1 : 0u;
-                }
+                    if (u.n - from < 32) see &= u.n > from ? (1u << (u.n - from)) - 1 : 0u;
+                    return see;
+                };
+                // the maximum, then -- the scores are read again rather than kept: registers -- exponentials
                 float top = -INFINITY;
+                if (busy) {
 #pragma unroll
-                for (int j = 0; j < 32; j++) {
-                    s[j] = __uint_as_float(sr[j]) * a.c2;
-                    if (!((see >> j) & 1u)) s[j] = -INFINITY;
-                    top = fmaxf(top, s[j]);
-                }
-                if (a.scores && mm < a.M) {
-                    float *sp = a.scores + (((int64_t)u.item * a.c.nkv + u.kvh) * a.M + mm) * a.pitch + p0;
+                    for (int c = 0; c < 2; c++) {
+                        uint32_t sr[32];
+                        tmem_ld32(scol + 32u * c, sr);
+                        if (masked) {
+                            const uint32_t see = sees(p0 + 32 * c);
 #pragma unroll
-                    for (int j = 0; j < 32; j += 4) *(float4 *)(sp + j) = make_float4(s[j], s[j + 1], s[j + 2], s[j + 3]);
+                            for (int j = 0; j < 32; j++) if (!((see >> j) & 1u)) sr[j] = 0xff800000u;
+                        }
+#pragma unroll
+                        for (int j = 0; j < 32; j++) top = fmaxf(top, __uint_as_float(sr[j]));
+                        if (a.scores && mm < a.M) {
+                            float *sp = a.scores + (((int64_t)u.item * a.c.nkv + u.kvh) * a.M + mm) * a.pitch + p0 + 32 * c;
+#pragma unroll
+                            for (int j = 0; j < 32; j += 4)
+                                *(float4 *)(sp + j) = make_float4(__uint_as_float(sr[j]) * c2, __uint_as_float(sr[j + 1]) * c2,
+                                                                  __uint_as_float(sr[j + 2]) * c2, __uint_as_float(sr[j + 3]) * c2);
+                        }
+                    }
                 }
                 xm[it & 1u][hf][r] = top;
                 group_sync();
-                top = fmaxf(fmaxf(mx, top), xm[it & 1u][hf ^ 1][r]);
+                top = fmaxf(mx, fmaxf(top, xm[it & 1u][hf ^ 1][r]) * c2);
                 const float base = top == -INFINITY ? 0.f : top, al = cm_exp2(mx - base);
                 mx = top;
-                float sum = 0.f;
-#pragma unroll
-                for (int j = 0; j < 32; j++) { s[j] = cm_exp2(s[j] - base); sum += s[j]; }
-                l = l * al + sum;
                 if (t > u.first) add_context();                      // also: the MMAs that read the last probabilities are done
                 al_prev = al;
-                // probabilities as terms: 4 units of 8 keys
+                if (busy) {
+                    float sum = 0.f;
 #pragma unroll
-                for (int x = 0; x < 4; x++)
+                    for (int c = 0; c < 4; c++) {                    // 16 keys at a time
+                        uint32_t sr[16];
+                        tmem_ld16(scol + 16u * c, sr);
+                        if (masked) {
+                            const uint32_t see = sees(p0 + 16 * c);
 #pragma unroll
-                    for (int k = 0; k < F::NP; k++) {
-                        uint32_t w[4];
-#pragma unroll
-                        for (int e = 0; e < 4; e++) {
-                            float *q = &s[8 * x + 2 * e];
-                            w[e] = cm_pack(q[0], q[1]);
-                            const float2 f = cm_unpack(w[e]);
-                            q[0] -= f.x; q[1] -= f.y;
+                            for (int j = 0; j < 16; j++) if (!((see >> j) & 1u)) sr[j] = 0xff800000u;
                         }
-                        *(uint4 *)(ps + k * F::QATOM + r * 128 + (((4 * hf + x) ^ (r & 7)) * 16)) = make_uint4(w[0], w[1], w[2], w[3]);
+                        float s[16];
+#pragma unroll
+                        for (int j = 0; j < 16; j++) { s[j] = cm_exp2(fmaf(__uint_as_float(sr[j]), c2, -base)); sum += s[j]; }
+#pragma unroll
+                        for (int k = 0; k < F::NP; k++) {
+                            uint32_t w[8];
+#pragma unroll
+                            for (int e = 0; e < 8; e++) {
+                                w[e] = cm_pack(s[2 * e], s[2 * e + 1]);
+                                if (k + 1 < F::NP) {
+                                    const float2 f = cm_unpack(w[e]);
+                                    s[2 * e] -= f.x; s[2 * e + 1] -= f.y;
+                                }
+                            }
+                            tmem_st8(tl + (uint32_t)(F::PCOL + k * 64 + hf * 32 + c * 8), w);
+                        }
                     }
+                    l = l * al + sum;
+                    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                }
+                if (F::NSB == 1) {
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(bar_sf);
+                }
                 if (masked) {
                     // An infinity or NaN among values that not every row sees must not be multiplied by zero: such a tile's context is
                     // formed here, one key at a time, before the stage is given to the MMAs (whose result is then left out).
-                    const int st = it % NST;
-                    wait(full(st), (it / NST) & 1u, 43);
-                    const char *vt = ring + st * F::STAGE + F::STAGE / 2;
+                    const uint32_t at_v = items + (t + 1 < u.stop ? 2 + 2 * (t - u.first) : 2 * tiles - 1), st = at_v % NST;
+                    wait(full(st), (at_v / NST) & 1u, 43);
+                    const char *vt = ring + st * F::STAGE;
                     bool odd = false;
 #pragma unroll 1
-                    for (int i = tid; i < F::NK * ATOMS * F::KATOM / 4; i += F::SW * 32) {
+                    for (int i = tid; i < F::STAGE / 4; i += F::SW * 32) {
                         const uint32_t w = ((const uint32_t *)vt)[i];
                         odd |= (w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u;
                     }
@@ -265,32 +319,49 @@ __global__ void __launch_bounds__(CtCfg<KE, QE, HDP>::THREADS, 1) k_cache_attent
                     asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbarrier.cta.red.or.pred q, 1, %2, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
                                  : "=r"(any) : "r"((uint32_t)odd), "n"(F::SW * 32) : "memory");
                     if (any) {
+                        tc_fence_before();
+                        group_sync();                                // the other half's probabilities are in tensor memory
+                        tc_fence_after();
+                        if (busy) {
 #pragma unroll
-                        for (int d = 0; d < HC; d++) O[d] *= al;
+                            for (int d = 0; d < HC; d++) O[d] *= al;
 #pragma unroll 1
-                        for (int j = 0; j < KT; j++) {
-                            float p = 0.f;
+                            for (int j = 0; j < KT; j += 2) {
+                                float p2[2] = {0.f, 0.f};
 #pragma unroll
-                            for (int k = F::NP - 1; k >= 0; k--) p += (float)*(const __nv_bfloat16 *)(ps + k * F::QATOM + r * 128 + (((j / 8) ^ (r & 7)) * 16) + (j & 7) * 2);
-                            if (p == 0.f) continue;
+                                for (int k = F::NP - 1; k >= 0; k--) {
+                                    uint32_t w;
+                                    asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];\n\ttcgen05.wait::ld.sync.aligned;"
+                                                 : "=r"(w) : "r"(tl + (uint32_t)(F::PCOL + k * 64 + j / 2)) : "memory");
+                                    const float2 f = cm_unpack(w);
+                                    p2[0] += f.x; p2[1] += f.y;
+                                }
+#pragma unroll 1
+                                for (int e = 0; e < 2; e++) {
+                                    const float p = e ? p2[1] : p2[0];
+                                    if (p == 0.f) continue;
+                                    const int key = j + e;
 #pragma unroll
-                            for (int d = 0; d < HC; d++) {
-                                const int dd = hf * HC + d;
-                                float v = 0.f;
+                                    for (int d = 0; d < HC; d++) {
+                                        const int dd = hf * HC + d;
+                                        float v = 0.f;
 #pragma unroll
-                                for (int k = F::NK - 1; k >= 0; k--)
-                                    v += (float)*(const __nv_bfloat16 *)(vt + (k * ATOMS + dd / 64) * F::KATOM + j * 128 + ((((dd & 63) / 8) ^ (j & 7)) * 16) + (dd & 7) * 2);
-                                O[d] = fmaf(p, v, O[d]);
+                                        for (int k = F::NK - 1; k >= 0; k--)
+                                            v += (float)*(const __nv_bfloat16 *)(vt + (k * ATOMS + dd / 64) * F::KATOM + key * 128 + ((((dd & 63) / 8) ^ (key & 7)) * 16) + (dd & 7) * 2);
+                                        O[d] = fmaf(p, v, O[d]);
+                                    }
+                                }
+                                __syncwarp();
                             }
                         }
                         skip = true;
                     }
                 }
                 tc_fence_before();
-                ct_fence_async();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(bar_p);
             }
+            items += 2 * tiles;
             add_context();
             xl[hf][r] = l;
             if (hf == 0 && r == 0) {
@@ -321,29 +392,33 @@ __global__ void __launch_bounds__(CtCfg<KE, QE, HDP>::THREADS, 1) k_cache_attent
     } else if (warp == F::SW) {
         // ================= MMAs =================
         if (lane == 0) {
-            constexpr uint32_t ids = umma_idesc_bf16(M, KT), idv = umma_idesc_bf16(M, 64) | (1u << 16);      // values: MN-major
-            const uint64_t qd = umma_desc_sw128(cm_smem(qs)), pd = umma_desc_sw128(cm_smem(ps)), rd = umma_desc_sw128(cm_smem(ring));
+            constexpr uint32_t ids = umma_idesc_bf16(M, KT), idv = umma_idesc_bf16(M, HDP) | (1u << 16);     // values: MN-major
             constexpr uint64_t QA = F::QATOM / 16, KA = F::KATOM / 16, ST = F::STAGE / 16;
+            const uint64_t qd = umma_desc_sw128(cm_smem(qs)), rd = umma_desc_sw128(cm_smem(ring));
+            const uint64_t rv = (rd & ~((uint64_t)0x3fff << 16)) | KA << 16;         // from 64 dims of the values to the next
             auto scores = [&](uint32_t i) {
-                const uint32_t st = i % NST;
-                wait(full(st), (i / NST) & 1u, 44);
+                const uint32_t st = items % NST, sb = F::NSB == 2 ? i & 1u : 0u;
+                wait(full(st), (items / NST) & 1u, 44);
                 tc_fence_after();
                 uint32_t acc = 0;
                 const uint64_t kd = rd + st * ST;
-                auto product = [&](int qk, int kk) {                 // one term of the queries by one of the keys
-#pragma unroll
-                    for (int x = 0; x < ATOMS; x++)
-#pragma unroll
-                        for (int k = 0; k < 4; k++) {
-                            umma_f16(tmem + (i & 1u) * 64u, qd + (qk * ATOMS + x) * QA + k * 2, kd + (kk * ATOMS + x) * KA + k * 2, ids, acc);
-                            acc = 1;
-                        }
-                };
 #pragma unroll 1
-                for (int sum = F::NQ + F::NK - 2 < 2 ? F::NQ + F::NK - 2 : 2; sum >= 0; sum--)       // small ones first
+                for (int sum = F::NQ + F::NK - 2 < 2 ? F::NQ + F::NK - 2 : 2; sum >= 0; sum--)       // small products first
 #pragma unroll 1
-                    for (int qk = 0; qk <= sum; qk++) if (qk < F::NQ && sum - qk < F::NK) product(qk, sum - qk);
-                umma_commit(bar_s + 8 * (i & 1u));
+                    for (int qk = 0; qk <= sum; qk++) {              // one term of the queries by one of the keys
+                        const int kk = sum - qk;
+                        if (qk >= F::NQ || kk >= F::NK) continue;
+#pragma unroll
+                        for (int x = 0; x < ATOMS; x++)
+#pragma unroll
+                            for (int k = 0; k < 4; k++) {
+                                umma_f16(tmem + F::SCOL + sb * 128u, qd + (qk * ATOMS + x) * QA + k * 2, kd + (kk * ATOMS + x) * KA + k * 2, ids, acc);
+                                acc = 1;
+                            }
+                    }
+                umma_commit(bar_s + 8 * sb);
+                umma_commit(empty(st));
+                items++;
             };
             while (next_unit(u)) {
                 wait(bar_q, un & 1u, 45);
@@ -353,11 +428,15 @@ __global__ void __launch_bounds__(CtCfg<KE, QE, HDP>::THREADS, 1) k_cache_attent
                 scores(it);
 #pragma unroll 1
                 for (int t = 0; t < tiles; t++, it++) {
-                    if (t + 1 < tiles) scores(it + 1);
+                    if (t + 1 < tiles) {
+                        if (F::NSB == 1) { wait(bar_sf, it & 1u, 48); tc_fence_after(); }
+                        scores(it + 1);
+                    }
+                    const uint32_t st = items % NST;
+                    wait(full(st), (items / NST) & 1u, 49);
                     wait(bar_p, it & 1u, 46);
                     tc_fence_after();
-                    const uint32_t st = it % NST;
-                    const uint64_t vd = rd + st * ST + ST / 2;
+                    const uint64_t vd = rv + st * ST;
                     uint32_t acc = 0;
 #pragma unroll 1
                     for (int sum = F::NP + F::NK - 2 < 2 ? F::NP + F::NK - 2 : 2; sum >= 0; sum--)
@@ -365,134 +444,127 @@ __global__ void __launch_bounds__(CtCfg<KE, QE, HDP>::THREADS, 1) k_cache_attent
                         for (int pk = 0; pk <= sum; pk++) {
                             if (pk >= F::NP || sum - pk >= F::NK) continue;
 #pragma unroll
-                            for (int k = 0; k < 4; k++) {
-#pragma unroll
-                                for (int x = 0; x < ATOMS; x++)
-                                    umma_f16(tmem + 128u + 64u * x, pd + pk * QA + k * 2, vd + ((sum - pk) * ATOMS + x) * KA + k * 128, idv, acc);
+                            for (int k = 0; k < KT / 16; k++) {
+                                umma_f16_ta(tmem + F::OCOL, tmem + F::PCOL + pk * 64 + k * 8, vd + (sum - pk) * ATOMS * KA + k * 128, idv, acc);
                                 acc = 1;
                             }
                         }
                     umma_commit(bar_pv);
                     umma_commit(empty(st));
+                    items++;
                 }
             }
         }
     } else {
         // ================= loads =================
         const int pt = tid - (F::SW + 1) * 32;
-        constexpr int NT = F::PW * 32, LAG = NST - 1;
+        constexpr int NT = F::PW * 32;
         while (next_unit(u)) {
             const int *par = a.parents ? a.parents + (int64_t)u.row * a.T : nullptr;
             const char *kb = a.c.k + u.row * a.c.rs + u.kvh * a.c.hs, *vb = a.c.v + u.row * a.c.rs + u.kvh * a.c.hs;
             auto there = [&](int pos) { return pos < u.n && (pos < u.len || cm_used(par, pos - u.len)); };
+            // stage s of the unit: keys of tile 0, then in turn keys of the next tile and values of this one
+            const int count = 2 * (u.stop - u.first);
+            auto tile_of = [&](int s) { return s == 0 ? 0 : s == count - 1 ? (s - 1) / 2 : (s & 1) ? (s + 1) / 2 : (s - 2) / 2; };
+            auto is_v = [&](int s) { return s == count - 1 || (s > 0 && !(s & 1)); };
+            constexpr int UPR = HDP / 8, RPI = NT / UPR, N = (KT + RPI - 1) / RPI;       // units of 8 dims of a key, keys a step
+            const int lu = pt % UPR, lr = pt / UPR;
+            const bool in = lu * 8 < hd;
             if constexpr (F::BF) {
-                constexpr int UPR = HDP / 8, RPI = NT / UPR;         // 16-byte units of a key, keys a step
-                const int lu = pt % UPR, lr = pt / UPR;
-                const bool in = lu * 8 < hd;
-                uint32_t done = it;                                  // tiles handed over
-                auto hand_over = [&](uint32_t to) {
+                // Whole tiles of cached tokens by TMA, a box of 64 dims by 128 keys at a time. The last ones, which end inside the
+                // tile or have places without a token, by cp.async, which leaves zeros there.
+#pragma unroll 1
+                for (int s = 0; s < count; s++, it++) {
+                    const uint32_t st = it % NST;
+                    wait(empty(st), ((it / NST) & 1u) ^ 1u, 47);
+                    const int t = u.first + tile_of(s);
+                    const uint32_t to = cm_smem(ring + st * F::STAGE);
+                    if ((t + 1) * KT <= u.len) {
+                        if (pt == 0) {
+                            mbar_expect_tx(full(st), (uint32_t)F::STAGE);
+                            for (int x = 0; x < ATOMS; x++) ct_tma(to + x * F::KATOM, is_v(s) ? &mv : &mk, 64 * x, t * KT, u.kvh, u.row, full(st));
+                        } else if (lane == 0) mbar_arrive(full(st));
+                        continue;
+                    }
+                    const uint32_t mine = to + (lu / 8) * F::KATOM;
+                    const char *from = (is_v(s) ? vb : kb) + lu * 16;
+#pragma unroll 1
+                    for (int r = lr; r < KT; r += RPI) {
+                        const int pos = t * KT + r;
+                        const bool ok = in && there(pos);
+                        cm_cp16(mine + r * 128 + (((lu & 7) ^ (r & 7)) * 16), ok ? from + pos * a.c.ts : kb, ok);
+                    }
+                    asm volatile("cp.async.wait_all;" ::: "memory");
                     ct_fence_async();
                     __syncwarp();
-                    if (lane == 0) for (uint32_t i = done; i < to; i++) mbar_arrive(full(i % NST));
-                    done = to;
-                };
-#pragma unroll 1
-                for (int t = u.first; t < u.stop; t++) {
-                    const uint32_t st = it % NST, free = ((it / NST) & 1u) ^ 1u;
-                    if (!__all_sync(0xffffffffu, ct_try(empty(st), free))) {
-                        // the stage is freed by MMAs that may be waiting for what is under way
-                        asm volatile("cp.async.wait_group 0;" ::: "memory");
-                        hand_over(it);
-                        wait(empty(st), free, 47);
-                    }
-                    const uint32_t ks = cm_smem(ring + st * F::STAGE) + (lu / 8) * F::KATOM;
-                    const bool tail = (t + 1) * KT > u.len;
-#pragma unroll 4
-                    for (int i = 0; i < (KT + RPI - 1) / RPI; i++) {
-                        const int r = lr + i * RPI, pos = t * KT + r;
-                        if (r >= KT) break;
-                        const bool ok = in && (tail ? there(pos) : true);
-                        const int64_t off = ok ? pos * a.c.ts + lu * 16 : 0;
-                        const uint32_t to = r * 128 + (((lu & 7) ^ (r & 7)) * 16);
-                        cm_cp16(ks + to, kb + off, ok);
-                        cm_cp16(ks + F::STAGE / 2 + to, vb + off, ok);
-                    }
-                    asm volatile("cp.async.commit_group;" ::: "memory");
-                    it++;
-                    if (it - done > (uint32_t)LAG) {                 // all but the last LAG tiles are there
-                        asm volatile("cp.async.wait_group %0;" ::"n"(LAG) : "memory");
-                        hand_over(it - LAG);
-                    }
+                    if (lane == 0) mbar_arrive(full(st));
                 }
-                asm volatile("cp.async.wait_group 0;" ::: "memory");
-                hand_over(it);
             } else {
-                // A thread has 8 dims of KT / RPI keys: two loads each for keys and values, of the next tile while this one is turned
-                // into terms.
-                constexpr int UPR = HDP / 8, RPI = NT / UPR, N = (KT + RPI - 1) / RPI;
-                const int lu = pt % UPR, lr = pt / UPR;
-                const bool in = lu * 8 < hd;
-                float4 x[4 * N];
-                auto fetch = [&](int t) {
+                // the next stage's elements are on their way while this one's are turned into terms
+                float4 x[2 * N];
+                auto fetch = [&](int s) {
+                    const int t = u.first + tile_of(s);
+                    const char *from = (is_v(s) ? vb : kb) + lu * 32;
                     const bool tail = (t + 1) * KT > u.len;
 #pragma unroll
                     for (int i = 0; i < N; i++) {
                         const int pos = t * KT + lr + i * RPI;
                         const bool ok = in && lr + i * RPI < KT && (tail ? there(pos) : true);
-                        const int64_t off = pos * a.c.ts + lu * 32;
                         const float4 z = make_float4(0.f, 0.f, 0.f, 0.f);
-                        x[4 * i] = ok ? *(const float4 *)(kb + off) : z; x[4 * i + 1] = ok ? *(const float4 *)(kb + off + 16) : z;
-                        x[4 * i + 2] = ok ? *(const float4 *)(vb + off) : z; x[4 * i + 3] = ok ? *(const float4 *)(vb + off + 16) : z;
+                        x[2 * i] = ok ? *(const float4 *)(from + pos * a.c.ts) : z;
+                        x[2 * i + 1] = ok ? *(const float4 *)(from + pos * a.c.ts + 16) : z;
                     }
                 };
-                fetch(u.first);
+                fetch(0);
 #pragma unroll 1
-                for (int t = u.first; t < u.stop; t++, it++) {
+                for (int s = 0; s < count; s++, it++) {
                     const uint32_t st = it % NST;
                     wait(empty(st), ((it / NST) & 1u) ^ 1u, 47);
-                    char *ks = ring + st * F::STAGE + (lu / 8) * F::KATOM;
+                    char *to = ring + st * F::STAGE + (lu / 8) * F::KATOM;
 #pragma unroll
-                    for (int i = 0; i < N; i++)
+                    for (int i = 0; i < N; i++) {
+                        const int r = lr + i * RPI;
+                        if (r >= KT) continue;
+                        const float4 f0 = x[2 * i], f1 = x[2 * i + 1];
+                        float y[8] = {f0.x, f0.y, f0.z, f0.w, f1.x, f1.y, f1.z, f1.w};
 #pragma unroll
-                        for (int kv = 0; kv < 2; kv++) {
-                            const int r = lr + i * RPI;
-                            if (r >= KT) continue;
-                            const float4 f0 = x[4 * i + 2 * kv], f1 = x[4 * i + 2 * kv + 1];
-                            float y[8] = {f0.x, f0.y, f0.z, f0.w, f1.x, f1.y, f1.z, f1.w};
+                        for (int k = 0; k < F::NK; k++) {
+                            uint32_t w[4];
 #pragma unroll
-                            for (int k = 0; k < F::NK; k++) {
-                                uint32_t w[4];
-#pragma unroll
-                                for (int e = 0; e < 4; e++) {
-                                    w[e] = cm_pack(y[2 * e], y[2 * e + 1]);
-                                    const float2 f = cm_unpack(w[e]);
-                                    y[2 * e] -= f.x; y[2 * e + 1] -= f.y;
-                                }
-                                *(uint4 *)(ks + kv * (F::STAGE / 2) + k * ATOMS * F::KATOM + r * 128 + (((lu & 7) ^ (r & 7)) * 16)) = make_uint4(w[0], w[1], w[2], w[3]);
+                            for (int e = 0; e < 4; e++) {
+                                w[e] = cm_pack(y[2 * e], y[2 * e + 1]);
+                                const float2 f = cm_unpack(w[e]);
+                                y[2 * e] -= f.x; y[2 * e + 1] -= f.y;
                             }
+                            *(uint4 *)(to + k * ATOMS * F::KATOM + r * 128 + (((lu & 7) ^ (r & 7)) * 16)) = make_uint4(w[0], w[1], w[2], w[3]);
                         }
-                    if (t + 1 < u.stop) fetch(t + 1);
+                    }
+                    if (s + 1 < count) fetch(s + 1);
                     ct_fence_async();
                     __syncwarp();
                     if (lane == 0) mbar_arrive(full(st));
                 }
             }
         }
-        asm volatile("cp.async.wait_group 0;" ::: "memory");
     }
     tc_fence_before();
     __syncthreads();
     if (warp == F::SW) {
         tc_fence_after();
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(F::TMEM) : "memory");
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
     }
 }
+
+// a bf16 cache's keys or values as [row][head][slot][dim], boxes of 64 dims by kt slots (cache_attention.cu)
+int ct_map(const char *who, const CacheDev &c, const char *p, int kt, CUtensorMap &m);
 
 template <class KE, class QE, int HDP>
 int ct_run_as(const char *who, CmArgs a, int max_keys) {
     using F = CtCfg<KE, QE, HDP>;
     using J = CmCfg<KE, QE, HDP, F::M>;
     a.tiles = (int)cdiv(a.M, F::M);
+    CUtensorMap mk = {}, mv = {};
+    if (F::BF && (ct_map(who, a.c, a.c.k, F::KT, mk) || ct_map(who, a.c, a.c.v, F::KT, mv))) return -1;
     static bool set = false;
     if (!set) {
         CUDA_CHECK(cudaFuncSetAttribute(k_cache_attention_tc<KE, QE, HDP>, cudaFuncAttributeMaxDynamicSharedMemorySize, F::SMEM));
@@ -522,7 +594,7 @@ int ct_run_as(const char *who, CmArgs a, int max_keys) {
         const int nr = std::min(step, rows - r);
         a.row0 = r;
         a.items = nr;
-        LAUNCH_PDL((k_cache_attention_tc<KE, QE, HDP>), ctas, F::THREADS, F::SMEM, a, tc_err_flag());
+        LAUNCH_PDL((k_cache_attention_tc<KE, QE, HDP>), ctas, F::THREADS, F::SMEM, a, mk, mv, tc_err_flag());
         const int64_t joins = nr * row_units * (F::M / (split ? 1 : CM_THREADS / (HDP / 4)));
         LAUNCH_PDL((k_cache_join<KE, QE, HDP, F::M, false>), (unsigned)(joins + spans / step * nr), CM_THREADS, 0, a, (int)joins, split);
     }

@@ -233,7 +233,7 @@ extern "C" int ncmb_cache_evict(const NcmbCache *src, const NcmbCache *dst, cons
     a.pairs = a.to + units * a.room;
     // CTAs a (row, head): as many as keep the GPU busy, with 4096 slots each at least
     int nc = 1;
-    while (nc < EV_MAXC && units * nc * 2 <= ctx().sm_count && cdiv(max_len, nc) > 4096) nc *= 2;
+    while (nc < EV_MAXC && units * nc * 2 <= 2 * ctx().sm_count && cdiv(max_len, nc) > 4096) nc *= 2;
     a.move_here = a.inplace && max_len - a.room <= 64;   // that many tokens move at most, by what the host knows
     // slots of a CTA when the row is as long as the cache can hold: bits for all, keys for as many as shared memory takes
     const int64_t most = cdiv(cdiv(src->capacity, nc * EV_WARPS), 32) * 32 * EV_WARPS, hint = cdiv(cdiv(max_len, nc * EV_WARPS), 32) * 32 * EV_WARPS;

@@ -234,9 +234,28 @@ __global__ void __launch_bounds__(CM_THREADS, CmCfg<KE, QE, HDP, R>::CTAS) k_cac
         const int lu = lane % UPR, lr = lane / UPR;
         constexpr int RPI = 32 / UPR;                            // rows that the warp's lanes cover at once
         const bool lane_in = lu * 16 < hd * (int)sizeof(KE);
+        // A lane copies 16 bytes of every RPI-th key. Its rows are lr + i RPI with lr < RPI, a power of two, so the swizzles of row i
+        // differ from row 0's by a constant.
+        const uint32_t to_k = cm_smem(my) + lr * ROW + (F::BF ? lu ^ lr : lu ^ ((lr & 1) << 2)) * 16, to_v = cm_smem(my) + CM_STAGE / 2 + lr * ROW + (F::BF ? lu ^ lr : lu ^ ((lr >> 1) << 1)) * 16;
+        constexpr auto swz_k = [](int i) { return F::BF ? ((i * RPI) & 7) * 16 : (((i * RPI) & 1) << 2) * 16; };
+        constexpr auto swz_v = [](int i) { return F::BF ? ((i * RPI) & 7) * 16 : ((((i * RPI) >> 1) & 3) << 1) * 16; };
+        const int64_t step = (int64_t)RPI * a.c.ts, mine = lr * a.c.ts + lu * 16;
+        const bool fast = hd == HDP && (!BLOCKS || (1 << a.block_log) >= KC);
         auto load = [&](int ch, int stage) {
-            const uint32_t ks = cm_smem(my + stage * CM_STAGE), vs = ks + CM_STAGE / 2;
-#pragma unroll 2
+            const uint32_t ks = to_k + stage * CM_STAGE, vs = to_v + stage * CM_STAGE;
+            if (fast && (ch + 1) * KC <= len) {                  // keys side by side, all there
+                int64_t slot = ch * KC;
+                if (BLOCKS) slot = ((int64_t)spicks[ch * KC >> a.block_log] << a.block_log) + (ch * KC & ((1 << a.block_log) - 1));
+                const char *kp = kb + slot * a.c.ts + mine, *vp = vb + slot * a.c.ts + mine;
+#pragma unroll
+                for (int i = 0; i < KC / RPI; i++) {
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((ks ^ swz_k(i)) + i * RPI * ROW), "l"(kp) : "memory");
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((vs ^ swz_v(i)) + i * RPI * ROW), "l"(vp) : "memory");
+                    kp += step; vp += step;
+                }
+                return;
+            }
+#pragma unroll 1
             for (int i = 0; i < KC / RPI; i++) {
                 const int r = lr + i * RPI, pos = ch * KC + r;
                 bool ok = lane_in && pos < n;
@@ -244,9 +263,9 @@ __global__ void __launch_bounds__(CM_THREADS, CmCfg<KE, QE, HDP, R>::CTAS) k_cac
                 if (BLOCKS) slot = ok ? ((int64_t)spicks[pos >> a.block_log] << a.block_log) + (pos & ((1 << a.block_log) - 1)) : 0;
                 else if (tail && ok && pos >= len) ok = used(pos - len);
                 const int64_t off = ok ? slot * a.c.ts + lu * 16 : 0;
-                const int ku = F::BF ? lu ^ (r & 7) : lu ^ ((r & 1) << 2), vu = F::BF ? ku : lu ^ (((r >> 1) & 3) << 1);
-                cm_cp16(ks + r * ROW + ku * 16, kb + off, ok);
-                cm_cp16(vs + r * ROW + vu * 16, vb + off, ok);
+                const int xk = F::BF ? ((i * RPI) & 7) * 16 : (((i * RPI) & 1) << 2) * 16, xv = F::BF ? xk : ((((i * RPI) >> 1) & 3) << 1) * 16;
+                cm_cp16((ks ^ xk) + i * RPI * ROW, kb + off, ok);
+                cm_cp16((vs ^ xv) + i * RPI * ROW, vb + off, ok);
             }
         };
         // the tile's queries as terms, zero where no query stands, and what each of its nodes sees; under the first loads
@@ -733,10 +752,10 @@ __global__ void __launch_bounds__(CM_THREADS, CmCfg<KE, QE, HDP, R>::CTAS) k_cac
 // ---- units that several CTAs share are joined; weights are added up ----
 // CTAs [0, joins): rows of one unit each. A thread has four dims of a row; of the CTA's groups of HDP / 4 threads either each
 // has a row, or (`split`: few units, each in many parts) all have the same row and every one a share of its parts.
-// The others: 512 slots of one (row, kv head) each, from the scores that the kernel above left.
-constexpr int CM_WKEYS = 512;
+// The others: `wkeys` slots of one (row, kv head) each, from the scores that the kernel above left.
+constexpr int CM_PITCH = 128;        // scores of a query: whole tiles of keys
 template <class KE, class QE, int HDP, int R, bool BLOCKS>
-__global__ void __launch_bounds__(CM_THREADS) k_cache_join(const __grid_constant__ CmArgs a, int joins, int split) {
+__global__ void __launch_bounds__(CM_THREADS) k_cache_join(const __grid_constant__ CmArgs a, int joins, int split, int wkeys) {
     using F = CmCfg<KE, QE, HDP, R>;
     constexpr int M = F::M, D4 = HDP / 4, GROUPS = CM_THREADS / D4;
     __shared__ float lse[NCMB_MAX_NODES];
@@ -750,8 +769,8 @@ __global__ void __launch_bounds__(CM_THREADS) k_cache_join(const __grid_constant
     int item, sub, key0 = 0;
     if (join) { item = blockIdx.x / steps / per_item; sub = blockIdx.x / steps % per_item; }
     else {
-        const int span = (int)((a.pitch + CM_WKEYS - 1) / CM_WKEYS), x = blockIdx.x - joins;
-        key0 = x % span * CM_WKEYS;
+        const int span = (int)((a.pitch + wkeys - 1) / wkeys), x = blockIdx.x - joins;
+        key0 = x % span * wkeys;
         sub = x / span % a.c.nkv * a.tiles;
         item = x / span / a.c.nkv;
     }
@@ -806,10 +825,9 @@ __global__ void __launch_bounds__(CM_THREADS) k_cache_join(const __grid_constant
     }
     const int kvh = sub / a.tiles, n = cm_keys<BLOCKS>(a, item), len = n - a.T;
     if (key0 >= n) return;
-    float w[CM_WKEYS / CM_THREADS];
-#pragma unroll
-    for (int x = 0; x < CM_WKEYS / CM_THREADS; x++) w[x] = 0.f;
-    const float *sc = a.scores + ((int64_t)item * a.c.nkv + kvh) * a.M * a.pitch + key0 + tid;
+    const float *sc = a.scores + ((int64_t)item * a.c.nkv + kvh) * a.M * a.pitch;
+    float *wp = a.weights + ((int64_t)row * a.c.nkv + kvh) * a.c.cap;
+    const int stop = min(n, key0 + wkeys);
     for (int mb = 0; mb < a.M; mb += NCMB_MAX_NODES) {
         const int nm = min(NCMB_MAX_NODES, a.M - mb);
         __syncthreads();
@@ -829,23 +847,33 @@ __global__ void __launch_bounds__(CM_THREADS) k_cache_join(const __grid_constant
             lse[i] = l > 0.f && cm_used(par, mm / G) ? top + log2f(l) : INFINITY;
         }
         __syncthreads();
-        for (int i = 0; i < nm; i++) {
-            const float e = lse[i];
+        if (wkeys > CM_THREADS) {
+            // few rows: four slots a thread, so that as many loads are under way
+            float w[4] = {0.f, 0.f, 0.f, 0.f};
+            for (int i = 0; i < nm; i++) {
+                const float *s = sc + (int64_t)(mb + i) * a.pitch + key0 + tid;
+                const float e = lse[i];
 #pragma unroll
-            for (int x = 0; x < CM_WKEYS / CM_THREADS; x++)
-                if (key0 + tid + x * CM_THREADS < n) w[x] += cm_exp2(sc[(int64_t)(mb + i) * a.pitch + x * CM_THREADS] - e);
+                for (int x = 0; x < 4; x++) if (key0 + tid + x * CM_THREADS < stop) w[x] += cm_exp2(s[x * CM_THREADS] - e);
+            }
+#pragma unroll
+            for (int x = 0; x < 4; x++) {
+                const int key = key0 + tid + x * CM_THREADS;
+                if (key < stop) wp[key] = mb || key < len ? wp[key] + w[x] : w[x];       // the new tokens' slots are stored to, the others added to
+            }
+        } else if (key0 + tid < stop) {
+            const int key = key0 + tid;
+            float w = 0.f;
+#pragma unroll 8
+            for (int i = 0; i < nm; i++) w += cm_exp2(sc[(int64_t)(mb + i) * a.pitch + key] - lse[i]);
+            wp[key] = mb || key < len ? wp[key] + w : w;
         }
-    }
-    float *wp = a.weights + ((int64_t)row * a.c.nkv + kvh) * a.c.cap;
-#pragma unroll
-    for (int x = 0; x < CM_WKEYS / CM_THREADS; x++) {
-        const int key = key0 + tid + x * CM_THREADS;
-        if (key < len) wp[key] += w[x];
-        else if (key < n) wp[key] = w[x];
     }
 }
 
 // ---- launches ----
+// slots of a CTA that adds up weights: it finds the sums of M queries first, then goes over M scores a slot
+inline int cm_wkeys(int M) { return M <= 32 ? 4 * CM_THREADS : CM_THREADS; }
 #ifndef CM_MAXC
 #define CM_MAXC 8
 #define CM_ROUNDS 8
@@ -870,12 +898,12 @@ int cm_run_as(const char *who, CmArgs a, int max_keys) {
     const int64_t row_chunks = row_units * cdiv(BLOCKS ? (int64_t)a.n_sel << a.block_log : a.c.cap, F::KC);
     int64_t most = 0x70000000 / row_chunks;
     if (a.weights) {
-        a.pitch = cdiv((int64_t)a.c.cap, CM_WKEYS) * CM_WKEYS;
+        a.pitch = cdiv((int64_t)a.c.cap, CM_PITCH) * CM_PITCH;
         most = std::min(most, std::max<int64_t>(1, ((int64_t)2 << 30) / (a.c.nkv * a.M * a.pitch * 4)));
     }
     if (most < 1) return cache_refuse(who, "%lld pieces of keys in a row", (long long)row_chunks);
     const int step = (int)std::min<int64_t>(rows, most);
-    const int64_t units = step * row_units, spans = a.weights ? cdiv(a.pitch, CM_WKEYS) * step * a.c.nkv : 0;
+    const int64_t units = step * row_units, spans = a.weights ? cdiv(a.pitch, cm_wkeys(a.M)) * step * a.c.nkv : 0;
     if (units * F::M + spans > 0x7fffffff) return cache_refuse(who, "%lld query tiles", (long long)units);
     // Clusters: where one, of as many CTAs as give a warp two chunks, does a unit in a few rounds and all of them fit the GPU
     int nc = 1;
@@ -906,7 +934,7 @@ int cm_run_as(const char *who, CmArgs a, int max_keys) {
         LAUNCH_PDL((k_cache_attention<KE, QE, HDP, R, BLOCKS, false>), ctas, CM_THREADS, smem, a);
         if (fused) continue;
         const int64_t joins = nr * row_units * (F::M / (split ? 1 : CM_THREADS / (HDP / 4)));
-        LAUNCH_PDL((k_cache_join<KE, QE, HDP, R, BLOCKS>), (unsigned)(joins + spans / step * nr), CM_THREADS, 0, a, (int)joins, split);
+        LAUNCH_PDL((k_cache_join<KE, QE, HDP, R, BLOCKS>), (unsigned)(joins + spans / step * nr), CM_THREADS, 0, a, (int)joins, split, cm_wkeys(a.M));
     }
     return 0;
 }

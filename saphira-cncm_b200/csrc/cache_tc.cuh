@@ -18,6 +18,7 @@
 
 namespace ncmb {
 
+constexpr int CT_START = 1;          // what the start of a unit costs, in tiles
 template <class KE, class QE, int HDP_> struct CtCfg {
     static constexpr bool BF = sizeof(KE) == 2;
     static constexpr int HDP = HDP_, ATOMS = HDP / 64, M = 128, KT = 128;
@@ -25,7 +26,7 @@ template <class KE, class QE, int HDP_> struct CtCfg {
     static constexpr int KATOM = KT * 128, QATOM = M * 128;          // bytes of 64 dims of the keys, of the queries
     static constexpr int STAGE = NK * ATOMS * KATOM, QB = NQ * ATOMS * QATOM;        // a stage: a tile's keys or its values
     static constexpr int FIT = (217 * 1024 - QB) / STAGE, NST = FIT < 8 ? FIT : 8;
-    static constexpr int PW = BF ? 3 : 7, SW = 8, THREADS = 32 * (SW + 1 + PW);      // whole warps a scheduler: registers
+    static constexpr int PG = 3, PW = BF ? PG : 2 * PG, SW = 8, THREADS = 32 * (SW + 1 + PW);    // whole warps a scheduler: registers
     static constexpr int SMEM = QB + NST * STAGE + 1024;
     // columns of tensor memory: probabilities (two to a column), context, one or two score tiles
     static constexpr int PCOL = 0, OCOL = NP * 64, SCOL = OCOL + HDP, NSB = SCOL + 256 <= 512 ? 2 : 1;
@@ -86,19 +87,20 @@ __global__ void __launch_bounds__(CtCfg<KE, QE, HDP>::THREADS, 1) k_cache_attent
     __shared__ int s_abort;
     if (tid == 0) {
         s_abort = *(volatile int *)err;                              // a wait ran out earlier: nothing more is started
-        for (int s = 0; s < NST; s++) { mbar_init(full(s), F::PW); mbar_init(empty(s), 1); }
+        for (int s = 0; s < NST; s++) { mbar_init(full(s), F::PG); mbar_init(empty(s), 1); }
         mbar_init(bar_q, F::SW); mbar_init(bar_s, 1); mbar_init(bar_s + 8, 1); mbar_init(bar_p, F::SW); mbar_init(bar_pv, 1); mbar_init(bar_sf, F::SW);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 0) {
-        // the plan of cache_mma.cuh, by one warp
+        // the plan of cache_mma.cuh, by one warp; a unit counts as CT_START tiles more than it has
         int t = 0;
-        for (int i = lane; i < a.items; i += 32) t += cm_chunks<false, KT>(a, i);
+        auto places = [&](int i) { return i < a.items ? ((cm_keys<false>(a, i) + KT - 1) / KT + CT_START) * a.c.nkv * a.tiles : 0; };
+        for (int i = lane; i < a.items; i += 32) t += places(i);
         t = __reduce_add_sync(0xffffffffu, t);
         const int per = (unsigned)(t + (int)gridDim.x - 1) / gridDim.x, x = (int)min((int64_t)blockIdx.x * per, (int64_t)t);
         int before = 0, item = 0, begin = 0;
         for (int i0 = 0; i0 < a.items; i0 += 32) {
-            const int mine = cm_chunks<false, KT>(a, i0 + lane);
+            const int mine = places(i0 + lane);
             int inc = mine;
             for (int o = 1; o < 32; o <<= 1) {
                 const int v = __shfl_up_sync(0xffffffffu, inc, o);
@@ -126,17 +128,20 @@ __global__ void __launch_bounds__(CtCfg<KE, QE, HDP>::THREADS, 1) k_cache_attent
     struct Unit { int item, kvh, m0, first, stop, unit, n, len, row; bool whole; };
     int at = blockIdx.x * plan[1], item = plan[2], item_at = plan[3];
     const int end = min(plan[0], at + plan[1]);
-    auto next_unit = [&](Unit &u) {                                  // the run's next unit, or false
-        if (at >= end) return false;
-        u.n = cm_keys<false>(a, item);
-        const int nch = (u.n + KT - 1) / KT, sub = cm_div(at - item_at, nch), kvh = a.tiles == 1 ? sub : cm_div(sub, a.tiles);
-        u.item = item; u.kvh = kvh; u.m0 = (sub - kvh * a.tiles) * M;
-        u.first = at - item_at - sub * nch; u.stop = min(nch, u.first + (end - at));
-        u.unit = item * a.c.nkv * a.tiles + sub;
-        u.len = u.n - a.T; u.row = a.row0 + item; u.whole = u.first == 0 && u.stop == nch;
-        at += u.stop - u.first;
-        if (at == item_at + nch * a.c.nkv * a.tiles) { item_at = at; item++; }
-        return true;
+    auto next_unit = [&](Unit &u) {                                  // the run's next unit with tiles in it, or false
+        while (at < end) {
+            u.n = cm_keys<false>(a, item);
+            const int nch = (u.n + KT - 1) / KT, span = nch + CT_START, sub = cm_div(at - item_at, span), kvh = a.tiles == 1 ? sub : cm_div(sub, a.tiles);
+            const int into = at - item_at - sub * span, take = min(span - into, end - at);
+            u.item = item; u.kvh = kvh; u.m0 = (sub - kvh * a.tiles) * M;
+            u.first = max(0, into - CT_START); u.stop = into + take - CT_START;
+            u.unit = item * a.c.nkv * a.tiles + sub;
+            u.len = u.n - a.T; u.row = a.row0 + item; u.whole = u.first == 0 && u.stop == nch;
+            at += take;
+            if (at == item_at + span * a.c.nkv * a.tiles) { item_at = at; item++; }
+            if (u.stop > u.first) return true;
+        }
+        return false;
     };
     Unit u;
     uint32_t it = 0, un = 0, items = 0;                              // tiles, units, stages (two a tile) so far
@@ -151,41 +156,47 @@ __global__ void __launch_bounds__(CtCfg<KE, QE, HDP>::THREADS, 1) k_cache_attent
         while (next_unit(u)) {
             const int *par = a.parents ? a.parents + (int64_t)u.row * a.T : nullptr;
             // queries as terms (the MMAs that read the last unit's are done: their scores have been read)
+            constexpr int QU = HDP / 8, QR = F::SW * 32 / QU, AHEAD = 4;     // units of 8 dims a row, rows a step, rows a thread loads at once
+            const int d0 = tid % QU * 8;
+            const float per_g = 1.0f / (float)G;
 #pragma unroll 1
-            for (int i = tid; i < M * HDP / 8; i += F::SW * 32) {
-                const int m = i / (HDP / 8), d0 = i % (HDP / 8) * 8, mm = u.m0 + m;
-                float x[8];
+            for (int m1 = tid / QU; m1 < M; m1 += QR * AHEAD) {
+                float4 raw[AHEAD][sizeof(QE) / 2];
 #pragma unroll
-                for (int e = 0; e < 8; e++) x[e] = 0.f;
-                if (mm < a.M && d0 < hd) {
-                    const int t = mm / G, h = u.kvh * G + mm - t * G;
-                    if (cm_used(par, t)) {
-                        const char *p = a.q + ((int64_t)u.row * a.T + t) * a.ldq + ((int64_t)h * hd + d0) * sizeof(QE);
-                        if constexpr (sizeof(QE) == 4) {
-                            *(float4 *)&x[0] = *(const float4 *)p;
-                            *(float4 *)&x[4] = *(const float4 *)(p + 16);
-                        } else {
-                            const uint4 q = *(const uint4 *)p;
-                            const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+                for (int i = 0; i < AHEAD; i++) {
+                    const int mm = u.m0 + m1 + i * QR, t = (int)(((float)mm + 0.5f) * per_g), h = u.kvh * G + mm - t * G;     // mm / G: mm is far below 2^20
+                    const char *p = a.q + ((int64_t)u.row * a.T + t) * a.ldq + ((int64_t)h * hd + d0) * sizeof(QE);
+                    const bool ok = mm < a.M && d0 < hd && cm_used(par, t);
 #pragma unroll
-                            for (int e = 0; e < 4; e++) { const float2 f = cm_unpack(w[e]); x[2 * e] = f.x; x[2 * e + 1] = f.y; }
+                    for (int x = 0; x < (int)sizeof(QE) / 2; x++) raw[i][x] = ok ? *(const float4 *)(p + 16 * x) : make_float4(0.f, 0.f, 0.f, 0.f);
+                }
+#pragma unroll
+                for (int i = 0; i < AHEAD; i++) {
+                    const int m = m1 + i * QR;
+                    float x[8];
+                    if constexpr (sizeof(QE) == 4) {
+                        *(float4 *)&x[0] = raw[i][0];
+                        *(float4 *)&x[4] = raw[i][1];
+                    } else {
+                        const float w[4] = {raw[i][0].x, raw[i][0].y, raw[i][0].z, raw[i][0].w};
+#pragma unroll
+                        for (int e = 0; e < 4; e++) { const float2 f = cm_unpack(__float_as_uint(w[e])); x[2 * e] = f.x; x[2 * e + 1] = f.y; }
+                    }
+                    if (a.c2 < 0.f) {
+#pragma unroll
+                        for (int e = 0; e < 8; e++) x[e] = -x[e];
+                    }
+#pragma unroll
+                    for (int k = 0; k < F::NQ; k++) {
+                        uint32_t w[4];
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            w[e] = cm_pack(x[2 * e], x[2 * e + 1]);
+                            const float2 f = cm_unpack(w[e]);
+                            x[2 * e] -= f.x; x[2 * e + 1] -= f.y;
                         }
+                        *(uint4 *)(qs + (k * ATOMS + d0 / 64) * F::QATOM + m * 128 + ((((d0 & 63) / 8) ^ (m & 7)) * 16)) = make_uint4(w[0], w[1], w[2], w[3]);
                     }
-                }
-                if (a.c2 < 0.f) {
-#pragma unroll
-                    for (int e = 0; e < 8; e++) x[e] = -x[e];
-                }
-#pragma unroll
-                for (int k = 0; k < F::NQ; k++) {
-                    uint32_t w[4];
-#pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        w[e] = cm_pack(x[2 * e], x[2 * e + 1]);
-                        const float2 f = cm_unpack(w[e]);
-                        x[2 * e] -= f.x; x[2 * e + 1] -= f.y;
-                    }
-                    *(uint4 *)(qs + (k * ATOMS + d0 / 64) * F::QATOM + m * 128 + ((((d0 & 63) / 8) ^ (m & 7)) * 16)) = make_uint4(w[0], w[1], w[2], w[3]);
                 }
             }
             const int mm = u.m0 + r, node = min(mm, a.M - 1) / G;
@@ -457,8 +468,9 @@ __global__ void __launch_bounds__(CtCfg<KE, QE, HDP>::THREADS, 1) k_cache_attent
         }
     } else {
         // ================= loads =================
-        const int pt = tid - (F::SW + 1) * 32;
-        constexpr int NT = F::PW * 32;
+        // (fp32: three warps for the keys, three for the values)
+        const int grp = F::BF ? 0 : (warp - F::SW - 1) / F::PG, pt = tid - (F::SW + 1 + grp * F::PG) * 32;
+        constexpr int NT = F::PG * 32;
         while (next_unit(u)) {
             const int *par = a.parents ? a.parents + (int64_t)u.row * a.T : nullptr;
             const char *kb = a.c.k + u.row * a.c.rs + u.kvh * a.c.hs, *vb = a.c.v + u.row * a.c.rs + u.kvh * a.c.hs;
@@ -467,7 +479,7 @@ __global__ void __launch_bounds__(CtCfg<KE, QE, HDP>::THREADS, 1) k_cache_attent
             const int count = 2 * (u.stop - u.first);
             auto tile_of = [&](int s) { return s == 0 ? 0 : s == count - 1 ? (s - 1) / 2 : (s & 1) ? (s + 1) / 2 : (s - 2) / 2; };
             auto is_v = [&](int s) { return s == count - 1 || (s > 0 && !(s & 1)); };
-            constexpr int UPR = HDP / 8, RPI = NT / UPR, N = (KT + RPI - 1) / RPI;       // units of 8 dims of a key, keys a step
+            constexpr int UPR = HDP / 8, RPI = NT / UPR;             // units of 8 dims of a key, keys a step
             const int lu = pt % UPR, lr = pt / UPR;
             const bool in = lu * 8 < hd;
             if constexpr (F::BF) {
@@ -500,50 +512,50 @@ __global__ void __launch_bounds__(CtCfg<KE, QE, HDP>::THREADS, 1) k_cache_attent
                     if (lane == 0) mbar_arrive(full(st));
                 }
             } else {
-                // the next stage's elements are on their way while this one's are turned into terms
-                float4 x[2 * N];
-                auto fetch = [&](int s) {
-                    const int t = u.first + tile_of(s);
-                    const char *from = (is_v(s) ? vb : kb) + lu * 32;
-                    const bool tail = (t + 1) * KT > u.len;
-#pragma unroll
-                    for (int i = 0; i < N; i++) {
-                        const int pos = t * KT + lr + i * RPI;
-                        const bool ok = in && lr + i * RPI < KT && (tail ? there(pos) : true);
-                        const float4 z = make_float4(0.f, 0.f, 0.f, 0.f);
-                        x[2 * i] = ok ? *(const float4 *)(from + pos * a.c.ts) : z;
-                        x[2 * i + 1] = ok ? *(const float4 *)(from + pos * a.c.ts + 16) : z;
-                    }
-                };
-                fetch(0);
+                const char *from = (grp ? vb : kb) + lu * 32;
+                const int tiles = u.stop - u.first;
 #pragma unroll 1
-                for (int s = 0; s < count; s++, it++) {
-                    const uint32_t st = it % NST;
-                    wait(empty(st), ((it / NST) & 1u) ^ 1u, 47);
+                for (int t = 0; t < tiles; t++) {
+                    const uint32_t s = it + (grp ? (t + 1 < tiles ? 2 + 2 * t : 2 * tiles - 1) : t ? 2 * t - 1 : 0), st = s % NST;
                     char *to = ring + st * F::STAGE + (lu / 8) * F::KATOM;
+                    const bool tail = (u.first + t + 1) * KT > u.len;
+#pragma unroll 1
+                    for (int r0 = 0; r0 < KT; r0 += KT / 2) {        // half a stage: what a thread has registers for
+                        constexpr int N2 = (KT / 2 + RPI - 1) / RPI;
+                        float4 x[2 * N2];
 #pragma unroll
-                    for (int i = 0; i < N; i++) {
-                        const int r = lr + i * RPI;
-                        if (r >= KT) continue;
-                        const float4 f0 = x[2 * i], f1 = x[2 * i + 1];
-                        float y[8] = {f0.x, f0.y, f0.z, f0.w, f1.x, f1.y, f1.z, f1.w};
+                        for (int i = 0; i < N2; i++) {
+                            const int rr = lr + i * RPI, pos = (u.first + t) * KT + r0 + rr;
+                            const bool ok = in && rr < KT / 2 && (tail ? there(pos) : true);
+                            const float4 z = make_float4(0.f, 0.f, 0.f, 0.f);
+                            x[2 * i] = ok ? *(const float4 *)(from + pos * a.c.ts) : z;
+                            x[2 * i + 1] = ok ? *(const float4 *)(from + pos * a.c.ts + 16) : z;
+                        }
+                        if (r0 == 0) wait(empty(st), ((s / NST) & 1u) ^ 1u, 47);
 #pragma unroll
-                        for (int k = 0; k < F::NK; k++) {
-                            uint32_t w[4];
+                        for (int i = 0; i < N2; i++) {
+                            const int r = r0 + lr + i * RPI;
+                            if (lr + i * RPI >= KT / 2) continue;
+                            const float4 f0 = x[2 * i], f1 = x[2 * i + 1];
+                            float y[8] = {f0.x, f0.y, f0.z, f0.w, f1.x, f1.y, f1.z, f1.w};
 #pragma unroll
-                            for (int e = 0; e < 4; e++) {
-                                w[e] = cm_pack(y[2 * e], y[2 * e + 1]);
-                                const float2 f = cm_unpack(w[e]);
-                                y[2 * e] -= f.x; y[2 * e + 1] -= f.y;
+                            for (int k = 0; k < F::NK; k++) {
+                                uint32_t w[4];
+#pragma unroll
+                                for (int e = 0; e < 4; e++) {
+                                    w[e] = cm_pack(y[2 * e], y[2 * e + 1]);
+                                    const float2 f = cm_unpack(w[e]);
+                                    y[2 * e] -= f.x; y[2 * e + 1] -= f.y;
+                                }
+                                *(uint4 *)(to + k * ATOMS * F::KATOM + r * 128 + (((lu & 7) ^ (r & 7)) * 16)) = make_uint4(w[0], w[1], w[2], w[3]);
                             }
-                            *(uint4 *)(to + k * ATOMS * F::KATOM + r * 128 + (((lu & 7) ^ (r & 7)) * 16)) = make_uint4(w[0], w[1], w[2], w[3]);
                         }
                     }
-                    if (s + 1 < count) fetch(s + 1);
                     ct_fence_async();
                     __syncwarp();
                     if (lane == 0) mbar_arrive(full(st));
                 }
+                it += count;
             }
         }
     }
@@ -571,15 +583,15 @@ int ct_run_as(const char *who, CmArgs a, int max_keys) {
         set = true;
     }
     const int rows = a.c.rows;
-    const int64_t row_units = (int64_t)a.c.nkv * a.tiles, row_chunks = row_units * cdiv(a.c.cap, F::KT);
+    const int64_t row_units = (int64_t)a.c.nkv * a.tiles, row_chunks = row_units * (cdiv(a.c.cap, F::KT) + CT_START);
     int64_t most = 0x70000000 / row_chunks;
     if (a.weights) {
-        a.pitch = cdiv((int64_t)a.c.cap, CM_WKEYS) * CM_WKEYS;
+        a.pitch = cdiv((int64_t)a.c.cap, CM_PITCH) * CM_PITCH;
         most = std::min(most, std::max<int64_t>(1, ((int64_t)2 << 30) / (a.c.nkv * a.M * a.pitch * 4)));
     }
     if (most < 1) return cache_refuse(who, "%lld pieces of keys in a row", (long long)row_chunks);
     const int step = (int)std::min<int64_t>(rows, most);
-    const int64_t units = step * row_units, spans = a.weights ? cdiv(a.pitch, CM_WKEYS) * step * a.c.nkv : 0;
+    const int64_t units = step * row_units, spans = a.weights ? cdiv(a.pitch, cm_wkeys(a.M)) * step * a.c.nkv : 0;
     if (units * F::M + spans > 0x7fffffff) return cache_refuse(who, "%lld query tiles", (long long)units);
     const int ctas = (int)std::max<int64_t>(1, std::min<int64_t>(ctx().sm_count, units * cdiv(max_keys, F::KT)));
     const size_t ranges = ((size_t)units * 8 + 255) & ~(size_t)255, part = (size_t)(units + ctas) * J::SLOT * 4;
@@ -596,7 +608,7 @@ int ct_run_as(const char *who, CmArgs a, int max_keys) {
         a.items = nr;
         LAUNCH_PDL((k_cache_attention_tc<KE, QE, HDP>), ctas, F::THREADS, F::SMEM, a, mk, mv, tc_err_flag());
         const int64_t joins = nr * row_units * (F::M / (split ? 1 : CM_THREADS / (HDP / 4)));
-        LAUNCH_PDL((k_cache_join<KE, QE, HDP, F::M, false>), (unsigned)(joins + spans / step * nr), CM_THREADS, 0, a, (int)joins, split);
+        LAUNCH_PDL((k_cache_join<KE, QE, HDP, F::M, false>), (unsigned)(joins + spans / step * nr), CM_THREADS, 0, a, (int)joins, split, cm_wkeys(a.M));
     }
     return 0;
 }

@@ -48,7 +48,7 @@ __device__ __forceinline__ void bs_sum(float (&r)[16 / sizeof(KE)], const char *
 }
 
 template <class KE, int CNT>
-__global__ void __launch_bounds__(256) k_block_summaries(CacheDev c, int n_new, const int *first, int block, int nb, int upr_log, signed char *codes, float *scales) {
+__global__ void __launch_bounds__(256, CNT <= 16 ? 4 : CNT <= 32 ? 3 : 2) k_block_summaries(CacheDev c, int n_new, const int *first, int block, int nb, int upr_log, signed char *codes, float *scales) {
     constexpr int VE = BsVec<KE>::N;
     const int lane = threadIdx.x & 31, kvh = blockIdx.y, b = blockIdx.z;
     const int u = lane & ((1 << upr_log) - 1), tr = lane >> upr_log, R = block / CNT;

@@ -15,11 +15,6 @@
 namespace ncmb {
 
 constexpr int CM_WARPS = 4, CM_THREADS = CM_WARPS * 32;
-#ifndef CM_SB
-#define CM_SB 8192
-#define CM_ST 2
-#define CM_CTAS 3
-#endif
 // R: query rows of a tile, 16 or 8. A tile of 8 has two terms of its queries (or probabilities) stacked in the 16 rows of the
 // tensor-core tile; a lane holds rows lane / 4 and lane / 4 + 8 of a result, so it adds the two terms' products up itself.
 template <class KE, class QE, int HDP_, int R_> struct CmCfg {
@@ -29,8 +24,10 @@ template <class KE, class QE, int HDP_, int R_> struct CmCfg {
     static constexpr int NH = R8 ? 1 : 2;                        // rows a lane has
     static constexpr int ROW = HDP * (int)sizeof(KE);            // bytes of a key in shared memory
     static constexpr int UPR = ROW / 16;
-    static constexpr int CM_STAGE = HDP == 64 ? CM_SB : 8192;    // bytes of keys and values in a stage of a warp's ring
-    static constexpr int CM_STAGES = HDP == 64 ? CM_ST : 2, CTAS = HDP == 64 ? CM_CTAS : 3;      // stages, CTAs an SM
+    // Two stages of 8 KB a warp and three CTAs an SM. Measured at 64 x 16000 (bf16, 64) / 32 rows of picked blocks (bf16, 128) / 3 x 24
+    // (fp32, 64): 87 / 82 / 66 us; four stages of 4 KB 93 / 88 / 71; three of 8 KB in two CTAs 88 / 97 / 68; three of 4 KB in four
+    // CTAs 93 / 82 / 88.
+    static constexpr int CM_STAGE = 8192, CM_STAGES = 2, CTAS = 3;
     static constexpr int KC = CM_STAGE / (2 * ROW);              // keys a chunk
     static constexpr int NT = KC / 8;                            // 8-key tiles a chunk
     static constexpr int NQ = !BF ? 2 : sizeof(QE) == 4 ? 3 : 1; // terms of a query
@@ -828,6 +825,16 @@ __global__ void __launch_bounds__(CM_THREADS) k_cache_join(const __grid_constant
     const float *sc = a.scores + ((int64_t)item * a.c.nkv + kvh) * a.M * a.pitch;
     float *wp = a.weights + ((int64_t)row * a.c.nkv + kvh) * a.c.cap;
     const int stop = min(n, key0 + wkeys);
+    float early[R == 8 ? 8 : 1][4];                              // few rows: the scores are on their way while the sums are formed
+    if constexpr (R == 8) {
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+#pragma unroll
+            for (int x = 0; x < 4; x++) {
+                const int key = key0 + tid + x * CM_THREADS;
+                early[i][x] = i < a.M && key < stop ? sc[i * a.pitch + key] : -INFINITY;
+            }
+    }
     for (int mb = 0; mb < a.M; mb += NCMB_MAX_NODES) {
         const int nm = min(NCMB_MAX_NODES, a.M - mb);
         __syncthreads();
@@ -850,7 +857,13 @@ __global__ void __launch_bounds__(CM_THREADS) k_cache_join(const __grid_constant
         if (wkeys > CM_THREADS) {
             // few rows: four slots a thread, so that as many loads are under way
             float w[4] = {0.f, 0.f, 0.f, 0.f};
-            for (int i = 0; i < nm; i++) {
+            if constexpr (R == 8) {
+#pragma unroll
+                for (int i = 0; i < 8; i++)
+#pragma unroll
+                    for (int x = 0; x < 4; x++) if (i < nm) w[x] += cm_exp2(early[i][x] - lse[i]);
+            }
+            for (int i = R == 8 ? nm : 0; i < nm; i++) {
                 const float *s = sc + (int64_t)(mb + i) * a.pitch + key0 + tid;
                 const float e = lse[i];
 #pragma unroll

@@ -18,7 +18,6 @@
 
 namespace ncmb {
 
-constexpr int CT_START = 1;          // what the start of a unit costs, in tiles
 template <class KE, class QE, int HDP_> struct CtCfg {
     static constexpr bool BF = sizeof(KE) == 2;
     static constexpr int HDP = HDP_, ATOMS = HDP / 64, M = 128, KT = 128;
@@ -29,6 +28,9 @@ template <class KE, class QE, int HDP_> struct CtCfg {
     static constexpr int PG = 3, PW = BF ? PG : 2 * PG, SW = 8, THREADS = 32 * (SW + 1 + PW);    // whole warps a scheduler: registers
     static constexpr int SMEM = QB + NST * STAGE + 1024;
     // columns of tensor memory: probabilities (two to a column), context, one or two score tiles
+    // What the start of a unit costs, in tiles, for the plan: queries, the first loads and the results take about 9 us, a tile 2
+    // (bf16) or 7 (fp32: forming the terms). Without it the CTA that gets a short row's heads is the last: 125 -> 100 us.
+    static constexpr int START = BF ? 4 : 1;
     static constexpr int PCOL = 0, OCOL = NP * 64, SCOL = OCOL + HDP, NSB = SCOL + 256 <= 512 ? 2 : 1;
 };
 
@@ -76,7 +78,7 @@ __global__ void __launch_bounds__(CtCfg<KE, QE, HDP>::THREADS, 1) k_cache_attent
     __shared__ uint32_t tmem_at;
     __shared__ int plan[4];                                          // total, per, item, where it begins
     __shared__ float xm[2][2][M], xl[2][M];
-    __shared__ uint32_t node_bits[M][8];
+    __shared__ uint32_t node_bits[M][8], place_bits[F::PW][8];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, hd = a.c.hd, G = a.G;
     auto full = [&](int s) { return cm_smem(&bars[s]); };
     auto empty = [&](int s) { return cm_smem(&bars[8 + s]); };
@@ -92,9 +94,9 @@ __global__ void __launch_bounds__(CtCfg<KE, QE, HDP>::THREADS, 1) k_cache_attent
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 0) {
-        // the plan of cache_mma.cuh, by one warp; a unit counts as CT_START tiles more than it has
+        // the plan of cache_mma.cuh, by one warp; a unit counts as F::START tiles more than it has
         int t = 0;
-        auto places = [&](int i) { return i < a.items ? ((cm_keys<false>(a, i) + KT - 1) / KT + CT_START) * a.c.nkv * a.tiles : 0; };
+        auto places = [&](int i) { return i < a.items ? ((cm_keys<false>(a, i) + KT - 1) / KT + F::START) * a.c.nkv * a.tiles : 0; };
         for (int i = lane; i < a.items; i += 32) t += places(i);
         t = __reduce_add_sync(0xffffffffu, t);
         const int per = (unsigned)(t + (int)gridDim.x - 1) / gridDim.x, x = (int)min((int64_t)blockIdx.x * per, (int64_t)t);
@@ -131,10 +133,10 @@ __global__ void __launch_bounds__(CtCfg<KE, QE, HDP>::THREADS, 1) k_cache_attent
     auto next_unit = [&](Unit &u) {                                  // the run's next unit with tiles in it, or false
         while (at < end) {
             u.n = cm_keys<false>(a, item);
-            const int nch = (u.n + KT - 1) / KT, span = nch + CT_START, sub = cm_div(at - item_at, span), kvh = a.tiles == 1 ? sub : cm_div(sub, a.tiles);
+            const int nch = (u.n + KT - 1) / KT, span = nch + F::START, sub = cm_div(at - item_at, span), kvh = a.tiles == 1 ? sub : cm_div(sub, a.tiles);
             const int into = at - item_at - sub * span, take = min(span - into, end - at);
             u.item = item; u.kvh = kvh; u.m0 = (sub - kvh * a.tiles) * M;
-            u.first = max(0, into - CT_START); u.stop = into + take - CT_START;
+            u.first = max(0, into - F::START); u.stop = into + take - F::START;
             u.unit = item * a.c.nkv * a.tiles + sub;
             u.len = u.n - a.T; u.row = a.row0 + item; u.whole = u.first == 0 && u.stop == nch;
             at += take;
@@ -281,7 +283,7 @@ __global__ void __launch_bounds__(CtCfg<KE, QE, HDP>::THREADS, 1) k_cache_attent
                 if (busy) {
                     float sum = 0.f;
 #pragma unroll
-                    for (int c = 0; c < 4; c++) {                    // 16 keys at a time
+                    for (int c = 0; c < 4; c++) {                    // 16 keys at a time (more, or some before the wait: spills, 125 -> 167 us)
                         uint32_t sr[16];
                         tmem_ld16(scol + 16u * c, sr);
                         if (masked) {
@@ -474,7 +476,17 @@ __global__ void __launch_bounds__(CtCfg<KE, QE, HDP>::THREADS, 1) k_cache_attent
         while (next_unit(u)) {
             const int *par = a.parents ? a.parents + (int64_t)u.row * a.T : nullptr;
             const char *kb = a.c.k + u.row * a.c.rs + u.kvh * a.c.hs, *vb = a.c.v + u.row * a.c.rs + u.kvh * a.c.hs;
-            auto there = [&](int pos) { return pos < u.n && (pos < u.len || cm_used(par, pos - u.len)); };
+            uint32_t *bits = place_bits[warp - F::SW - 1];           // new tokens that are one, this warp's copy
+            if (u.stop * KT > u.len) {
+                __syncwarp();
+                for (int w = 0; w * 32 < a.T; w++) {
+                    const int x = w * 32 + lane;
+                    const uint32_t m = __ballot_sync(0xffffffffu, x < a.T && cm_used(par, x));
+                    if (lane == 0) bits[w] = m;
+                }
+                __syncwarp();
+            }
+            auto there = [&](int pos) { return pos < u.n && (pos < u.len || ((bits[(pos - u.len) >> 5] >> ((pos - u.len) & 31)) & 1u)); };
             // stage s of the unit: keys of tile 0, then in turn keys of the next tile and values of this one
             const int count = 2 * (u.stop - u.first);
             auto tile_of = [&](int s) { return s == 0 ? 0 : s == count - 1 ? (s - 1) / 2 : (s & 1) ? (s + 1) / 2 : (s - 2) / 2; };
@@ -500,7 +512,7 @@ __global__ void __launch_bounds__(CtCfg<KE, QE, HDP>::THREADS, 1) k_cache_attent
                     }
                     const uint32_t mine = to + (lu / 8) * F::KATOM;
                     const char *from = (is_v(s) ? vb : kb) + lu * 16;
-#pragma unroll 1
+#pragma unroll 4
                     for (int r = lr; r < KT; r += RPI) {
                         const int pos = t * KT + r;
                         const bool ok = in && there(pos);
@@ -583,7 +595,7 @@ int ct_run_as(const char *who, CmArgs a, int max_keys) {
         set = true;
     }
     const int rows = a.c.rows;
-    const int64_t row_units = (int64_t)a.c.nkv * a.tiles, row_chunks = row_units * (cdiv(a.c.cap, F::KT) + CT_START);
+    const int64_t row_units = (int64_t)a.c.nkv * a.tiles, row_chunks = row_units * (cdiv(a.c.cap, F::KT) + F::START);
     int64_t most = 0x70000000 / row_chunks;
     if (a.weights) {
         a.pitch = cdiv((int64_t)a.c.cap, CM_PITCH) * CM_PITCH;

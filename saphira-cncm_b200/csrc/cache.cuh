@@ -107,8 +107,9 @@ __device__ uint32_t select_kth(SelShared &s, int n, uint32_t k, uint32_t &ties, 
             cg::cluster_group cl = cg::this_cluster();
             cl.sync();
             c = make_uint4(0, 0, 0, 0);
-#pragma unroll 1
-            for (int r = 0; r < (int)cl.num_blocks(); r++) {
+#pragma unroll
+            for (int r = 0; r < 8; r++) {            // loads from the other CTAs all at once: each takes some 600 cycles
+                if (r >= (int)cl.num_blocks()) break;
                 const uint4 v = *(const uint4 *)(cl.map_shared_rank(hist, r) + b);
                 c.x += v.x; c.y += v.y; c.z += v.z; c.w += v.w;
             }

@@ -14,7 +14,7 @@
 
 namespace ncmb {
 
-constexpr int CM_WARPS = 4, CM_THREADS = CM_WARPS * 32;
+constexpr int CM_WARPS = 4, CM_THREADS = CM_WARPS * 32, CM_MAXC = 8;      // CM_MAXC: CTAs of a cluster
 // R: query rows of a tile, 16 or 8. A tile of 8 has two terms of its queries (or probabilities) stacked in the 16 rows of the
 // tensor-core tile; a lane holds rows lane / 4 and lane / 4 + 8 of a result, so it adds the two terms' products up itself.
 template <class KE, class QE, int HDP_, int R_> struct CmCfg {
@@ -640,26 +640,40 @@ __global__ void __launch_bounds__(CM_THREADS, CmCfg<KE, QE, HDP, R>::CTAS) k_cac
             else *(uint2 *)p = make_uint2(cm_pack(o.x * r, o.y * r), cm_pack(o.z * r, o.w * r));
         };
         if constexpr (CL) {
-            // a thread has the same four dims of a row in every CTA; row m's factors: every CTA's maximum against the cluster's
+            // the warps' contexts first, then the CTAs': a thread has the same four dims of a row in every CTA, scaled by that CTA's
+            // maximum against the cluster's. Loads from the others all at once: each takes some 600 cycles.
+#pragma unroll 1
+            for (int i = tid; i < nm * (HDP / 4); i += CM_THREADS) {
+                float4 *p = (float4 *)ctx_sh + i;
+                float4 o = *p;
+#pragma unroll
+                for (int w = 1; w < CM_WARPS; w++) {
+                    const float4 x = p[w * M * HDP / 4];
+                    o.x += x.x; o.y += x.y; o.z += x.z; o.w += x.w;
+                }
+                *p = o;
+            }
             cl.sync();
 #pragma unroll 1
             for (int i = rank * CM_THREADS + tid; i < nm * (HDP / 4); i += nc * CM_THREADS) {
                 const int m = i / (HDP / 4), d = i % (HDP / 4) * 4;
-                float top = -INFINITY, l = 0.f;
-                float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 1
-                for (int r = 0; r < nc; r++) top = fmaxf(top, *cl.map_shared_rank(&cmax[m], r));
-                const float base = top == -INFINITY ? 0.f : top;
-#pragma unroll 1
-                for (int r = 0; r < nc; r++) {
-                    const float f = cm_exp2(*cl.map_shared_rank(&cmax[m], r) - base);
-                    const float *cs = cl.map_shared_rank(ctx_sh, r) + m * HDP + d;
-                    l = fmaf(*cl.map_shared_rank(&wl[0][m], r), f, l);
+                float cm[CM_MAXC], cw[CM_MAXC], top = -INFINITY, l = 0.f;
+                float4 x[CM_MAXC], o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-                    for (int w = 0; w < CM_WARPS; w++) {
-                        const float4 x = *(const float4 *)(cs + w * M * HDP);
-                        o.x = fmaf(x.x, f, o.x); o.y = fmaf(x.y, f, o.y); o.z = fmaf(x.z, f, o.z); o.w = fmaf(x.w, f, o.w);
-                    }
+                for (int r = 0; r < CM_MAXC; r++) {
+                    const int rr = min(r, nc - 1);
+                    cm[r] = *cl.map_shared_rank(&cmax[m], rr);
+                    cw[r] = *cl.map_shared_rank(&wl[0][m], rr);
+                    x[r] = *((const float4 *)cl.map_shared_rank(ctx_sh, rr) + i);
+                    if (r >= nc) cm[r] = -INFINITY;
+                    top = fmaxf(top, cm[r]);
+                }
+                const float base = top == -INFINITY ? 0.f : top;
+#pragma unroll
+                for (int r = 0; r < CM_MAXC; r++) {
+                    const float f = cm_exp2(cm[r] - base);
+                    l = fmaf(cw[r], f, l);
+                    o.x = fmaf(x[r].x, f, o.x); o.y = fmaf(x[r].y, f, o.y); o.z = fmaf(x[r].z, f, o.z); o.w = fmaf(x[r].w, f, o.w);
                 }
                 if (d < hd) write(m, d, o, l);
             }
@@ -887,13 +901,7 @@ __global__ void __launch_bounds__(CM_THREADS) k_cache_join(const __grid_constant
 // ---- launches ----
 // slots of a CTA that adds up weights: it finds the sums of M queries first, then goes over M scores a slot
 inline int cm_wkeys(int M) { return M <= 32 ? 4 * CM_THREADS : CM_THREADS; }
-#ifndef CM_MAXC
-#define CM_MAXC 8
-#define CM_ROUNDS 8
-#endif
-#ifndef CM_FUSED
-#define CM_FUSED 24
-#endif
+constexpr int CM_ROUNDS = 8, CM_FUSED = 24;
 template <class KE, class QE, int HDP, int R, bool BLOCKS>
 int cm_run_as(const char *who, CmArgs a, int max_keys) {
     using F = CmCfg<KE, QE, HDP, R>;

@@ -6,6 +6,8 @@
 // is one token over budget moves one token, and in place no source is a target.
 #include "cache.cuh"
 
+#include <type_traits>
+
 namespace ncmb {
 namespace {
 
@@ -76,22 +78,31 @@ __global__ void __launch_bounds__(EV_THREADS) k_cache_evict(EvictArgs a) {
     uint32_t bound = 0, ties = 0xffffffffu;              // all are kept where there is room for all
     if (n2 < n) bound = select_kth<EV_THREADS, CL>(sel, hi - lo, (uint32_t)n2, ties, key);
 
-    // how many of something the slots before this warp's hold, given its own count; total: all CTAs'
+    // how many of something (of N things) the slots before this warp's hold, given its own counts; total: all CTAs'
     const int w0 = lo + warp * per_warp, w1 = min(hi, w0 + per_warp);
-    auto before = [&](int which, int mine, int &total) {
-        if (lane == 0) wcount[which][warp] = mine;
+    auto before = [&](auto first, int *mine, int *total) {
+        constexpr int N = decltype(first)::value == 0 ? 1 : 3, AT = decltype(first)::value;
+#pragma unroll
+        for (int i = 0; i < N; i++) if (lane == 0) wcount[AT + i][warp] = mine[i];
         __syncthreads();
-        const int v = lane < EV_WARPS ? wcount[which][lane] : 0;
-        int lead = __reduce_add_sync(0xffffffffu, lane < warp ? v : 0);
-        total = __reduce_add_sync(0xffffffffu, v);
-        if constexpr (CL) {
-            if (tid == 0) share[which] = total;
-            cl.sync();
-            const int o = lane < nc ? *cl.map_shared_rank(&share[which], lane) : 0;
-            lead += __reduce_add_sync(0xffffffffu, lane < rank ? o : 0);
-            total = __reduce_add_sync(0xffffffffu, o);
+        int v[N];
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            v[i] = lane < EV_WARPS ? wcount[AT + i][lane] : 0;
+            mine[i] = __reduce_add_sync(0xffffffffu, lane < warp ? v[i] : 0);
+            total[i] = __reduce_add_sync(0xffffffffu, v[i]);
         }
-        return lead;
+        if constexpr (CL) {
+#pragma unroll
+            for (int i = 0; i < N; i++) if (tid == 0) share[AT + i] = total[i];
+            cl.sync();
+#pragma unroll
+            for (int i = 0; i < N; i++) {
+                const int o = lane < nc ? *cl.map_shared_rank(&share[AT + i], lane) : 0;
+                mine[i] += __reduce_add_sync(0xffffffffu, lane < rank ? o : 0);
+                total[i] = __reduce_add_sync(0xffffffffu, o);
+            }
+        }
     };
     int all;
     uint32_t tied = 0;                                   // ties before, of which the lower ones are kept
@@ -99,7 +110,8 @@ __global__ void __launch_bounds__(EV_THREADS) k_cache_evict(EvictArgs a) {
         int mine = 0;
 #pragma unroll 1
         for (int s = w0; s < w1; s += 32) mine += __popc(__ballot_sync(0xffffffffu, s + lane < w1 && key(s + lane - lo) == bound));
-        tied = (uint32_t)before(0, mine, all);
+        before(std::integral_constant<int, 0>(), &mine, &all);
+        tied = (uint32_t)mine;
     }
     int freed = 0, beyond = 0, stay = 0;
 #pragma unroll 1
@@ -116,10 +128,10 @@ __global__ void __launch_bounds__(EV_THREADS) k_cache_evict(EvictArgs a) {
         beyond += __popc(km & ~below);
         stay += __popc(km & below);
     }
-    int moves;
-    freed = before(1, freed, moves);
-    beyond = before(2, beyond, all);
-    if (!a.inplace) stay = moves + before(3, stay, all);
+    int count[3] = {freed, beyond, stay}, totals[3];
+    before(std::integral_constant<int, 1>(), count, totals);
+    const int moves = totals[0];
+    freed = count[0]; beyond = count[1]; stay = moves + count[2];
     // pairs (from, to): moves, then -- to another cache -- the tokens that keep their slot
     int *from = a.from + u * a.room, *to = a.to + u * a.room;
     __syncwarp();
@@ -162,7 +174,7 @@ __global__ void __launch_bounds__(EV_THREADS) k_cache_evict(EvictArgs a) {
 }
 
 // The tokens that move, over the whole GPU. A thread has 16 bytes of a token's keys or values, of EV_AHEAD tokens.
-constexpr int EV_MTHREADS = 256, EV_AHEAD = 4;
+constexpr int EV_MTHREADS = 256, EV_AHEAD = 4;       // 8 ahead: 38 us where 4 take 28
 __global__ void __launch_bounds__(EV_MTHREADS) k_cache_move(EvictArgs a, int ul) {
     const int kvh = blockIdx.y, b = blockIdx.z, tid = threadIdx.x;
     const int x = tid & ((1 << ul) - 1), is_v = (tid >> ul) & 1, tok = tid >> (ul + 1), tpc = EV_MTHREADS >> (ul + 1);

@@ -426,7 +426,8 @@ void   ncmb_lm_nll(NcmbLM *m, const int *ids, int B, int T, const int *lens, dou
  * max_len (these four calls): an upper bound on the lengths that the host knows, by which the launch is sized; 0 =
  * capacity. Results are right where it is exceeded, only slower.
  * All four queue kernels on the library's stream and return 0, or print one line to stderr and return -1 for arguments
- * they refuse (nothing is queued then). Rounding: scores, exponentials, sums and weights are fp32 whatever the cache's
+ * they refuse (nothing is queued then). The wide tiles' waits are bounded and reported like the GEMM engines'
+ * (ncmb_gemm_tc_check). Rounding: scores, exponentials, sums and weights are fp32 whatever the cache's
  * type. A call's scratch memory is kept for the next one and grows on demand. No counterpart in the reference. */
 enum { NCMB_F32 = 0, NCMB_BF16 = 1 };
 #define NCMB_MAX_NODES 256
@@ -448,6 +449,9 @@ typedef struct {
  * T tokens and the query heads that share the kv head: added to slots [0, len[b]), stored to the T new ones. */
 int ncmb_cache_attention(const NcmbCache *c, const void *q, int64_t ldq, void *out, int64_t ldo, int act_type, int n_head,
                          int T, const int *parents, float scale, int max_len, float *weights);
+/* Diagnostic: which tiles ncmb_cache_attention takes for more than 16 query rows a kv head (T * n_head / n_kv): 0 by size
+ * (default), 1 tiles of 16 rows, 2 tiles of 128 rows where they take the shape. No counterpart in the reference. */
+void ncmb_set_cache_variant(int variant);
 /* Holds every (row, kv head) of a cache to `budget` tokens: kept are the `recent` tokens latest in the text, then those
  * with the largest weights, ties by the lower slot (a NaN weight ranks below all). With n = min(len[b], budget), kept
  * tokens of slots below n keep their slot and the freed slots below n take the kept tokens from beyond, both ascending:

@@ -182,6 +182,7 @@ _SIGS = {
     "ncmb_lm_nll": (None, [_P, _P, _I, _I, _P, _P]),
     "ncmb_weights_import_safetensors": (_I, [C.POINTER(WeightStore), C.c_char_p, _I]),
     "ncmb_cache_attention": (_I, [C.POINTER(KVCache), _P, _I64, _P, _I64, _I, _I, _I, _P, _F, _I, _P]),
+    "ncmb_set_cache_variant": (None, [_I]),
     "ncmb_cache_evict": (_I, [C.POINTER(KVCache), C.POINTER(KVCache), _P, _P, _P, _P, _P, _P, _I, _I, _I, _P]),
     "ncmb_block_summaries": (_I, [C.POINTER(KVCache), _I, _P, _I, _I, _P, _P]),
     "ncmb_block_attention": (_I, [C.POINTER(KVCache), _P, _I64, _P, _I64, _I, _I, _I, _I, _P, _P, _I, _I, _I, _F, _I, _P]),

@@ -83,21 +83,48 @@ int ct_map(const char *who, const CacheDev &c, const char *p, int kt, CUtensorMa
 
 namespace {
 
+int g_variant = 0;                   // ncmb_set_cache_variant
+
+// Which tiles: 16 (8) query rows on mma.sync, keys straight from a warp's ring, or 128 rows on tcgen05. By the times that a sweep
+// over 1 - 64 rows of 500 - 30000 tokens, 3 - 64 new tokens and 33 - 448 query rows a kv head gave, in us:
+//   narrow  8 + tiles of 16 rows x (NARROW x keys + 0.013)
+//   wide   14 + WIDE x tiles of 128 rows x (tiles of 128 keys + START), over the SMs
+// e.g. bf16 cache, fp32 queries, 2 x 64, narrow against wide: 1 x 4000 x 112 rows 11.1 / 16.8, 16 x 4000 x 56 rows 37 / 36,
+// x 448 rows 154 / 103; 8 x 128: 1 x 500 x 64 rows 11.9 / 24, 16 x 4000 x 64 rows 283 / 148, x 256 rows 1052 / 278.
+template <class KE, class QE, int HDP> struct Cost {
+    static constexpr bool Q32 = sizeof(QE) == 4;
+    static constexpr double NARROW = sizeof(KE) == 4 ? 111e-6 : HDP == 64 ? (Q32 ? 42e-6 : 30e-6) : (Q32 ? 126e-6 : 71e-6);
+    static constexpr double WIDE = sizeof(KE) == 4 ? 4.7 : HDP == 64 ? (Q32 ? 2.9 : 2.05) : (Q32 ? 4.3 : 2.3);
+};
+template <class KE, class QE, int HDP>
+bool takes_wide(const CmArgs &a, int max_keys) {
+    using F = CtCfg<KE, QE, HDP>;
+    using C = Cost<KE, QE, HDP>;
+    if (a.M <= 16 || g_variant == 1) return false;
+    if (g_variant == 2) return true;
+    const double heads = (double)a.c.rows * a.c.nkv;
+    const double narrow = 8 + heads * cdiv(a.M, 16) * (C::NARROW * max_keys + 0.013);
+    const double wide = 14 + C::WIDE * ceil(heads * cdiv(a.M, F::M) * (cdiv(max_keys, F::KT) + F::START) / ctx().sm_count);
+    return wide < narrow;
+}
+
+template <class KE, class QE, int HDP>
+int run_attention_hd(const char *who, const CmArgs &a, int max_keys) {
+    // (the terms of an fp32 cache's keys of more than 64 dims do not fit shared memory beside the queries')
+    if constexpr (sizeof(KE) == 2 || HDP == 64) { if (takes_wide<KE, QE, HDP>(a, max_keys)) return ct_run_as<KE, QE, HDP>(who, a, max_keys); }
+    return a.M <= 8 ? cm_run_as<KE, QE, HDP, 8, false>(who, a, max_keys) : cm_run_as<KE, QE, HDP, 16, false>(who, a, max_keys);
+}
 template <class KE, class QE>
 int run_attention(const char *who, const CmArgs &a, int max_keys) {
-    static const int dev = getenv("NCM_CT") ? atoi(getenv("NCM_CT")) : 1;
-    if (a.c.hd <= 64) {
-        if (dev && a.M > 16) return ct_run_as<KE, QE, 64>(who, a, max_keys);
-        return a.M <= 8 ? cm_run_as<KE, QE, 64, 8, false>(who, a, max_keys) : cm_run_as<KE, QE, 64, 16, false>(who, a, max_keys);
-    }
-    if constexpr (sizeof(KE) == 2) { if (dev && a.M > 16) return ct_run_as<KE, QE, 128>(who, a, max_keys); }
-    return a.M <= 8 ? cm_run_as<KE, QE, 128, 8, false>(who, a, max_keys) : cm_run_as<KE, QE, 128, 16, false>(who, a, max_keys);
+    return a.c.hd <= 64 ? run_attention_hd<KE, QE, 64>(who, a, max_keys) : run_attention_hd<KE, QE, 128>(who, a, max_keys);
 }
 
 } // namespace
 } // namespace ncmb
 
 using namespace ncmb;
+
+extern "C" void ncmb_set_cache_variant(int variant) { g_variant = variant; }
 
 extern "C" int ncmb_cache_attention(const NcmbCache *c, const void *q, int64_t ldq, void *out, int64_t ldo, int act_type, int n_head,
                                     int T, const int *parents, float scale, int max_len, float *weights) {

@@ -48,11 +48,12 @@ __device__ __forceinline__ int cache_len(const CacheDev &c, int row, int n_new) 
 // a launch in clusters of nc CTAs along x, started under its predecessor
 template <typename... KArgs, typename... Args>
 void cache_launch(void (*kernel)(KArgs...), dim3 grid, int threads, size_t smem, int nc, Args... args) {
+    static const bool off = getenv("NCM_B200_NO_PDL") != nullptr;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid; cfg.blockDim = dim3(threads); cfg.dynamicSmemBytes = smem; cfg.stream = stream();
     cudaLaunchAttribute at[2];
     at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at[0].val.programmaticStreamSerializationAllowed = 1;
+    at[0].val.programmaticStreamSerializationAllowed = off ? 0 : 1;
     at[1].id = cudaLaunchAttributeClusterDimension;
     at[1].val.clusterDim.x = nc; at[1].val.clusterDim.y = 1; at[1].val.clusterDim.z = 1;
     cfg.attrs = at; cfg.numAttrs = nc > 1 ? 2 : 1;

@@ -144,6 +144,8 @@ extern "C" int ncmb_cache_attention(const NcmbCache *c, const void *q, int64_t l
     a.H = n_head; a.G = n_head / c->n_kv; a.T = T; a.M = T * a.G; a.parents = parents; a.weights = weights;
     a.c2 = (scale == 0.f ? 1.0f / sqrtf((float)c->hd) : scale) * 1.44269504f;
     if (max_len <= 0 || max_len > c->capacity - T) max_len = c->capacity - T;
+    const double keys = (double)c->rows * c->n_kv * (max_len + T);      // by the bound: lengths are on the device
+    ProfScope prof(NCMB_K_ATTN, 4.0 * keys * a.M * c->hd, 2.0 * keys * c->hd * cache_elem(c));
     if (c->type == NCMB_F32) return run_attention<float, float>(who, a, max_len + T);
     if (act_type == NCMB_F32) return run_attention<__nv_bfloat16, float>(who, a, max_len + T);
     return run_attention<__nv_bfloat16, __nv_bfloat16>(who, a, max_len + T);

@@ -284,6 +284,7 @@ extern "C" int ncmb_block_summaries(const NcmbCache *c, int n_new, const int *fi
     const int nb = (int)cdiv(c->capacity, block);
     if (max_len <= 0 || max_len > c->capacity - n_new) max_len = c->capacity - n_new;
     const int hint = (int)cdiv((int64_t)max_len + n_new, block);
+    ProfScope prof(NCMB_K_ATTN, 0, (double)c->rows * c->n_kv * hint * block * c->hd * cache_elem(c));
     if (c->type == NCMB_F32) run_summaries<float>(d, n_new, first, block, nb, hint, codes, scales);
     else run_summaries<__nv_bfloat16>(d, n_new, first, block, nb, hint, codes, scales);
     return 0;
@@ -313,6 +314,7 @@ extern "C" int ncmb_block_attention(const NcmbCache *c, const void *q, int64_t l
     a.scale = scale == 0.f ? 1.0f / sqrtf((float)c->hd) : scale;
     const int64_t units = (int64_t)c->rows * T * c->n_kv;
     if (max_len <= 0 || max_len > c->capacity - T) max_len = c->capacity - T;
+    ProfScope prof(NCMB_K_ATTN, 4.0 * units * a.G * c->hd * n_sel * block, 2.0 * units * n_sel * block * c->hd * cache_elem(c));
     // CTAs a (row, token, head): as many as keep the GPU busy, with 512 blocks each at least. One row of 2047 blocks, the whole call:
     // with 256 / 512 / 1024 / 2048 blocks a CTA 20.0 / 18.1 / 20.3 / 24.4 us.
     int nc = 1;

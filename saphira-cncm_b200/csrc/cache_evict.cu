@@ -251,6 +251,7 @@ extern "C" int ncmb_cache_evict(const NcmbCache *src, const NcmbCache *dst, cons
     const int64_t most = cdiv(cdiv(src->capacity, nc * EV_WARPS), 32) * 32 * EV_WARPS, hint = cdiv(cdiv(max_len, nc * EV_WARPS), 32) * 32 * EV_WARPS;
     a.kcap = (int)(hint < EV_KEYS ? hint : EV_KEYS);
     const size_t smem = (size_t)a.kcap * 4 + (size_t)most / 8;
+    ProfScope prof(NCMB_K_ATTN, 0, 4.0 * units * max_len);
     auto kernel = nc > 1 ? k_cache_evict<true> : k_cache_evict<false>;
     if (smem > 20000) CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     cache_launch(kernel, dim3(nc, src->n_kv, src->rows), EV_THREADS, smem, nc, a);

@@ -171,20 +171,24 @@ __global__ void __launch_bounds__(BP_THREADS) k_block_pick(BlockArgs a) {
     // A tile of 8 blocks a warp at a time, the next one's codes on their way. Not unrolled: the whole of it runs a few times only, and
     // code that runs once is paced by instruction fetches (four tiles at once: 13000 cycles for 512 blocks of 128 dims).
     int2 ahead[4];
-    auto fetch = [&](int i) {
+    float scale_ahead;
+    auto fetch = [&](int i0) {
+        const int i = i0 + g4, j = i0 + 2 * c4 + (g4 & 1);
 #pragma unroll
         for (int s = 0; s < 4; s++) {
             ahead[s] = make_int2(0, 0);
             if (32 * s + 8 * c4 < hd && i < hi) ahead[s] = *(const int2 *)(codes + (int64_t)i * hd + 32 * s + 8 * c4);
         }
+        scale_ahead = j < hi ? scales[j] : 0.f;
     };
-    fetch(lo + warp * 8 + g4);
+    fetch(lo + warp * 8);
 #pragma unroll 1
     for (int i0 = lo + warp * 8; i0 < hi; i0 += BP_WARPS * 8) {
         int2 cd[4];
 #pragma unroll
         for (int s = 0; s < 4; s++) cd[s] = ahead[s];
-        fetch(i0 + BP_WARPS * 8 + g4);
+        const float block_scale = scale_ahead;
+        fetch(i0 + BP_WARPS * 8);
         float best[2] = {-INFINITY, -INFINITY};
 #pragma unroll 1
         for (int tt = 0; tt < gt; tt++) {
@@ -212,7 +216,7 @@ __global__ void __launch_bounds__(BP_THREADS) k_block_pick(BlockArgs a) {
         const int i = i0 + 2 * c4 + (g4 & 1);                                // lanes with g4 = 0, 1 have a block each
         if (g4 < 2 && i < hi) {
             const bool always = i < a.n_first || i > cur - a.n_last;
-            keys[i - lo] = always ? 0xffffffffu : float_key(__fmul_rn(g4 ? best[1] : best[0], scales[i]));
+            keys[i - lo] = always ? 0xffffffffu : float_key(__fmul_rn(g4 ? best[1] : best[0], block_scale));
         }
     }
     __syncthreads();

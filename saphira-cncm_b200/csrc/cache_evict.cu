@@ -15,6 +15,7 @@ namespace cg = cooperative_groups;
 
 constexpr int EV_THREADS = 512, EV_WARPS = EV_THREADS / 32, EV_MAXC = 8;
 constexpr int EV_KEYS = 24576;       // keys a CTA holds in shared memory; beyond, they are read again
+constexpr int EV_FEW = 8;
 constexpr int EV_MOST = 393216;      // slots of a row: a bit for each and EV_KEYS keys fit one CTA
 
 struct EvictArgs {
@@ -60,20 +61,83 @@ __global__ void __launch_bounds__(EV_THREADS) k_cache_evict(EvictArgs a) {
     const int per_warp = ((n + nc * EV_WARPS - 1) / (nc * EV_WARPS) + 31) & ~31;
     const int per = per_warp * EV_WARPS, lo = min(n, rank * per), hi = min(n, lo + per);
     auto place = [&](int s) { return s < known ? pos[s] : seen - n + s; };
-    if (tid == 0) maxpos = INT_MIN;
-    __syncthreads();
+    // the latest place in the text: of the tokens since the last eviction it is seen - 1
     int last = known < n ? seen - 1 : INT_MIN;
-    for (int s = lo + tid; s < min(hi, lo + a.kcap); s += EV_THREADS) keys[s - lo] = float_key(w[s]);
-    for (int s = lo + tid; s < min(hi, known); s += EV_THREADS) last = max(last, pos[s]);
-    last = __reduce_max_sync(0xffffffffu, last);
-    if (lane == 0) atomicMax(&maxpos, last);
-    sync();
-    if constexpr (CL) { for (int r = 0; r < nc; r++) last = max(last, *cl.map_shared_rank(&maxpos, r)); }
-    else last = maxpos;
     auto latest = [&](int s) { return (int64_t)place(s) > (int64_t)last - a.recent; };
+    if (known == 0) {
+        for (int s = lo + tid; s < min(hi, lo + a.kcap); s += EV_THREADS) keys[s - lo] = latest(s) ? 0xffffffffu : float_key(w[s]);
+    } else {
+        if (tid == 0) maxpos = INT_MIN;
+        __syncthreads();
+        for (int s = lo + tid; s < min(hi, lo + a.kcap); s += EV_THREADS) keys[s - lo] = float_key(w[s]);
+        for (int s = lo + tid; s < min(hi, known); s += EV_THREADS) last = max(last, pos[s]);
+        last = __reduce_max_sync(0xffffffffu, last);
+        if (lane == 0) atomicMax(&maxpos, last);
+        sync();
+        if constexpr (CL) { for (int r = 0; r < nc; r++) last = max(last, *cl.map_shared_rank(&maxpos, r)); }
+        else last = maxpos;
 #pragma unroll 1
-    for (int s = lo + tid; s < min(hi, lo + a.kcap); s += EV_THREADS) if (latest(s)) keys[s - lo] = 0xffffffffu;
+        for (int s = lo + tid; s < min(hi, lo + a.kcap); s += EV_THREADS) if (latest(s)) keys[s - lo] = 0xffffffffu;
+    }
     __syncthreads();
+    const char *k = a.c.k + b * a.c.rs + kvh * a.c.hs, *v = a.c.v + b * a.c.rs + kvh * a.c.hs;
+    char *k2 = a.k2 + b * a.rs2 + kvh * a.hs2, *v2 = a.v2 + b * a.rs2 + kvh * a.hs2;
+    const int units = a.c.hd * a.es / 16;                // of 16 bytes in a token's keys
+    auto move = [&](int64_t f, int64_t t) {              // a warp
+        if (lane < units) {
+            const int4 kx = *(const int4 *)(k + f * a.c.ts + lane * 16), vx = *(const int4 *)(v + f * a.c.ts + lane * 16);
+            *(int4 *)(k2 + t * a.ts2 + lane * 16) = kx;
+            *(int4 *)(v2 + t * a.ts2 + lane * 16) = vx;
+        }
+    };
+    if (!CL && a.inplace && n - n2 <= EV_FEW && n <= a.kcap) {
+        // A few tokens over budget, as after a decode step: the lowest keys one after another (of equal ones the highest slot goes)
+        // instead of a selection among all. One over 2048, 64 rows: 4.3 us a call, by selection 9.6.
+        __shared__ unsigned long long low[2];
+        __shared__ int gone[EV_FEW], from[EV_FEW], to[EV_FEW], moves;
+#pragma unroll 1
+        for (int d = 0; d < n - n2; d++) {
+            if (tid == 0) low[d & 1] = ~0ull;
+            __syncthreads();
+            uint32_t best = 0xffffffffu, at = 0;         // smallest key, then largest slot
+            bool any = false;
+#pragma unroll 4
+            for (int s = tid; s < n; s += EV_THREADS) {
+                bool out = false;
+                for (int x = 0; x < d; x++) out |= gone[x] == s;
+                if (!out && (!any || keys[s] <= best)) { best = keys[s]; at = s; any = true; }
+            }
+            const uint32_t wmin = __reduce_min_sync(0xffffffffu, best);
+            const uint32_t wat = __reduce_max_sync(0xffffffffu, any && best == wmin ? at + 1 : 0u);      // 0: no slot in this warp
+            if (lane == 0 && wat) atomicMin(&low[d & 1], (unsigned long long)wmin << 32 | (0xffffffffu - wat));
+            __syncthreads();
+            if (tid == 0) gone[d] = (int)(0xffffffffu - (uint32_t)low[d & 1]) - 1;
+            __syncthreads();
+        }
+        if (tid == 0) {
+            int m = 0;
+            for (int s = n2; s < n; s++) {               // kept ones from beyond, ascending
+                bool out = false;
+                for (int x = 0; x < n - n2; x++) out |= gone[x] == s;
+                if (!out) from[m++] = s;
+            }
+            for (int i = 0, last = -1; i < m; i++) {     // freed slots, ascending
+                int next = n2;
+                for (int x = 0; x < n - n2; x++) if (gone[x] > last && gone[x] < next) next = gone[x];
+                to[i] = last = next;
+            }
+            moves = m;
+            a.pairs[u] = 0;                              // nothing is left for k_cache_move
+        }
+        __syncthreads();
+        for (int s = known + tid; s < n2; s += EV_THREADS) a.pos2[u * a.cap2 + s] = seen - n + s;
+        __syncthreads();                                 // a freed slot's place is written last
+        for (int i = warp; i < moves; i += EV_WARPS) {
+            if (lane == 0) { a.w2[u * a.cap2 + to[i]] = w[from[i]]; a.pos2[u * a.cap2 + to[i]] = place(from[i]); }
+            move(from[i], to[i]);
+        }
+        return;
+    }
     auto key = [&](int i) { return i < a.kcap ? keys[i] : latest(lo + i) ? 0xffffffffu : float_key(w[lo + i]); };
     uint32_t bound = 0, ties = 0xffffffffu;              // all are kept where there is room for all
     if (n2 < n) bound = select_kth<EV_THREADS, CL>(sel, hi - lo, (uint32_t)n2, ties, key);
@@ -160,17 +224,7 @@ __global__ void __launch_bounds__(EV_THREADS) k_cache_evict(EvictArgs a) {
     }
     if (rank == 0 && tid == 0) a.pairs[u] = pairs;
     if (!a.move_here) return;
-    const char *k = a.c.k + b * a.c.rs + kvh * a.c.hs, *v = a.c.v + b * a.c.rs + kvh * a.c.hs;
-    char *k2 = a.k2 + b * a.rs2 + kvh * a.hs2, *v2 = a.v2 + b * a.rs2 + kvh * a.hs2;
-    const int units = a.c.hd * a.es / 16;                // of 16 bytes in a token's keys
-    for (int p = rank * EV_WARPS + warp; p < pairs; p += nc * EV_WARPS) {
-        const int64_t f = from[p], t = to[p];
-        if (lane < units) {
-            const int4 kx = *(const int4 *)(k + f * a.c.ts + lane * 16), vx = *(const int4 *)(v + f * a.c.ts + lane * 16);
-            *(int4 *)(k2 + t * a.ts2 + lane * 16) = kx;
-            *(int4 *)(v2 + t * a.ts2 + lane * 16) = vx;
-        }
-    }
+    for (int p = rank * EV_WARPS + warp; p < pairs; p += nc * EV_WARPS) move(from[p], to[p]);
 }
 
 // The tokens that move, over the whole GPU. A thread has 16 bytes of a token's keys or values, of EV_AHEAD tokens.
@@ -247,6 +301,7 @@ extern "C" int ncmb_cache_evict(const NcmbCache *src, const NcmbCache *dst, cons
     int nc = 1;
     while (nc < EV_MAXC && units * nc * 2 <= 2 * ctx().sm_count && cdiv(max_len, nc) > 4096) nc *= 2;
     a.move_here = a.inplace && max_len - a.room <= 64;   // that many tokens move at most, by what the host knows
+    if (a.inplace && max_len - a.room <= EV_FEW && max_len <= EV_KEYS) nc = 1;       // no selection: one CTA is enough
     // slots of a CTA when the row is as long as the cache can hold: bits for all, keys for as many as shared memory takes
     const int64_t most = cdiv(cdiv(src->capacity, nc * EV_WARPS), 32) * 32 * EV_WARPS, hint = cdiv(cdiv(max_len, nc * EV_WARPS), 32) * 32 * EV_WARPS;
     a.kcap = (int)(hint < EV_KEYS ? hint : EV_KEYS);

@@ -839,8 +839,10 @@ __global__ void __launch_bounds__(CM_THREADS) k_cache_join(const __grid_constant
     const float *sc = a.scores + ((int64_t)item * a.c.nkv + kvh) * a.M * a.pitch;
     float *wp = a.weights + ((int64_t)row * a.c.nkv + kvh) * a.c.cap;
     const int stop = min(n, key0 + wkeys);
-    float early[R == 8 ? 8 : 1][4];                              // few rows: the scores are on their way while the sums are formed
+    float early[R == 8 ? 8 : 1][4], old[4];                      // few rows: scores and weights are on their way while the sums are formed
     if constexpr (R == 8) {
+#pragma unroll
+        for (int x = 0; x < 4; x++) old[x] = key0 + tid + x * CM_THREADS < min(stop, len) ? wp[key0 + tid + x * CM_THREADS] : 0.f;
 #pragma unroll
         for (int i = 0; i < 8; i++)
 #pragma unroll
@@ -886,7 +888,8 @@ __global__ void __launch_bounds__(CM_THREADS) k_cache_join(const __grid_constant
 #pragma unroll
             for (int x = 0; x < 4; x++) {
                 const int key = key0 + tid + x * CM_THREADS;
-                if (key < stop) wp[key] = mb || key < len ? wp[key] + w[x] : w[x];       // the new tokens' slots are stored to, the others added to
+                if (key >= stop) continue;                       // the new tokens' slots are stored to, the others added to
+                wp[key] = R == 8 ? old[x] + w[x] : mb || key < len ? wp[key] + w[x] : w[x];
             }
         } else if (key0 + tid < stop) {
             const int key = key0 + tid;

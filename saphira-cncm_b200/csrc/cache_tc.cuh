@@ -9,9 +9,11 @@
 // write the results), warp 8 issues the MMAs, the others load: keys of the next tile, values of this one, in turn through
 // one ring -- bf16 by cp.async, fp32 through registers, where the terms are formed.
 //
-// Tiles are 128 keys wide because MMAs are paced by operand fetch: 128 x 64 x 16 takes about 100 cycles, as long as
-// 128 x 128 x 16, and probabilities in shared memory would be fetched again by every MMA (64-key tiles with probabilities
-// in shared memory: 2.5 times the time of this one).
+// Tiles are 128 keys wide and probabilities stand in tensor memory because MMAs are paced by operand fetch: 64-wide ones took about
+// 100 cycles each with both operands in shared memory, 128-wide ones 90 with A in tensor memory (arithmetic: 16 and 32). Bound by
+// the chain of a tile: products with the values, then the exponentials of the next tile, which wait for the tensor memory that
+// the products read: 3900 cycles for 64 KB of keys and values at head dim 128. 16 rows of up to 8192 tokens, 32 heads over 8 x
+// 128, 16 drafted tokens: 105 us, of which 51 are the time the bytes take (64-key tiles by cp.async: 179).
 #pragma once
 #include "cache_mma.cuh"
 #include "tc_common.cuh"

@@ -452,10 +452,11 @@ int ncmb_cache_attention(const NcmbCache *c, const void *q, int64_t ldq, void *o
 /* Diagnostic: which tiles ncmb_cache_attention takes for more than 16 query rows a kv head (T * n_head / n_kv): 0 by size
  * (default), 1 tiles of 16 rows, 2 tiles of 128 rows where they take the shape. No counterpart in the reference. */
 void ncmb_set_cache_variant(int variant);
-/* Holds every (row, kv head) of a cache to `budget` tokens: kept are the `recent` tokens latest in the text, then those
- * with the largest weights, ties by the lower slot (a NaN weight ranks below all). With n = min(len[b], budget), kept
- * tokens of slots below n keep their slot and the freed slots below n take the kept tokens from beyond, both ascending:
- * attention does not depend on the order, and a step that is one token over budget moves one token.
+/* Holds every (row, kv head) of a cache to `budget` tokens: kept are the tokens in the text's last min(recent, budget)
+ * places, then those with the largest weights, ties by the lower slot (a NaN weight ranks below all); so recent >=
+ * budget is a sliding window. With n = min(len[b], budget), kept tokens of slots below n keep their slot and the freed
+ * slots below n take the kept tokens from beyond, both ascending: attention does not depend on the order, and a step
+ * that is one token over budget moves one token.
  * dst == src (same k and v): in place. Else dst is another cache that does not overlap src, of the same type, rows,
  * n_kv and hd and of a capacity of budget (or of src's capacity, if less) at least; only its k, v and strides are used.
  * weights [rows][n_kv][src->capacity], weights_dst [rows][n_kv][dst->capacity] (the same array in place).

@@ -1,6 +1,6 @@
 // A cache held to a budget of tokens by the attention each has received (ncmb_cache_evict, include/ncm_b200.h).
 //
-// Per (row, kv head) of n tokens, n2 = min(n, budget) are kept: key = the weight as an ordered integer, the `recent`
+// Per (row, kv head) of n tokens, n2 = min(n, budget) are kept: key = the weight as an ordered integer, the min(recent, budget)
 // latest tokens above all; the n2-th largest key by three counting passes; of the tokens that tie with it those in the
 // lower slots. Kept tokens below slot n2 stay where they are and the others take the freed slots in order, so a step that
 // is one token over budget moves one token, and in place no source is a target.
@@ -292,7 +292,8 @@ extern "C" int ncmb_cache_evict(const NcmbCache *src, const NcmbCache *dst, cons
     if (!a.inplace && overlaps(a.c, d, es)) return cache_refuse(who, "the two caches overlap");
     ensure_device();
     a.k2 = (char *)dst->k; a.v2 = (char *)dst->v; a.rs2 = d.rs; a.hs2 = d.hs; a.ts2 = d.ts; a.cap2 = d.cap;
-    a.budget = budget; a.recent = recent; a.es = es;
+    // The latest tokens rank alike, so no more of them than the budget holds may count as such: else the lower slots stay, the oldest.
+    a.budget = budget; a.recent = recent < budget ? recent : budget; a.es = es;
     a.w = weights; a.w2 = weights_dst; a.pos = pos; a.pos2 = pos_dst; a.known = known; a.seen = seen; a.len2 = len_dst;
     if (max_len <= 0 || max_len > src->capacity) max_len = src->capacity;
     const int64_t units = (int64_t)src->rows * src->n_kv;

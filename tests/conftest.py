@@ -15,6 +15,15 @@ def pytest_configure(config):
     config.addinivalue_line("markers", "gpu: needs a CUDA device (run on the B200 box)")
 
 
+# Cases that stand as they were written although what they expect is wrong -- with more `recent` tokens than the budget holds they want
+# the oldest of them kept; test_gpu_cache_eviction_windows.py has what is right. They fail, after everything else has run.
+OLDEST_KEPT = "test_gpu_cache_operators.py::test_eviction[lens7-300-5000-0-"
+
+
+def pytest_collection_modifyitems(items):
+    items.sort(key=lambda item: OLDEST_KEPT in item.nodeid)
+
+
 @pytest.fixture(scope="session")
 def model_dir(tmp_path_factory):
     return str(tmp_path_factory.mktemp("models"))

@@ -447,10 +447,14 @@ __global__ void __launch_bounds__(CM_THREADS, CmCfg<KE, QE, HDP, R>::CTAS) k_cac
 #pragma unroll
                 for (int hh = 0; hh < NH; hh++) {
                     const int mm = m0 + g + 8 * hh;
-                    if (mm < a.M) {
+                    if (mm >= a.M) continue;
+                    if (par && !used(mm / G)) {                  // no token, no share: its scores are zeros by keys that may hold anything
 #pragma unroll
-                        for (int j = 0; j < NT; j++) *(float2 *)(sp + mm * a.pitch + 8 * j) = make_float2(S[j][2 * hh], S[j][2 * hh + 1]);
+                        for (int j = 0; j < NT; j++) *(float2 *)(sp + mm * a.pitch + 8 * j) = make_float2(-INFINITY, -INFINITY);
+                        continue;
                     }
+#pragma unroll
+                    for (int j = 0; j < NT; j++) *(float2 *)(sp + mm * a.pitch + 8 * j) = make_float2(S[j][2 * hh], S[j][2 * hh + 1]);
                 }
             }
             float al[NH];
@@ -638,7 +642,8 @@ __global__ void __launch_bounds__(CM_THREADS, CmCfg<KE, QE, HDP, R>::CTAS) k_cac
         const int nm = min(M, a.M - m0);                         // rows that hold a query
         auto write = [&](int m, int d, float4 o, float l) {      // a result, four dims of a row
             const int mm = m0 + m, t = BLOCKS ? tok : mm / G, h = kvh * G + mm % G;
-            const float r = l > 0.f && (BLOCKS || used(t)) ? 1.f / l : 0.f;
+            const float r = l > 0.f ? 1.f / l : 0.f;
+            if (!BLOCKS && !used(t)) o = make_float4(0.f, 0.f, 0.f, 0.f);        // not by r = 0: values may hold infinities
             QE *p = (QE *)(a.out + ((int64_t)row * a.T + t) * a.ldo) + (int64_t)h * hd + d;
             if constexpr (sizeof(QE) == 4) *(float4 *)p = make_float4(o.x * r, o.y * r, o.z * r, o.w * r);
             else *(uint2 *)p = make_uint2(cm_pack(o.x * r, o.y * r), cm_pack(o.z * r, o.w * r));
@@ -833,7 +838,8 @@ __global__ void __launch_bounds__(CM_THREADS) k_cache_join(const __grid_constant
         }
         if (mm >= a.M || d >= hd) return;
         const int t = BLOCKS ? item % a.T : mm / G, h = kvh * G + mm % G;
-        const float r = l > 0.f && (BLOCKS || cm_used(par, t)) ? 1.f / l : 0.f;
+        const float r = l > 0.f ? 1.f / l : 0.f;
+        if (!BLOCKS && !cm_used(par, t)) o = make_float4(0.f, 0.f, 0.f, 0.f);
         QE *out = (QE *)(a.out + ((int64_t)row * a.T + t) * a.ldo) + (int64_t)h * hd + d;
         cm_put(out, o.x * r); cm_put(out + 1, o.y * r); cm_put(out + 2, o.z * r); cm_put(out + 3, o.w * r);
         return;

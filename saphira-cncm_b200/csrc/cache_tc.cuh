@@ -268,6 +268,10 @@ __global__ void __launch_bounds__(CtCfg<KE, QE, HDP>::THREADS, 1) k_cache_attent
                         for (int j = 0; j < 32; j++) top = fmaxf(top, __uint_as_float(sr[j]));
                         if (a.scores && mm < a.M) {
                             float *sp = a.scores + (((int64_t)u.item * a.c.nkv + u.kvh) * a.M + mm) * a.pitch + p0 + 32 * c;
+                            if (!row_used) {                         // no token, no share: its scores are zeros by keys that may hold anything
+#pragma unroll
+                                for (int j = 0; j < 32; j++) sr[j] = 0xff800000u;
+                            }
 #pragma unroll
                             for (int j = 0; j < 32; j += 4)
                                 *(float4 *)(sp + j) = make_float4(__uint_as_float(sr[j]) * c2, __uint_as_float(sr[j + 1]) * c2,
@@ -389,7 +393,11 @@ __global__ void __launch_bounds__(CtCfg<KE, QE, HDP>::THREADS, 1) k_cache_attent
             if (hf == 0) { slot[r] = mx; slot[M + r] = l; }
             if (mm < a.M) {
                 if (u.whole) {
-                    const float f = l > 0.f && row_used ? 1.f / l : 0.f;
+                    const float f = l > 0.f ? 1.f / l : 0.f;
+                    if (!row_used) {                                 // not by f = 0: values may hold infinities
+#pragma unroll
+                        for (int d = 0; d < HC; d++) O[d] = 0.f;
+                    }
                     QE *o = (QE *)(a.out + ((int64_t)u.row * a.T + node) * a.ldo) + (int64_t)(u.kvh * G + mm - node * G) * hd + hf * HC;
 #pragma unroll
                     for (int d = 0; d < HC; d += 4) {

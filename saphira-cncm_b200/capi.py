@@ -47,15 +47,23 @@ class KVCache(C.Structure):
 
     @classmethod
     def of(cls, k, v, length):
-        """From device arrays with ``data_ptr`` / ``stride`` / ``shape`` (torch tensors): k and v as views
-        [rows][n_kv][capacity][hd] of one layout, length int32[rows]. The caller keeps the arrays alive."""
+        """From torch tensors: k and v as float32 or bfloat16 views [rows][n_kv][capacity][hd] of one layout, length
+        int32[rows], contiguous. The cache keeps them alive (``held``)."""
+        kinds = {"torch.float32": F32, "torch.bfloat16": BF16}
+        if len(k.shape) != 4:
+            raise ValueError("keys and values are [rows][n_kv][capacity][hd]")
         if tuple(k.shape) != tuple(v.shape) or tuple(k.stride()) != tuple(v.stride()) or k.dtype != v.dtype:
             raise ValueError("keys and values differ in shape, strides or type")
         if k.stride(3) != 1 and k.shape[3] > 1:
             raise ValueError("the head dim has to be contiguous")
-        kind = {4: F32, 2: BF16}[k.element_size()]
+        if str(k.dtype) not in kinds:
+            raise ValueError("a cache of %s: float32 or bfloat16" % k.dtype)
         b, h, n, d = k.shape
-        c = cls(k.data_ptr(), v.data_ptr(), kind, b, h, d, n, k.stride(0), k.stride(1), k.stride(2), length.data_ptr())
+        if str(length.dtype) != "torch.int32" or tuple(length.shape) != (b,) or (b > 1 and length.stride(0) != 1):
+            raise ValueError("lengths are a contiguous int32[rows]")
+        if k.device != v.device or k.device != length.device:
+            raise ValueError("keys, values and lengths are on different devices")
+        c = cls(k.data_ptr(), v.data_ptr(), kinds[str(k.dtype)], b, h, d, n, k.stride(0), k.stride(1), k.stride(2), length.data_ptr())
         c.held = (k, v, length)
         return c
 

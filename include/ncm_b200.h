@@ -463,7 +463,8 @@ void ncmb_set_cache_variant(int variant);
  * pos / pos_dst, int arrays of the same shapes: place in the text of each slot's token. Input pos is read for slots
  * below known[b] only (device int[rows], NULL = 0: none); a slot beyond is the place seen[b] - len[b] + slot, that is,
  * seen[b] (device int[rows]) tokens of the text have passed and the last ones stand in order. So known = the len_dst of
- * the eviction before. len_dst: device int[rows], receives n; must not be src->len. len at most 393216. */
+ * the eviction before. len_dst: device int[rows], receives n; may be the array of known or seen, but not share memory with
+ * src->len. len at most 393216. */
 int ncmb_cache_evict(const NcmbCache *src, const NcmbCache *dst, const float *weights, float *weights_dst, const int *pos,
                      int *pos_dst, const int *known, const int *seen, int budget, int recent, int max_len, int *len_dst);
 /* Mean keys of blocks of `block` (16, 32, 64 or 128) slots in 8 bits, for the call below. Slots [0, len[b] + n_new) hold

@@ -279,8 +279,10 @@ extern "C" int ncmb_cache_evict(const NcmbCache *src, const NcmbCache *dst, cons
     if (budget < 1 || recent < 0) return cache_refuse(who, "budget %d, recent %d", budget, recent);
     if (src->capacity > EV_MOST) return cache_refuse(who, "capacity %d: at most %d slots", src->capacity, EV_MOST);
     if (!weights || !weights_dst || !pos || !pos_dst || !seen || !len_dst) return cache_refuse(who, "a null pointer");
-    if (len_dst == src->len) return cache_refuse(who, "len_dst has to be another array than the lengths of the cache");
     if (src->rows == 0) return 0;
+    const int64_t rows = src->rows;
+    auto with_len_dst = [&](const int *p) { return p < len_dst + rows && len_dst < p + rows; };
+    if (with_len_dst(src->len)) return cache_refuse(who, "len_dst has to be another array than the lengths of the cache");
     a.inplace = src->k == dst->k && src->v == dst->v;
     if (a.inplace && (src->capacity != dst->capacity || src->row_stride != dst->row_stride || src->head_stride != dst->head_stride || src->token_stride != dst->token_stride))
         return cache_refuse(who, "one cache with two layouts");
@@ -297,10 +299,19 @@ extern "C" int ncmb_cache_evict(const NcmbCache *src, const NcmbCache *dst, cons
     a.w = weights; a.w2 = weights_dst; a.pos = pos; a.pos2 = pos_dst; a.known = known; a.seen = seen; a.len2 = len_dst;
     if (max_len <= 0 || max_len > src->capacity) max_len = src->capacity;
     const int64_t units = (int64_t)src->rows * src->n_kv;
-    a.from = (int *)cache_scratch(who, units * a.room * 8 + units * 4);
+    a.from = (int *)cache_scratch(who, units * a.room * 8 + units * 4 + rows * 8);
     if (!a.from) return -1;
     a.to = a.from + units * a.room;
     a.pairs = a.to + units * a.room;
+    // A row's new length is stored by its first CTA when others may not have read `known` or `seen` yet: where these are the array of the
+    // lengths -- the last call's len_dst is this one's known -- the kernel reads copies.
+    int *copy = a.pairs + units;
+    for (const int **x : {&a.known, &a.seen}) {
+        if (!*x || !with_len_dst(*x)) continue;
+        CUDA_CHECK(cudaMemcpyAsync(copy, *x, rows * 4, cudaMemcpyDeviceToDevice, stream()));
+        *x = copy;
+        copy += rows;
+    }
     // CTAs a (row, head): as many as keep the GPU busy, with 4096 slots each at least
     int nc = 1;
     while (nc < EV_MAXC && units * nc * 2 <= 2 * ctx().sm_count && cdiv(max_len, nc) > 4096) nc *= 2;

@@ -55,6 +55,8 @@ struct CmArgs {
     float c2;                        // scale * log2(e)
     float *part;                     // partial results, one slot a (CTA + unit)
     int2 *range;                     // first and last CTA of each unit
+    int ctas;                        // CTAs of the attention kernel
+    const int *err;                  // wide tiles: set when a wait ran out, and then `range` and `part` may be what was there before
     int *done;                       // chunks of each unit that are in `part`, zero between calls; null: k_cache_join joins
     float *scores;                   // [row][kv head][M][pitch], or null
     int64_t pitch;
@@ -774,6 +776,11 @@ __global__ void __launch_bounds__(CM_THREADS, CmCfg<KE, QE, HDP, R>::CTAS) k_cac
 // has a row, or (`split`: few units, each in many parts) all have the same row and every one a share of its parts.
 // The others: `wkeys` slots of one (row, kv head) each, from the scores that the kernel above left.
 constexpr int CM_PITCH = 128;        // scores of a query: whole tiles of keys
+// The CTAs that have a part of a unit; none (0, -1) for a range that the attention kernel cannot have written: `part` is not read by it
+__device__ __forceinline__ int2 cm_range(const CmArgs &a, int64_t unit) {
+    const int2 r = a.range[unit];
+    return r.x >= 0 && r.x <= r.y && r.y < a.ctas ? r : make_int2(0, -1);
+}
 template <class KE, class QE, int HDP, int R, bool BLOCKS>
 __global__ void __launch_bounds__(CM_THREADS) k_cache_join(const __grid_constant__ CmArgs a, int joins, int split, int wkeys) {
     using F = CmCfg<KE, QE, HDP, R>;
@@ -784,6 +791,7 @@ __global__ void __launch_bounds__(CM_THREADS) k_cache_join(const __grid_constant
     const int tid = threadIdx.x, G = a.G, hd = a.c.hd;
     pdl_wait();
     pdl_launch_dependents();           // after the wait: one kernel ahead, not a queue of them that takes the SMs' room
+    const int gave_up = a.err ? __ldcg(a.err) : 0;               // CTAs that saw it set have left without a result
     const bool join = (int)blockIdx.x < joins;
     const int per_item = a.c.nkv * a.tiles, rows = split ? 1 : GROUPS, steps = M / rows;      // rows a CTA, CTAs a unit
     int item, sub, key0 = 0;
@@ -798,9 +806,9 @@ __global__ void __launch_bounds__(CM_THREADS) k_cache_join(const __grid_constant
     const int *par = a.parents ? a.parents + (int64_t)row * a.T : nullptr;
     const int64_t unit0 = (int64_t)item * per_item + sub;
     if (join) {
-        const int2 cr = a.range[unit0];                          // CTAs that have a part of it
+        const int2 cr = cm_range(a, unit0);
         const int c0 = cr.x, c1 = cr.y;
-        if (c0 == c1) return;                                    // written already
+        if (c0 >= c1 || gave_up) return;                         // written already
         const float *slot = a.part + ((int64_t)c0 + (int64_t)item * per_item + sub) * F::SLOT;
         const int grp = tid / D4, d = tid % D4 * 4, kvh = sub / a.tiles;
         const int m = (int)(blockIdx.x % steps) * rows + (split ? 0 : grp), mm = sub % a.tiles * M + m;
@@ -845,7 +853,7 @@ __global__ void __launch_bounds__(CM_THREADS) k_cache_join(const __grid_constant
         return;
     }
     const int kvh = sub / a.tiles, n = cm_keys<BLOCKS>(a, item), len = n - a.T;
-    if (key0 >= n) return;
+    if (key0 >= n || gave_up) return;
     const float *sc = a.scores + ((int64_t)item * a.c.nkv + kvh) * a.M * a.pitch;
     float *wp = a.weights + ((int64_t)row * a.c.nkv + kvh) * a.c.cap;
     const int stop = min(n, key0 + wkeys);
@@ -867,7 +875,7 @@ __global__ void __launch_bounds__(CM_THREADS) k_cache_join(const __grid_constant
         for (int i = tid; i < nm; i += CM_THREADS) {
             const int mm = mb + i, m = mm % M;
             const int64_t u = unit0 + mm / M;
-            const int2 cr = a.range[u];
+            const int2 cr = cm_range(a, u);
             const float *slot = a.part + (cr.x + u) * F::SLOT;
             float top = -INFINITY, l = 0.f;
 #pragma unroll 4
@@ -956,6 +964,7 @@ int cm_run_as(const char *who, CmArgs a, int max_keys) {
     a.scores = a.weights ? (float *)scratch : nullptr;
     a.range = (int2 *)(scratch + sc);
     a.part = (float *)(scratch + sc + ranges);
+    a.ctas = ctas;
     // Few parts a unit: the CTA that finishes it joins them. Many: a kernel of its own, which has a CTA for each row of a
     // unit; it also adds up weights.
     const bool fused = !a.weights && ctas <= CM_FUSED * units;

@@ -623,6 +623,8 @@ int ct_run_as(const char *who, CmArgs a, int max_keys) {
     a.scores = a.weights ? (float *)scratch : nullptr;
     a.range = (int2 *)(scratch + sc);
     a.part = (float *)(scratch + sc + ranges);
+    a.ctas = ctas;
+    a.err = tc_err_flag();
     const int split = ctas > 4 * units;
     for (int r = 0; r < rows; r += step) {
         const int nr = std::min(step, rows - r);

@@ -791,7 +791,7 @@ __global__ void __launch_bounds__(CM_THREADS) k_cache_join(const __grid_constant
     const int tid = threadIdx.x, G = a.G, hd = a.c.hd;
     pdl_wait();
     pdl_launch_dependents();           // after the wait: one kernel ahead, not a queue of them that takes the SMs' room
-    const int gave_up = a.err ? __ldcg(a.err) : 0;               // CTAs that saw it set have left without a result
+    const int gave_up = a.err ? *a.err : 0;               // CTAs that saw it set have left without a result
     const bool join = (int)blockIdx.x < joins;
     const int per_item = a.c.nkv * a.tiles, rows = split ? 1 : GROUPS, steps = M / rows;      // rows a CTA, CTAs a unit
     int item, sub, key0 = 0;

@@ -39,10 +39,13 @@ template <class KE, class QE, int HDP_> struct CtCfg {
 __host__ __device__ constexpr uint32_t umma_idesc_bf16(int M, int N) {
     return (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
 }
+// Every wait is bounded. The warps of the softmax, which meet at barriers of their own, go on without waiting once one has run out;
+// whoever starts copies or MMAs starts no more, and nobody leaves before those under way have ended (or a limit has passed).
 struct CtWait {
-    int *err; bool dead;
+    int *err, *any;                  // any: in shared memory, for the whole CTA
+    bool dead;
     __device__ __forceinline__ void operator()(uint32_t bar, uint32_t parity, int code) {
-        if (!dead && !mbar_wait(bar, parity, err, code)) dead = true;
+        if (!dead && !mbar_wait(bar, parity, err, code)) { dead = true; *any = 1; }
     }
 };
 // the same MMA with A in tensor memory (16-bit elements, two to a column)
@@ -86,13 +89,14 @@ __global__ void __launch_bounds__(CtCfg<KE, QE, HDP>::THREADS, 1) k_cache_attent
     auto empty = [&](int s) { return cm_smem(&bars[8 + s]); };
     const uint32_t bar_q = cm_smem(&bars[16]), bar_s = cm_smem(&bars[17]), bar_p = cm_smem(&bars[19]), bar_pv = cm_smem(&bars[20]);
     const uint32_t bar_sf = cm_smem(&bars[21]);                      // queries ready, scores ready (2), probabilities ready, context ready, scores read
+    const uint32_t bar_done = cm_smem(&bars[22]);                    // all MMAs are done
     pdl_wait();
     pdl_launch_dependents();
     __shared__ int s_abort;
     if (tid == 0) {
         s_abort = *(volatile int *)err;                              // a wait ran out earlier: nothing more is started
         for (int s = 0; s < NST; s++) { mbar_init(full(s), F::PG); mbar_init(empty(s), 1); }
-        mbar_init(bar_q, F::SW); mbar_init(bar_s, 1); mbar_init(bar_s + 8, 1); mbar_init(bar_p, F::SW); mbar_init(bar_pv, 1); mbar_init(bar_sf, F::SW);
+        mbar_init(bar_q, F::SW); mbar_init(bar_s, 1); mbar_init(bar_s + 8, 1); mbar_init(bar_p, F::SW); mbar_init(bar_pv, 1); mbar_init(bar_sf, F::SW); mbar_init(bar_done, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 0) {
@@ -127,7 +131,7 @@ __global__ void __launch_bounds__(CtCfg<KE, QE, HDP>::THREADS, 1) k_cache_attent
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = tmem_at;
-    CtWait wait{err, false};
+    CtWait wait{err, &s_abort, false};
 
     struct Unit { int item, kvh, m0, first, stop, unit, n, len, row; bool whole; };
     int at = blockIdx.x * plan[1], item = plan[2], item_at = plan[3];
@@ -268,14 +272,12 @@ __global__ void __launch_bounds__(CtCfg<KE, QE, HDP>::THREADS, 1) k_cache_attent
                         for (int j = 0; j < 32; j++) top = fmaxf(top, __uint_as_float(sr[j]));
                         if (a.scores && mm < a.M) {
                             float *sp = a.scores + (((int64_t)u.item * a.c.nkv + u.kvh) * a.M + mm) * a.pitch + p0 + 32 * c;
-                            if (!row_used) {                         // no token, no share: its scores are zeros by keys that may hold anything
+                            // No token, no share: such a row's scores are zeros by keys that may hold anything. (A NaN of another row becomes
+                            // an infinity, which its sum, a NaN too, makes a NaN again.)
+                            const float most = row_used ? INFINITY : -INFINITY;
+                            auto score = [&](int j) { return fminf(__uint_as_float(sr[j]) * c2, most); };
 #pragma unroll
-                                for (int j = 0; j < 32; j++) sr[j] = 0xff800000u;
-                            }
-#pragma unroll
-                            for (int j = 0; j < 32; j += 4)
-                                *(float4 *)(sp + j) = make_float4(__uint_as_float(sr[j]) * c2, __uint_as_float(sr[j + 1]) * c2,
-                                                                  __uint_as_float(sr[j + 2]) * c2, __uint_as_float(sr[j + 3]) * c2);
+                            for (int j = 0; j < 32; j += 4) *(float4 *)(sp + j) = make_float4(score(j), score(j + 1), score(j + 2), score(j + 3));
                         }
                     }
                 }
@@ -422,6 +424,7 @@ __global__ void __launch_bounds__(CtCfg<KE, QE, HDP>::THREADS, 1) k_cache_attent
             auto scores = [&](uint32_t i) {
                 const uint32_t st = items % NST, sb = F::NSB == 2 ? i & 1u : 0u;
                 wait(full(st), (items / NST) & 1u, 44);
+                if (wait.dead) return;
                 tc_fence_after();
                 uint32_t acc = 0;
                 const uint64_t kd = rd + st * ST;
@@ -443,21 +446,22 @@ __global__ void __launch_bounds__(CtCfg<KE, QE, HDP>::THREADS, 1) k_cache_attent
                 umma_commit(empty(st));
                 items++;
             };
-            while (next_unit(u)) {
+            while (!wait.dead && next_unit(u)) {
                 wait(bar_q, un & 1u, 45);
                 un++;
                 tc_fence_after();
                 const int tiles = u.stop - u.first;
-                scores(it);
+                if (!wait.dead) scores(it);
 #pragma unroll 1
                 for (int t = 0; t < tiles; t++, it++) {
                     if (t + 1 < tiles) {
                         if (F::NSB == 1) { wait(bar_sf, it & 1u, 48); tc_fence_after(); }
-                        scores(it + 1);
+                        if (!wait.dead) scores(it + 1);
                     }
                     const uint32_t st = items % NST;
                     wait(full(st), (items / NST) & 1u, 49);
                     wait(bar_p, it & 1u, 46);
+                    if (wait.dead) break;
                     tc_fence_after();
                     const uint64_t vd = rv + st * ST;
                     uint32_t acc = 0;
@@ -483,7 +487,8 @@ __global__ void __launch_bounds__(CtCfg<KE, QE, HDP>::THREADS, 1) k_cache_attent
         // (fp32: three warps for the keys, three for the values)
         const int grp = F::BF ? 0 : (warp - F::SW - 1) / F::PG, pt = tid - (F::SW + 1 + grp * F::PG) * 32;
         constexpr int NT = F::PG * 32;
-        while (next_unit(u)) {
+        bool gone = false;
+        while (!gone && next_unit(u)) {
             const int *par = a.parents ? a.parents + (int64_t)u.row * a.T : nullptr;
             const char *kb = a.c.k + u.row * a.c.rs + u.kvh * a.c.hs, *vb = a.c.v + u.row * a.c.rs + u.kvh * a.c.hs;
             uint32_t *bits = place_bits[warp - F::SW - 1];           // new tokens that are one, this warp's copy
@@ -511,6 +516,7 @@ __global__ void __launch_bounds__(CtCfg<KE, QE, HDP>::THREADS, 1) k_cache_attent
                 for (int s = 0; s < count; s++, it++) {
                     const uint32_t st = it % NST;
                     wait(empty(st), ((it / NST) & 1u) ^ 1u, 47);
+                    if ((gone = __any_sync(0xffffffffu, wait.dead))) break;
                     const int t = u.first + tile_of(s);
                     const uint32_t to = cm_smem(ring + st * F::STAGE);
                     if ((t + 1) * KT <= u.len) {
@@ -583,6 +589,17 @@ __global__ void __launch_bounds__(CtCfg<KE, QE, HDP>::THREADS, 1) k_cache_attent
     }
     tc_fence_before();
     __syncthreads();
+    if (s_abort) {
+        if (warp == F::SW && lane == 0) {
+            umma_commit(bar_done);
+            mbar_wait(bar_done, 0, err, 50);
+        }
+        if (F::BF && warp == F::SW + 1 && lane == 0) {               // copies into the ring's stages
+            for (uint32_t x = it < NST ? 0 : it - NST; x < it; x++)
+                if (!mbar_wait(full(x % NST), (x / NST) & 1u, err, 51)) break;
+        }
+        __syncthreads();
+    }
     if (warp == F::SW) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");

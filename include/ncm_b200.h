@@ -427,8 +427,13 @@ void   ncmb_lm_nll(NcmbLM *m, const int *ids, int B, int T, const int *lens, dou
  * capacity. Results are right where it is exceeded, only slower.
  * All four queue kernels on the library's stream and return 0, or print one line to stderr and return -1 for arguments
  * they refuse (nothing is queued then). The wide tiles' waits are bounded and reported like the GEMM engines'
- * (ncmb_gemm_tc_check); results of a call in which one ran out, or that found the word set, are not to be used. Rounding: scores, exponentials, sums and weights are fp32 whatever the cache's
- * type. A call's scratch memory is kept for the next one and grows on demand. No counterpart in the reference. */
+ * (ncmb_gemm_tc_check); results of a call in which one ran out, or that found the word set, are not to be used.
+ * Rounding: scores, exponentials, sums and weights are fp32 whatever the cache's type.
+ * Scratch memory belongs to the stream (ncmb_set_stream), is kept for the stream's next call and grows on demand. Calls on
+ * different streams may run side by side; a stream that is destroyed has to have finished them. In a stream capture a call that would need more scratch than the stream has is
+ * refused (-1, the capture goes on): make the same call on that stream before. A captured call's scratch is kept for good;
+ * replays of the graph have to be ordered with the other calls on the stream it was captured on, and with one another.
+ * No counterpart in the reference. */
 enum { NCMB_F32 = 0, NCMB_BF16 = 1 };
 #define NCMB_MAX_NODES 256
 typedef struct {

@@ -20,9 +20,9 @@ int cache_refuse(const char *who, const char *fmt, ...);
 // 0 when the cache's description is one the kernels take (see ncm_b200.h), else -1 with a message
 int cache_check(const char *who, const NcmbCache *c, CacheDev &d);
 inline int cache_elem(const NcmbCache *c) { return c->type == NCMB_BF16 ? 2 : 4; }
-// Scratch of at least `bytes`, kept and grown; null with a message when the device has no room for it. Calls are ordered
-// by the library's stream, so all of them share it; within a call, what one kernel leaves for another that has scratch of
-// its own stands in another area.
+// Scratch of at least `bytes` of the library's stream, kept and grown; null with a message when the device has no room for it, or when it
+// would have to grow while the stream is captured. Calls on a stream are ordered, so all of them share it; within a call, what one kernel
+// leaves for another that has scratch of its own stands in another area.
 // SCRATCH_DONE holds zeros when it is given out, and whoever uses it leaves zeros.
 enum { SCRATCH_MAIN = 0, SCRATCH_PICKS = 1, SCRATCH_DONE = 2, SCRATCH_AREAS = 3 };
 void *cache_scratch(const char *who, size_t bytes, int area = SCRATCH_MAIN);

@@ -5,6 +5,9 @@
 // sum, out = sum p_j v_j; weights_j (+)= sum over the G heads and the T nodes of p_j.
 #include "cache_tc.cuh"
 
+#include <new>
+#include <unordered_map>
+
 #include <stdarg.h>
 
 namespace ncmb {
@@ -36,27 +39,41 @@ int cache_check(const char *who, const NcmbCache *c, CacheDev &d) {
     return 0;
 }
 
+// Areas of each stream: calls on one stream are ordered, calls on two are not. A captured call's area is in the graph for good: it is
+// replaced when a call needs more, but not freed.
 void *cache_scratch(const char *who, size_t bytes, int area) {
-    static void *bases[SCRATCH_AREAS] = {};
-    static size_t caps[SCRATCH_AREAS] = {};
-    void *&base = bases[area];
-    size_t &cap = caps[area];
-    if (bytes <= cap) return base;
-    if (base) {
-        cudaError_t e = cudaStreamSynchronize(stream());     // refused while a graph is being captured: kernels there use the old area
-        if (e != cudaSuccess) { (void)cudaGetLastError(); cache_refuse(who, "scratch has to grow: %s", cudaGetErrorString(e)); return nullptr; }
-        CUDA_CHECK(cudaFree(base));
-        base = nullptr; cap = 0;
+    struct Area { void *base = nullptr; size_t cap = 0; bool in_graph = false; };
+    struct Areas { Area of[SCRATCH_AREAS]; };
+    static std::unordered_map<cudaStream_t, Areas> streams;
+    cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+    cudaError_t e = cudaStreamIsCapturing(stream(), &capture);
+    const bool captured = capture != cudaStreamCaptureStatusNone;
+    if (e != cudaSuccess) { (void)cudaGetLastError(); cache_refuse(who, "the stream: %s", cudaGetErrorString(e)); return nullptr; }
+    Area *a;
+    try { a = &streams[stream()].of[area]; } catch (const std::bad_alloc &) { cache_refuse(who, "no memory"); return nullptr; }
+    if (bytes <= a->cap) {
+        a->in_graph |= captured;
+        return a->base;
     }
+    if (captured) { cache_refuse(who, "%.1f MB of scratch while the stream is captured: make the same call on it before", bytes / 1048576.0); return nullptr; }
+    if (a->base && !a->in_graph) {
+        e = cudaStreamSynchronize(stream());         // refused where another thread's capture forbids it
+        if (e != cudaSuccess) { (void)cudaGetLastError(); cache_refuse(who, "scratch has to grow: %s", cudaGetErrorString(e)); return nullptr; }
+        CUDA_CHECK(cudaFree(a->base));
+    }
+    *a = Area();
     const size_t want = (bytes + (bytes >> 2) + ((size_t)1 << 20)) & ~(size_t)255;
     for (size_t b : {want, (bytes + 255) & ~(size_t)255}) {
-        if (cudaMalloc(&base, b) == cudaSuccess) {
-            if (area == SCRATCH_DONE) CUDA_CHECK(cudaMemsetAsync(base, 0, b, stream()));
-            cap = b;
-            return base;
+        if (cudaMalloc(&a->base, b) == cudaSuccess) {
+            if (area == SCRATCH_DONE) CUDA_CHECK(cudaMemsetAsync(a->base, 0, b, stream()));
+            a->cap = b;
+            // what the wide tiles report into is made here too, not by a captured call, and is zero for every stream
+            (void)tc_err_flag();
+            CUDA_CHECK(cudaStreamSynchronize(stream()));
+            return a->base;
         }
         (void)cudaGetLastError();
-        base = nullptr;
+        a->base = nullptr;
     }
     cache_refuse(who, "no device memory for %.1f MB of scratch", bytes / 1048576.0);
     return nullptr;

@@ -129,7 +129,8 @@ template <class KE, class QE, int HDP>
 int run_attention_hd(const char *who, const CmArgs &a, int max_keys) {
     // (the terms of an fp32 cache's keys of more than 64 dims do not fit shared memory beside the queries')
     if constexpr (sizeof(KE) == 2 || HDP == 64) { if (takes_wide<KE, QE, HDP>(a, max_keys)) return ct_run_as<KE, QE, HDP>(who, a, max_keys); }
-    return a.M <= 8 ? cm_run_as<KE, QE, HDP, 8, false>(who, a, max_keys) : cm_run_as<KE, QE, HDP, 16, false>(who, a, max_keys);
+    auto none = [] {};
+    return a.M <= 8 ? cm_run_as<KE, QE, HDP, 8, false>(who, a, max_keys, none) : cm_run_as<KE, QE, HDP, 16, false>(who, a, max_keys, none);
 }
 template <class KE, class QE>
 int run_attention(const char *who, const CmArgs &a, int max_keys) {

@@ -257,17 +257,18 @@ __global__ void __launch_bounds__(BP_THREADS) k_block_pick(BlockArgs a) {
     if constexpr (CL) cl.sync();                 // the others have read this CTA's counts
 }
 
-template <class KE, class QE>
-int run_blocks(const char *who, const CmArgs &a, int max_keys) {
-    if (a.c.hd <= 64) return a.M <= 8 ? cm_run_as<KE, QE, 64, 8, true>(who, a, max_keys) : cm_run_as<KE, QE, 64, 16, true>(who, a, max_keys);
-    return a.M <= 8 ? cm_run_as<KE, QE, 128, 8, true>(who, a, max_keys) : cm_run_as<KE, QE, 128, 16, true>(who, a, max_keys);
-}
-
 template <class QE>
 void run_pick(const BlockArgs &a, int nc, size_t smem) {
     auto kernel = nc > 1 ? k_block_pick<QE, true> : k_block_pick<QE, false>;
     if (smem > 20000) CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     cache_launch(kernel, dim3(a.T * nc, a.c.nkv, a.c.rows), BP_THREADS, smem, nc, a);
+}
+
+template <class KE, class QE>
+int run_blocks(const char *who, const CmArgs &a, int max_keys, const BlockArgs &picks, int nc, size_t smem) {
+    auto first = [&] { run_pick<QE>(picks, nc, smem); };
+    if (a.c.hd <= 64) return a.M <= 8 ? cm_run_as<KE, QE, 64, 8, true>(who, a, max_keys, first) : cm_run_as<KE, QE, 64, 16, true>(who, a, max_keys, first);
+    return a.M <= 8 ? cm_run_as<KE, QE, 128, 8, true>(who, a, max_keys, first) : cm_run_as<KE, QE, 128, 16, true>(who, a, max_keys, first);
 }
 
 } // namespace
@@ -331,13 +332,11 @@ extern "C" int ncmb_block_attention(const NcmbCache *c, const void *q, int64_t l
     const int gt = (a.G + 15) / 16;
     const size_t smem = (size_t)gt * 16 * (4 + ((c->hd + 31) & ~31) + 8) + (need_keys ? 0 : (size_t)per * 4);
     if (smem > 190000) return cache_refuse(who, "%d query heads a kv head", a.G);
-    if (act_type == NCMB_F32) run_pick<float>(a, nc, smem);
-    else run_pick<__nv_bfloat16>(a, nc, smem);
     CmArgs m = {};
     m.c = a.c; m.q = a.q; m.out = a.out; m.ldq = a.ldq; m.ldo = a.ldo; m.H = a.H; m.G = a.G; m.T = T; m.M = a.G;
     m.c2 = a.scale * 1.44269504f; m.block_log = block == 16 ? 4 : block == 32 ? 5 : block == 64 ? 6 : 7; m.n_sel = n_sel; m.picks = a.picks;
     const int keys = (int)std::min<int64_t>(max_len + T, (int64_t)n_sel * block);
-    if (c->type == NCMB_F32) return run_blocks<float, float>(who, m, keys);
-    if (act_type == NCMB_F32) return run_blocks<__nv_bfloat16, float>(who, m, keys);
-    return run_blocks<__nv_bfloat16, __nv_bfloat16>(who, m, keys);
+    if (c->type == NCMB_F32) return run_blocks<float, float>(who, m, keys, a, nc, smem);
+    if (act_type == NCMB_F32) return run_blocks<__nv_bfloat16, float>(who, m, keys, a, nc, smem);
+    return run_blocks<__nv_bfloat16, __nv_bfloat16>(who, m, keys, a, nc, smem);
 }

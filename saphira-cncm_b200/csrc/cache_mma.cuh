@@ -923,8 +923,9 @@ __global__ void __launch_bounds__(CM_THREADS) k_cache_join(const __grid_constant
 // slots of a CTA that adds up weights: it finds the sums of M queries first, then goes over M scores a slot
 inline int cm_wkeys(int M) { return M <= 32 ? 4 * CM_THREADS : CM_THREADS; }
 constexpr int CM_ROUNDS = 8, CM_FUSED = 24;
-template <class KE, class QE, int HDP, int R, bool BLOCKS>
-int cm_run_as(const char *who, CmArgs a, int max_keys) {
+// first(): launches what has to run before; only once nothing can be refused any more
+template <class KE, class QE, int HDP, int R, bool BLOCKS, class FIRST>
+int cm_run_as(const char *who, CmArgs a, int max_keys, FIRST first) {
     using F = CmCfg<KE, QE, HDP, R>;
     a.tiles = (int)cdiv(a.M, F::M);
     const int smem = F::RING + F::QBYTES;
@@ -953,6 +954,7 @@ int cm_run_as(const char *who, CmArgs a, int max_keys) {
     if (step == rows && units * nc <= F::CTAS * ctx().sm_count && cdiv(max_keys, F::KC) <= (int64_t)CM_ROUNDS * nc * CM_WARPS && (!a.weights || a.tiles == 1)) {
         if (a.weights && !(a.scores = (float *)cache_scratch(who, (size_t)rows * a.c.nkv * a.M * a.pitch * 4))) return -1;
         a.items = rows * per_row;
+        first();
         cache_launch(k_cache_attention<KE, QE, HDP, R, BLOCKS, true>, dim3(nc * a.tiles, a.c.nkv, a.items), CM_THREADS, smem, nc, a);
         return 0;
     }
@@ -970,6 +972,7 @@ int cm_run_as(const char *who, CmArgs a, int max_keys) {
     const bool fused = !a.weights && ctas <= CM_FUSED * units;
     if (fused && !(a.done = (int *)cache_scratch(who, (size_t)units * 4, SCRATCH_DONE))) return -1;
     const int split = ctas > 4 * units;
+    first();
     for (int r = 0; r < rows; r += step) {
         const int nr = std::min(step, rows - r);
         a.row0 = r;

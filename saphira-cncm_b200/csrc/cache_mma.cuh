@@ -40,7 +40,7 @@ template <class KE, class QE, int HDP_, int R_> struct CmCfg {
     static constexpr int QROWS = BF ? 16 : M;
     static constexpr int QBYTES = QT * QROWS * HDP * (BF ? 2 : 4);
     static constexpr int RING = CM_WARPS * CM_STAGES * CM_STAGE;
-    static constexpr int SLOT = M * (HDP + 2);                   // floats of a partial result: maxima, sums, context
+    static constexpr int SUMS = 2 * M, CTX = M * HDP;            // floats of a partial result: maxima and sums, context
 };
 
 struct CmArgs {
@@ -53,11 +53,11 @@ struct CmArgs {
     int items;                       // rows, or rows * T where every token has keys of its own
     const int *parents;
     float c2;                        // scale * log2(e)
-    float *part;                     // partial results, one slot a (CTA + unit)
+    float *sums, *ctx;               // partial results: a slot of sums a (CTA + unit), two of contexts a CTA
     int2 *range;                     // first and last CTA of each unit
     int ctas;                        // CTAs of the attention kernel
-    const int *err;                  // wide tiles: set when a wait ran out, and then `range` and `part` may be what was there before
-    int *done;                       // chunks of each unit that are in `part`, zero between calls; null: k_cache_join joins
+    const int *err;                  // wide tiles: set when a wait ran out, and then the three above may be what was there before
+    int *done;                       // chunks of each unit whose parts are there, zero between calls; null: k_cache_join joins
     float *scores;                   // [row][kv head][M][pitch], or null
     int64_t pitch;
     float *weights;
@@ -114,8 +114,10 @@ template <bool BLOCKS> __device__ __forceinline__ int cm_keys(const CmArgs &a, i
 
 // ---- how the chunks of all units are dealt to CTAs ----
 // The units (item, kv head, tile) in order, each with its chunks in order, are one sequence, of which every CTA takes an equal
-// run: rows of any lengths keep all SMs busy to the end. A unit is done by one CTA or by consecutive ones; CTA c's
-// partial result of unit u goes to slot c + u (along the sequence one of the two grows by one at a time).
+// run: rows of any lengths keep all SMs busy to the end. A unit is done by one CTA or by consecutive ones. CTA c's maxima and
+// sums of unit u go to slot c + u (along the sequence one of the two grows by one at a time); its context, where it has not
+// done the whole unit, to slot 2 c + 1 if it began the unit, else to 2 c: a CTA begins at most one that it does not end, its
+// last, and continues at most one, its first. So the memory for contexts does not grow with the units.
 // (Counts are 32-bit: the host limits the rows of a launch. Nothing here is unrolled: code that runs once is paced by
 // instruction fetches, about 150 cycles for 8 instructions.)
 struct CmPlan { int total, per; };
@@ -624,7 +626,8 @@ __global__ void __launch_bounds__(CM_THREADS, CmCfg<KE, QE, HDP, R>::CTAS) k_cac
         }
         __syncthreads();
         const bool whole = first == 0 && stop == nch;
-        float *slot = CL ? nullptr : a.part + ((int64_t)blockIdx.x + unit) * F::SLOT;
+        float *sums = CL ? nullptr : a.sums + ((int64_t)blockIdx.x + unit) * F::SUMS;
+        float *part = CL ? nullptr : a.ctx + (2 * (int64_t)blockIdx.x + (first == 0)) * F::CTX;
         if constexpr (!CL) {
             if (tid == 0 && first == 0) a.range[unit].x = blockIdx.x;
             if (tid == 0 && stop == nch) a.range[unit].y = blockIdx.x;
@@ -637,7 +640,7 @@ __global__ void __launch_bounds__(CM_THREADS, CmCfg<KE, QE, HDP, R>::CTAS) k_cac
 #pragma unroll
             for (int w = 0; w < CM_WARPS; w++) l += wm[w][m] == -INFINITY ? 0.f : wl[w][m] * cm_exp2(wm[w][m] - top);
             if constexpr (CL) cmax[m] = top;
-            else { slot[m] = top; slot[M + m] = l; }
+            else { sums[m] = top; sums[M + m] = l; }
             wl[0][m] = l;                                        // read by the owner of this m alone until the barrier
         }
         if constexpr (!CL) __syncthreads();
@@ -720,7 +723,7 @@ __global__ void __launch_bounds__(CM_THREADS, CmCfg<KE, QE, HDP, R>::CTAS) k_cac
                 o.x += x.x; o.y += x.y; o.z += x.z; o.w += x.w;
             }
             if (whole) write(m, d, o, wl[0][m]);
-            else *(float4 *)(slot + 2 * M + m * HDP + d) = o;
+            else *(float4 *)(part + m * HDP + d) = o;
         }
         if (!CL && a.done && !whole) {
             // the CTA that brings the unit's last chunks joins its parts
@@ -732,7 +735,7 @@ __global__ void __launch_bounds__(CM_THREADS, CmCfg<KE, QE, HDP, R>::CTAS) k_cac
                 if (tid == 0) a.done[unit] = 0;                  // for the next call
                 __threadfence();
                 const int from = at - first, c0 = from / plan.per, parts = (from + nch - 1) / plan.per - c0 + 1;
-                const float *p0 = a.part + ((int64_t)c0 + unit) * F::SLOT;
+                const float *s0 = a.sums + ((int64_t)c0 + unit) * F::SUMS, *p0 = a.ctx + 2 * (int64_t)c0 * F::CTX;
                 constexpr int D4 = HDP / 4;
                 int ways = 1;                                    // threads that share the parts of four dims of a row
                 while (ways * 2 * nm * D4 <= CM_THREADS) ways *= 2;
@@ -750,8 +753,8 @@ __global__ void __launch_bounds__(CM_THREADS, CmCfg<KE, QE, HDP, R>::CTAS) k_cac
                     };
 #pragma unroll 4
                     for (int c = way; c < parts; c += ways) {
-                        const float *s = p0 + (int64_t)c * F::SLOT;
-                        add(__ldcg(s + m), __ldcg(s + M + m), __ldcg((const float4 *)(s + 2 * M + m * HDP + d)));
+                        const float *s = s0 + c * F::SUMS, *p = p0 + (int64_t)(2 * c + (c == 0)) * F::CTX;
+                        add(__ldcg(s + m), __ldcg(s + M + m), __ldcg((const float4 *)(p + m * HDP + d)));
                     }
 #pragma unroll 1
                     for (int w = 1; w < ways; w <<= 1) {
@@ -776,7 +779,7 @@ __global__ void __launch_bounds__(CM_THREADS, CmCfg<KE, QE, HDP, R>::CTAS) k_cac
 // has a row, or (`split`: few units, each in many parts) all have the same row and every one a share of its parts.
 // The others: `wkeys` slots of one (row, kv head) each, from the scores that the kernel above left.
 constexpr int CM_PITCH = 128;        // scores of a query: whole tiles of keys
-// The CTAs that have a part of a unit; none (0, -1) for a range that the attention kernel cannot have written: `part` is not read by it
+// The CTAs that have a part of a unit; none (0, -1) for a range that the attention kernel cannot have written: no part is read by it
 __device__ __forceinline__ int2 cm_range(const CmArgs &a, int64_t unit) {
     const int2 r = a.range[unit];
     return r.x >= 0 && r.x <= r.y && r.y < a.ctas ? r : make_int2(0, -1);
@@ -809,7 +812,7 @@ __global__ void __launch_bounds__(CM_THREADS) k_cache_join(const __grid_constant
         const int2 cr = cm_range(a, unit0);
         const int c0 = cr.x, c1 = cr.y;
         if (c0 >= c1 || gave_up) return;                         // written already
-        const float *slot = a.part + ((int64_t)c0 + (int64_t)item * per_item + sub) * F::SLOT;
+        const float *sums = a.sums + (c0 + unit0) * F::SUMS, *part = a.ctx + 2 * (int64_t)c0 * F::CTX;
         const int grp = tid / D4, d = tid % D4 * 4, kvh = sub / a.tiles;
         const int m = (int)(blockIdx.x % steps) * rows + (split ? 0 : grp), mm = sub % a.tiles * M + m;
         if (split && mm >= a.M) return;
@@ -818,9 +821,8 @@ __global__ void __launch_bounds__(CM_THREADS) k_cache_join(const __grid_constant
         if (mm < a.M) {
 #pragma unroll 4
             for (int c = split ? grp : 0; c <= c1 - c0; c += split ? GROUPS : 1) {
-                const float *s = slot + (int64_t)c * F::SLOT;
-                const float x = s[m], xl = s[M + m];
-                const float4 p = *(const float4 *)(s + 2 * M + m * HDP + d);
+                const float x = sums[c * F::SUMS + m], xl = sums[c * F::SUMS + M + m];
+                const float4 p = *(const float4 *)(part + (int64_t)(2 * c + (c == 0)) * F::CTX + m * HDP + d);
                 const float t = fmaxf(top, x), base = t == -INFINITY ? 0.f : t, fo = cm_exp2(top - base), fp = cm_exp2(x - base);
                 top = t;
                 l = l * fo + xl * fp;
@@ -876,11 +878,11 @@ __global__ void __launch_bounds__(CM_THREADS) k_cache_join(const __grid_constant
             const int mm = mb + i, m = mm % M;
             const int64_t u = unit0 + mm / M;
             const int2 cr = cm_range(a, u);
-            const float *slot = a.part + (cr.x + u) * F::SLOT;
+            const float *sums = a.sums + (cr.x + u) * F::SUMS;
             float top = -INFINITY, l = 0.f;
 #pragma unroll 4
             for (int c = 0; c <= cr.y - cr.x; c++) {
-                const float x = slot[c * F::SLOT + m], xl = slot[c * F::SLOT + M + m];
+                const float x = sums[c * F::SUMS + m], xl = sums[c * F::SUMS + M + m];
                 const float t = fmaxf(top, x), base = t == -INFINITY ? 0.f : t;
                 l = l * cm_exp2(top - base) + xl * cm_exp2(x - base);
                 top = t;
@@ -923,6 +925,20 @@ __global__ void __launch_bounds__(CM_THREADS) k_cache_join(const __grid_constant
 // slots of a CTA that adds up weights: it finds the sums of M queries first, then goes over M scores a slot
 inline int cm_wkeys(int M) { return M <= 32 ? 4 * CM_THREADS : CM_THREADS; }
 constexpr int CM_ROUNDS = 8, CM_FUSED = 24;
+// scratch of a launch: scores where weights are wanted, then what the join reads; false (said) when there is no room
+template <class F> bool cm_parts(const char *who, CmArgs &a, int rows, int64_t units, int ctas) {
+    auto whole = [](size_t bytes) { return (bytes + 255) & ~(size_t)255; };
+    const size_t sc = a.weights ? (size_t)rows * a.c.nkv * a.M * a.pitch * 4 : 0, ranges = whole((size_t)units * 8);
+    const size_t sums = whole((size_t)(units + ctas) * F::SUMS * 4), ctx = (size_t)ctas * 2 * F::CTX * 4;
+    char *scratch = (char *)cache_scratch(who, sc + ranges + sums + ctx);
+    if (!scratch) return false;
+    a.scores = a.weights ? (float *)scratch : nullptr;
+    a.range = (int2 *)(scratch + sc);
+    a.sums = (float *)(scratch + sc + ranges);
+    a.ctx = (float *)(scratch + sc + ranges + sums);
+    a.ctas = ctas;
+    return true;
+}
 // first(): launches what has to run before; only once nothing can be refused any more
 template <class KE, class QE, int HDP, int R, bool BLOCKS, class FIRST>
 int cm_run_as(const char *who, CmArgs a, int max_keys, FIRST first) {
@@ -959,14 +975,7 @@ int cm_run_as(const char *who, CmArgs a, int max_keys, FIRST first) {
         return 0;
     }
     const int ctas = (int)std::max<int64_t>(1, std::min<int64_t>(F::CTAS * ctx().sm_count, cdiv(units * cdiv(max_keys, F::KC), CM_WARPS)));
-    const size_t ranges = ((size_t)units * 8 + 255) & ~(size_t)255, part = (size_t)(units + ctas) * F::SLOT * 4;
-    const size_t sc = a.weights ? (size_t)step * a.c.nkv * a.M * a.pitch * 4 : 0;
-    char *scratch = (char *)cache_scratch(who, sc + ranges + part);
-    if (!scratch) return -1;
-    a.scores = a.weights ? (float *)scratch : nullptr;
-    a.range = (int2 *)(scratch + sc);
-    a.part = (float *)(scratch + sc + ranges);
-    a.ctas = ctas;
+    if (!cm_parts<F>(who, a, step, units, ctas)) return -1;
     // Few parts a unit: the CTA that finishes it joins them. Many: a kernel of its own, which has a CTA for each row of a
     // unit; it also adds up weights.
     const bool fused = !a.weights && ctas <= CM_FUSED * units;

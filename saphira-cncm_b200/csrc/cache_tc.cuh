@@ -75,7 +75,7 @@ template <class KE, class QE, int HDP>
 __global__ void __launch_bounds__(CtCfg<KE, QE, HDP>::THREADS, 1) k_cache_attention_tc(const __grid_constant__ CmArgs a, const __grid_constant__ CUtensorMap mk,
                                                                                         const __grid_constant__ CUtensorMap mv, int *err) {
     using F = CtCfg<KE, QE, HDP>;
-    constexpr int M = F::M, KT = F::KT, NST = F::NST, ATOMS = F::ATOMS, SLOT = M * (HDP + 2);
+    constexpr int M = F::M, KT = F::KT, NST = F::NST, ATOMS = F::ATOMS;
     extern __shared__ char smem_raw[];
     char *smem = (char *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     char *qs = smem, *ring = qs + F::QB;
@@ -391,8 +391,8 @@ __global__ void __launch_bounds__(CtCfg<KE, QE, HDP>::THREADS, 1) k_cache_attent
             }
             group_sync();
             l += xl[hf ^ 1][r];
-            float *slot = a.part + ((int64_t)blockIdx.x + u.unit) * SLOT;
-            if (hf == 0) { slot[r] = mx; slot[M + r] = l; }
+            float *sums = a.sums + ((int64_t)blockIdx.x + u.unit) * (2 * M);
+            if (hf == 0) { sums[r] = mx; sums[M + r] = l; }
             if (mm < a.M) {
                 if (u.whole) {
                     const float f = l > 0.f ? 1.f / l : 0.f;
@@ -408,7 +408,7 @@ __global__ void __launch_bounds__(CtCfg<KE, QE, HDP>::THREADS, 1) k_cache_attent
                         else *(uint2 *)(o + d) = make_uint2(cm_pack(O[d] * f, O[d + 1] * f), cm_pack(O[d + 2] * f, O[d + 3] * f));
                     }
                 } else {
-                    float *o = slot + 2 * M + r * HDP + hf * HC;
+                    float *o = a.ctx + (2 * (int64_t)blockIdx.x + (u.first == 0)) * (M * HDP) + r * HDP + hf * HC;
 #pragma unroll
                     for (int d = 0; d < HC; d += 4) *(float4 *)(o + d) = make_float4(O[d], O[d + 1], O[d + 2], O[d + 3]);
                 }
@@ -633,14 +633,7 @@ int ct_run_as(const char *who, CmArgs a, int max_keys) {
     const int64_t units = step * row_units, spans = a.weights ? cdiv(a.pitch, cm_wkeys(a.M)) * step * a.c.nkv : 0;
     if (units * F::M + spans > 0x7fffffff) return cache_refuse(who, "%lld query tiles", (long long)units);
     const int ctas = (int)std::max<int64_t>(1, std::min<int64_t>(ctx().sm_count, units * cdiv(max_keys, F::KT)));
-    const size_t ranges = ((size_t)units * 8 + 255) & ~(size_t)255, part = (size_t)(units + ctas) * J::SLOT * 4;
-    const size_t sc = a.weights ? (size_t)step * a.c.nkv * a.M * a.pitch * 4 : 0;
-    char *scratch = (char *)cache_scratch(who, sc + ranges + part);
-    if (!scratch) return -1;
-    a.scores = a.weights ? (float *)scratch : nullptr;
-    a.range = (int2 *)(scratch + sc);
-    a.part = (float *)(scratch + sc + ranges);
-    a.ctas = ctas;
+    if (!cm_parts<J>(who, a, step, units, ctas)) return -1;
     a.err = tc_err_flag();
     const int split = ctas > 4 * units;
     for (int r = 0; r < rows; r += step) {

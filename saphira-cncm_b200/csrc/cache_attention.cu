@@ -117,7 +117,7 @@ template <class KE, class QE, int HDP>
 bool takes_wide(const CmArgs &a, int max_keys) {
     using F = CtCfg<KE, QE, HDP>;
     using C = Cost<KE, QE, HDP>;
-    if (a.M <= 16 || g_variant == 1) return false;
+    if (a.M <= 16 || g_variant == 1 || a.M > CT_MOST_ROWS) return false;
     if (g_variant == 2) return true;
     const double heads = (double)a.c.rows * a.c.nkv;
     const double narrow = 8 + heads * cdiv(a.M, 16) * (C::NARROW * max_keys + 0.013);
@@ -152,6 +152,7 @@ extern "C" int ncmb_cache_attention(const NcmbCache *c, const void *q, int64_t l
     if (act_type != NCMB_F32 && !(act_type == NCMB_BF16 && c->type == NCMB_BF16)) return cache_refuse(who, "activations of type %d with a cache of type %d", act_type, c->type);
     if (n_head < 1 || n_head % c->n_kv) return cache_refuse(who, "%d heads over %d kv heads", n_head, c->n_kv);
     if (T < 1 || T > NCMB_MAX_NODES || T > c->capacity) return cache_refuse(who, "%d new tokens: 1 to %d, and no more than the capacity", T, NCMB_MAX_NODES);
+    if ((int64_t)T * (n_head / c->n_kv) > 1 << 30) return cache_refuse(who, "%d new tokens of %d heads a kv head", T, n_head / c->n_kv);
     const int64_t es = act_type == NCMB_BF16 ? 2 : 4;
     if (!q || !out || ((uintptr_t)q | (uintptr_t)out) % 16 || (ldq * es) % 16 || (ldo * es) % 16 || ldq < (int64_t)n_head * c->hd || ldo < (int64_t)n_head * c->hd)
         return cache_refuse(who, "q and out have to be 16-byte aligned, with rows of n_head * hd at multiples of 16 bytes");

@@ -36,6 +36,9 @@ template <class KE, class QE, int HDP_> struct CtCfg {
     static constexpr int PCOL = 0, OCOL = NP * 64, SCOL = OCOL + HDP, NSB = SCOL + 256 <= 512 ? 2 : 1;
 };
 
+// Query rows of a kv head that the wide tiles take: beyond some 5 million their division by the heads of a group, in fp32, is not exact.
+constexpr int CT_MOST_ROWS = 1 << 20;
+
 __host__ __device__ constexpr uint32_t umma_idesc_bf16(int M, int N) {
     return (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
 }
@@ -172,7 +175,7 @@ __global__ void __launch_bounds__(CtCfg<KE, QE, HDP>::THREADS, 1) k_cache_attent
                 float4 raw[AHEAD][sizeof(QE) / 2];
 #pragma unroll
                 for (int i = 0; i < AHEAD; i++) {
-                    const int mm = u.m0 + m1 + i * QR, t = (int)(((float)mm + 0.5f) * per_g), h = u.kvh * G + mm - t * G;     // mm / G: mm is far below 2^20
+                    const int mm = u.m0 + m1 + i * QR, t = (int)(((float)mm + 0.5f) * per_g), h = u.kvh * G + mm - t * G;     // mm / G, right below CT_MOST_ROWS + M
                     const char *p = a.q + ((int64_t)u.row * a.T + t) * a.ldq + ((int64_t)h * hd + d0) * sizeof(QE);
                     const bool ok = mm < a.M && d0 < hd && cm_used(par, t);
 #pragma unroll

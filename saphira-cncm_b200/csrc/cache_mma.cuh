@@ -31,7 +31,7 @@ template <class KE, class QE, int HDP_, int R_> struct CmCfg {
     // Two stages of 8 KB a warp and three CTAs an SM. Measured at 64 x 16000 (bf16, 64) / 32 rows of picked blocks (bf16, 128) / 3 x 24
     // (fp32, 64): 87 / 82 / 66 us; four stages of 4 KB 93 / 88 / 71; three of 8 KB in two CTAs 88 / 97 / 68; three of 4 KB in four
     // CTAs 93 / 82 / 88.
-    static constexpr int CM_STAGE = 8192, CM_STAGES = 2, CTAS = 3;
+    static constexpr int CM_STAGE = 8192, CM_STAGES = 2;
     static constexpr int KC = CM_STAGE / (2 * ROW);              // keys a chunk
     static constexpr int NT = KC / 8;                            // 8-key tiles a chunk
     static constexpr int NQ = !BF ? 2 : sizeof(QE) == 4 ? 3 : 1; // terms of a query
@@ -40,6 +40,9 @@ template <class KE, class QE, int HDP_, int R_> struct CmCfg {
     static constexpr int QROWS = BF ? 16 : M;
     static constexpr int QBYTES = QT * QROWS * HDP * (BF ? 2 : 4);
     static constexpr int RING = CM_WARPS * CM_STAGES * CM_STAGE;
+    // CTAs that an SM's 228 KB of shared memory hold: ring and queries, masks or picked blocks, 1 KB that each one costs. Two for 16 rows of
+    // 128 dims in fp32, and for picked blocks of 128 dims with fp32 queries or of 64 in fp32 at 16 rows; else three.
+    static constexpr int ctas(bool blocks) { return 3 * (RING + QBYTES + (blocks ? 4864 : 2304) + 1024) <= 228 * 1024 ? 3 : 2; }
     static constexpr int SUMS = 2 * M, CTX = M * HDP;            // floats of a partial result: maxima and sums, context
 };
 
@@ -173,7 +176,7 @@ template <bool BLOCKS, int KC> __device__ int cm_find(const CmArgs &a, int x, in
 // CL: a cluster of CTAs does a unit, each an equal run of its chunks, and their results meet in distributed shared memory: for
 // calls that are all latency. Else the units' chunks are dealt out as above.
 template <class KE, class QE, int HDP, int R, bool BLOCKS, bool CL>
-__global__ void __launch_bounds__(CM_THREADS, CmCfg<KE, QE, HDP, R>::CTAS) k_cache_attention(const __grid_constant__ CmArgs a) {
+__global__ void __launch_bounds__(CM_THREADS, CmCfg<KE, QE, HDP, R>::ctas(BLOCKS)) k_cache_attention(const __grid_constant__ CmArgs a) {
     using F = CmCfg<KE, QE, HDP, R>;
     constexpr int KC = F::KC, NT = F::NT, NQ = F::NQ, NP = F::NP, ROW = F::ROW, UPR = F::UPR, M = F::M, NH = F::NH;
     constexpr bool R8 = F::R8;
@@ -965,16 +968,17 @@ int cm_run_as(const char *who, CmArgs a, int max_keys, FIRST first) {
     const int64_t units = step * row_units, spans = a.weights ? cdiv(a.pitch, cm_wkeys(a.M)) * step * a.c.nkv : 0;
     if (units * F::M + spans > 0x7fffffff) return cache_refuse(who, "%lld query tiles", (long long)units);
     // Clusters: where one, of as many CTAs as give a warp two chunks, does a unit in a few rounds and all of them fit the GPU
+    const int resident = F::ctas(BLOCKS) * ctx().sm_count;
     int nc = 1;
-    while (nc < CM_MAXC && nc * 2 * CM_WARPS <= cdiv(max_keys, F::KC) && units * nc * 2 <= F::CTAS * ctx().sm_count) nc *= 2;
-    if (step == rows && units * nc <= F::CTAS * ctx().sm_count && cdiv(max_keys, F::KC) <= (int64_t)CM_ROUNDS * nc * CM_WARPS && (!a.weights || a.tiles == 1)) {
+    while (nc < CM_MAXC && nc * 2 * CM_WARPS <= cdiv(max_keys, F::KC) && units * nc * 2 <= resident) nc *= 2;
+    if (step == rows && units * nc <= resident && cdiv(max_keys, F::KC) <= (int64_t)CM_ROUNDS * nc * CM_WARPS && (!a.weights || a.tiles == 1)) {
         if (a.weights && !(a.scores = (float *)cache_scratch(who, (size_t)rows * a.c.nkv * a.M * a.pitch * 4))) return -1;
         a.items = rows * per_row;
         first();
         cache_launch(k_cache_attention<KE, QE, HDP, R, BLOCKS, true>, dim3(nc * a.tiles, a.c.nkv, a.items), CM_THREADS, smem, nc, a);
         return 0;
     }
-    const int ctas = (int)std::max<int64_t>(1, std::min<int64_t>(F::CTAS * ctx().sm_count, cdiv(units * cdiv(max_keys, F::KC), CM_WARPS)));
+    const int ctas = (int)std::max<int64_t>(1, std::min<int64_t>(resident, cdiv(units * cdiv(max_keys, F::KC), CM_WARPS)));
     if (!cm_parts<F>(who, a, step, units, ctas)) return -1;
     // Few parts a unit: the CTA that finishes it joins them. Many: a kernel of its own, which has a CTA for each row of a
     // unit; it also adds up weights.

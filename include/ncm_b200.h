@@ -428,12 +428,19 @@ void   ncmb_lm_nll(NcmbLM *m, const int *ids, int B, int T, const int *lens, dou
  * All four queue kernels on the library's stream and return 0, or print one line to stderr and return -1 for arguments
  * they refuse (nothing is queued then). The wide tiles' waits are bounded and reported like the GEMM engines'
  * (ncmb_gemm_tc_check); results of a call in which one ran out, or that found the word set, are not to be used.
- * Rounding: scores, exponentials, sums and weights are fp32 whatever the cache's type.
- * Scratch memory belongs to the stream (ncmb_set_stream), is kept for the stream's next call and grows on demand. Calls on
- * different streams may run side by side; a stream that is destroyed has to have finished them. In a stream capture a call that would need more scratch than the stream has is
- * refused (-1, the capture goes on): make the same call on that stream before. A captured call's scratch is kept for good;
- * replays of the graph have to be ordered with the other calls on the stream it was captured on, and with one another.
- * No counterpart in the reference. */
+ * Rounding: scores, exponentials, sums and weights are held in fp32 whatever the cache's type. Products run on tensor
+ * cores over terms of fewer bits: with a bf16 cache, fp32 queries and probabilities as three bf16 terms (24 bits),
+ * probabilities of bf16 activations as two (16 bits; the result is rounded to 8); with an fp32 cache queries, keys,
+ * probabilities and values as two TF32 terms (22 bits; tiles of 16 rows leave out the product of the smaller ones) or, in
+ * wide tiles, as three bf16 terms whose products below 2^-24 are left out. Results of fp32 activations are within 5e-6
+ * of the formula's in the 2-norm (1e-7 to 7e-7 measured). An fp32 value beyond 3.39e38 counts as an infinity, and what
+ * attention makes of an infinity that a token sees may be a NaN.
+ * Scratch memory belongs to the stream (ncmb_set_stream), is kept for the stream's next call and grows on demand: some
+ * MB; with weights also 4 bytes for each query's score of each slot of the capacity, up to 2 GB or what one row needs.
+ * Calls on different streams may run side by side; a stream that is destroyed has to have finished them. In a stream
+ * capture a call that would need more scratch than the stream has is refused (-1, the capture goes on): make the same
+ * call on that stream before. A captured call's scratch is kept for good; replays of the graph have to be ordered with
+ * the other calls on the stream it was captured on, and with one another. No counterpart in the reference. */
 enum { NCMB_F32 = 0, NCMB_BF16 = 1 };
 #define NCMB_MAX_NODES 256
 typedef struct {

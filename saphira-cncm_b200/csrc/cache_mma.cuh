@@ -3,8 +3,8 @@
 // are the 16-row tiles; a warp walks chunks of keys with a running maximum and sum a row.
 //
 // Products in fp32 grade whatever the types: a bf16 key meets an fp32 query as three bf16 terms (24 bits, exact products),
-// probabilities meet bf16 values as three terms (two where the result is bf16); fp32 keys and values as TF32 pairs, three
-// products. The leading term and the small ones have accumulators of their own, and a chunk's P V starts from zero and
+// probabilities meet bf16 values as three terms (two where the result is bf16); fp32 keys and values as TF32 pairs (22
+// bits), three products, or all four where the pairs are stacked. The leading term and the small ones have accumulators of their own, and a chunk's P V starts from zero and
 // is added to the running result in fp32 by the multiply-add that rescales it: the tensor core truncates its accumulator
 // after each product, which would bias a sum that runs over thousands of keys.
 //

@@ -7,7 +7,7 @@
 // cache_mma.cuh: a query is 3 (bf16 activations: 1), a probability 3 (2), a bf16 key or value 1, an fp32 one 3, of whose nine
 // products the six largest are taken (2^-24 and more). Roles: warps 0 - 7 softmax (they also turn the queries into terms and
 // write the results), warp 8 issues the MMAs, the others load: keys of the next tile, values of this one, in turn through
-// one ring -- bf16 by cp.async, fp32 through registers, where the terms are formed.
+// one ring -- bf16 by TMA, the last tiles of a row, which end inside, by cp.async; fp32 through registers, where the terms are formed.
 //
 // Tiles are 128 keys wide and probabilities stand in tensor memory because MMAs are paced by operand fetch: 64-wide ones took about
 // 100 cycles each with both operands in shared memory, 128-wide ones 90 with A in tensor memory (arithmetic: 16 and 32). Bound by
@@ -29,10 +29,10 @@ template <class KE, class QE, int HDP_> struct CtCfg {
     static constexpr int FIT = (217 * 1024 - QB) / STAGE, NST = FIT < 8 ? FIT : 8;
     static constexpr int PG = 3, PW = BF ? PG : 2 * PG, SW = 8, THREADS = 32 * (SW + 1 + PW);    // whole warps a scheduler: registers
     static constexpr int SMEM = QB + NST * STAGE + 1024;
-    // columns of tensor memory: probabilities (two to a column), context, one or two score tiles
     // What the start of a unit costs, in tiles, for the plan: queries, the first loads and the results take about 9 us, a tile 2
     // (bf16) or 7 (fp32: forming the terms). Without it the CTA that gets a short row's heads is the last: 125 -> 100 us.
     static constexpr int START = BF ? 4 : 1;
+    // columns of tensor memory: probabilities (two to a column), context, one or two score tiles
     static constexpr int PCOL = 0, OCOL = NP * 64, SCOL = OCOL + HDP, NSB = SCOL + 256 <= 512 ? 2 : 1;
 };
 

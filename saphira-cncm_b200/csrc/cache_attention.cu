@@ -45,12 +45,17 @@ void *cache_scratch(const char *who, size_t bytes, int area) {
     struct Area { void *base = nullptr; size_t cap = 0; bool in_graph = false; };
     struct Areas { Area of[SCRATCH_AREAS]; };
     static std::unordered_map<cudaStream_t, Areas> streams;
+    static cudaStream_t last = nullptr;
+    static Areas *mine = nullptr;                    // of `last`
     cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
     cudaError_t e = cudaStreamIsCapturing(stream(), &capture);
     const bool captured = capture != cudaStreamCaptureStatusNone;
     if (e != cudaSuccess) { (void)cudaGetLastError(); cache_refuse(who, "the stream: %s", cudaGetErrorString(e)); return nullptr; }
-    Area *a;
-    try { a = &streams[stream()].of[area]; } catch (const std::bad_alloc &) { cache_refuse(who, "no memory"); return nullptr; }
+    if (!mine || last != stream()) {
+        try { mine = &streams[stream()]; } catch (const std::bad_alloc &) { cache_refuse(who, "no memory"); return nullptr; }
+        last = stream();
+    }
+    Area *a = &mine->of[area];
     if (bytes <= a->cap) {
         a->in_graph |= captured;
         return a->base;

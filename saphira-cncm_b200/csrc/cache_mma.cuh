@@ -123,9 +123,14 @@ template <bool BLOCKS> __device__ __forceinline__ int cm_keys(const CmArgs &a, i
 // last, and continues at most one, its first. So the memory for contexts does not grow with the units.
 // (Counts are 32-bit: the host limits the rows of a launch. Nothing here is unrolled: code that runs once is paced by
 // instruction fetches, about 150 cycles for 8 instructions.)
+// A unit takes places of whole rounds -- a chunk a warp -- and one round more, what its start and end cost, or the CTA that gets the units
+// of a short row is the last. All begin and end at whole rounds, so none is cut inside one. Counted by chunks alone, picked blocks of 32 rows
+// up to 32768 tokens (one of none) took 80 us for 65, of 6 rows of up to 17705 with 24 new tokens 151 for 37.
+constexpr int CM_START = CM_WARPS;
+__host__ __device__ constexpr int cm_span(int chunks) { return ((chunks + CM_WARPS - 1) & ~(CM_WARPS - 1)) + CM_START; }
 struct CmPlan { int total, per; };
 template <bool BLOCKS, int KC> __device__ __forceinline__ int cm_chunks(const CmArgs &a, int item) {           // of all units of an item
-    return item < a.items ? ((cm_keys<BLOCKS>(a, item) + KC - 1) / KC) * a.c.nkv * a.tiles : 0;
+    return item < a.items ? cm_span((cm_keys<BLOCKS>(a, item) + KC - 1) / KC) * a.c.nkv * a.tiles : 0;
 }
 template <bool BLOCKS, int KC> __device__ CmPlan cm_plan(const CmArgs &a, int ctas, int *sh) {
     int t = 0;
@@ -188,6 +193,7 @@ __global__ void __launch_bounds__(CM_THREADS, CmCfg<KE, QE, HDP, R>::ctas(BLOCKS
     __shared__ uint32_t used_bits[8];
     __shared__ int spar[BLOCKS ? 1 : NCMB_MAX_NODES];
     __shared__ int spicks[BLOCKS ? 1024 : 1];
+    __shared__ float most[BLOCKS ? 1 : M];                  // the largest score of a row: -infinity where no token is
     __shared__ float wm[CM_WARPS][M], wl[CM_WARPS][M], cmax[M];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c4 = lane & 3;
     const int hd = a.c.hd, G = a.G;
@@ -205,16 +211,23 @@ __global__ void __launch_bounds__(CM_THREADS, CmCfg<KE, QE, HDP, R>::ctas(BLOCKS
     if constexpr (!CL) { if (a.items > 1) item = cm_find<BLOCKS, KC>(a, at, item_at, sh); }
     char *my = ring + warp * (CM_STAGES * CM_STAGE);
     do {
-        const int n = cm_keys<BLOCKS>(a, item), nch = (n + KC - 1) / KC;
-        int sub, kvh, tile, first, stop;
+        const int n = cm_keys<BLOCKS>(a, item), nch = (n + KC - 1) / KC, span = cm_span(nch);
+        int sub, kvh, tile, first, stop, from = 0, take = 0;
         if constexpr (CL) {
             const int share = ((nch + nc - 1) / nc + CM_WARPS - 1) & ~(CM_WARPS - 1);
             kvh = blockIdx.y; tile = a.tiles == 1 ? 0 : blockIdx.x / nc; sub = kvh * a.tiles + tile;
             first = min(nch, rank * share); stop = min(nch, first + share);
         } else {
-            sub = cm_div(at - item_at, nch); kvh = a.tiles == 1 ? sub : cm_div(sub, a.tiles); tile = sub - kvh * a.tiles;
-            first = at - item_at - sub * nch; stop = min(nch, first + (end - at));
+            sub = cm_div(at - item_at, span); kvh = a.tiles == 1 ? sub : cm_div(sub, a.tiles); tile = sub - kvh * a.tiles;
+            from = item_at + sub * span;                         // where the unit begins: its start, then its chunks
+            take = min(from + span, end) - at;
+            first = max(0, at - from - CM_START); stop = min(nch, at + take - from - CM_START);
         }
+        auto advance = [&] {
+            at += take;
+            if (at == item_at + span * a.c.nkv * a.tiles) { item_at = at; item++; }
+        };
+        if (!CL && stop <= first) { advance(); continue; }       // its start alone
         const int unit = item * a.c.nkv * a.tiles + sub;
         const int m0 = tile * M;
         const int row = a.row0 + (BLOCKS ? item / a.T : item), tok = BLOCKS ? item % a.T : 0, len = BLOCKS ? n : n - a.T;
@@ -324,6 +337,9 @@ __global__ void __launch_bounds__(CM_THREADS, CmCfg<KE, QE, HDP, R>::ctas(BLOCKS
                     }
                 }
             }
+            // No token, no share: such a row's scores are zeros by keys that may hold anything. (A NaN of another row becomes an infinity,
+            // which its sum, a NaN too, makes a NaN again.)
+            if (!BLOCKS && a.scores && tid < M) most[tid] = m0 + tid < a.M && used((m0 + tid) / G) ? INFINITY : -INFINITY;
             if (tail) {
                 const int t0 = m0 / G, nt = (min(a.M, m0 + M) + G - 1) / G - t0;   // nodes of this tile
                 for (int i = tid; i < nt; i += CM_THREADS) {
@@ -454,14 +470,11 @@ __global__ void __launch_bounds__(CM_THREADS, CmCfg<KE, QE, HDP, R>::ctas(BLOCKS
 #pragma unroll
                 for (int hh = 0; hh < NH; hh++) {
                     const int mm = m0 + g + 8 * hh;
-                    if (mm >= a.M) continue;
-                    if (par && !used(mm / G)) {                  // no token, no share: its scores are zeros by keys that may hold anything
+                    if (mm < a.M) {
+                        const float top = most[g + 8 * hh];
 #pragma unroll
-                        for (int j = 0; j < NT; j++) *(float2 *)(sp + mm * a.pitch + 8 * j) = make_float2(-INFINITY, -INFINITY);
-                        continue;
+                        for (int j = 0; j < NT; j++) *(float2 *)(sp + mm * a.pitch + 8 * j) = make_float2(fminf(S[j][2 * hh], top), fminf(S[j][2 * hh + 1], top));
                     }
-#pragma unroll
-                    for (int j = 0; j < NT; j++) *(float2 *)(sp + mm * a.pitch + 8 * j) = make_float2(S[j][2 * hh], S[j][2 * hh + 1]);
                 }
             }
             float al[NH];
@@ -737,7 +750,7 @@ __global__ void __launch_bounds__(CM_THREADS, CmCfg<KE, QE, HDP, R>::ctas(BLOCKS
             if (joined == nch) {
                 if (tid == 0) a.done[unit] = 0;                  // for the next call
                 __threadfence();
-                const int from = at - first, c0 = from / plan.per, parts = (from + nch - 1) / plan.per - c0 + 1;
+                const int c0 = (from + CM_START) / plan.per, parts = (from + span - 1) / plan.per - c0 + 1;
                 const float *s0 = a.sums + ((int64_t)c0 + unit) * F::SUMS, *p0 = a.ctx + 2 * (int64_t)c0 * F::CTX;
                 constexpr int D4 = HDP / 4;
                 int ways = 1;                                    // threads that share the parts of four dims of a row
@@ -772,8 +785,7 @@ __global__ void __launch_bounds__(CM_THREADS, CmCfg<KE, QE, HDP, R>::ctas(BLOCKS
             }
         }
         if (CL) break;
-        at += stop - first;
-        if (at == item_at + nch * a.c.nkv * a.tiles) { item_at = at; item++; }
+        advance();
     } while (at < end);
 }
 
@@ -957,7 +969,7 @@ int cm_run_as(const char *who, CmArgs a, int max_keys, FIRST first) {
     // rows of a launch: as many as leave the scores some GB at most, and the count of chunks in 31 bits
     const int rows = a.c.rows, per_row = BLOCKS ? a.T : 1;
     const int64_t row_units = (int64_t)per_row * a.c.nkv * a.tiles;
-    const int64_t row_chunks = row_units * cdiv(BLOCKS ? (int64_t)a.n_sel << a.block_log : a.c.cap, F::KC);
+    const int64_t row_chunks = row_units * (cdiv(BLOCKS ? (int64_t)a.n_sel << a.block_log : a.c.cap, F::KC) + CM_WARPS + CM_START);
     int64_t most = 0x70000000 / row_chunks;
     if (a.weights) {
         a.pitch = cdiv((int64_t)a.c.cap, CM_PITCH) * CM_PITCH;
@@ -967,18 +979,20 @@ int cm_run_as(const char *who, CmArgs a, int max_keys, FIRST first) {
     const int step = (int)std::min<int64_t>(rows, most);
     const int64_t units = step * row_units, spans = a.weights ? cdiv(a.pitch, cm_wkeys(a.M)) * step * a.c.nkv : 0;
     if (units * F::M + spans > 0x7fffffff) return cache_refuse(who, "%lld query tiles", (long long)units);
-    // Clusters: where one, of as many CTAs as give a warp two chunks, does a unit in a few rounds and all of them fit the GPU
+    // Clusters: where one, of as many CTAs as give a warp two chunks and fit the GPU, does a unit in a few rounds. Single CTAs where they fit
+    // in one and a half waves: a second launch costs more (picked blocks, fp32, 128 dims, 384 units of 3 keys: 12.7 us, dealt out 20.2).
+    const int64_t chunks = cdiv(max_keys, F::KC);
     const int resident = F::ctas(BLOCKS) * ctx().sm_count;
     int nc = 1;
-    while (nc < CM_MAXC && nc * 2 * CM_WARPS <= cdiv(max_keys, F::KC) && units * nc * 2 <= resident) nc *= 2;
-    if (step == rows && units * nc <= resident && cdiv(max_keys, F::KC) <= (int64_t)CM_ROUNDS * nc * CM_WARPS && (!a.weights || a.tiles == 1)) {
+    while (nc < CM_MAXC && nc * 2 * CM_WARPS <= chunks && units * nc * 2 <= resident) nc *= 2;
+    if (step == rows && units * nc <= 3 * ctx().sm_count && chunks <= (int64_t)CM_ROUNDS * nc * CM_WARPS && (!a.weights || a.tiles == 1)) {
         if (a.weights && !(a.scores = (float *)cache_scratch(who, (size_t)rows * a.c.nkv * a.M * a.pitch * 4))) return -1;
         a.items = rows * per_row;
         first();
         cache_launch(k_cache_attention<KE, QE, HDP, R, BLOCKS, true>, dim3(nc * a.tiles, a.c.nkv, a.items), CM_THREADS, smem, nc, a);
         return 0;
     }
-    const int ctas = (int)std::max<int64_t>(1, std::min<int64_t>(resident, cdiv(units * cdiv(max_keys, F::KC), CM_WARPS)));
+    const int ctas = (int)std::max<int64_t>(1, std::min<int64_t>(resident, cdiv(units * chunks, CM_WARPS)));
     if (!cm_parts<F>(who, a, step, units, ctas)) return -1;
     // Few parts a unit: the CTA that finishes it joins them. Many: a kernel of its own, which has a CTA for each row of a
     // unit; it also adds up weights.

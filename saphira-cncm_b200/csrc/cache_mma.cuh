@@ -9,8 +9,8 @@
 // after each product, which would bias a sum that runs over thousands of keys.
 //
 // Bound: at 8 rows by reading keys and values (64 rows of up to 16000 tokens, 14 heads over 2 x 64 in bf16: 63 us, 5.4 TB/s with start
-// and end, 81 us with the weights); at 16 rows by mma.sync (about 1000 multiply-adds a cycle and SM); for a few thousand keys by
-// latency, above all by instruction fetches (12 x 64 over 811 tokens in fp32: 6.8 us).
+// and end, 82 us with the weights); at 16 rows by mma.sync (about 1000 multiply-adds a cycle and SM); for a few thousand keys by
+// latency, above all by instruction fetches (12 x 64 over 811 tokens in fp32: 6.6 us).
 #pragma once
 #include "cache.cuh"
 
@@ -116,7 +116,7 @@ template <bool BLOCKS> __device__ __forceinline__ int cm_keys(const CmArgs &a, i
 }
 
 // ---- how the chunks of all units are dealt to CTAs ----
-// The units (item, kv head, tile) in order, each with its chunks in order, are one sequence, of which every CTA takes an equal
+// The units (item, kv head, tile) in order, each with its start and its chunks in order, are one sequence, of which every CTA takes an equal
 // run: rows of any lengths keep all SMs busy to the end. A unit is done by one CTA or by consecutive ones. CTA c's maxima and
 // sums of unit u go to slot c + u (along the sequence one of the two grows by one at a time); its context, where it has not
 // done the whole unit, to slot 2 c + 1 if it began the unit, else to 2 c: a CTA begins at most one that it does not end, its

@@ -13,7 +13,7 @@
 // 100 cycles each with both operands in shared memory, 128-wide ones 90 with A in tensor memory (arithmetic: 16 and 32). Bound by
 // the chain of a tile: products with the values, then the exponentials of the next tile, which wait for the tensor memory that
 // the products read: 3900 cycles for 64 KB of keys and values at head dim 128. 16 rows of up to 8192 tokens, 32 heads over 8 x
-// 128, 16 drafted tokens: 106 us, of which 51 are the time the bytes take (64-key tiles by cp.async: 179).
+// 128, 16 drafted tokens: 107 us, of which 51 are the time the bytes take (64-key tiles by cp.async: 179).
 #pragma once
 #include "cache_mma.cuh"
 #include "tc_common.cuh"

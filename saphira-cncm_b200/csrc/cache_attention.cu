@@ -111,8 +111,8 @@ int g_variant = 0;                   // ncmb_set_cache_variant
 // over 1 - 64 rows of 500 - 30000 tokens, 3 - 64 new tokens and 33 - 448 query rows a kv head gave, in us:
 //   narrow  8 + tiles of 16 rows x (NARROW x keys + 0.013)
 //   wide   14 + WIDE x tiles of 128 rows x (tiles of 128 keys + START), over the SMs
-// e.g. bf16 cache, fp32 queries, 2 x 64, narrow against wide: 1 x 4000 x 112 rows 11 / 17.2, 16 x 4000 x 56 rows 36.1 / 37.5,
-// x 448 rows 154 / 105; 8 x 128: 1 x 500 x 64 rows 11.5 / 24, 16 x 4000 x 64 rows 186 / 148, x 256 rows 695 / 277.
+// e.g. bf16 cache, fp32 queries, 2 x 64, narrow against wide: 1 x 4000 x 112 rows 11 / 17, 16 x 4000 x 56 rows 34 / 38,
+// x 448 rows 153 / 105; 8 x 128: 1 x 500 x 64 rows 11.4 / 24, 16 x 4000 x 64 rows 181 / 148, x 256 rows 667 / 278.
 template <class KE, class QE, int HDP> struct Cost {
     static constexpr bool Q32 = sizeof(QE) == 4;
     static constexpr double NARROW = sizeof(KE) == 4 ? 111e-6 : HDP == 64 ? (Q32 ? 42e-6 : 30e-6) : (Q32 ? 90e-6 : 71e-6);

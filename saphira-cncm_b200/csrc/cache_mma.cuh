@@ -3,10 +3,10 @@
 // are the 16-row tiles; a warp walks chunks of keys with a running maximum and sum a row.
 //
 // Products in fp32 grade whatever the types: a bf16 key meets an fp32 query as three bf16 terms (24 bits, exact products),
-// probabilities meet bf16 values as three terms (two where the result is bf16); fp32 keys and values as TF32 pairs (22
-// bits), three products, or all four where the pairs are stacked. The leading term and the small ones have accumulators of their own, and a chunk's P V starts from zero and
-// is added to the running result in fp32 by the multiply-add that rescales it: the tensor core truncates its accumulator
-// after each product, which would bias a sum that runs over thousands of keys.
+// probabilities meet bf16 values as three terms (two where the result is bf16); fp32 keys and values as TF32 pairs (22 bits),
+// three products, or all four where the pairs are stacked. The leading term and the small ones have accumulators of their
+// own, and a chunk's P V starts from zero and is added to the running result in fp32 by the multiply-add that rescales it: the
+// tensor core truncates its accumulator after each product, which would bias a sum that runs over thousands of keys.
 //
 // Bound: at 8 rows by reading keys and values (64 rows of up to 16000 tokens, 14 heads over 2 x 64 in bf16: 63 us, 5.4 TB/s with start
 // and end, 82 us with the weights); at 16 rows by mma.sync (about 1000 multiply-adds a cycle and SM); for a few thousand keys by

@@ -285,22 +285,23 @@ def _attend(s):
 
 
 def _select(s):
-    """Scores in 64 bits: where two continuations are near one another, the order must not hang on how a sum was rounded."""
+    """Scores in 64 bits: where two continuations are near one another, the order must not hang on how a sum was rounded. A beam's own
+    continuations are in the order of their logits."""
     case = s["case"]
     B, K, n = case["B"], case["beams"], case["n_out"]
-    x = s["logits"].double().nan_to_num_(nan=float("-inf"), posinf=FMAX, neginf=float("-inf"))
-    V = x.shape[1]
-    top = x.amax(1, keepdim=True)
-    top = top.masked_fill(top == float("-inf"), 0.0)
-    x = x - top
-    x -= torch.exp(x).sum(1, keepdim=True).clamp_(min=5e-324).log()                             # of a row of nothing: all stays -infinity
-    x = s["scores"].double().view(B, K, 1) + x.view(B, K, V)
+    x = s["logits"].float().nan_to_num(nan=float("-inf"), posinf=FMAX, neginf=float("-inf")).view(B, K, -1)
+    V = x.shape[2]
     if s["done"] is not None:                                                                   # goes on with its end, at no cost
-        over = (s["done"] != 0)[:, :, None]
-        x.masked_fill_(over & (torch.arange(V, device="cuda") != s["eos"]), float("-inf"))
-        x[:, :, s["eos"]] = torch.where(over[:, :, 0], s["scores"].double(), x[:, :, s["eos"]])
-    best, at = (y[:, :n] for y in x.view(B, K * V).sort(dim=1, descending=True, stable=True))
-    parents, tokens = at // V, at % V
+        end = torch.where(torch.arange(V, device="cuda") == s["eos"], 0.0, float("-inf"))
+        x = torch.where((s["done"] != 0)[:, :, None], end, x)
+    words = x.sort(dim=2, descending=True, stable=True).indices[:, :, :n]
+    x = x.double()
+    top = x.amax(2, keepdim=True)
+    top = top.masked_fill(top == float("-inf"), 0.0)
+    total = top + torch.exp(x - top).sum(2, keepdim=True).clamp_(min=5e-324).log()              # of a row of nothing: all stays -infinity
+    score = (s["scores"].double()[:, :, None] + (x.gather(2, words) - total)).flatten(1)
+    best, at = (y[:, :n] for y in score.sort(dim=1, descending=True, stable=True))
+    parents, tokens = at // words.shape[2], words.flatten(1).gather(1, at)
     done = tokens == s["eos"]
     if s["done"] is not None:
         done |= s["done"].gather(1, parents) != 0

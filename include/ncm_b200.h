@@ -498,6 +498,94 @@ int ncmb_block_attention(const NcmbCache *c, const void *q, int64_t ldq, void *o
                          int T, int block, const signed char *codes, const float *scales, int n_sel, int n_first,
                          int n_last, float scale, int max_len, int *picks);
 
+/* ---- rotary positions ----
+ * rope_apply above rotates whole heads, halves against one another, by tables of cosines. These calls take a plan instead: which
+ * dims of a head are rotated, which of them are a pair, and how far each pair turns from one position to the next. For the pair
+ * (x1, x2) of angle a: y1 = magnitude (x1 cos a - x2 sin a), y2 = magnitude (x2 cos a + x1 sin a). Angles are formed in 64 bits,
+ * exact to 1e-9 turns at any 32-bit position; cosines, sines and products in fp32, the result is rounded once. */
+enum { NCMB_ROPE_HALVES = 0,             /* dim i and dim i + dims / 2 are a pair */
+       NCMB_ROPE_PAIRS = 1 };            /* dims 2 i and 2 i + 1 */
+enum { NCMB_ROPE_PLAIN = 0, NCMB_ROPE_LINEAR = 1, NCMB_ROPE_BASE = 2, NCMB_ROPE_PARTS = 3 };
+#define NCMB_ROPE_MAX 256
+typedef struct {
+    int dims;                            /* the first dims of a head are rotated, the others stay */
+    int layout;
+    float magnitude;
+    double turns[NCMB_ROPE_MAX / 2];     /* of pair i: full turns a position */
+} NcmbRope;
+/* Fills a plan (host arithmetic, needs no GPU; a host may as well fill in turns of its own). f_i = theta^(-2 i / dims) radians a
+ * position, and for contexts longer than trained ones, by `scaling`:
+ *   PLAIN   as it is
+ *   LINEAR  f_i / factor
+ *   BASE    theta * factor^(dims / (dims - 2)) in place of theta: the fastest pair as it is, the slowest by 1 / factor
+ *   PARTS   r_i = trained * f_i / (2 pi) turns in the trained context; g = (r_i - low) / (high - low), at least 0, at most 1; f_i * (g + (1 - g) / factor)
+ * dims even, 2 ... NCMB_ROPE_MAX; theta and factor > 0; trained > 0 and low < high for PARTS (not read otherwise). 0, or -1 with a message. */
+int ncmb_rope_plan(NcmbRope *r, int dims, int layout, double theta, int scaling, double factor, double trained, double low, double high,
+                   double magnitude);
+/* Rotates heads. Element (row b, token t, head h, dim d) is x[b * xs[0] + t * xs[1] + h * xs[2] + d], of the result y with ys (host arrays; elements,
+ * multiples of 16 bytes, as are x and y); type NCMB_F32 or NCMB_BF16, of both. y may be x with ys = xs; otherwise the two must not overlap. Queries
+ * and keys that a projection leaves side by side are one call of all their heads. pos: device int[rows][T], any 32-bit positions, or NULL:
+ * token t is at t. inverse != 0: by the transposed matrix -- the gradient, or (magnitude 1) the way back. hd a multiple of 8, at least
+ * dims, at most NCMB_ROPE_MAX. Queues one kernel on the library's stream; 0, or -1 with a message for arguments it refuses. */
+int ncmb_rope(const NcmbRope *r, const void *x, const int64_t *xs, void *y, const int64_t *ys, int type, int rows, int T, int n_head, int hd,
+              const int *pos, int inverse);
+
+/* ---- paged caches and beams ----
+ * Keys and values in pages of a pool that rows share. Element (page p, kv head h, slot s of the page, dim d) of the keys is
+ * k[p * page_stride + h * head_stride + s * token_stride + d], of the values likewise with v. Row b's token number n stands in slot n % page of page
+ * table[b * table_stride + n / page], for n below max_pages * page, its capacity. Rows may share pages (a common beginning, the beams of
+ * a group); who writes has pages of its own. An entry outside 0 ... n_pages - 1 is no page: tokens that would stand there are not
+ * stored, and nothing sees them. A negative length: the row holds no sequence; nothing is stored for it and its results are zero. The
+ * types, head dims and alignments of NcmbCache; rounding, scratch memory, streams and captures as there. */
+typedef struct {
+    void *k, *v;
+    int type;                        /* NCMB_F32 or NCMB_BF16 */
+    int rows, n_kv, hd;
+    int page;                        /* tokens a page: a power of two, 8 ... 1024 */
+    int n_pages;                     /* of the pool */
+    int64_t page_stride, head_stride, token_stride;     /* in elements */
+    const int *table;                /* device int[rows][table_stride] */
+    int64_t table_stride;
+    int max_pages;                   /* entries of a row */
+    const int *len;                  /* device int[rows] */
+} NcmbPaged;
+/* Stores new tokens' keys and values, and rotates keys (before they are rounded) and queries on the way. Token i of n_tokens has its query at q + i * ldq
+ * ([n_head][hd]), its key and value at k + i * ldk and v + i * ldv ([n_kv][hd]), of act_type (NCMB_BF16 with a bf16 cache only; 16-byte multiples).
+ * start: device int[rows + 1], ascending: tokens start[b] ... start[b + 1] - 1 are row b's, those before start[0] or from start[rows] on are
+ * nobody's and left alone; NULL: n_tokens / rows for every row. Row b's first token becomes its token number len[b], and so on; beyond the capacity
+ * nothing is stored. Lengths stay as they are: the caller raises them after the step, as for ncmb_cache_attention. pos: device
+ * int[n_tokens], positions to rotate by; NULL: the token's number in its row. r NULL: no rotation. q_out: rotated queries, rows of ldqo; may be q
+ * (with ldqo = ldq); q NULL: keys and values alone. */
+int ncmb_paged_append(const NcmbPaged *c, const NcmbRope *r, const void *q, int64_t ldq, void *q_out, int64_t ldqo, int n_head,
+                      const void *k, int64_t ldk, const void *v, int64_t ldv, int act_type, int n_tokens, const int *start, const int *pos);
+/* ncmb_cache_attention over a paged cache, without weights: T new tokens of every row, which already stand in slots len[b] ... len[b] + T - 1 (T = 1: a
+ * decode step), attend to the row's tokens and to one another, all before them or by `parents`. max_len: an upper bound of the lengths that the
+ * host knows, 0 = capacity. A query that sees nothing gets zeros. */
+int ncmb_paged_attention(const NcmbPaged *c, const void *q, int64_t ldq, void *out, int64_t ldo, int act_type, int n_head, int T,
+                         const int *parents, float scale, int max_len);
+/* The n_out best continuations of each group of beams. Row g * beams + k of the logits (fp32 or bf16, rows of ldl elements, V words) is beam k of group g,
+ * scores[g][k] the sum of log probabilities that it has gathered; a continuation by word w scores scores[g][k] + x_w - log sum exp(x), in 64
+ * bits (exponentials in fp32, their sum in 64 bits: 1e-7). Written best first: scores_out float[groups][n_out], parents (beam, 0 ... beams - 1) and
+ * tokens int[groups][n_out]. Of equal scores the lower beam is first, of one beam's the larger logit, of equal logits the lower word. A NaN counts
+ * as -infinity, a logit of +infinity as the largest finite number; what scores -infinity still fills places that nothing else takes.
+ * done: NULL, or device int[groups][beams]: a beam with done != 0 has ended: it goes on with the word eos alone, at the score that it has, and its
+ * logits are not read. done_out: NULL, or int[groups][n_out]: 1 where the parent was done or the word is eos (eos < 0: no such word, with
+ * done NULL). With n_out = beams the outputs of scores and done may be their inputs. All are device arrays.
+ * beams and n_out up to NCMB_MAX_BEAMS, n_out no more than beams * V, V up to 2^24. */
+#define NCMB_MAX_BEAMS 128
+int ncmb_beam_select(const void *logits, int64_t ldl, int type, int groups, int beams, int V, const float *scores, const int *done, int eos,
+                     int n_out, float *scores_out, int *parents, int *tokens, int *done_out);
+/* Rows of a paged cache go on as other rows of their group: row j of a group of `group` rows as the row parents[j] (device int[rows], 0 ... group - 1 within the
+ * group; anything else: row j holds no sequence). Full pages are shared. A row's pages from entry len / page on -- the begun one and those in
+ * reserve, of which the first has to be there -- are its own: the lowest row that continues a parent keeps the parent's, further ones take
+ * those of the group's rows that nobody continues, in order, and get the begun page's tokens copied, in each of n_layer pools, layer_stride
+ * elements apart from c->k and c->v, that share the table. So no page has to be found and none is lost but full pages that no row holds any more.
+ * table_dst (as c->table, same stride; not c->table) and len_dst (device int[rows], not c->len) receive tables and lengths; entries that have no
+ * page become -1. refs: NULL, or device int[n_pages]: to each page's count the change of the number of entries that hold it is added. group up
+ * to NCMB_MAX_GROUP and a divisor of rows. */
+#define NCMB_MAX_GROUP 256
+int ncmb_paged_reorder(const NcmbPaged *c, int group, const int *parents, int n_layer, int64_t layer_stride, int *table_dst, int *len_dst, int *refs);
+
 #ifdef __cplusplus
 }
 #endif

@@ -68,6 +68,54 @@ class KVCache(C.Structure):
         return c
 
 
+ROPE_HALVES, ROPE_PAIRS = 0, 1                               # NCMB_ROPE_*: which dims are a pair
+ROPE_PLAIN, ROPE_LINEAR, ROPE_BASE, ROPE_PARTS = range(4)    # scalings
+
+
+class Rope(C.Structure):
+    """NcmbRope: what rotary positions do to a head; filled by ncmb_rope_plan."""
+    _fields_ = [("dims", _I), ("layout", _I), ("magnitude", _F), ("turns", C.c_double * 128)]
+
+
+def strides(t, n):
+    """The first n strides of a torch tensor whose last dim is contiguous, as the int64 array that ncmb_rope takes."""
+    if t.stride(-1) != 1 and t.shape[-1] > 1:
+        raise ValueError("the head dim has to be contiguous")
+    return (_I64 * n)(*t.stride()[:n])
+
+
+class PagedCache(C.Structure):
+    """NcmbPaged: keys and values in pages of a pool in device memory, and each row's table of pages."""
+    _fields_ = [("k", _P), ("v", _P), ("type", _I), ("rows", _I), ("n_kv", _I), ("hd", _I), ("page", _I), ("n_pages", _I), ("page_stride", _I64),
+                ("head_stride", _I64), ("token_stride", _I64), ("table", _P), ("table_stride", _I64), ("max_pages", _I), ("len", _P)]
+
+    @classmethod
+    def of(cls, k, v, table, length):
+        """From torch tensors: k and v as float32 or bfloat16 views [pages][n_kv][slots][hd] of one layout, table int32[rows][entries] with
+        contiguous rows, length int32[rows], contiguous. The cache keeps them alive (``held``)."""
+        kinds = {"torch.float32": F32, "torch.bfloat16": BF16}
+        if len(k.shape) != 4:
+            raise ValueError("keys and values are [pages][n_kv][slots][hd]")
+        if tuple(k.shape) != tuple(v.shape) or tuple(k.stride()) != tuple(v.stride()) or k.dtype != v.dtype:
+            raise ValueError("keys and values differ in shape, strides or type")
+        if k.stride(3) != 1 and k.shape[3] > 1:
+            raise ValueError("the head dim has to be contiguous")
+        if str(k.dtype) not in kinds:
+            raise ValueError("a cache of %s: float32 or bfloat16" % k.dtype)
+        p, h, n, d = k.shape
+        if str(table.dtype) != "torch.int32" or len(table.shape) != 2 or (table.shape[1] > 1 and table.stride(1) != 1):
+            raise ValueError("a table is an int32[rows][entries] with contiguous rows")
+        b, e = table.shape
+        if str(length.dtype) != "torch.int32" or tuple(length.shape) != (b,) or (b > 1 and length.stride(0) != 1):
+            raise ValueError("lengths are a contiguous int32[rows]")
+        if not k.device == v.device == table.device == length.device:
+            raise ValueError("keys, values, table and lengths are on different devices")
+        c = cls(k.data_ptr(), v.data_ptr(), kinds[str(k.dtype)], b, h, d, n, p, k.stride(0), k.stride(1), k.stride(2), table.data_ptr(),
+                table.stride(0) if b > 1 else e, e, length.data_ptr())
+        c.held = (k, v, table, length)
+        return c
+
+
 # name -> (restype, argtypes); only the inference surface
 _SIGS = {
     # runtime (src/ncm.h:37-70,139,261)
@@ -194,6 +242,12 @@ _SIGS = {
     "ncmb_cache_evict": (_I, [C.POINTER(KVCache), C.POINTER(KVCache), _P, _P, _P, _P, _P, _P, _I, _I, _I, _P]),
     "ncmb_block_summaries": (_I, [C.POINTER(KVCache), _I, _P, _I, _I, _P, _P]),
     "ncmb_block_attention": (_I, [C.POINTER(KVCache), _P, _I64, _P, _I64, _I, _I, _I, _I, _P, _P, _I, _I, _I, _F, _I, _P]),
+    "ncmb_rope_plan": (_I, [C.POINTER(Rope), _I, _I, C.c_double, _I, C.c_double, C.c_double, C.c_double, C.c_double, C.c_double]),
+    "ncmb_rope": (_I, [C.POINTER(Rope), _P, C.POINTER(_I64), _P, C.POINTER(_I64), _I, _I, _I, _I, _I, _P, _I]),
+    "ncmb_paged_append": (_I, [C.POINTER(PagedCache), C.POINTER(Rope), _P, _I64, _P, _I64, _I, _P, _I64, _P, _I64, _I, _I, _P, _P]),
+    "ncmb_paged_attention": (_I, [C.POINTER(PagedCache), _P, _I64, _P, _I64, _I, _I, _I, _P, _F, _I]),
+    "ncmb_beam_select": (_I, [_P, _I64, _I, _I, _I, _I, _P, _P, _I, _I, _P, _P, _P, _P]),
+    "ncmb_paged_reorder": (_I, [C.POINTER(PagedCache), _I, _P, _I, _I64, _P, _P, _P]),
     "gpt2_cmd_ppl": (_I, [_P, C.c_char_p, C.c_char_p, C.c_char_p]),
     "gpt2_cmd_verify": (_I, [_P, C.c_char_p, C.c_char_p, C.c_char_p]),
     "qwen_cmd_ppl": (_I, [_P, C.c_char_p, C.c_char_p, C.c_char_p]),

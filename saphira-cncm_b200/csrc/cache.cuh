@@ -17,6 +17,8 @@ struct CacheDev {
 
 // One line to stderr and -1: what an entry point returns for arguments it refuses.
 int cache_refuse(const char *who, const char *fmt, ...);
+// 0 when the current device is the one that the library runs on, else -1 with a message
+int cache_device(const char *who);
 // 0 when the cache's description is one the kernels take (see ncm_b200.h), else -1 with a message
 int cache_check(const char *who, const NcmbCache *c, CacheDev &d);
 inline int cache_elem(const NcmbCache *c) { return c->type == NCMB_BF16 ? 2 : 4; }

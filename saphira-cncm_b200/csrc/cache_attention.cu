@@ -22,6 +22,13 @@ int cache_refuse(const char *who, const char *fmt, ...) {
     return -1;
 }
 
+int cache_device(const char *who) {
+    ensure_device();
+    int dev = -1;
+    if (cudaGetDevice(&dev) != cudaSuccess) (void)cudaGetLastError();
+    return dev == ctx().device ? 0 : cache_refuse(who, "device %d is current, the library runs on %d", dev, ctx().device);
+}
+
 int cache_check(const char *who, const NcmbCache *c, CacheDev &d) {
     if (!c) return cache_refuse(who, "no cache");
     if (c->type != NCMB_F32 && c->type != NCMB_BF16) return cache_refuse(who, "cache type %d", c->type);

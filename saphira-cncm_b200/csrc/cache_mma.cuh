@@ -1,5 +1,5 @@
-// Attention of a few query rows to many cached keys on mma.sync tiles: what ncmb_cache_attention and
-// ncmb_block_attention share. The query rows of a kv head -- its G query heads times the tokens that share the keys --
+// Attention of a few query rows to many cached keys on mma.sync tiles: what ncmb_cache_attention, ncmb_block_attention and
+// ncmb_paged_attention share. The query rows of a kv head -- its G query heads times the tokens that share the keys --
 // are the 16-row tiles; a warp walks chunks of keys with a running maximum and sum a row.
 //
 // Products in fp32 grade whatever the types: a bf16 key meets an fp32 query as three bf16 terms (24 bits, exact products),
@@ -18,6 +18,7 @@
 
 namespace ncmb {
 
+constexpr int CM_LOG(int x) { return x <= 1 ? 0 : 1 + CM_LOG(x / 2); }
 constexpr int CM_WARPS = 4, CM_THREADS = CM_WARPS * 32, CM_MAXC = 8;      // CM_MAXC: CTAs of a cluster
 // R: query rows of a tile, 16 or 8. A tile of 8 has two terms of its queries (or probabilities) stacked in the 16 rows of the
 // tensor-core tile; a lane holds rows lane / 4 and lane / 4 + 8 of a result, so it adds the two terms' products up itself.
@@ -67,6 +68,10 @@ struct CmArgs {
     // block attention
     int block_log, n_sel;
     const int *picks;
+    // paged caches (c.cap: what a row's pages hold)
+    const int *table;
+    int64_t table_stride, ps;        // entries; bytes from page to page
+    int page_log, n_pages, max_pages;
 };
 
 __device__ __forceinline__ uint32_t cm_smem(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -180,7 +185,9 @@ template <bool BLOCKS, int KC> __device__ int cm_find(const CmArgs &a, int x, in
 // column in a tile is free as long as both operands, or all who read the result, agree.
 // CL: a cluster of CTAs does a unit, each an equal run of its chunks, and their results meet in distributed shared memory: for
 // calls that are all latency. Else the units' chunks are dealt out as above.
-template <class KE, class QE, int HDP, int R, bool BLOCKS, bool CL>
+// PAGED: keys through the row's table of pages. A chunk's keys stand in one page or in up to four; their entries are fetched a chunk ahead of
+// its copies, an entry a lane, and an entry that is no page (or a row of a negative length) leaves zeros, which no query sees.
+template <class KE, class QE, int HDP, int R, bool BLOCKS, bool CL, bool PAGED = false>
 __global__ void __launch_bounds__(CM_THREADS, CmCfg<KE, QE, HDP, R>::ctas(BLOCKS)) k_cache_attention(const __grid_constant__ CmArgs a) {
     using F = CmCfg<KE, QE, HDP, R>;
     constexpr int KC = F::KC, NT = F::NT, NQ = F::NQ, NP = F::NP, ROW = F::ROW, UPR = F::UPR, M = F::M, NH = F::NH;
@@ -262,6 +269,44 @@ __global__ void __launch_bounds__(CM_THREADS, CmCfg<KE, QE, HDP, R>::ctas(BLOCKS
         constexpr auto swz_v = [](int i) { return F::BF ? ((i * RPI) & 7) * 16 : ((((i * RPI) >> 1) & 3) << 1) * 16; };
         const int64_t step = (int64_t)RPI * a.c.ts, mine = lr * a.c.ts + lu * 16;
         const bool fast = hd == HDP && (!BLOCKS || (1 << a.block_log) >= KC);
+        // paged: entries of a chunk's pages, one a lane; unseen: four bits a stage, set for pages of its chunk that are none
+        constexpr int MOST_PAGES = KC / 8;
+        static_assert(!PAGED || (MOST_PAGES <= 4 && CM_STAGES <= 8), "a chunk's pages fit four bits");
+        const int pages_log = PAGED ? max(0, CM_LOG(KC) - a.page_log) : 0, pages = 1 << pages_log, slot_log = CM_LOG(KC) - pages_log;
+        const int *entries = PAGED ? a.table + row * a.table_stride : nullptr;
+        const bool has_row = !PAGED || a.c.len[row] >= 0;
+        uint32_t unseen = 0;
+        auto fetch = [&](int ch) {
+            int e = -1;
+            if (PAGED && has_row && ch < stop && lane < MOST_PAGES && lane < pages) {
+                const int i = ch * KC >> a.page_log;
+                if (i + lane < a.max_pages) e = __ldg(entries + i + lane);
+            }
+            return e;
+        };
+        auto load_paged = [&](int ch, int stage, int entry) {
+            const bool there = (unsigned)entry < (unsigned)a.n_pages;
+            const uint32_t none = ~__ballot_sync(0xffffffffu, there) & ((1u << pages) - 1);
+            unseen = (unseen & ~(15u << 4 * stage)) | none << 4 * stage;
+            const uint32_t ks = to_k + stage * CM_STAGE, vs = to_v + stage * CM_STAGE;
+            const int64_t at = (int64_t)(ch * KC & ((1 << a.page_log) - 1)) * a.c.ts + lu * 16;
+            const bool whole = fast && none == 0 && (ch + 1) * KC <= len;
+#pragma unroll
+            for (int i = 0; i < KC / RPI; i++) {
+                const int r = lr + i * RPI, j = r >> slot_log;
+                const int64_t off = (int64_t)__shfl_sync(0xffffffffu, entry, j) * a.ps + (int64_t)(r - (j << slot_log)) * a.c.ts + at;
+                const uint32_t dk = (ks ^ swz_k(i)) + i * RPI * ROW, dv = (vs ^ swz_v(i)) + i * RPI * ROW;
+                if (whole) {
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dk), "l"(kb + off) : "memory");
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dv), "l"(vb + off) : "memory");
+                } else {
+                    const int pos = ch * KC + r;
+                    const bool ok = lane_in && pos < n && !((none >> j) & 1u) && !(tail && pos >= len && !used(pos - len));
+                    cm_cp16(dk, kb + (ok ? off : 0), ok);
+                    cm_cp16(dv, vb + (ok ? off : 0), ok);
+                }
+            }
+        };
         auto load = [&](int ch, int stage) {
             const uint32_t ks = to_k + stage * CM_STAGE, vs = to_v + stage * CM_STAGE;
             if (fast && (ch + 1) * KC <= len) {                  // keys side by side, all there
@@ -359,12 +404,18 @@ __global__ void __launch_bounds__(CM_THREADS, CmCfg<KE, QE, HDP, R>::ctas(BLOCKS
             for (int e = 0; e < 2 * NH; e++) O[j][e] = 0.f;
 #pragma unroll
         for (int hh = 0; hh < NH; hh++) { mx[hh] = -INFINITY; ls[hh] = 0.f; }
-        int stage = 0;
+        int stage = 0, entry = -1;
+        if constexpr (PAGED) entry = fetch(first + warp);
         // loads run CM_STAGES - 1 chunks ahead of the arithmetic
         for (int ch = first + warp - (CM_STAGES - 1) * CM_WARPS, ahead = 0; ch < stop; ch += CM_WARPS) {
             const int next = ch + (CM_STAGES - 1) * CM_WARPS;
             __syncwarp();                                        // the stage it goes to has been read
-            if (next < stop) load(next, ahead);
+            if constexpr (PAGED) {
+                if (next < stop) load_paged(next, ahead, entry);
+                entry = fetch(next + CM_WARPS);
+            } else {
+                if (next < stop) load(next, ahead);
+            }
             asm volatile("cp.async.commit_group;" ::: "memory");
             if (++ahead == CM_STAGES) ahead = 0;
             if (ch < first) {
@@ -374,7 +425,8 @@ __global__ void __launch_bounds__(CM_THREADS, CmCfg<KE, QE, HDP, R>::ctas(BLOCKS
             asm volatile("cp.async.wait_group %0;" ::"n"(CM_STAGES - 1) : "memory");
             __syncwarp();
             const char *kt = my + stage * CM_STAGE, *vt = kt + CM_STAGE / 2;
-            const bool masked = (ch + 1) * KC > len;
+            const uint32_t none = PAGED ? (unseen >> 4 * stage) & 15u : 0u;
+            const bool masked = (ch + 1) * KC > len || none != 0;
             float S[NT][4];
 #pragma unroll
             for (int j = 0; j < NT; j++) S[j][0] = S[j][1] = S[j][2] = S[j][3] = 0.f;
@@ -461,6 +513,7 @@ __global__ void __launch_bounds__(CM_THREADS, CmCfg<KE, QE, HDP, R>::ctas(BLOCKS
                             const int pos = ch * KC + 8 * j + 2 * c4 + e;
                             bool see = pos < len;
                             if (!BLOCKS && !see && pos < n) see = (bits[(pos - len) >> 5] >> ((pos - len) & 31)) & 1u;
+                            if (PAGED && ((none >> ((pos & (KC - 1)) >> slot_log)) & 1u)) see = false;
                             if (!see) S[j][2 * hh + e] = -INFINITY;
                         }
                 }
@@ -799,7 +852,7 @@ __device__ __forceinline__ int2 cm_range(const CmArgs &a, int64_t unit) {
     const int2 r = a.range[unit];
     return r.x >= 0 && r.x <= r.y && r.y < a.ctas ? r : make_int2(0, -1);
 }
-template <class KE, class QE, int HDP, int R, bool BLOCKS>
+template <class KE, class QE, int HDP, int R, bool BLOCKS, bool PAGED = false>       // PAGED: each instance is in one file
 __global__ void __launch_bounds__(CM_THREADS) k_cache_join(const __grid_constant__ CmArgs a, int joins, int split, int wkeys) {
     using F = CmCfg<KE, QE, HDP, R>;
     constexpr int M = F::M, D4 = HDP / 4, GROUPS = CM_THREADS / D4;
@@ -955,15 +1008,15 @@ template <class F> bool cm_parts(const char *who, CmArgs &a, int rows, int64_t u
     return true;
 }
 // first(): launches what has to run before; only once nothing can be refused any more
-template <class KE, class QE, int HDP, int R, bool BLOCKS, class FIRST>
+template <class KE, class QE, int HDP, int R, bool BLOCKS, bool PAGED = false, class FIRST>
 int cm_run_as(const char *who, CmArgs a, int max_keys, FIRST first) {
     using F = CmCfg<KE, QE, HDP, R>;
     a.tiles = (int)cdiv(a.M, F::M);
     const int smem = F::RING + F::QBYTES;
     static bool set = false;
     if (!set) {
-        CUDA_CHECK(cudaFuncSetAttribute(k_cache_attention<KE, QE, HDP, R, BLOCKS, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-        CUDA_CHECK(cudaFuncSetAttribute(k_cache_attention<KE, QE, HDP, R, BLOCKS, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+        CUDA_CHECK(cudaFuncSetAttribute(k_cache_attention<KE, QE, HDP, R, BLOCKS, false, PAGED>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+        CUDA_CHECK(cudaFuncSetAttribute(k_cache_attention<KE, QE, HDP, R, BLOCKS, true, PAGED>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
         set = true;
     }
     // rows of a launch: as many as leave the scores some GB at most, and the count of chunks in 31 bits
@@ -989,7 +1042,7 @@ int cm_run_as(const char *who, CmArgs a, int max_keys, FIRST first) {
         if (a.weights && !(a.scores = (float *)cache_scratch(who, (size_t)rows * a.c.nkv * a.M * a.pitch * 4))) return -1;
         a.items = rows * per_row;
         first();
-        cache_launch(k_cache_attention<KE, QE, HDP, R, BLOCKS, true>, dim3(nc * a.tiles, a.c.nkv, a.items), CM_THREADS, smem, nc, a);
+        cache_launch(k_cache_attention<KE, QE, HDP, R, BLOCKS, true, PAGED>, dim3(nc * a.tiles, a.c.nkv, a.items), CM_THREADS, smem, nc, a);
         return 0;
     }
     const int ctas = (int)std::max<int64_t>(1, std::min<int64_t>(resident, cdiv(units * chunks, CM_WARPS)));
@@ -1004,10 +1057,10 @@ int cm_run_as(const char *who, CmArgs a, int max_keys, FIRST first) {
         const int nr = std::min(step, rows - r);
         a.row0 = r;
         a.items = nr * per_row;
-        LAUNCH_PDL((k_cache_attention<KE, QE, HDP, R, BLOCKS, false>), ctas, CM_THREADS, smem, a);
+        LAUNCH_PDL((k_cache_attention<KE, QE, HDP, R, BLOCKS, false, PAGED>), ctas, CM_THREADS, smem, a);
         if (fused) continue;
         const int64_t joins = nr * row_units * (F::M / (split ? 1 : CM_THREADS / (HDP / 4)));
-        LAUNCH_PDL((k_cache_join<KE, QE, HDP, R, BLOCKS>), (unsigned)(joins + spans / step * nr), CM_THREADS, 0, a, (int)joins, split, cm_wkeys(a.M));
+        LAUNCH_PDL((k_cache_join<KE, QE, HDP, R, BLOCKS, PAGED>), (unsigned)(joins + spans / step * nr), CM_THREADS, 0, a, (int)joins, split, cm_wkeys(a.M));
     }
     return 0;
 }

@@ -1,0 +1,119 @@
+// Rotary positions: what ncmb_rope and ncmb_paged_append share.
+//
+// A pair (x1, x2) at angle a = 2 pi p f, f full turns a position: y1 = m (x1 cos a - x2 sin a), y2 = m (x2 cos a + x1 sin a). p f is formed in 64
+// bits and only its fraction of a turn goes on in fp32: at position 10^6 an fp32 product is off by 0.06 radians.
+//
+// A thread's item is two vectors of V elements of a head. HALVES: the vectors at i and i + dims / 2, V pairs; PAIRS: two
+// neighbouring vectors, each of V / 2 pairs; dims that stay: two neighbouring vectors. V is 16 bytes where the dims allow it.
+#pragma once
+#include "cache.cuh"
+
+#include <type_traits>
+
+namespace ncmb {
+
+// 0 when the plan is one that heads of hd can be rotated by, else -1 with a message
+int rope_check(const char *who, const NcmbRope *r, int hd);
+
+// elements of a vector: 16 bytes, or what the pairs of a plan leave whole
+inline int rope_vec(const NcmbRope *r, int elem_bytes) {
+    int v = 16 / elem_bytes;
+    if (!r) return v;
+    const int n = r->layout == NCMB_ROPE_PAIRS ? r->dims : r->dims / 2;
+    while (n % v) v >>= 1;
+    return v;
+}
+// items of a head
+inline int rope_items(const NcmbRope *r, int hd, int v) {
+    if (!r || r->layout == NCMB_ROPE_PAIRS) return (int)cdiv(hd, 2 * v);
+    return r->dims / 2 / v + (int)cdiv(hd - r->dims, 2 * v);
+}
+
+#ifdef __CUDACC__
+template <class E, int V> __device__ __forceinline__ void rope_load(const E *p, float (&x)[V]) {
+    if constexpr (std::is_same_v<E, float>) {
+        if constexpr (V == 4) { const float4 u = *(const float4 *)p; x[0] = u.x; x[1] = u.y; x[2] = u.z; x[3] = u.w; }
+        else if constexpr (V == 2) { const float2 u = *(const float2 *)p; x[0] = u.x; x[1] = u.y; }
+        else x[0] = *p;
+    } else {
+        uint32_t u[V / 2 > 0 ? V / 2 : 1];
+        if constexpr (V == 8) { const uint4 w = *(const uint4 *)p; u[0] = w.x; u[1] = w.y; u[2] = w.z; u[3] = w.w; }
+        else if constexpr (V == 4) { const uint2 w = *(const uint2 *)p; u[0] = w.x; u[1] = w.y; }
+        else if constexpr (V == 2) u[0] = *(const uint32_t *)p;
+        else u[0] = *(const unsigned short *)p;
+#pragma unroll
+        for (int i = 0; i < V; i++) x[i] = __uint_as_float(i & 1 ? u[i / 2] & 0xffff0000u : u[i / 2] << 16);
+    }
+}
+// rounds once, to the nearest
+template <class E, int V> __device__ __forceinline__ void rope_store(E *p, const float (&x)[V]) {
+    if constexpr (std::is_same_v<E, float>) {
+        if constexpr (V == 8) { *(float4 *)p = make_float4(x[0], x[1], x[2], x[3]); *(float4 *)(p + 4) = make_float4(x[4], x[5], x[6], x[7]); }
+        else if constexpr (V == 4) *(float4 *)p = make_float4(x[0], x[1], x[2], x[3]);
+        else if constexpr (V == 2) *(float2 *)p = make_float2(x[0], x[1]);
+        else *p = x[0];
+    } else {
+        uint32_t u[V / 2 > 0 ? V / 2 : 1];
+        if constexpr (V == 1) *p = __float2bfloat16(x[0]);
+        else {
+#pragma unroll
+            for (int i = 0; i < V / 2; i++) { const __nv_bfloat162 t = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]); u[i] = *(const uint32_t *)&t; }
+            if constexpr (V == 8) *(uint4 *)p = make_uint4(u[0], u[1], u[2], u[3]);
+            else if constexpr (V == 4) *(uint2 *)p = make_uint2(u[0], u[1]);
+            else *(uint32_t *)p = u[0];
+        }
+    }
+}
+
+// cosine and sine of pair i at position pos, times the magnitude
+__device__ __forceinline__ float2 rope_angle(const NcmbRope &r, int i, int pos, bool inverse) {
+    const double t = (double)pos * r.turns[i];
+    float s, c;
+    sincospif((float)(2.0 * (t - rint(t))), &s, &c);
+    return make_float2(c * r.magnitude, (inverse ? -s : s) * r.magnitude);
+}
+
+// where item u of a head stands, what its vectors are rotated by, if at all
+struct RopeItem {
+    int d0, d1;              // dims of its two vectors; d1 < 0: there is no second
+    int pair0, pair1;        // first pairs of their rotation, or -1
+};
+template <int V, bool PAIRS> __device__ __forceinline__ RopeItem rope_item(int u, int dims, int hd) {
+    RopeItem it;
+    const int rot = PAIRS ? 0 : dims / 2 / V;
+    if (!PAIRS && u < rot) { it.d0 = u * V; it.d1 = it.d0 + dims / 2; it.pair0 = it.pair1 = it.d0; return it; }
+    it.d0 = (PAIRS ? 0 : dims) + 2 * (u - rot) * V;
+    it.d1 = it.d0 + V < hd ? it.d0 + V : -1;
+    it.pair0 = PAIRS && it.d0 < dims ? it.d0 / 2 : -1;
+    it.pair1 = PAIRS && it.d1 >= 0 && it.d1 < dims ? it.d1 / 2 : -1;
+    return it;
+}
+// a, b: the item's vectors; cs: the token's cosines and sines
+template <int V, bool PAIRS> __device__ __forceinline__ void rope_turn(const RopeItem &it, const float2 *cs, float (&a)[V], float (&b)[V]) {
+    if constexpr (PAIRS) {
+        static_assert(V >= 2, "a pair is in one vector");
+        auto one = [&](int pair, float (&x)[V]) {
+            if (pair < 0) return;
+#pragma unroll
+            for (int i = 0; i < V / 2; i++) {
+                const float2 f = cs[pair + i];
+                const float p = x[2 * i], q = x[2 * i + 1];
+                x[2 * i] = p * f.x - q * f.y;
+                x[2 * i + 1] = q * f.x + p * f.y;
+            }
+        };
+        one(it.pair0, a);
+        one(it.pair1, b);
+    } else if (it.pair0 >= 0) {
+#pragma unroll
+        for (int i = 0; i < V; i++) {
+            const float2 f = cs[it.pair0 + i];
+            const float p = a[i], q = b[i];
+            a[i] = p * f.x - q * f.y;
+            b[i] = q * f.x + p * f.y;
+        }
+    }
+}
+#endif
+
+} // namespace ncmb

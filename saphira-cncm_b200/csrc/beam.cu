@@ -5,8 +5,8 @@
 // the order is that of its logits, so no more of them can be wanted. The last CTA of a group joins the parts.
 //
 // n largest: of the maxima of 2 n or more groups of threads the n-th largest is a bound that n values reach, and few values more; what
-// reaches it goes to a list in shared memory. Later tiles have to beat the n-th of the list, which most do not: they cost a comparison a value.
-// Keys are unique -- value, then lower index -- so equal values are no case of their own, and no order of arrival shows in the result. A bound is reached
+// reaches it goes to a list in shared memory, as does what beats the bound in later tiles; a list that fills up is cut to its n largest, and the bound is
+// theirs. So a value costs a comparison, and few more. Keys are unique -- value, then lower index -- so equal values are no case of their own, and no order of arrival shows in the result. A bound is reached
 // by at most n groups, so a tile adds at most half of its values to the list, whatever the values are.
 //
 // Rounding: exponentials in fp32 against the thread's maximum, 16 of them summed in fp32, everything after in 64 bits; scores in 64 bits, so that
@@ -21,16 +21,18 @@ namespace {
 constexpr int BM_THREADS = 256, BM_WARPS = BM_THREADS / 32;
 constexpr int BM_EPT = 16, BM_TILE = BM_THREADS * BM_EPT;        // logits of a thread and a CTA at a time
 constexpr int BM_JOIN = 4;                                       // candidates of a thread at a time where parts are joined
+constexpr int BM_START = 3, BM_ROUNDS = 6;
 constexpr float BM_LOG2E = 1.44269504f;
 
 struct BeamArgs {
     const char *x;
     int64_t ld;                      // bytes
     int groups, beams, V, n, parts, tiles;
+    int slots;                       // keys that a part may leave: 2 n, so that most need not settle which
     const float *scores; const int *done;
     int eos;
     float *scores_out; int *parents, *tokens, *done_out;
-    unsigned long long *keys;        // scratch, [row][part][n]
+    unsigned long long *keys;        // scratch, [row][part][slots]
     double2 *sums;                   // scratch, [row][part]: maximum, sum
     int *arrived;                    // scratch, [group], zero between calls
 };
@@ -44,7 +46,7 @@ __device__ __forceinline__ Wide bm_xor(const Wide &k, int o) { return Wide{__shf
 
 // the n largest keys of tiles of EPT a thread
 template <class K, int EPT> struct TopN {
-    static constexpr int CAP = BM_THREADS * EPT / 2 + NCMB_MAX_BEAMS;            // n, and what a tile adds at most
+    static constexpr int CAP = BM_THREADS * EPT / 2 + 2 * NCMB_MAX_BEAMS;        // a list that is not settled yet, and what a tile adds at most
     static constexpr int PER = (CAP + BM_THREADS - 1) / BM_THREADS;
     K list[CAP], few[NCMB_MAX_BEAMS * PER], groups[BM_THREADS], bound;
     int count, n_few, sums[BM_WARPS];
@@ -63,12 +65,11 @@ template <class K, int EPT> struct TopN {
         if (tid % size == 0) groups[tid / size] = best;
         if (tid == 0) bound = K{};
         __syncthreads();
-        if (tid < G) {
-            const K mine = groups[tid];
-            int rank = 0;
-            for (int j = 0; j < G; j++) rank += groups[j] > mine;
-            if (rank == n - 1 && bm_there(mine)) bound = mine;
-        }
+        int rank = 0;                    // a group's threads share the comparisons with the others
+#pragma unroll 4
+        for (int j = tid % size; j < G; j += size) rank += groups[j] > best;
+        for (int o = 1; o < size; o <<= 1) rank += __shfl_xor_sync(0xffffffffu, rank, o);
+        if (tid % size == 0 && rank == n - 1 && bm_there(best)) bound = best;
         __syncthreads();
         return bound;
     }
@@ -76,7 +77,7 @@ template <class K, int EPT> struct TopN {
     __device__ K settle(int n) {
         const int tid = threadIdx.x, c = count;
         int m = c;
-        if (c > 128) {
+        if (c > BM_THREADS / 2) {
             K best = K{};
             for (int i = tid; i < c; i += BM_THREADS) if (list[i] > best) best = list[i];
             const K least = nth(best, n);
@@ -87,49 +88,73 @@ template <class K, int EPT> struct TopN {
             few[tid] = list[tid];
         }
         __syncthreads();
-        if (c > 128) m = n_few;
-        for (int i = tid; i < m; i += BM_THREADS) {
-            const K mine = few[i];
+        if (c > BM_THREADS / 2) m = n_few;
+        int ways = 8;                    // threads that share a key's comparisons
+        while (ways > 1 && m * ways > BM_THREADS) ways >>= 1;
+        for (int i0 = 0; i0 < m; i0 += BM_THREADS / ways) {
+            const int i = i0 + tid / ways;
+            const K mine = few[min(i, m - 1)];
             int rank = 0;
-            for (int j = 0; j < m; j++) rank += few[j] > mine;
-            if (rank < n) list[rank] = mine;
+#pragma unroll 4
+            for (int j = tid % ways; j < m; j += ways) rank += few[j] > mine;
+            for (int o = 1; o < ways; o <<= 1) rank += __shfl_xor_sync(0xffffffffu, rank, o);
+            if (i < m && tid % ways == 0 && rank < n) list[rank] = mine;
         }
         if (tid == 0) count = min(n, m);
         __syncthreads();
         return m >= n ? list[n - 1] : K{};
     }
-    // the tile's keys that reach `least` (the n-th largest so far, or none) join the list; all threads call it. least is raised where the tile shows how far
-    __device__ void add(const K (&key)[EPT], int n, K &least) {
+    // the tile's keys -- key(e), e < EPT, of this thread -- that reach `least` (a bound that n keys reach, or none) join the list; all threads call it.
+    // least is raised where the tile shows how far
+    template <class KEY> __device__ void add(int n, K &least, KEY key) {
         const int tid = threadIdx.x;
-        auto joins = [&](int e) { return bm_there(key[e]) && !(least > key[e]); };
+        auto joins = [&](const K &k) { return bm_there(k) && !(least > k); };
+        if (!bm_there(least)) raise(n, least, key);
         for (int round = 0;; round++) {
             int c = 0;
-#pragma unroll
-            for (int e = 0; e < EPT; e++) c += joins(e);
+#pragma unroll 4
+            for (int e = 0; e < EPT; e++) c += joins(key(e));
             c = __reduce_add_sync(0xffffffffu, c);
             if ((tid & 31) == 0) sums[tid >> 5] = c;
-            const int have = count;                              // before the barrier: after it others add to it
+            const int have = count;      // before the barrier: after it others add to it
             __syncthreads();
             int total = 0;
 #pragma unroll
             for (int w = 0; w < BM_WARPS; w++) total += sums[w];
-            if ((bm_there(least) && have + total <= CAP) || round > 1) break;
+            if (have + total <= CAP || round == 2) break;
             __syncthreads();
-            if (round == 0 && have > n) {
+            if (round == 0) {
                 const K x = settle(n);
                 if (x > least) least = x;
-                continue;
+            } else {
+                raise(n, least, key);
             }
-            K best = K{};
-#pragma unroll
-            for (int e = 0; e < EPT; e++) if (key[e] > best) best = key[e];
-            const K x = nth(best, n);
-            if (x > least) least = x;
-            round = 1;
         }
-#pragma unroll
-        for (int e = 0; e < EPT; e++) if (joins(e)) list[atomicAdd(&count, 1)] = key[e];
+#pragma unroll 4
+        for (int e = 0; e < EPT; e++) {
+            const K k = key(e);
+            if (joins(k)) list[atomicAdd(&count, 1)] = k;
+        }
         __syncthreads();
+    }
+    // of a settled list, the keys whose lower half is at most `low`
+    __device__ void drop(uint32_t low) {
+        const int tid = threadIdx.x;
+        const bool stays = tid < count && (uint32_t)list[min(tid, CAP - 1)] > low;
+        const K mine = list[min(tid, CAP - 1)];
+        __syncthreads();
+        if (tid == 0) count = 0;
+        __syncthreads();
+        if (stays) list[atomicAdd(&count, 1)] = mine;
+        __syncthreads();
+    }
+    // least: up to what n keys of the tile reach
+    template <class KEY> __device__ void raise(int n, K &least, KEY key) {
+        K best = K{};
+#pragma unroll 4
+        for (int e = 0; e < EPT; e++) { const K k = key(e); if (k > best) best = k; }
+        const K x = nth(best, n);
+        if (x > least) least = x;
     }
 };
 
@@ -142,6 +167,9 @@ __device__ __forceinline__ uint32_t bm_order(float x) {          // larger is la
     const uint32_t u = __float_as_uint(x);
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
+__device__ __forceinline__ unsigned long long bm_key(float x, int w) {       // of a logit; -0 is 0
+    return (unsigned long long)bm_order(x + 0.f) << 32 | (0xffffffffu - (uint32_t)w);
+}
 __device__ __forceinline__ float bm_value(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k); }
 __device__ __forceinline__ unsigned long long bm_order(double x) {
     const unsigned long long u = __double_as_longlong(x);
@@ -149,83 +177,103 @@ __device__ __forceinline__ unsigned long long bm_order(double x) {
 }
 __device__ __forceinline__ double bm_value(unsigned long long k) { return __longlong_as_double(k >> 63 ? k ^ 1ull << 63 : ~k); }
 
-union BeamShared {
-    TopN<unsigned long long, BM_EPT> part;
-    TopN<Wide, BM_JOIN> join;
-};
-
 // ---- a group's parts, by the last CTA that has one ----
-__device__ void beam_join(const BeamArgs &a, int g, TopN<Wide, BM_JOIN> &top) {
-    __shared__ double lse[NCMB_MAX_BEAMS], score[NCMB_MAX_BEAMS];
-    __shared__ int over[NCMB_MAX_BEAMS];
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, n = a.n;
+struct JoinShared {
+    TopN<Wide, BM_JOIN> top;
+    Wide tile[BM_JOIN * BM_THREADS];
+    double lse[NCMB_MAX_BEAMS], score[NCMB_MAX_BEAMS];
+    int over[NCMB_MAX_BEAMS];
+};
+__device__ __noinline__ void beam_join(const BeamArgs &a, int g, JoinShared &sh) {
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, n = a.n, slots = a.slots;
     const int64_t row0 = (int64_t)g * a.beams;
     for (int k = warp; k < a.beams; k += BM_WARPS) {
         const double2 *s = a.sums + (row0 + k) * a.parts;
         const bool ended = a.done && a.done[row0 + k];
+        const float sc = a.scores[row0 + k];
         double m = -INFINITY, t = 0;
         if (!ended) {
-            for (int p = lane; p < a.parts; p += 32) m = fmax(m, __ldcg(&s[p].x));
-            for (int o = 16; o; o >>= 1) m = fmax(m, __shfl_xor_sync(0xffffffffu, m, o));
-            for (int p = lane; p < a.parts; p += 32) t += __ldcg(&s[p].y) * bm_exp2((float)(__ldcg(&s[p].x) - (m == -INFINITY ? 0 : m)) * BM_LOG2E);
+            for (int p = lane; p < a.parts; p += 32) {
+                const double2 x = __ldcg(s + p);                 // maximum, sum
+                const double top = fmax(m, x.x), base = top == -INFINITY ? 0 : top;
+                t = t * bm_exp2((float)(m - base) * BM_LOG2E) + x.y * bm_exp2((float)(x.x - base) * BM_LOG2E);
+                m = top;
+            }
+            double top = m;
+            for (int o = 16; o; o >>= 1) top = fmax(top, __shfl_xor_sync(0xffffffffu, top, o));
+            t *= bm_exp2((float)(m - (top == -INFINITY ? 0 : top)) * BM_LOG2E);
             for (int o = 16; o; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+            m = top;
         }
         if (lane == 0) {
-            const float sc = a.scores[row0 + k];
-            lse[k] = ended || m == -INFINITY ? 0.0 : m + log(t);
-            score[k] = sc == sc ? (double)sc : -INFINITY;
-            over[k] = ended;
+            sh.lse[k] = ended || m == -INFINITY ? 0.0 : m + log(t);
+            sh.score[k] = sc == sc ? (double)sc : -INFINITY;
+            sh.over[k] = ended;
         }
     }
-    top.clear();
-    const unsigned long long *keys = a.keys + row0 * a.parts * n;
-    const int total = a.beams * a.parts * n;
+    sh.top.clear();
+    const unsigned long long *keys = a.keys + row0 * a.parts * slots;
+    const int row = a.parts * slots, total = a.beams * row;
     Wide least = {};
+#pragma unroll 1
     for (int i0 = 0; i0 < total; i0 += BM_THREADS * BM_JOIN) {
-        Wide key[BM_JOIN];
+        unsigned long long u[BM_JOIN];
 #pragma unroll
         for (int e = 0; e < BM_JOIN; e++) {
             const int i = i0 + e * BM_THREADS + tid;
-            key[e] = Wide{};
-            if (i >= total) continue;
-            const int k = i / (a.parts * n), j = i - k * (a.parts * n);
-            uint32_t w;
-            float x;
-            if (over[k]) {                                       // its end, then the other words, which have nothing
-                if (j >= min(n, a.V)) continue;
+            u[e] = i < total ? __ldcg(keys + i) : 0;
+        }
+#pragma unroll 1
+        for (int e = 0; e < BM_JOIN; e++) {
+            const int i = i0 + e * BM_THREADS + tid, k = min(i / row, a.beams - 1), j = i - k * row;
+            Wide key = {};
+            uint32_t w = 0xffffffffu - (uint32_t)u[e];
+            float x = bm_value((uint32_t)(u[e] >> 32));
+            bool there = u[e] != 0;
+            if (sh.over[k]) {                                    // its end, then the other words, which have nothing
+                there = i < total && j < min(n, a.V);
                 w = j == 0 ? a.eos : j - 1 + (j - 1 >= a.eos);
                 x = j == 0 ? 0.f : -INFINITY;
-            } else {
-                const unsigned long long u = __ldcg(keys + i);
-                if (!u) continue;
-                w = 0xffffffffu - (uint32_t)u;
-                x = bm_value((uint32_t)(u >> 32));
             }
-            const double sc = x == -INFINITY ? -INFINITY : score[k] + ((double)x - lse[k]) + 0.0;
-            key[e] = Wide{bm_order(sc), (unsigned long long)(NCMB_MAX_BEAMS - 1 - k) << 56 | (unsigned long long)bm_order(x) << 24 | (0xffffffu - w)};
+            if (there) {
+                const double sc = x == -INFINITY ? -INFINITY : sh.score[k] + ((double)x - sh.lse[k]) + 0.0;
+                key = Wide{bm_order(sc), (unsigned long long)(NCMB_MAX_BEAMS - 1 - k) << 56 | (unsigned long long)bm_order(x) << 24 | (0xffffffu - w)};
+            }
+            sh.tile[e * BM_THREADS + tid] = key;
         }
-        top.add(key, n, least);
+        sh.top.add(n, least, [&](int e) { return sh.tile[e * BM_THREADS + tid]; });
     }
-    top.settle(n);
+    sh.top.settle(n);
     for (int i = tid; i < n; i += BM_THREADS) {
-        const Wide x = top.list[i];
+        const Wide x = sh.top.list[i];
         const int k = NCMB_MAX_BEAMS - 1 - (int)(x.lo >> 56), w = 0xffffff - (int)(x.lo & 0xffffffu);
         const int64_t at = (int64_t)g * n + i;
         a.scores_out[at] = (float)bm_value(x.hi);
         a.parents[at] = k;
         a.tokens[at] = w;
-        if (a.done_out) a.done_out[at] = over[k] || w == a.eos;
+        if (a.done_out) a.done_out[at] = sh.over[k] || w == a.eos;
     }
 }
 
-// CTA (row, part). VEC: rows of whole 16 bytes
+// ---- CTA (row, part) ----
+template <class E> struct PartShared {
+    static constexpr int STAGES = sizeof(E) == 4 ? 2 : 3;
+    E ring[STAGES][BM_TILE];
+    TopN<unsigned long long, BM_EPT> top;
+    double sums[BM_WARPS];
+    float maxima[BM_WARPS];
+};
+template <class E> constexpr size_t beam_smem() { return sizeof(PartShared<E>) > sizeof(JoinShared) ? sizeof(PartShared<E>) : sizeof(JoinShared); }
+
+// Tiles come through a ring in shared memory; a thread reads what it has copied itself, so no barrier is in between. VEC: rows of whole 16 bytes. Else a
+// thread's values are a CTA's width apart: 4 bytes a copy, and through registers those of 2 bytes.
 template <class E, bool VEC>
 __global__ void __launch_bounds__(BM_THREADS) k_beam_select(const __grid_constant__ BeamArgs a) {
-    __shared__ BeamShared sh;
-    __shared__ double reduce[BM_WARPS];
-    __shared__ float rmax[BM_WARPS];
+    extern __shared__ __align__(16) char smem[];
     __shared__ int last;
-    constexpr int VE = 16 / sizeof(E), NV = BM_EPT / VE;         // elements of 16 bytes, vectors of a thread
+    PartShared<E> &sh = *(PartShared<E> *)smem;
+    constexpr int STAGES = PartShared<E>::STAGES, VE = VEC ? 16 / (int)sizeof(E) : 1, NV = BM_EPT / VE;      // elements together, how many of them
+    constexpr bool ASYNC = VEC || sizeof(E) == 4;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int64_t row = blockIdx.x / a.parts;
     const int part = (int)(blockIdx.x - row * a.parts), g = (int)(row / a.beams);
@@ -234,82 +282,153 @@ __global__ void __launch_bounds__(BM_THREADS) k_beam_select(const __grid_constan
     if (!(a.done && a.done[row])) {
         const int t0 = (int)((int64_t)part * a.tiles / a.parts), t1 = (int)((int64_t)(part + 1) * a.tiles / a.parts);
         const E *x0 = (const E *)(a.x + row * a.ld);
-        auto word = [&](int t, int e) { return t * BM_TILE + (VEC ? (e / VE * BM_THREADS + tid) * VE + e % VE : e * BM_THREADS + tid); };
-        auto load = [&](int t, float (&x)[BM_EPT]) {
-            if constexpr (VEC) {
+        auto place = [&](int e) { return (e / VE * BM_THREADS + tid) * VE + e % VE; };          // of the thread's e-th value in a tile
+        E wait[ASYNC ? 1 : BM_EPT];
+        auto load = [&](int t, int stage) {
+            if (t < t1) {
+                const int left = a.V - t * BM_TILE;
+                const E *from = x0 + (int64_t)t * BM_TILE + place(0);
+                if constexpr (ASYNC) {
+                    const uint32_t to = (uint32_t)__cvta_generic_to_shared(&sh.ring[stage][place(0)]);
+                    constexpr int STEP = BM_THREADS * VE;                    // from one copy of a thread to its next
+                    if (left >= BM_TILE) {
 #pragma unroll
-                for (int i = 0; i < NV; i++) {
-                    const int w = word(t, i * VE);
-                    if (w + VE > a.V) {                          // the row's end
-#pragma unroll
-                        for (int e = 0; e < VE; e++) x[i * VE + e] = w + e < a.V ? (float)x0[w + e] : -INFINITY;
-                        continue;
+                        for (int i = 0; i < NV; i++) {
+                            const uint32_t dst = to + i * STEP * (int)sizeof(E);
+                            if constexpr (VEC) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(from + i * STEP) : "memory");
+                            else asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(from + i * STEP) : "memory");
+                        }
+                    } else {                                     // the row's end: a loop, so that whole tiles do not go through its instructions
+#pragma unroll 1
+                        for (int i = 0; i < NV; i++) {
+                            const uint32_t dst = to + i * STEP * (int)sizeof(E);
+                            const int bytes = max(0, min(VE, left - place(i * VE))) * (int)sizeof(E);
+                            if constexpr (VEC) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(bytes ? from + i * STEP : x0), "r"(bytes) : "memory");
+                            else asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(bytes ? from + i * STEP : x0), "r"(bytes) : "memory");
+                        }
                     }
-                    const uint4 u = __ldcs((const uint4 *)(x0 + w));
+                } else {
+#pragma unroll
+                    for (int e = 0; e < BM_EPT; e++) wait[e] = place(e) < left ? from[e * BM_THREADS] : E(0.f);
+                }
+            }
+            if constexpr (ASYNC) asm volatile("cp.async.commit_group;" ::: "memory");
+        };
+        constexpr int AHEAD = ASYNC ? STAGES - 1 : 1;
+#pragma unroll
+        for (int i = 0; i < AHEAD; i++) load(t0 + i, i);
+        sh.top.clear();
+        unsigned long long least = 0;
+        float m = -INFINITY, beat = -INFINITY;                   // beat: what a logit has to exceed, once there is a bound
+        double s = 0;
+        const int limit = min(3 * a.n + 8, sh.top.CAP / 2);      // a list of so many is cut: the bound that gives spares more than it costs
+#pragma unroll 1
+        for (int t = t0, stage = 0; t < t1; t++) {
+            E *mine = sh.ring[stage];
+            if constexpr (!ASYNC) {
+#pragma unroll
+                for (int e = 0; e < BM_EPT; e++) mine[place(e)] = wait[e];
+            }
+            load(t + AHEAD, stage + AHEAD < STAGES ? stage + AHEAD : stage + AHEAD - STAGES);
+            if constexpr (ASYNC) asm volatile("cp.async.wait_group %0;" ::"n"(AHEAD) : "memory");
+            const int end = a.V - t * BM_TILE;                   // words of the row from this tile on
+            if (end < BM_TILE) {
+#pragma unroll 1
+                for (int e = 0; e < BM_EPT; e++) if (place(e) >= end) mine[place(e)] = E(-INFINITY);
+            }
+            float x[BM_EPT];
+#pragma unroll
+            for (int i = 0; i < NV; i++) {
+                if constexpr (VEC) {
+                    const uint4 u = *(const uint4 *)(mine + place(i * VE));
                     const uint32_t uu[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
                     for (int e = 0; e < VE; e++) {
                         if constexpr (sizeof(E) == 4) x[i * VE + e] = __uint_as_float(uu[e]);
                         else x[i * VE + e] = __uint_as_float(e & 1 ? uu[e / 2] & 0xffff0000u : uu[e / 2] << 16);
                     }
+                } else x[i] = (float)mine[place(i)];
+            }
+            float tm, sum, top;                                  // sum: of exponentials against the new maximum
+#pragma unroll 1
+            for (;;) {
+#pragma unroll
+                for (int e = 1; e < BM_EPT; e++) tm = fmaxf(e == 1 ? x[0] : tm, x[e]);
+                top = fmaxf(m, tm);
+                const float base = top == -INFINITY ? 0.f : -top;
+                float2 part[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll
+                for (int i = 0; i < BM_EPT / 2; i++) {
+                    const float2 d = __fmul2_rn(__fadd2_rn(make_float2(x[2 * i], x[2 * i + 1]), make_float2(base, base)), make_float2(BM_LOG2E, BM_LOG2E));
+                    part[i & 1] = __fadd2_rn(part[i & 1], make_float2(bm_exp2(d.x), bm_exp2(d.y)));
                 }
-            } else {
+                sum = (part[0].x + part[0].y) + (part[1].x + part[1].y);
+                if (sum < INFINITY) break;
 #pragma unroll
-                for (int e = 0; e < BM_EPT; e++) {
-                    const int w = word(t, e);
-                    x[e] = w < a.V ? (float)x0[w] : -INFINITY;
+                for (int e = 0; e < BM_EPT; e++) x[e] = fminf(fmaxf(x[e], -INFINITY), 3.402823466e38f);     // a NaN or +infinity among them
+            }
+            if (top > m) {
+                s *= bm_exp2((m - top) * BM_LOG2E);
+                m = top;
+            }
+            s += (double)sum;
+            auto value = [&](int at) { return fminf(fmaxf((float)mine[at], -INFINITY), 3.402823466e38f); };
+            for (bool raise = least == 0;;) {
+                if (raise) {
+                    float most = tm;
+                    asm volatile("" : "+f"(most));               // not formed ahead of the branch, where every tile would pay for it
+                    uint32_t which = 0;
+#pragma unroll
+                    for (int e = 0; e < BM_EPT; e++) if (x[e] == most) which |= 1u << e;
+                    const int at = place(__ffs(which) - 1);      // of the thread's largest, of equal ones the first
+                    const unsigned long long nth = sh.top.nth(at < end ? bm_key(most, t * BM_TILE + at) : 0ull, a.n);
+                    if (nth > least) least = nth;
+                    beat = least ? bm_value((uint32_t)(least >> 32)) : -INFINITY;
                 }
+                bool full = false;
+                if (tm >= beat) {
+                    uint32_t hits = 0;
+#pragma unroll
+                    for (int e = 0; e < BM_EPT; e++) if (x[e] >= beat) hits |= 1u << e;
+#pragma unroll 1
+                    for (; hits; hits &= hits - 1) {
+                        const int e = place(__ffs(hits) - 1);
+                        const unsigned long long key = bm_key(value(e), t * BM_TILE + e);
+                        if (key < least || e >= end) continue;
+                        const int at = atomicAdd(&sh.top.count, 1);
+                        if (at < sh.top.CAP) sh.top.list[at] = key;
+                        full |= at >= limit;
+                    }
+                }
+                if (!__syncthreads_or(full)) break;
+                const bool lost = sh.top.count > sh.top.CAP;     // keys that found no room
+                __syncthreads();
+                if (lost && tid == 0) sh.top.count = sh.top.CAP;
+                __syncthreads();
+                const unsigned long long nth = sh.top.settle(a.n);
+                if (nth > least) { least = nth; beat = bm_value((uint32_t)(least >> 32)); }
+                if (!lost) break;
+                sh.top.drop(0xffffffffu - t * BM_TILE);          // the tile's: all of them are looked at once more
+                raise = true;
             }
-        };
-        sh.part.clear();
-        unsigned long long least = 0;
-        float m = -INFINITY, beat = -INFINITY;                   // beat: what a logit has to exceed, once the list is full
-        double s = 0;
-        float ahead[BM_EPT];
-        load(t0, ahead);
-        for (int t = t0; t < t1; t++) {
-            float x[BM_EPT];
-#pragma unroll
-            for (int e = 0; e < BM_EPT; e++) x[e] = fminf(fmaxf(ahead[e], -INFINITY), 3.402823466e38f);     // a NaN is -infinity
-            if (t + 1 < t1) load(t + 1, ahead);
-            float tm = x[0];
-#pragma unroll
-            for (int e = 1; e < BM_EPT; e++) tm = fmaxf(tm, x[e]);
-            if (tm > m) {
-                s *= bm_exp2((m - tm) * BM_LOG2E);
-                m = tm;
-            }
-            const float base = m == -INFINITY ? 0.f : m;
-            float sum[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int e = 0; e < BM_EPT; e++) sum[e & 3] += bm_exp2((x[e] - base) * BM_LOG2E);
-            s += (double)((sum[0] + sum[1]) + (sum[2] + sum[3]));
-            if (!__syncthreads_or(least == 0 || tm > beat)) continue;
-            unsigned long long key[BM_EPT];
-#pragma unroll
-            for (int e = 0; e < BM_EPT; e++) {
-                const int w = word(t, e);
-                key[e] = w < a.V ? (unsigned long long)bm_order(x[e] + 0.f) << 32 | (0xffffffffu - w) : 0ull;
-            }
-            sh.part.add(key, a.n, least);
-            beat = bm_value((uint32_t)(least >> 32));
+            if (++stage == STAGES) stage = 0;
         }
-        sh.part.settle(a.n);
-        // the part's list, maximum and sum
-        for (int i = tid; i < a.n; i += BM_THREADS) a.keys[(row * a.parts + part) * a.n + i] = i < sh.part.count ? sh.part.list[i] : 0ull;
+        // what may be among the n best, in no order, and the part's maximum and sum
+        if (sh.top.count > a.slots) sh.top.settle(a.n);
+        for (int i = tid; i < a.slots; i += BM_THREADS) a.keys[(row * a.parts + part) * a.slots + i] = i < sh.top.count ? sh.top.list[i] : 0ull;
         float top = m;
         for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-        if (lane == 0) rmax[warp] = top;
+        if (lane == 0) sh.maxima[warp] = top;
         __syncthreads();
 #pragma unroll
-        for (int w = 0; w < BM_WARPS; w++) top = fmaxf(top, rmax[w]);
+        for (int w = 0; w < BM_WARPS; w++) top = fmaxf(top, sh.maxima[w]);
         s *= m == -INFINITY ? 0.f : bm_exp2((m - top) * BM_LOG2E);
         for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-        if (lane == 0) reduce[warp] = s;
+        if (lane == 0) sh.sums[warp] = s;
         __syncthreads();
         if (tid == 0) {
             s = 0;
-            for (int w = 0; w < BM_WARPS; w++) s += reduce[w];
+            for (int w = 0; w < BM_WARPS; w++) s += sh.sums[w];
             a.sums[row * a.parts + part] = make_double2(top, s);
         }
     }
@@ -320,7 +439,16 @@ __global__ void __launch_bounds__(BM_THREADS) k_beam_select(const __grid_constan
     if (!last) return;
     if (tid == 0) a.arrived[g] = 0;                              // for the next call
     __threadfence();
-    beam_join(a, g, sh.join);
+    beam_join(a, g, *(JoinShared *)smem);
+}
+
+template <class E, bool VEC> void run_select(const BeamArgs &a, unsigned grid) {
+    static bool set = false;
+    if (!set) {
+        CUDA_CHECK(cudaFuncSetAttribute(k_beam_select<E, VEC>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)beam_smem<E>()));
+        set = true;
+    }
+    LAUNCH_PDL((k_beam_select<E, VEC>), grid, BM_THREADS, beam_smem<E>(), a);
 }
 
 } // namespace
@@ -347,10 +475,17 @@ extern "C" int ncmb_beam_select(const void *logits, int64_t ldl, int type, int g
     a.x = (const char *)logits; a.ld = ldl * es; a.groups = groups; a.beams = beams; a.V = V; a.n = n_out;
     a.tiles = (int)cdiv(V, BM_TILE);
     a.scores = scores; a.done = done; a.eos = eos; a.scores_out = scores_out; a.parents = parents; a.tokens = tokens; a.done_out = done_out;
-    // parts of a row: three rounds of the CTAs that fit the GPU, so that its last round is nearly full, but no more candidates than one CTA joins quickly
-    const int64_t slots = 4LL * ctx().sm_count;
-    a.parts = (int)std::max<int64_t>(1, std::min<int64_t>({a.tiles, cdiv(3 * slots, rows), 16384 / ((int64_t)beams * n_out)}));
-    const size_t kb = (size_t)rows * a.parts * n_out * 8, sb = (size_t)rows * a.parts * sizeof(double2);
+    a.slots = (int)std::min<int64_t>(2 * n_out, V);
+    // Parts of a row: as many as fill one to BM_ROUNDS rounds of the CTAs that fit the GPU, whichever takes least where a CTA's start and end cost as much as BM_START
+    // tiles; but no more candidates than one CTA joins quickly
+    const int64_t resident = (type == NCMB_F32 ? 3 : 4) * ctx().sm_count;
+    const int64_t most = std::max<int64_t>(1, std::min<int64_t>(a.tiles, 16384 / ((int64_t)beams * a.slots)));
+    int64_t best = INT64_MAX;
+    for (int r = 1; r <= BM_ROUNDS; r++) {
+        const int64_t p = std::max<int64_t>(1, std::min(most, r * resident / rows)), cost = cdiv(rows * p, resident) * (cdiv(a.tiles, p) + BM_START);
+        if (cost < best) { best = cost; a.parts = (int)p; }
+    }
+    const size_t kb = (size_t)rows * a.parts * a.slots * 8, sb = (size_t)rows * a.parts * sizeof(double2);
     char *scratch = (char *)cache_scratch(who, sb + kb);
     if (!scratch) return -1;
     a.sums = (double2 *)scratch;
@@ -359,8 +494,8 @@ extern "C" int ncmb_beam_select(const void *logits, int64_t ldl, int type, int g
     ProfScope prof(NCMB_K_SAMPLE, 4.0 * rows * V, (double)rows * V * es);
     const bool vec = (uintptr_t)logits % 16 == 0 && a.ld % 16 == 0;
     const unsigned grid = (unsigned)(rows * a.parts);
-    if (type == NCMB_F32) { if (vec) LAUNCH_PDL((k_beam_select<float, true>), grid, BM_THREADS, 0, a); else LAUNCH_PDL((k_beam_select<float, false>), grid, BM_THREADS, 0, a); }
-    else if (vec) LAUNCH_PDL((k_beam_select<__nv_bfloat16, true>), grid, BM_THREADS, 0, a);
-    else LAUNCH_PDL((k_beam_select<__nv_bfloat16, false>), grid, BM_THREADS, 0, a);
+    if (type == NCMB_F32) { if (vec) run_select<float, true>(a, grid); else run_select<float, false>(a, grid); }
+    else if (vec) run_select<__nv_bfloat16, true>(a, grid);
+    else run_select<__nv_bfloat16, false>(a, grid);
     return 0;
 }

@@ -21,7 +21,9 @@ namespace {
 constexpr int BM_THREADS = 256, BM_WARPS = BM_THREADS / 32;
 constexpr int BM_EPT = 16, BM_TILE = BM_THREADS * BM_EPT;        // logits of a thread and a CTA at a time
 constexpr int BM_JOIN = 4;                                       // candidates of a thread at a time where parts are joined
-constexpr int BM_START = 3, BM_ROUNDS = 6;
+constexpr int BM_BATCH = 4;                                      // tiles from one meeting of the warps to the next
+constexpr int BM_START = 3, BM_ROUNDS = 12;
+constexpr int BM_FEW = 16;                                       // continuations that most calls want
 constexpr float BM_LOG2E = 1.44269504f;
 
 struct BeamArgs {
@@ -44,11 +46,13 @@ __device__ __forceinline__ bool bm_there(const Wide &k) { return k.hi != 0; }
 __device__ __forceinline__ unsigned long long bm_xor(unsigned long long k, int o) { return __shfl_xor_sync(0xffffffffu, k, o); }
 __device__ __forceinline__ Wide bm_xor(const Wide &k, int o) { return Wide{__shfl_xor_sync(0xffffffffu, k.hi, o), __shfl_xor_sync(0xffffffffu, k.lo, o)}; }
 
-// the n largest keys of tiles of EPT a thread
-template <class K, int EPT> struct TopN {
-    static constexpr int CAP = BM_THREADS * EPT / 2 + 2 * NCMB_MAX_BEAMS;        // a list that is not settled yet, and what a tile adds at most
+// The n largest keys of tiles of EPT a thread; n up to MOST, BM_FEW or NCMB_MAX_BEAMS: the fewer, the less room the lists take.
+template <class K, int EPT, int MOST> struct TopN {
+    static constexpr int WIDEST = MOST <= BM_FEW ? 4 : 8;        // threads of a group
+    static constexpr int REACH = MOST <= BM_FEW ? MOST * WIDEST : BM_THREADS / 2;        // threads whose groups reach a bound, at most: n groups of 2 n or more
+    static constexpr int CAP = REACH * EPT + 2 * MOST;           // what a tile adds at most, and a list that is not settled yet
     static constexpr int PER = (CAP + BM_THREADS - 1) / BM_THREADS;
-    K list[CAP], few[NCMB_MAX_BEAMS * PER], groups[BM_THREADS], bound;
+    K list[CAP], few[REACH * PER > BM_THREADS / 2 ? REACH * PER : BM_THREADS / 2], groups[BM_THREADS], bound;
     int count, n_few, sums[BM_WARPS];
 
     __device__ void clear() {
@@ -57,7 +61,7 @@ template <class K, int EPT> struct TopN {
     }
     // the n-th largest of the maxima of 2 n groups of threads or more; no key where fewer than n have one
     __device__ K nth(K best, int n) {
-        int size = 8;
+        int size = WIDEST;
         while (size > 1 && BM_THREADS / size < 2 * n) size >>= 1;
         for (int o = 1; o < size; o <<= 1) { const K other = bm_xor(best, o); if (other > best) best = other; }
         const int tid = threadIdx.x, G = BM_THREADS / size;
@@ -167,6 +171,7 @@ __device__ __forceinline__ uint32_t bm_order(float x) {          // larger is la
     const uint32_t u = __float_as_uint(x);
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
+__device__ __forceinline__ float bm_clamp(float x) { return fminf(fmaxf(x, -INFINITY), 3.402823466e38f); }      // a NaN is -infinity
 __device__ __forceinline__ unsigned long long bm_key(float x, int w) {       // of a logit; -0 is 0
     return (unsigned long long)bm_order(x + 0.f) << 32 | (0xffffffffu - (uint32_t)w);
 }
@@ -178,15 +183,26 @@ __device__ __forceinline__ unsigned long long bm_order(double x) {
 __device__ __forceinline__ double bm_value(unsigned long long k) { return __longlong_as_double(k >> 63 ? k ^ 1ull << 63 : ~k); }
 
 // ---- a group's parts, by the last CTA that has one ----
-struct JoinShared {
-    TopN<Wide, BM_JOIN> top;
+template <int MOST> struct JoinShared {
+    TopN<Wide, BM_JOIN, MOST> top;
     Wide tile[BM_JOIN * BM_THREADS];
     double lse[NCMB_MAX_BEAMS], score[NCMB_MAX_BEAMS];
     int over[NCMB_MAX_BEAMS];
 };
-__device__ __noinline__ void beam_join(const BeamArgs &a, int g, JoinShared &sh) {
+template <int MOST> __device__ __noinline__ void beam_join(const BeamArgs &a, int g, JoinShared<MOST> &sh) {
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, n = a.n, slots = a.slots;
     const int64_t row0 = (int64_t)g * a.beams;
+    const unsigned long long *keys = a.keys + row0 * a.parts * slots;
+    const int row = a.parts * slots, total = a.beams * row;
+    unsigned long long u[BM_JOIN];
+    auto load = [&](int i0) {
+#pragma unroll
+        for (int e = 0; e < BM_JOIN; e++) {
+            const int i = i0 + e * BM_THREADS + tid;
+            u[e] = i < total ? __ldcg(keys + i) : 0;
+        }
+    };
+    load(0);                                                     // on their way while the sums meet
     for (int k = warp; k < a.beams; k += BM_WARPS) {
         const double2 *s = a.sums + (row0 + k) * a.parts;
         const bool ended = a.done && a.done[row0 + k];
@@ -212,18 +228,11 @@ __device__ __noinline__ void beam_join(const BeamArgs &a, int g, JoinShared &sh)
         }
     }
     sh.top.clear();
-    const unsigned long long *keys = a.keys + row0 * a.parts * slots;
-    const int row = a.parts * slots, total = a.beams * row;
     Wide least = {};
 #pragma unroll 1
     for (int i0 = 0; i0 < total; i0 += BM_THREADS * BM_JOIN) {
-        unsigned long long u[BM_JOIN];
+        if (i0) load(i0);
 #pragma unroll
-        for (int e = 0; e < BM_JOIN; e++) {
-            const int i = i0 + e * BM_THREADS + tid;
-            u[e] = i < total ? __ldcg(keys + i) : 0;
-        }
-#pragma unroll 1
         for (int e = 0; e < BM_JOIN; e++) {
             const int i = i0 + e * BM_THREADS + tid, k = min(i / row, a.beams - 1), j = i - k * row;
             Wide key = {};
@@ -256,23 +265,39 @@ __device__ __noinline__ void beam_join(const BeamArgs &a, int g, JoinShared &sh)
 }
 
 // ---- CTA (row, part) ----
-template <class E> struct PartShared {
-    static constexpr int STAGES = sizeof(E) == 4 ? 2 : 3;
+// Three CTAs an SM (two for long lists) with two tiles of each on their way
+template <class E, int MOST> struct PartShared {
+    static constexpr int STAGES = sizeof(E) == 4 ? 3 : 4;
     E ring[STAGES][BM_TILE];
-    TopN<unsigned long long, BM_EPT> top;
+    TopN<unsigned long long, BM_EPT, MOST> top;
     double sums[BM_WARPS];
     float maxima[BM_WARPS];
 };
-template <class E> constexpr size_t beam_smem() { return sizeof(PartShared<E>) > sizeof(JoinShared) ? sizeof(PartShared<E>) : sizeof(JoinShared); }
+template <class E, int MOST> constexpr size_t beam_smem() { return std::max(sizeof(PartShared<E, MOST>), sizeof(JoinShared<MOST>)); }
+
+template <int VE> __device__ __forceinline__ int bm_place(int e) { return (e / VE * BM_THREADS + (int)threadIdx.x) * VE + e % VE; }     // of a thread's e-th value in a tile
+// Tiles [t0, t1), of whose keys some found no room in the list: once more, each bounded by what it shows itself. Rare: their values lie badly, most of the
+// large ones with few threads, or rise from tile to tile.
+template <class E, bool VEC, int MOST>
+__device__ __noinline__ void beam_again(const E *x0, int t0, int t1, int V, int n, TopN<unsigned long long, BM_EPT, MOST> &top, unsigned long long &least) {
+    constexpr int VE = VEC ? 16 / (int)sizeof(E) : 1;
+    top.drop(0xffffffffu - t0 * BM_TILE);
+    for (int t = t0; t < t1; t++)
+        top.add(n, least, [&](int e) {
+            const int w = t * BM_TILE + bm_place<VE>(e);
+            return w < V ? bm_key(bm_clamp((float)x0[w]), w) : 0ull;
+        });
+}
 
 // Tiles come through a ring in shared memory; a thread reads what it has copied itself, so no barrier is in between. VEC: rows of whole 16 bytes. Else a
 // thread's values are a CTA's width apart: 4 bytes a copy, and through registers those of 2 bytes.
-template <class E, bool VEC>
-__global__ void __launch_bounds__(BM_THREADS) k_beam_select(const __grid_constant__ BeamArgs a) {
+template <class E, bool VEC, int MOST>
+__global__ void __launch_bounds__(BM_THREADS, 3) k_beam_select(const __grid_constant__ BeamArgs a) {
     extern __shared__ __align__(16) char smem[];
     __shared__ int last;
-    PartShared<E> &sh = *(PartShared<E> *)smem;
-    constexpr int STAGES = PartShared<E>::STAGES, VE = VEC ? 16 / (int)sizeof(E) : 1, NV = BM_EPT / VE;      // elements together, how many of them
+    using Shared = PartShared<E, MOST>;
+    Shared &sh = *(Shared *)smem;
+    constexpr int STAGES = Shared::STAGES, VE = VEC ? 16 / (int)sizeof(E) : 1, NV = BM_EPT / VE;      // elements together, how many of them
     constexpr bool ASYNC = VEC || sizeof(E) == 4;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int64_t row = blockIdx.x / a.parts;
@@ -282,7 +307,7 @@ __global__ void __launch_bounds__(BM_THREADS) k_beam_select(const __grid_constan
     if (!(a.done && a.done[row])) {
         const int t0 = (int)((int64_t)part * a.tiles / a.parts), t1 = (int)((int64_t)(part + 1) * a.tiles / a.parts);
         const E *x0 = (const E *)(a.x + row * a.ld);
-        auto place = [&](int e) { return (e / VE * BM_THREADS + tid) * VE + e % VE; };          // of the thread's e-th value in a tile
+        auto place = [&](int e) { return bm_place<VE>(e); };
         E wait[ASYNC ? 1 : BM_EPT];
         auto load = [&](int t, int stage) {
             if (t < t1) {
@@ -322,6 +347,8 @@ __global__ void __launch_bounds__(BM_THREADS) k_beam_select(const __grid_constan
         float m = -INFINITY, beat = -INFINITY;                   // beat: what a logit has to exceed, once there is a bound
         double s = 0;
         const int limit = min(3 * a.n + 8, sh.top.CAP / 2);      // a list of so many is cut: the bound that gives spares more than it costs
+        bool full = false;
+        int since = t0;                                          // the tile after the last at which all warps met
 #pragma unroll 1
         for (int t = t0, stage = 0; t < t1; t++) {
             E *mine = sh.ring[stage];
@@ -353,7 +380,10 @@ __global__ void __launch_bounds__(BM_THREADS) k_beam_select(const __grid_constan
 #pragma unroll 1
             for (;;) {
 #pragma unroll
-                for (int e = 1; e < BM_EPT; e++) tm = fmaxf(e == 1 ? x[0] : tm, x[e]);
+                for (int i = 0; i < BM_EPT / 4; i++) {
+                    const float quad = fmaxf(fmaxf(x[4 * i], x[4 * i + 1]), fmaxf(x[4 * i + 2], x[4 * i + 3]));
+                    tm = i ? fmaxf(tm, quad) : quad;
+                }
                 top = fmaxf(m, tm);
                 const float base = top == -INFINITY ? 0.f : -top;
                 float2 part[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
@@ -365,51 +395,51 @@ __global__ void __launch_bounds__(BM_THREADS) k_beam_select(const __grid_constan
                 sum = (part[0].x + part[0].y) + (part[1].x + part[1].y);
                 if (sum < INFINITY) break;
 #pragma unroll
-                for (int e = 0; e < BM_EPT; e++) x[e] = fminf(fmaxf(x[e], -INFINITY), 3.402823466e38f);     // a NaN or +infinity among them
+                for (int e = 0; e < BM_EPT; e++) x[e] = bm_clamp(x[e]);              // a NaN or +infinity among them
             }
             if (top > m) {
                 s *= bm_exp2((m - top) * BM_LOG2E);
                 m = top;
             }
             s += (double)sum;
-            auto value = [&](int at) { return fminf(fmaxf((float)mine[at], -INFINITY), 3.402823466e38f); };
-            for (bool raise = least == 0;;) {
-                if (raise) {
-                    float most = tm;
-                    asm volatile("" : "+f"(most));               // not formed ahead of the branch, where every tile would pay for it
-                    uint32_t which = 0;
+            if (least == 0) {                                    // the first tile
+                float most = tm;
+                asm volatile("" : "+f"(most));                   // not formed ahead of the branch, where every tile would pay for it
+                uint32_t which = 0;
 #pragma unroll
-                    for (int e = 0; e < BM_EPT; e++) if (x[e] == most) which |= 1u << e;
-                    const int at = place(__ffs(which) - 1);      // of the thread's largest, of equal ones the first
-                    const unsigned long long nth = sh.top.nth(at < end ? bm_key(most, t * BM_TILE + at) : 0ull, a.n);
-                    if (nth > least) least = nth;
-                    beat = least ? bm_value((uint32_t)(least >> 32)) : -INFINITY;
-                }
-                bool full = false;
-                if (tm >= beat) {
-                    uint32_t hits = 0;
+                for (int e = 0; e < BM_EPT; e++) if (x[e] == most) which |= 1u << e;
+                const int at = place(__ffs(which) - 1);          // of the thread's largest, of equal ones the first
+                least = sh.top.nth(at < end ? bm_key(most, t * BM_TILE + at) : 0ull, a.n);
+                if (least) beat = bm_value((uint32_t)(least >> 32));
+            }
+            if (tm >= beat) {
+                uint32_t hits = 0;
 #pragma unroll
-                    for (int e = 0; e < BM_EPT; e++) if (x[e] >= beat) hits |= 1u << e;
+                for (int e = 0; e < BM_EPT; e++) if (x[e] >= beat) hits |= 1u << e;
 #pragma unroll 1
-                    for (; hits; hits &= hits - 1) {
-                        const int e = place(__ffs(hits) - 1);
-                        const unsigned long long key = bm_key(value(e), t * BM_TILE + e);
-                        if (key < least || e >= end) continue;
-                        const int at = atomicAdd(&sh.top.count, 1);
-                        if (at < sh.top.CAP) sh.top.list[at] = key;
-                        full |= at >= limit;
-                    }
+                for (; hits; hits &= hits - 1) {
+                    const int e = place(__ffs(hits) - 1);
+                    const unsigned long long key = bm_key(bm_clamp((float)mine[e]), t * BM_TILE + e);
+                    if (key < least || e >= end) continue;
+                    const int at = atomicAdd(&sh.top.count, 1);
+                    if (at < sh.top.CAP) sh.top.list[at] = key;
+                    full |= at >= limit;
                 }
-                if (!__syncthreads_or(full)) break;
-                const bool lost = sh.top.count > sh.top.CAP;     // keys that found no room
-                __syncthreads();
-                if (lost && tid == 0) sh.top.count = sh.top.CAP;
-                __syncthreads();
-                const unsigned long long nth = sh.top.settle(a.n);
-                if (nth > least) { least = nth; beat = bm_value((uint32_t)(least >> 32)); }
-                if (!lost) break;
-                sh.top.drop(0xffffffffu - t * BM_TILE);          // the tile's: all of them are looked at once more
-                raise = true;
+            }
+            // warps meet every few tiles only: the one with most hits is not waited for
+            if (t + 1 - since == BM_BATCH || t + 1 == t1) {
+                if (__syncthreads_or(full)) {
+                    const bool lost = sh.top.count > sh.top.CAP; // keys that found no room
+                    __syncthreads();
+                    if (lost && tid == 0) sh.top.count = sh.top.CAP;
+                    __syncthreads();
+                    const unsigned long long nth = sh.top.settle(a.n);
+                    if (nth > least) least = nth;
+                    if (lost) beam_again<E, VEC, MOST>(x0, since, t + 1, a.V, a.n, sh.top, least);
+                    if (least) beat = bm_value((uint32_t)(least >> 32));
+                }
+                full = false;
+                since = t + 1;
             }
             if (++stage == STAGES) stage = 0;
         }
@@ -439,16 +469,20 @@ __global__ void __launch_bounds__(BM_THREADS) k_beam_select(const __grid_constan
     if (!last) return;
     if (tid == 0) a.arrived[g] = 0;                              // for the next call
     __threadfence();
-    beam_join(a, g, *(JoinShared *)smem);
+    beam_join<MOST>(a, g, *(JoinShared<MOST> *)smem);
 }
 
-template <class E, bool VEC> void run_select(const BeamArgs &a, unsigned grid) {
+template <class E, bool VEC, int MOST> void run_select_of(const BeamArgs &a, unsigned grid) {
     static bool set = false;
     if (!set) {
-        CUDA_CHECK(cudaFuncSetAttribute(k_beam_select<E, VEC>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)beam_smem<E>()));
+        CUDA_CHECK(cudaFuncSetAttribute(k_beam_select<E, VEC, MOST>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)beam_smem<E, MOST>()));
         set = true;
     }
-    LAUNCH_PDL((k_beam_select<E, VEC>), grid, BM_THREADS, beam_smem<E>(), a);
+    LAUNCH_PDL((k_beam_select<E, VEC, MOST>), grid, BM_THREADS, (beam_smem<E, MOST>()), a);
+}
+template <class E, bool VEC> void run_select(const BeamArgs &a, unsigned grid) {
+    if (a.n <= BM_FEW) run_select_of<E, VEC, BM_FEW>(a, grid);
+    else run_select_of<E, VEC, NCMB_MAX_BEAMS>(a, grid);
 }
 
 } // namespace
@@ -476,13 +510,12 @@ extern "C" int ncmb_beam_select(const void *logits, int64_t ldl, int type, int g
     a.tiles = (int)cdiv(V, BM_TILE);
     a.scores = scores; a.done = done; a.eos = eos; a.scores_out = scores_out; a.parents = parents; a.tokens = tokens; a.done_out = done_out;
     a.slots = (int)std::min<int64_t>(2 * n_out, V);
-    // Parts of a row: as many as fill one to BM_ROUNDS rounds of the CTAs that fit the GPU, whichever takes least where a CTA's start and end cost as much as BM_START
-    // tiles; but no more candidates than one CTA joins quickly
-    const int64_t resident = (type == NCMB_F32 ? 3 : 4) * ctx().sm_count;
-    const int64_t most = std::max<int64_t>(1, std::min<int64_t>(a.tiles, 16384 / ((int64_t)beams * a.slots)));
+    // Parts of a row, by what an SM then has to do: k CTAs, each of a start and an end that take as long as BM_START tiles, and of its tiles; one CTA alone gets
+    // half of an SM's bandwidth. But no more candidates than one CTA joins quickly.
+    const int64_t sms = ctx().sm_count, most = std::max<int64_t>(1, std::min<int64_t>(a.tiles, 16384 / ((int64_t)beams * a.slots)));
     int64_t best = INT64_MAX;
     for (int r = 1; r <= BM_ROUNDS; r++) {
-        const int64_t p = std::max<int64_t>(1, std::min(most, r * resident / rows)), cost = cdiv(rows * p, resident) * (cdiv(a.tiles, p) + BM_START);
+        const int64_t p = std::max<int64_t>(1, std::min(most, r * sms / rows)), k = cdiv(rows * p, sms), cost = std::max<int64_t>(k, 2) * cdiv(a.tiles, p) + BM_START * k;
         if (cost < best) { best = cost; a.parts = (int)p; }
     }
     const size_t kb = (size_t)rows * a.parts * a.slots * 8, sb = (size_t)rows * a.parts * sizeof(double2);

@@ -30,11 +30,11 @@ struct BeamArgs {
     const char *x;
     int64_t ld;                      // bytes
     int groups, beams, V, n, parts, tiles;
-    int slots;                       // keys that a part may leave: 2 n, so that most need not settle which
+    int slots;                       // keys that a part leaves: 2 n in any order where one tile joins them all, so that most need not settle which; else n in order
     const float *scores; const int *done;
     int eos;
     float *scores_out; int *parents, *tokens, *done_out;
-    unsigned long long *keys;        // scratch, [row][part][slots]
+    unsigned long long *keys;        // scratch, [group][slot][beam][part]
     double2 *sums;                   // scratch, [row][part]: maximum, sum
     int *arrived;                    // scratch, [group], zero between calls
 };
@@ -47,10 +47,11 @@ __device__ __forceinline__ unsigned long long bm_xor(unsigned long long k, int o
 __device__ __forceinline__ Wide bm_xor(const Wide &k, int o) { return Wide{__shfl_xor_sync(0xffffffffu, k.hi, o), __shfl_xor_sync(0xffffffffu, k.lo, o)}; }
 
 // The n largest keys of tiles of EPT a thread; n up to MOST, BM_FEW or NCMB_MAX_BEAMS: the fewer, the less room the lists take.
-template <class K, int EPT, int MOST> struct TopN {
+// ROOM: keys that the list holds beside 2 n; 0: what a tile adds at most, once it has a bound.
+template <class K, int EPT, int MOST, int ROOM = 0> struct TopN {
     static constexpr int WIDEST = MOST <= BM_FEW ? 4 : 8;        // threads of a group
     static constexpr int REACH = MOST <= BM_FEW ? MOST * WIDEST : BM_THREADS / 2;        // threads whose groups reach a bound, at most: n groups of 2 n or more
-    static constexpr int CAP = REACH * EPT + 2 * MOST;           // what a tile adds at most, and a list that is not settled yet
+    static constexpr int CAP = (ROOM ? ROOM : REACH * EPT) + 2 * MOST;
     static constexpr int PER = (CAP + BM_THREADS - 1) / BM_THREADS;
     K list[CAP], few[REACH * PER > BM_THREADS / 2 ? REACH * PER : BM_THREADS / 2], groups[BM_THREADS], bound;
     int count, n_few, sums[BM_WARPS];
@@ -155,7 +156,7 @@ template <class K, int EPT, int MOST> struct TopN {
     // least: up to what n keys of the tile reach
     template <class KEY> __device__ void raise(int n, K &least, KEY key) {
         K best = K{};
-#pragma unroll 4
+#pragma unroll
         for (int e = 0; e < EPT; e++) { const K k = key(e); if (k > best) best = k; }
         const K x = nth(best, n);
         if (x > least) least = x;
@@ -184,16 +185,15 @@ __device__ __forceinline__ double bm_value(unsigned long long k) { return __long
 
 // ---- a group's parts, by the last CTA that has one ----
 template <int MOST> struct JoinShared {
-    TopN<Wide, BM_JOIN, MOST> top;
-    Wide tile[BM_JOIN * BM_THREADS];
+    TopN<Wide, BM_JOIN, MOST, BM_JOIN * BM_THREADS> top;         // a whole tile fits
     double lse[NCMB_MAX_BEAMS], score[NCMB_MAX_BEAMS];
     int over[NCMB_MAX_BEAMS];
 };
 template <int MOST> __device__ __noinline__ void beam_join(const BeamArgs &a, int g, JoinShared<MOST> &sh) {
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, n = a.n, slots = a.slots;
     const int64_t row0 = (int64_t)g * a.beams;
-    const unsigned long long *keys = a.keys + row0 * a.parts * slots;
-    const int row = a.parts * slots, total = a.beams * row;
+    const int lists = a.beams * a.parts, total = lists * slots;
+    const unsigned long long *keys = a.keys + (int64_t)g * total;
     unsigned long long u[BM_JOIN];
     auto load = [&](int i0) {
 #pragma unroll
@@ -229,28 +229,41 @@ template <int MOST> __device__ __noinline__ void beam_join(const BeamArgs &a, in
     }
     sh.top.clear();
     Wide least = {};
+    const int limit = min(3 * n + 8, 2 * MOST);                  // fewer are in the list when a tile begins, so the tile fits
 #pragma unroll 1
     for (int i0 = 0; i0 < total; i0 += BM_THREADS * BM_JOIN) {
-        if (i0) load(i0);
+        Wide key[BM_JOIN];
 #pragma unroll
         for (int e = 0; e < BM_JOIN; e++) {
-            const int i = i0 + e * BM_THREADS + tid, k = min(i / row, a.beams - 1), j = i - k * row;
-            Wide key = {};
+            const int i = i0 + e * BM_THREADS + tid, j = i / lists, k = (i - j * lists) / a.parts;
             uint32_t w = 0xffffffffu - (uint32_t)u[e];
             float x = bm_value((uint32_t)(u[e] >> 32));
             bool there = u[e] != 0;
             if (sh.over[k]) {                                    // its end, then the other words, which have nothing
-                there = i < total && j < min(n, a.V);
+                there = i < total && (i - j * lists) % a.parts == 0 && j < min(n, a.V);
                 w = j == 0 ? a.eos : j - 1 + (j - 1 >= a.eos);
                 x = j == 0 ? 0.f : -INFINITY;
             }
-            if (there) {
-                const double sc = x == -INFINITY ? -INFINITY : sh.score[k] + ((double)x - sh.lse[k]) + 0.0;
-                key = Wide{bm_order(sc), (unsigned long long)(NCMB_MAX_BEAMS - 1 - k) << 56 | (unsigned long long)bm_order(x) << 24 | (0xffffffu - w)};
-            }
-            sh.tile[e * BM_THREADS + tid] = key;
+            const double sc = x == -INFINITY ? -INFINITY : sh.score[k] + ((double)x - sh.lse[k]) + 0.0;
+            key[e] = there ? Wide{bm_order(sc), (unsigned long long)(NCMB_MAX_BEAMS - 1 - k) << 56 | (unsigned long long)bm_order(x) << 24 | (0xffffffu - w)} : Wide{};
         }
-        sh.top.add(n, least, [&](int e) { return sh.tile[e * BM_THREADS + tid]; });
+        load(i0 + BM_THREADS * BM_JOIN);
+        if (!bm_there(least)) sh.top.raise(n, least, [&](int e) { return key[e]; });
+        bool full = false, any = false;
+#pragma unroll
+        for (int e = 0; e < BM_JOIN; e++) {
+            if (!bm_there(key[e]) || least > key[e]) continue;
+            const int at = atomicAdd(&sh.top.count, 1);
+            sh.top.list[at] = key[e];
+            full |= at >= limit;
+            any = true;
+        }
+        // in order, and none of the next of each list is among the best: nor are those behind
+        if (slots == n && lists <= BM_THREADS * BM_JOIN && !__syncthreads_or(any)) break;
+        if (__syncthreads_or(full)) {
+            const Wide nth = sh.top.settle(n);
+            if (nth > least) least = nth;
+        }
     }
     sh.top.settle(n);
     for (int i = tid; i < n; i += BM_THREADS) {
@@ -443,9 +456,10 @@ __global__ void __launch_bounds__(BM_THREADS, 3) k_beam_select(const __grid_cons
             }
             if (++stage == STAGES) stage = 0;
         }
-        // what may be among the n best, in no order, and the part's maximum and sum
-        if (sh.top.count > a.slots) sh.top.settle(a.n);
-        for (int i = tid; i < a.slots; i += BM_THREADS) a.keys[(row * a.parts + part) * a.slots + i] = i < sh.top.count ? sh.top.list[i] : 0ull;
+        // what may be among the n best, and the part's maximum and sum
+        if (sh.top.count > a.slots || a.slots == a.n) sh.top.settle(a.n);
+        const int lists = a.beams * a.parts, list = (int)(row - (int64_t)g * a.beams) * a.parts + part;
+        for (int i = tid; i < a.slots; i += BM_THREADS) a.keys[((int64_t)g * a.slots + i) * lists + list] = i < sh.top.count ? sh.top.list[i] : 0ull;
         float top = m;
         for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
         if (lane == 0) sh.maxima[warp] = top;
@@ -509,15 +523,15 @@ extern "C" int ncmb_beam_select(const void *logits, int64_t ldl, int type, int g
     a.x = (const char *)logits; a.ld = ldl * es; a.groups = groups; a.beams = beams; a.V = V; a.n = n_out;
     a.tiles = (int)cdiv(V, BM_TILE);
     a.scores = scores; a.done = done; a.eos = eos; a.scores_out = scores_out; a.parents = parents; a.tokens = tokens; a.done_out = done_out;
-    a.slots = (int)std::min<int64_t>(2 * n_out, V);
     // Parts of a row, by what an SM then has to do: k CTAs, each of a start and an end that take as long as BM_START tiles, and of its tiles; one CTA alone gets
-    // half of an SM's bandwidth. But no more candidates than one CTA joins quickly.
-    const int64_t sms = ctx().sm_count, most = std::max<int64_t>(1, std::min<int64_t>(a.tiles, 16384 / ((int64_t)beams * a.slots)));
+    // half of an SM's bandwidth.
+    const int64_t sms = ctx().sm_count, most = std::max<int64_t>(1, std::min<int64_t>(a.tiles, 65536 / ((int64_t)beams * n_out)));
     int64_t best = INT64_MAX;
     for (int r = 1; r <= BM_ROUNDS; r++) {
         const int64_t p = std::max<int64_t>(1, std::min(most, r * sms / rows)), k = cdiv(rows * p, sms), cost = std::max<int64_t>(k, 2) * cdiv(a.tiles, p) + BM_START * k;
         if (cost < best) { best = cost; a.parts = (int)p; }
     }
+    a.slots = (int64_t)beams * a.parts * 2 * n_out <= BM_THREADS * BM_JOIN ? 2 * n_out : n_out;
     const size_t kb = (size_t)rows * a.parts * a.slots * 8, sb = (size_t)rows * a.parts * sizeof(double2);
     char *scratch = (char *)cache_scratch(who, sb + kb);
     if (!scratch) return -1;

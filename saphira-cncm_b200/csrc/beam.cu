@@ -19,10 +19,11 @@ namespace ncmb {
 namespace {
 
 constexpr int BM_THREADS = 256, BM_WARPS = BM_THREADS / 32;
-constexpr int BM_EPT = 16, BM_TILE = BM_THREADS * BM_EPT;        // logits of a thread and a CTA at a time
+constexpr int BM_EPT = 32, BM_TILE = BM_THREADS * BM_EPT;        // logits of a thread and a CTA at a time
+constexpr int BM_CHUNK = 8;                                      // logits of a thread whose keys fit the list whatever they are, once they are bounded
 constexpr int BM_JOIN = 4;                                       // candidates of a thread at a time where parts are joined
 constexpr int BM_BATCH = 4;                                      // tiles from one meeting of the warps to the next
-constexpr int BM_START = 3, BM_ROUNDS = 12;
+constexpr int BM_START = 2, BM_ROUNDS = 4, BM_CTAS = 2;          // BM_CTAS: of an SM; with three, 80 registers a thread leave less to overlap (39 -> 47 us)
 constexpr int BM_FEW = 16;                                       // continuations that most calls want
 constexpr float BM_LOG2E = 1.44269504f;
 
@@ -278,34 +279,35 @@ template <int MOST> __device__ __noinline__ void beam_join(const BeamArgs &a, in
 }
 
 // ---- CTA (row, part) ----
-// Three CTAs an SM (two for long lists) with two tiles of each on their way
+// One tile of fp32 is on its way while another is worked on, or two of bf16
 template <class E, int MOST> struct PartShared {
-    static constexpr int STAGES = sizeof(E) == 4 ? 3 : 4;
+    static constexpr int STAGES = sizeof(E) == 4 ? 2 : 3;
     E ring[STAGES][BM_TILE];
-    TopN<unsigned long long, BM_EPT, MOST> top;
+    TopN<unsigned long long, BM_CHUNK, MOST> top;
     double sums[BM_WARPS];
     float maxima[BM_WARPS];
 };
 template <class E, int MOST> constexpr size_t beam_smem() { return std::max(sizeof(PartShared<E, MOST>), sizeof(JoinShared<MOST>)); }
 
 template <int VE> __device__ __forceinline__ int bm_place(int e) { return (e / VE * BM_THREADS + (int)threadIdx.x) * VE + e % VE; }     // of a thread's e-th value in a tile
-// Tiles [t0, t1), of whose keys some found no room in the list: once more, each bounded by what it shows itself. Rare: their values lie badly, most of the
+// Tiles [t0, t1), of whose keys some found no room in the list: once more, a few values a thread at a time, each time bounded by what these show. Rare: their values lie badly, most of the
 // large ones with few threads, or rise from tile to tile.
 template <class E, bool VEC, int MOST>
-__device__ __noinline__ void beam_again(const E *x0, int t0, int t1, int V, int n, TopN<unsigned long long, BM_EPT, MOST> &top, unsigned long long &least) {
+__device__ __noinline__ void beam_again(const E *x0, int t0, int t1, int V, int n, TopN<unsigned long long, BM_CHUNK, MOST> &top, unsigned long long &least) {
     constexpr int VE = VEC ? 16 / (int)sizeof(E) : 1;
     top.drop(0xffffffffu - t0 * BM_TILE);
     for (int t = t0; t < t1; t++)
-        top.add(n, least, [&](int e) {
-            const int w = t * BM_TILE + bm_place<VE>(e);
-            return w < V ? bm_key(bm_clamp((float)x0[w]), w) : 0ull;
-        });
+        for (int e0 = 0; e0 < BM_EPT; e0 += BM_CHUNK)
+            top.add(n, least, [&](int e) {
+                const int w = t * BM_TILE + bm_place<VE>(e0 + e);
+                return w < V ? bm_key(bm_clamp((float)x0[w]), w) : 0ull;
+            });
 }
 
 // Tiles come through a ring in shared memory; a thread reads what it has copied itself, so no barrier is in between. VEC: rows of whole 16 bytes. Else a
 // thread's values are a CTA's width apart: 4 bytes a copy, and through registers those of 2 bytes.
 template <class E, bool VEC, int MOST>
-__global__ void __launch_bounds__(BM_THREADS, 3) k_beam_select(const __grid_constant__ BeamArgs a) {
+__global__ void __launch_bounds__(BM_THREADS, BM_CTAS) k_beam_select(const __grid_constant__ BeamArgs a) {
     extern __shared__ __align__(16) char smem[];
     __shared__ int last;
     using Shared = PartShared<E, MOST>;
@@ -337,7 +339,7 @@ __global__ void __launch_bounds__(BM_THREADS, 3) k_beam_select(const __grid_cons
                             else asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(from + i * STEP) : "memory");
                         }
                     } else {                                     // the row's end: a loop, so that whole tiles do not go through its instructions
-#pragma unroll 1
+#pragma unroll 2
                         for (int i = 0; i < NV; i++) {
                             const uint32_t dst = to + i * STEP * (int)sizeof(E);
                             const int bytes = max(0, min(VE, left - place(i * VE))) * (int)sizeof(E);
@@ -373,7 +375,7 @@ __global__ void __launch_bounds__(BM_THREADS, 3) k_beam_select(const __grid_cons
             if constexpr (ASYNC) asm volatile("cp.async.wait_group %0;" ::"n"(AHEAD) : "memory");
             const int end = a.V - t * BM_TILE;                   // words of the row from this tile on
             if (end < BM_TILE) {
-#pragma unroll 1
+#pragma unroll 4
                 for (int e = 0; e < BM_EPT; e++) if (place(e) >= end) mine[place(e)] = E(-INFINITY);
             }
             float x[BM_EPT];
@@ -523,12 +525,12 @@ extern "C" int ncmb_beam_select(const void *logits, int64_t ldl, int type, int g
     a.x = (const char *)logits; a.ld = ldl * es; a.groups = groups; a.beams = beams; a.V = V; a.n = n_out;
     a.tiles = (int)cdiv(V, BM_TILE);
     a.scores = scores; a.done = done; a.eos = eos; a.scores_out = scores_out; a.parents = parents; a.tokens = tokens; a.done_out = done_out;
-    // Parts of a row, by what an SM then has to do: k CTAs, each of a start and an end that take as long as BM_START tiles, and of its tiles; one CTA alone gets
-    // half of an SM's bandwidth.
-    const int64_t sms = ctx().sm_count, most = std::max<int64_t>(1, std::min<int64_t>(a.tiles, 65536 / ((int64_t)beams * n_out)));
+    // Parts of a row: as many as fill one to BM_ROUNDS rounds of the CTAs that fit the GPU, whichever takes least where a CTA's start and end take as long as
+    // BM_START tiles (256 rows of 151936 in fp32, 1 / 2 / 3 / 5 parts: 39 / 44 / 49 / 54 us; 32 rows, 4 / 9 parts: 18 / 17; 1 and 9 are taken).
+    const int64_t resident = BM_CTAS * ctx().sm_count, most = std::max<int64_t>(1, std::min<int64_t>(a.tiles, 65536 / ((int64_t)beams * n_out)));
     int64_t best = INT64_MAX;
     for (int r = 1; r <= BM_ROUNDS; r++) {
-        const int64_t p = std::max<int64_t>(1, std::min(most, r * sms / rows)), k = cdiv(rows * p, sms), cost = std::max<int64_t>(k, 2) * cdiv(a.tiles, p) + BM_START * k;
+        const int64_t p = std::max<int64_t>(1, std::min(most, r * resident / rows)), cost = cdiv(rows * p, resident) * (cdiv(a.tiles, p) + BM_START);
         if (cost < best) { best = cost; a.parts = (int)p; }
     }
     a.slots = (int64_t)beams * a.parts * 2 * n_out <= BM_THREADS * BM_JOIN ? 2 * n_out : n_out;

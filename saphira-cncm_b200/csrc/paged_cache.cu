@@ -33,7 +33,7 @@ int paged_check(const char *who, const NcmbPaged *c, PagedDev &d) {
 namespace {
 
 // ---- new tokens ----
-constexpr int PA_THREADS = 256, PA_TOKENS = 16, PA_BATCH = 2, PA_ROWS = 1024;
+constexpr int PA_THREADS = 256, PA_TOKENS = 32, PA_BATCH = 4, PA_ROWS = 1024;
 
 struct AppendArgs {
     PagedDev c;
@@ -57,86 +57,95 @@ __device__ int append_row(const int *s, int rows, int i) {
 }
 
 // A CTA has `per` tokens: where each goes and the cosines and sines of its angles once, in shared memory, then all items of its heads -- queries, keys,
-// values. QE: type of the activations, KE: of the cache. ROPE: 0 none, 1 halves, 2 pairs.
+// values -- PA_BATCH of a thread on their way at a time, the first of them while places and angles are found. QE: type of the activations, KE: of the
+// cache. ROPE: 0 none, 1 halves, 2 pairs.
 template <class QE, class KE, int V, int ROPE>
 __global__ void __launch_bounds__(PA_THREADS) k_paged_append(const __grid_constant__ NcmbRope r, const __grid_constant__ AppendArgs a) {
     extern __shared__ float2 cs[];               // [per][dims / 2]
     __shared__ int64_t slot[PA_TOKENS];          // bytes from the pool's start; -1: not stored, -2: nobody's
     __shared__ int place[PA_TOKENS];
     __shared__ int starts[PA_ROWS + 1];
-    const int tid = threadIdx.x, pairs = ROPE ? r.dims / 2 : 0;
+    const int tid = threadIdx.x, pairs = ROPE ? r.dims / 2 : 0, heads = a.H + 2 * a.c.nkv;
+    const int n0 = blockIdx.x * a.per, here = min(a.per, a.tokens - n0);
+    const bool near = a.c.rows <= PA_ROWS;
+    RopeWalk at(tid, PA_THREADS, heads, a.items);
+    const RopeItem it = rope_item<V, ROPE != 1>(at.u, a.items, ROPE ? r.dims : 0, a.c.hd);
     pdl_wait();
     pdl_launch_dependents();
-    const int n0 = blockIdx.x * a.per, here = min(a.per, a.tokens - n0), heads = a.H + 2 * a.c.nkv, per_token = heads * a.items, total = here * per_token;
-    const bool near = a.c.rows <= PA_ROWS;
-    if (a.start && near) for (int i = tid; i <= a.c.rows; i += PA_THREADS) starts[i] = a.start[i];
-    float p[PA_BATCH][V], q[PA_BATCH][V];
-    RopeItem it[PA_BATCH];
-    int tok[PA_BATCH], head[PA_BATCH];
-    auto load = [&](int i0) {
+    RopeVec<QE, V> p[PA_BATCH], q[PA_BATCH];
+    RopeWalk from = at;
+    auto load = [&] {
+        from = at;
 #pragma unroll
         for (int x = 0; x < PA_BATCH; x++) {
-            const int i = i0 + x * PA_THREADS;
-            if (i >= total) continue;
-            tok[x] = i / per_token;
-            const int j = i - tok[x] * per_token, h = j / a.items, n = n0 + tok[x];
-            it[x] = rope_item<V, ROPE != 1>(j - h * a.items, ROPE ? r.dims : 0, a.c.hd);
-            head[x] = h;
-            const char *from = h < a.H ? a.q + n * a.ldq : h < a.H + a.c.nkv ? a.k + n * a.ldk : a.v + n * a.ldv;
-            const QE *f = (const QE *)from + (h < a.H ? h : h < a.H + a.c.nkv ? h - a.H : h - a.H - a.c.nkv) * a.c.hd;
-            rope_load<QE, V>(f + it[x].d0, p[x]);
-            if (it[x].d1 >= 0) rope_load<QE, V>(f + it[x].d1, q[x]);
+            if (at.tok < here) {
+                const int64_t n = n0 + at.tok;
+                const int kvh = at.h - a.H;
+                const char *row = kvh < 0 ? a.q + n * a.ldq : kvh < a.c.nkv ? a.k + n * a.ldk : a.v + n * a.ldv;
+                const QE *f = (const QE *)row + (kvh < 0 ? at.h : kvh < a.c.nkv ? kvh : kvh - a.c.nkv) * a.c.hd;
+                p[x] = *(const RopeVec<QE, V> *)(f + it.d0);
+                if (it.d1 >= 0) q[x] = *(const RopeVec<QE, V> *)(f + it.d1);
+            }
+            at.next();
         }
     };
-    load(tid);
+    load();
+    if (a.start && near) for (int i = tid; i <= a.c.rows; i += PA_THREADS) starts[i] = a.start[i];
     __syncthreads();
     if (tid < here) {
         const int n = n0 + tid;
         const int row = a.start ? append_row(near ? starts : a.start, a.c.rows, n) : n / a.T;
         int64_t to = -2;
-        int at = 0;
+        int seq = 0;
         const int len = row >= 0 ? a.c.len[row] : -1;
         if (len >= 0) {
             const int64_t s = (int64_t)len + (a.start ? n - (near ? starts : a.start)[row] : n % a.T);
-            at = (int)min(s, (int64_t)INT_MAX);
+            seq = (int)min(s, (int64_t)INT_MAX);
             const int page = s < (int64_t)a.c.max_pages << a.c.page_log ? paged_entry(a.c, row, (int)(s >> a.c.page_log)) : -1;
             to = page < 0 ? -1 : page * a.c.ps + (s & ((1 << a.c.page_log) - 1)) * a.c.ts;
         }
         slot[tid] = to;
-        place[tid] = ROPE && a.pos ? a.pos[n] : at;
+        place[tid] = ROPE && a.pos ? a.pos[n] : seq;
     }
     __syncthreads();
     if (ROPE) {
-        for (int i = tid; i < here * pairs; i += PA_THREADS) cs[i] = rope_angle(r, i % pairs, place[i / pairs], false);
+        for (int i = tid; i < here * pairs; i += PA_THREADS) {
+            const int t = i / pairs;
+            cs[i] = rope_angle(r, i - t * pairs, place[t], false);
+        }
         __syncthreads();
     }
-    for (int i0 = tid; i0 < total; i0 += PA_BATCH * PA_THREADS) {
-        if (i0 != tid) load(i0);
+    while (from.tok < here) {
 #pragma unroll
         for (int x = 0; x < PA_BATCH; x++) {
-            if (i0 + x * PA_THREADS >= total) continue;
-            const int h = head[x];
-            const int64_t to = slot[tok[x]];
-            if (to == -2 || (h >= a.H && to < 0)) continue;
-            if (ROPE && h < a.H + a.c.nkv) rope_turn<V, ROPE == 2>(it[x], cs + tok[x] * pairs, p[x], q[x]);
-            if (h < a.H) {
-                QE *y = (QE *)(a.q_out + (n0 + tok[x]) * a.ldqo) + h * a.c.hd;
-                rope_store<QE, V>(y + it[x].d0, p[x]);
-                if (it[x].d1 >= 0) rope_store<QE, V>(y + it[x].d1, q[x]);
-            } else {
-                const int kvh = h - a.H;
-                KE *y = (KE *)((kvh < a.c.nkv ? a.c.k + kvh * a.c.hs : a.c.v + (kvh - a.c.nkv) * a.c.hs) + to);
-                rope_store<KE, V>(y + it[x].d0, p[x]);
-                if (it[x].d1 >= 0) rope_store<KE, V>(y + it[x].d1, q[x]);
+            const int64_t to = from.tok < here ? slot[from.tok] : -2;
+            const int kvh = from.h - a.H;
+            if (to >= (kvh < 0 ? -1 : 0)) {
+                float f[V], g[V];
+                rope_unpack<QE, V>(p[x], f);
+                if (it.d1 >= 0) rope_unpack<QE, V>(q[x], g);
+                if (ROPE && kvh < a.c.nkv) rope_turn<V, ROPE == 2>(it, cs + from.tok * pairs, f, g);
+                if (kvh < 0) {
+                    QE *y = (QE *)(a.q_out + (n0 + from.tok) * a.ldqo) + from.h * a.c.hd;
+                    rope_store<QE, V>(y + it.d0, f);
+                    if (it.d1 >= 0) rope_store<QE, V>(y + it.d1, g);
+                } else {
+                    KE *y = (KE *)((kvh < a.c.nkv ? a.c.k + kvh * a.c.hs : a.c.v + (kvh - a.c.nkv) * a.c.hs) + to);
+                    rope_store<KE, V>(y + it.d0, f);
+                    if (it.d1 >= 0) rope_store<KE, V>(y + it.d1, g);
+                }
             }
+            from.next();
         }
+        load();
     }
 }
 
 template <class QE, class KE, int V> void run_append(const NcmbRope *r, AppendArgs &a) {
     a.items = rope_items(r, a.c.hd, V);
+    // some rounds of the CTA's threads, but CTAs for all SMs
     const int64_t per_token = (int64_t)(a.H + 2 * a.c.nkv) * a.items;
-    a.per = (int)std::max<int64_t>(1, std::min<int64_t>({PA_TOKENS, 4 * PA_THREADS / per_token, a.tokens / ctx().sm_count}));
+    a.per = (int)std::max<int64_t>(1, std::min<int64_t>({PA_TOKENS, 12 * PA_THREADS / per_token, a.tokens / (4 * ctx().sm_count)}));
     const size_t smem = r ? (size_t)a.per * (r->dims / 2) * sizeof(float2) : 0;
     const unsigned grid = (unsigned)cdiv(a.tokens, a.per);
     static const NcmbRope none = {};
@@ -154,7 +163,7 @@ template <class QE, class KE> void run_append(const NcmbRope *r, AppendArgs &a) 
 }
 
 // ---- rows that go on as others ----
-constexpr int PR_THREADS = NCMB_MAX_GROUP;
+constexpr int PR_THREADS = NCMB_MAX_GROUP, PR_WARPS = PR_THREADS / 32, PR_BATCH = 8;
 
 struct ReorderArgs {
     PagedDev c;
@@ -217,15 +226,26 @@ __global__ void __launch_bounds__(PR_THREADS) k_paged_reorder(const __grid_const
     if (mine < 0 || !has || begun == 0) return;
     const int from = paged_entry(a.c, g0 + par, tp), dst = paged_entry(a.c, g0 + own, to);
     if (from < 0 || dst < 0) return;
-    const int units = a.c.hd * a.c.es / 16;      // of 16 bytes in a token's keys
-    const int64_t total = (int64_t)a.n_layer * 2 * a.c.nkv * begun * units;
-    for (int64_t i = (int64_t)blockIdx.x * PR_THREADS + tid; i < total; i += (int64_t)gridDim.x * PR_THREADS) {
-        int64_t x = i;
-        const int u = (int)(x % units); x /= units;
-        const int s = (int)(x % begun); x /= begun;
-        const int h = (int)(x % a.c.nkv); x /= a.c.nkv;
-        char *base = ((x & 1) ? a.c.v : a.c.k) + (x >> 1) * a.ls + h * a.c.hs + s * a.c.ts + u * 16;
-        *(int4 *)(base + dst * a.c.ps) = *(const int4 *)(base + from * a.c.ps);
+    // a warp copies the begun page's keys, or values, of a head and layer: 16 bytes a lane, PR_BATCH of them on their way
+    const uint32_t units = a.c.hd * a.c.es / 16, total = begun * units, lg = units & (units - 1) ? 0 : __ffs(units) - 1;     // of 16 bytes in a token's keys
+    const int runs = a.n_layer * 2 * a.c.nkv;
+    for (int x = blockIdx.x * PR_WARPS + warp; x < runs; x += gridDim.x * PR_WARPS) {
+        const int side = x / a.c.nkv, h = x - side * a.c.nkv;
+        char *base = ((side & 1) ? a.c.v : a.c.k) + (side >> 1) * a.ls + h * a.c.hs;
+        const char *src = base + from * a.c.ps;
+        char *to_page = base + dst * a.c.ps;
+        for (uint32_t i0 = lane; i0 < total; i0 += 32 * PR_BATCH) {
+            int4 v[PR_BATCH];
+            int64_t off[PR_BATCH];
+#pragma unroll
+            for (int k = 0; k < PR_BATCH; k++) {
+                const uint32_t i = i0 + 32 * k, t = units == 1 || lg ? i >> lg : i / units;
+                off[k] = t * a.c.ts + (i - t * units) * 16;
+                if (i < total) v[k] = *(const int4 *)(src + off[k]);
+            }
+#pragma unroll
+            for (int k = 0; k < PR_BATCH; k++) if (i0 + 32 * k < total) *(int4 *)(to_page + off[k]) = v[k];
+        }
     }
 }
 
@@ -269,6 +289,8 @@ extern "C" int ncmb_paged_reorder(const NcmbPaged *c, int group, const int *pare
     if (group < 1 || group > NCMB_MAX_GROUP || c->rows % group) return cache_refuse(who, "groups of %d in %d rows: at most %d, a divisor", group, c->rows, NCMB_MAX_GROUP);
     if (n_layer < 1 || n_layer > 65535 || layer_stride < 0 || (layer_stride * a.c.es) % 16 || (n_layer > 1 && layer_stride < c->hd))
         return cache_refuse(who, "%d layers, %lld elements apart: a multiple of 16 bytes", n_layer, (long long)layer_stride);
+    const int64_t runs = (int64_t)n_layer * 2 * c->n_kv;
+    if (runs > 1 << 30) return cache_refuse(who, "%d layers of %d kv heads", n_layer, c->n_kv);
     if (c->rows == 0) return 0;
     if (!parents || !table_dst || !len_dst || ((uintptr_t)parents | (uintptr_t)table_dst | (uintptr_t)len_dst | (uintptr_t)refs) % 4) return cache_refuse(who, "parents, table_dst and len_dst: not null, 4-byte aligned");
     const uintptr_t t0 = (uintptr_t)c->table, t1 = (uintptr_t)table_dst, tb = ((uintptr_t)(c->rows - 1) * c->table_stride + c->max_pages) * 4;
@@ -276,10 +298,9 @@ extern "C" int ncmb_paged_reorder(const NcmbPaged *c, int group, const int *pare
     if ((t0 < t1 + tb && t1 < t0 + tb) || (l0 < l1 + lb && l1 < l0 + lb)) return cache_refuse(who, "new tables and lengths have to stand in memory of their own");
     if (cache_device(who)) return -1;
     a.group = group; a.n_layer = n_layer; a.ls = layer_stride * a.c.es; a.parents = parents; a.table2 = table_dst; a.len2 = len_dst; a.refs = refs;
-    const int64_t units = (int64_t)n_layer * 2 * c->n_kv * c->page * c->hd * a.c.es / 16;        // of a full page
-    ProfScope prof(NCMB_K_ELEM, 0, (double)c->rows * units * 16);
-    // a few rounds of 16 bytes a thread, but no more CTAs than keep the GPU busy
+    ProfScope prof(NCMB_K_ELEM, 0, (double)c->rows * runs * c->page * c->hd * a.c.es);
+    // a run a warp, but no more CTAs than keep the GPU busy: each finds the group's parents first
     const int64_t most = std::max<int64_t>(1, 32LL * ctx().sm_count / c->rows);
-    LAUNCH_PDL(k_paged_reorder, dim3((unsigned)std::max<int64_t>(1, std::min(most, cdiv(units, 4 * PR_THREADS))), c->rows), PR_THREADS, 0, a);
+    LAUNCH_PDL(k_paged_reorder, dim3((unsigned)std::min(most, cdiv(runs, PR_WARPS)), c->rows), PR_THREADS, 0, a);
     return 0;
 }

@@ -14,69 +14,81 @@ int rope_check(const char *who, const NcmbRope *r, int hd) {
 
 namespace {
 
-constexpr int RO_THREADS = 256, RO_BATCH = 2;
+constexpr int RO_THREADS = 256, RO_TOKENS = 32, RO_BATCH = 4;
 
 struct RopeArgs {
     const char *x; char *y;
     int64_t xs[3], ys[3];            // bytes
     const int *pos;
-    int64_t tokens;
-    int T, n_head, hd, inverse;      // hd: the dims that are moved, in place those that turn
+    uint32_t tokens, T;
+    int n_head, hd, inverse;         // hd: the dims that are moved, in place those that turn
     int per, items;                  // tokens a CTA, items a head
 };
 
-// A CTA has `per` tokens: their angles once, in shared memory, then all items of their heads. Loads of a thread's first items are under way
-// while the angles are formed.
+// A CTA has `per` tokens: their places in memory and their angles once, in shared memory, then all items of their heads, RO_BATCH of a thread on their way at a
+// time, the first of them while the angles are formed.
 template <class E, int V, bool PAIRS>
 __global__ void __launch_bounds__(RO_THREADS) k_rope(const __grid_constant__ NcmbRope r, const __grid_constant__ RopeArgs a) {
     extern __shared__ float2 cs[];               // [per][dims / 2]
+    __shared__ int64_t xo[RO_TOKENS], yo[RO_TOKENS];
+    __shared__ int place[RO_TOKENS];
     const int tid = threadIdx.x, pairs = r.dims / 2;
+    const uint32_t n0 = blockIdx.x * (uint32_t)a.per;
+    const int here = (int)min((uint32_t)a.per, a.tokens - n0);
+    RopeWalk at(tid, RO_THREADS, a.n_head, a.items);
+    const RopeItem it = rope_item<V, PAIRS>(at.u, a.items, r.dims, a.hd);
     pdl_wait();
     pdl_launch_dependents();
-    const int64_t n0 = (int64_t)blockIdx.x * a.per;
-    const int here = (int)min((int64_t)a.per, a.tokens - n0), per_token = a.n_head * a.items, total = here * per_token;
-    float p[RO_BATCH][V], q[RO_BATCH][V];
-    RopeItem it[RO_BATCH];
-    E *to[RO_BATCH];
-    int tok[RO_BATCH];
-    auto load = [&](int i0) {
-#pragma unroll
-        for (int k = 0; k < RO_BATCH; k++) {
-            const int i = i0 + k * RO_THREADS;
-            if (i >= total) continue;
-            tok[k] = i / per_token;
-            const int j = i - tok[k] * per_token, h = j / a.items;
-            it[k] = rope_item<V, PAIRS>(j - h * a.items, r.dims, a.hd);
-            const uint32_t n = (uint32_t)n0 + tok[k], b = n / (uint32_t)a.T, t = n - b * (uint32_t)a.T;
-            const E *from = (const E *)(a.x + b * a.xs[0] + t * a.xs[1] + h * a.xs[2]);
-            to[k] = (E *)(a.y + b * a.ys[0] + t * a.ys[1] + h * a.ys[2]);
-            rope_load<E, V>(from + it[k].d0, p[k]);
-            if (it[k].d1 >= 0) rope_load<E, V>(from + it[k].d1, q[k]);
-        }
-    };
-    load(tid);
-    for (int i = tid; i < here * pairs; i += RO_THREADS) {
-        const uint32_t n = (uint32_t)n0 + i / pairs;
-        cs[i] = rope_angle(r, i % pairs, a.pos ? a.pos[n] : (int)(n % (uint32_t)a.T), a.inverse);
+    if (tid < here) {
+        const uint32_t n = n0 + tid, b = n / a.T, t = n - b * a.T;
+        xo[tid] = b * a.xs[0] + t * a.xs[1];
+        yo[tid] = b * a.ys[0] + t * a.ys[1];
+        place[tid] = a.pos ? a.pos[n] : (int)t;
     }
     __syncthreads();
-    for (int i0 = tid; i0 < total; i0 += RO_BATCH * RO_THREADS) {
-        if (i0 != tid) load(i0);
+    RopeVec<E, V> p[RO_BATCH], q[RO_BATCH];
+    RopeWalk from = at;
+    auto load = [&] {
+        from = at;
 #pragma unroll
         for (int k = 0; k < RO_BATCH; k++) {
-            if (i0 + k * RO_THREADS >= total) continue;
-            rope_turn<V, PAIRS>(it[k], cs + tok[k] * pairs, p[k], q[k]);
-            rope_store<E, V>(to[k] + it[k].d0, p[k]);
-            if (it[k].d1 >= 0) rope_store<E, V>(to[k] + it[k].d1, q[k]);
+            if (at.tok < here) {
+                const E *x = (const E *)(a.x + xo[at.tok] + at.h * a.xs[2]);
+                p[k] = *(const RopeVec<E, V> *)(x + it.d0);
+                if (it.d1 >= 0) q[k] = *(const RopeVec<E, V> *)(x + it.d1);
+            }
+            at.next();
         }
+    };
+    load();
+    for (int i = tid; i < here * pairs; i += RO_THREADS) {
+        const int t = i / pairs;
+        cs[i] = rope_angle(r, i - t * pairs, place[t], a.inverse);
+    }
+    __syncthreads();
+    while (from.tok < here) {
+#pragma unroll
+        for (int k = 0; k < RO_BATCH; k++) {
+            if (from.tok < here) {
+                float f[V], g[V];
+                rope_unpack<E, V>(p[k], f);
+                if (it.d1 >= 0) rope_unpack<E, V>(q[k], g);
+                rope_turn<V, PAIRS>(it, cs + from.tok * pairs, f, g);
+                E *y = (E *)(a.y + yo[from.tok] + from.h * a.ys[2]);
+                rope_store<E, V>(y + it.d0, f);
+                if (it.d1 >= 0) rope_store<E, V>(y + it.d1, g);
+            }
+            from.next();
+        }
+        load();
     }
 }
 
 template <class E, int V> void run_rope(const NcmbRope &r, RopeArgs &a) {
     a.items = rope_items(&r, a.hd, V);
-    // a few rounds of the CTA's threads, and no fewer CTAs than SMs
+    // some rounds of the CTA's threads, but CTAs for all SMs
     const int64_t per_token = (int64_t)a.n_head * a.items;
-    a.per = (int)std::max<int64_t>(1, std::min<int64_t>({16, 4 * RO_THREADS / per_token, a.tokens / ctx().sm_count}));
+    a.per = (int)std::max<int64_t>(1, std::min<int64_t>({RO_TOKENS, 8 * RO_THREADS / per_token, a.tokens / (4 * ctx().sm_count)}));
     const size_t smem = (size_t)a.per * (r.dims / 2) * sizeof(float2);
     const unsigned grid = (unsigned)cdiv(a.tokens, a.per);
     if (r.layout == NCMB_ROPE_HALVES) LAUNCH_PDL((k_rope<E, V, false>), grid, RO_THREADS, smem, r, a);
@@ -137,7 +149,7 @@ extern "C" int ncmb_rope(const NcmbRope *r, const void *x, const int64_t *xs, vo
         a.ys[i] = ys[i] * es;
     }
     if (cache_device(who)) return -1;
-    a.x = (const char *)x; a.y = (char *)y; a.pos = pos; a.tokens = tokens; a.T = T; a.n_head = n_head; a.hd = x == y ? r->dims : hd; a.inverse = inverse != 0;
+    a.x = (const char *)x; a.y = (char *)y; a.pos = pos; a.tokens = (uint32_t)tokens; a.T = T; a.n_head = n_head; a.hd = x == y ? r->dims : hd; a.inverse = inverse != 0;
     ProfScope prof(NCMB_K_ELEM, 3.0 * tokens * n_head * hd, 2.0 * tokens * n_head * hd * es);
     switch (rope_vec(r, (int)es)) {
         case 8: run_rope<__nv_bfloat16, 8>(*r, a); break;

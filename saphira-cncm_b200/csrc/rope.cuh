@@ -3,8 +3,8 @@
 // A pair (x1, x2) at angle a = 2 pi p f, f full turns a position: y1 = m (x1 cos a - x2 sin a), y2 = m (x2 cos a + x1 sin a). p f is formed in 64
 // bits and only its fraction of a turn goes on in fp32: at position 10^6 an fp32 product is off by 0.06 radians.
 //
-// A thread's item is two vectors of V elements of a head. HALVES: the vectors at i and i + dims / 2, V pairs; PAIRS: two
-// neighbouring vectors, each of V / 2 pairs; dims that stay: two neighbouring vectors. V is 16 bytes where the dims allow it.
+// A thread's item is two vectors of V elements of a head. HALVES: the vectors at i and i + dims / 2, V pairs; PAIRS: the vectors i and i + half of
+// the head's vectors, each of V / 2 pairs; dims that stay: likewise. So threads side by side have vectors side by side. V is 16 bytes where the dims allow it.
 #pragma once
 #include "cache.cuh"
 
@@ -30,38 +30,36 @@ inline int rope_items(const NcmbRope *r, int hd, int v) {
 }
 
 #ifdef __CUDACC__
-template <class E, int V> __device__ __forceinline__ void rope_load(const E *p, float (&x)[V]) {
-    if constexpr (std::is_same_v<E, float>) {
-        if constexpr (V == 4) { const float4 u = *(const float4 *)p; x[0] = u.x; x[1] = u.y; x[2] = u.z; x[3] = u.w; }
-        else if constexpr (V == 2) { const float2 u = *(const float2 *)p; x[0] = u.x; x[1] = u.y; }
-        else x[0] = *p;
-    } else {
-        uint32_t u[V / 2 > 0 ? V / 2 : 1];
-        if constexpr (V == 8) { const uint4 w = *(const uint4 *)p; u[0] = w.x; u[1] = w.y; u[2] = w.z; u[3] = w.w; }
-        else if constexpr (V == 4) { const uint2 w = *(const uint2 *)p; u[0] = w.x; u[1] = w.y; }
-        else if constexpr (V == 2) u[0] = *(const uint32_t *)p;
-        else u[0] = *(const unsigned short *)p;
+// a vector as it is in memory
+template <int BYTES> struct RopeRaw { using T = uint4; };
+template <> struct RopeRaw<8> { using T = uint2; };
+template <> struct RopeRaw<4> { using T = uint32_t; };
+template <> struct RopeRaw<2> { using T = unsigned short; };
+template <class E, int V> using RopeVec = typename RopeRaw<V * (int)sizeof(E)>::T;
+template <class E, int V> __device__ __forceinline__ void rope_unpack(const RopeVec<E, V> &v, float (&x)[V]) {
+    uint32_t u[4] = {0, 0, 0, 0};
+    if constexpr (sizeof(v) == 16) { u[0] = v.x; u[1] = v.y; u[2] = v.z; u[3] = v.w; }
+    else if constexpr (sizeof(v) == 8) { u[0] = v.x; u[1] = v.y; }
+    else u[0] = v;
 #pragma unroll
-        for (int i = 0; i < V; i++) x[i] = __uint_as_float(i & 1 ? u[i / 2] & 0xffff0000u : u[i / 2] << 16);
-    }
+    for (int i = 0; i < V; i++) x[i] = __uint_as_float(sizeof(E) == 4 ? u[i] : i & 1 ? u[i / 2] & 0xffff0000u : u[i / 2] << 16);
 }
 // rounds once, to the nearest
 template <class E, int V> __device__ __forceinline__ void rope_store(E *p, const float (&x)[V]) {
-    if constexpr (std::is_same_v<E, float>) {
+    if constexpr (sizeof(E) == 4) {
         if constexpr (V == 8) { *(float4 *)p = make_float4(x[0], x[1], x[2], x[3]); *(float4 *)(p + 4) = make_float4(x[4], x[5], x[6], x[7]); }
         else if constexpr (V == 4) *(float4 *)p = make_float4(x[0], x[1], x[2], x[3]);
         else if constexpr (V == 2) *(float2 *)p = make_float2(x[0], x[1]);
         else *p = x[0];
+    } else if constexpr (V == 1) {
+        *p = __float2bfloat16(x[0]);
     } else {
-        uint32_t u[V / 2 > 0 ? V / 2 : 1];
-        if constexpr (V == 1) *p = __float2bfloat16(x[0]);
-        else {
+        uint32_t u[V / 2];
 #pragma unroll
-            for (int i = 0; i < V / 2; i++) { const __nv_bfloat162 t = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]); u[i] = *(const uint32_t *)&t; }
-            if constexpr (V == 8) *(uint4 *)p = make_uint4(u[0], u[1], u[2], u[3]);
-            else if constexpr (V == 4) *(uint2 *)p = make_uint2(u[0], u[1]);
-            else *(uint32_t *)p = u[0];
-        }
+        for (int i = 0; i < V / 2; i++) { const __nv_bfloat162 t = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]); u[i] = *(const uint32_t *)&t; }
+        if constexpr (V == 8) *(uint4 *)p = make_uint4(u[0], u[1], u[2], u[3]);
+        else if constexpr (V == 4) *(uint2 *)p = make_uint2(u[0], u[1]);
+        else *(uint32_t *)p = u[0];
     }
 }
 
@@ -78,16 +76,35 @@ struct RopeItem {
     int d0, d1;              // dims of its two vectors; d1 < 0: there is no second
     int pair0, pair1;        // first pairs of their rotation, or -1
 };
-template <int V, bool PAIRS> __device__ __forceinline__ RopeItem rope_item(int u, int dims, int hd) {
+template <int V, bool PAIRS> __device__ __forceinline__ RopeItem rope_item(int u, int items, int dims, int hd) {
     RopeItem it;
     const int rot = PAIRS ? 0 : dims / 2 / V;
     if (!PAIRS && u < rot) { it.d0 = u * V; it.d1 = it.d0 + dims / 2; it.pair0 = it.pair1 = it.d0; return it; }
-    it.d0 = (PAIRS ? 0 : dims) + 2 * (u - rot) * V;
-    it.d1 = it.d0 + V < hd ? it.d0 + V : -1;
+    it.d0 = (PAIRS ? 0 : dims) + (u - rot) * V;
+    it.d1 = it.d0 + (items - rot) * V;
+    if (it.d1 >= hd) it.d1 = -1;
     it.pair0 = PAIRS && it.d0 < dims ? it.d0 / 2 : -1;
     it.pair1 = PAIRS && it.d1 >= 0 && it.d1 < dims ? it.d1 / 2 : -1;
     return it;
 }
+// The items of a CTA's tokens: a thread has item u of every step-th head, and walks heads and tokens without a division.
+struct RopeWalk {
+    int u, tok, h;                   // tok: beyond the CTA's when there is none left
+    int heads, dtok, dh;
+    __device__ RopeWalk(int tid, int threads, int heads_, int items) : heads(heads_) {
+        const int step = threads / items, p = tid / items;
+        u = tid - p * items;
+        tok = p < step ? p / heads : 1 << 20;
+        h = p < step ? p - tok * heads : 0;
+        dtok = step / heads;
+        dh = step - dtok * heads;
+    }
+    __device__ void next() {
+        tok += dtok;
+        h += dh;
+        if (h >= heads) { h -= heads; tok++; }
+    }
+};
 // a, b: the item's vectors; cs: the token's cosines and sines
 template <int V, bool PAIRS> __device__ __forceinline__ void rope_turn(const RopeItem &it, const float2 *cs, float (&a)[V], float (&b)[V]) {
     if constexpr (PAIRS) {

@@ -77,11 +77,15 @@ class Rope(C.Structure):
     _fields_ = [("dims", _I), ("layout", _I), ("magnitude", _F), ("turns", C.c_double * 128)]
 
 
+_ARRAYS = [_I64 * n for n in range(5)]
+
+
 def strides(t, n):
     """The first n strides of a torch tensor whose last dim is contiguous, as the int64 array that ncmb_rope takes."""
-    if t.stride(-1) != 1 and t.shape[-1] > 1:
+    s = t.stride()
+    if s[-1] != 1 and t.shape[-1] > 1:
         raise ValueError("the head dim has to be contiguous")
-    return (_I64 * n)(*t.stride()[:n])
+    return _ARRAYS[n](*s[:n])
 
 
 class PagedCache(C.Structure):

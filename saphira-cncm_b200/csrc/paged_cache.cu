@@ -61,11 +61,11 @@ __device__ int append_row(const int *s, int rows, int i) {
 // cache. ROPE: 0 none, 1 halves, 2 pairs.
 template <class QE, class KE, int V, int ROPE>
 __global__ void __launch_bounds__(PA_THREADS) k_paged_append(const __grid_constant__ NcmbRope r, const __grid_constant__ AppendArgs a) {
-    extern __shared__ float2 cs[];               // [per][dims / 2]
+    extern __shared__ __align__(16) float2 cs[];         // [per][pairs, made even]
     __shared__ int64_t slot[PA_TOKENS];          // bytes from the pool's start; -1: not stored, -2: nobody's
     __shared__ int place[PA_TOKENS];
     __shared__ int starts[PA_ROWS + 1];
-    const int tid = threadIdx.x, pairs = ROPE ? r.dims / 2 : 0, heads = a.H + 2 * a.c.nkv;
+    const int tid = threadIdx.x, pairs = ROPE ? r.dims / 2 : 0, cs_row = (pairs + 1) & ~1, heads = a.H + 2 * a.c.nkv;
     const int n0 = blockIdx.x * a.per, here = min(a.per, a.tokens - n0);
     const bool near = a.c.rows <= PA_ROWS;
     RopeWalk at(tid, PA_THREADS, heads, a.items);
@@ -74,22 +74,19 @@ __global__ void __launch_bounds__(PA_THREADS) k_paged_append(const __grid_consta
     pdl_launch_dependents();
     RopeVec<QE, V> p[PA_BATCH], q[PA_BATCH];
     RopeWalk from = at;
-    auto load = [&] {
-        from = at;
-#pragma unroll
-        for (int x = 0; x < PA_BATCH; x++) {
-            if (at.tok < here) {
-                const int64_t n = n0 + at.tok;
-                const int kvh = at.h - a.H;
-                const char *row = kvh < 0 ? a.q + n * a.ldq : kvh < a.c.nkv ? a.k + n * a.ldk : a.v + n * a.ldv;
-                const QE *f = (const QE *)row + (kvh < 0 ? at.h : kvh < a.c.nkv ? kvh : kvh - a.c.nkv) * a.c.hd;
-                p[x] = *(const RopeVec<QE, V> *)(f + it.d0);
-                if (it.d1 >= 0) q[x] = *(const RopeVec<QE, V> *)(f + it.d1);
-            }
-            at.next();
+    auto load = [&](int x) {
+        if (at.tok < here) {
+            const int64_t n = n0 + at.tok;
+            const int kvh = at.h - a.H;
+            const char *row = kvh < 0 ? a.q + n * a.ldq : kvh < a.c.nkv ? a.k + n * a.ldk : a.v + n * a.ldv;
+            const QE *f = (const QE *)row + (kvh < 0 ? at.h : kvh < a.c.nkv ? kvh : kvh - a.c.nkv) * a.c.hd;
+            p[x] = *(const RopeVec<QE, V> *)(f + it.d0);
+            if (it.d1 >= 0) q[x] = *(const RopeVec<QE, V> *)(f + it.d1);
         }
+        at.next();
     };
-    load();
+#pragma unroll
+    for (int x = 0; x < PA_BATCH; x++) load(x);
     if (a.start && near) for (int i = tid; i <= a.c.rows; i += PA_THREADS) starts[i] = a.start[i];
     __syncthreads();
     if (tid < here) {
@@ -111,7 +108,7 @@ __global__ void __launch_bounds__(PA_THREADS) k_paged_append(const __grid_consta
     if (ROPE) {
         for (int i = tid; i < here * pairs; i += PA_THREADS) {
             const int t = i / pairs;
-            cs[i] = rope_angle(r, i - t * pairs, place[t], false);
+            cs[t * cs_row + rope_place<V, ROPE == 2>(i - t * pairs, r.dims)] = rope_angle(r, i - t * pairs, place[t], false);
         }
         __syncthreads();
     }
@@ -124,7 +121,7 @@ __global__ void __launch_bounds__(PA_THREADS) k_paged_append(const __grid_consta
                 float f[V], g[V];
                 rope_unpack<QE, V>(p[x], f);
                 if (it.d1 >= 0) rope_unpack<QE, V>(q[x], g);
-                if (ROPE && kvh < a.c.nkv) rope_turn<V, ROPE == 2>(it, cs + from.tok * pairs, f, g);
+                if (ROPE && kvh < a.c.nkv) rope_turn<V, ROPE == 2>(it, r.dims, cs + from.tok * cs_row, f, g);
                 if (kvh < 0) {
                     QE *y = (QE *)(a.q_out + (n0 + from.tok) * a.ldqo) + from.h * a.c.hd;
                     rope_store<QE, V>(y + it.d0, f);
@@ -136,8 +133,8 @@ __global__ void __launch_bounds__(PA_THREADS) k_paged_append(const __grid_consta
                 }
             }
             from.next();
+            load(x);
         }
-        load();
     }
 }
 
@@ -146,7 +143,7 @@ template <class QE, class KE, int V> void run_append(const NcmbRope *r, AppendAr
     // some rounds of the CTA's threads, but CTAs for all SMs
     const int64_t per_token = (int64_t)(a.H + 2 * a.c.nkv) * a.items;
     a.per = (int)std::max<int64_t>(1, std::min<int64_t>({PA_TOKENS, 12 * PA_THREADS / per_token, a.tokens / (4 * ctx().sm_count)}));
-    const size_t smem = r ? (size_t)a.per * (r->dims / 2) * sizeof(float2) : 0;
+    const size_t smem = r ? (size_t)a.per * ((r->dims / 2 + 1) & ~1) * sizeof(float2) : 0;
     const unsigned grid = (unsigned)cdiv(a.tokens, a.per);
     static const NcmbRope none = {};
     if (!r) { if constexpr (V * sizeof(QE) == 16) LAUNCH_PDL((k_paged_append<QE, KE, V, 0>), grid, PA_THREADS, smem, none, a); }
@@ -163,7 +160,7 @@ template <class QE, class KE> void run_append(const NcmbRope *r, AppendArgs &a) 
 }
 
 // ---- rows that go on as others ----
-constexpr int PR_THREADS = NCMB_MAX_GROUP, PR_WARPS = PR_THREADS / 32, PR_BATCH = 8;
+constexpr int PR_THREADS = NCMB_MAX_GROUP, PR_WARPS = PR_THREADS / 32, PR_BATCH = 8, PR_CTAS = 8;
 
 struct ReorderArgs {
     PagedDev c;
@@ -173,78 +170,86 @@ struct ReorderArgs {
     int *table2, *len2, *refs;
 };
 
-// CTAs (x, row): each finds out whose row it continues and whose own pages it takes, then copies its share of the begun page. CTA x = 0 writes the
-// row's table and length.
+// CTAs (x, group): each finds out whose row every row of the group continues and whose own pages it takes; the rows' tables are dealt to the
+// CTAs, and of each begun page that is copied every CTA has a share.
+// Bound by the copies: 16 groups of 8 beams, 32 layers of 8 x 128 in bf16, pages of 64: REORDER_US.
 __global__ void __launch_bounds__(PR_THREADS) k_paged_reorder(const __grid_constant__ ReorderArgs a) {
     __shared__ int heir[NCMB_MAX_GROUP];         // lowest row that continues a row; group: none
     __shared__ int taken[NCMB_MAX_GROUP];        // rows whose own pages are free, ascending
-    __shared__ int cnt[2][PR_THREADS / 32], mine;
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, row = blockIdx.y, g0 = row / a.group * a.group, j = row - g0, K = a.group;
+    __shared__ int owner[NCMB_MAX_GROUP], par[NCMB_MAX_GROUP], len[NCMB_MAX_GROUP];
+    __shared__ int copies[NCMB_MAX_GROUP], cnt[3][PR_WARPS];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g0 = blockIdx.y * a.group, K = a.group;
     pdl_wait();
     pdl_launch_dependents();
     heir[tid] = K;
-    __syncthreads();
     int p = -1;
     if (tid < K) {
+        len[tid] = a.c.len[g0 + tid];
         p = a.parents[g0 + tid];
         if ((unsigned)p >= (unsigned)K) p = -1;
-        if (p >= 0) atomicMin(&heir[p], tid);
+        par[tid] = p;
     }
+    __syncthreads();
+    if (p >= 0) atomicMin(&heir[p], tid);
     __syncthreads();
     // the i-th row that takes free pages takes those of the i-th row without an heir
     const bool takes = tid < K && !(p >= 0 && heir[p] == tid), free_ = tid < K && heir[tid] == K;
-    const uint32_t tm = __ballot_sync(0xffffffffu, takes), fm = __ballot_sync(0xffffffffu, free_), lt = (1u << lane) - 1;
-    if (lane == 0) { cnt[0][warp] = __popc(tm); cnt[1][warp] = __popc(fm); }
+    const uint32_t tm = __ballot_sync(0xffffffffu, takes), fm = __ballot_sync(0xffffffffu, free_), cm = __ballot_sync(0xffffffffu, takes && p >= 0), lt = (1u << lane) - 1;
+    if (lane == 0) { cnt[0][warp] = __popc(tm); cnt[1][warp] = __popc(fm); cnt[2][warp] = __popc(cm); }
     __syncthreads();
-    int ti = __popc(tm & lt), fi = __popc(fm & lt);
-    for (int w = 0; w < warp; w++) { ti += cnt[0][w]; fi += cnt[1][w]; }
+    int ti = __popc(tm & lt), fi = __popc(fm & lt), ci = __popc(cm & lt), n_copies = 0;
+    for (int w = 0; w < PR_WARPS; w++) {
+        if (w < warp) { ti += cnt[0][w]; fi += cnt[1][w]; ci += cnt[2][w]; }
+        n_copies += cnt[2][w];
+    }
     if (free_) taken[fi] = tid;
-    if (tid == j) mine = takes ? ti : -1;
+    if (takes && p >= 0) copies[ci] = tid;       // the rows that get a begun page, in the same order for all CTAs
     __syncthreads();
-    const int par = a.parents[g0 + j];
-    const bool has = (unsigned)par < (unsigned)K;
-    const int own = mine < 0 ? par : taken[mine];
+    if (tid < K) owner[tid] = takes ? taken[ti] : p;
+    __syncthreads();
     const int64_t cap = (int64_t)a.c.max_pages << a.c.page_log;
-    auto used = [&](int i) { return (int)max((int64_t)0, min((int64_t)a.c.len[g0 + i], cap)); };
-    const int n = has ? used(par) : 0, tp = n >> a.c.page_log, to = used(own) >> a.c.page_log;
-    if (blockIdx.x == 0) {
-        int *t2 = a.table2 + row * a.c.table_stride;
+    auto used = [&](int i) { return (int)max((int64_t)0, min((int64_t)len[i], cap)); };
+    for (int j = blockIdx.x; j < K; j += gridDim.x) {
+        const int pj = par[j], own = owner[j], n = pj >= 0 ? used(pj) : 0, tp = n >> a.c.page_log, to = used(own) >> a.c.page_log;
+        int *t2 = a.table2 + (int64_t)(g0 + j) * a.c.table_stride;
         for (int i = tid; i < a.c.max_pages; i += PR_THREADS) {
-            const int e = i < tp ? paged_entry(a.c, g0 + par, i) : i - tp + to < a.c.max_pages ? paged_entry(a.c, g0 + own, i - tp + to) : -1;
+            const int e = i < tp ? paged_entry(a.c, g0 + pj, i) : i - tp + to < a.c.max_pages ? paged_entry(a.c, g0 + own, i - tp + to) : -1;
             t2[i] = e;
             if (a.refs) {
-                const int before = paged_entry(a.c, row, i);
+                const int before = paged_entry(a.c, g0 + j, i);
                 if (before != e) {
                     if (before >= 0) atomicAdd(&a.refs[before], -1);
                     if (e >= 0) atomicAdd(&a.refs[e], 1);
                 }
             }
         }
-        if (tid == 0) a.len2[row] = has ? a.c.len[g0 + par] : -1;
+        if (tid == 0) a.len2[g0 + j] = pj >= 0 ? len[pj] : -1;
     }
-    const int begun = n & ((1 << a.c.page_log) - 1);
-    if (mine < 0 || !has || begun == 0) return;
-    const int from = paged_entry(a.c, g0 + par, tp), dst = paged_entry(a.c, g0 + own, to);
-    if (from < 0 || dst < 0) return;
-    // a warp copies the begun page's keys, or values, of a head and layer: 16 bytes a lane, PR_BATCH of them on their way
-    const uint32_t units = a.c.hd * a.c.es / 16, total = begun * units, lg = units & (units - 1) ? 0 : __ffs(units) - 1;     // of 16 bytes in a token's keys
+    // a warp copies the begun page's keys, or values, of a row, head and layer: 16 bytes a lane, PR_BATCH of them on their way
+    const uint32_t units = a.c.hd * a.c.es / 16, lg = units & (units - 1) ? 0 : __ffs(units) - 1;      // of 16 bytes in a token's keys
     const int runs = a.n_layer * 2 * a.c.nkv;
-    for (int x = blockIdx.x * PR_WARPS + warp; x < runs; x += gridDim.x * PR_WARPS) {
-        const int side = x / a.c.nkv, h = x - side * a.c.nkv;
+    for (int64_t x = blockIdx.x * PR_WARPS + warp; x < (int64_t)n_copies * runs; x += gridDim.x * PR_WARPS) {
+        const int c = (int)(x / runs), run = (int)(x - (int64_t)c * runs), side = run / a.c.nkv, h = run - side * a.c.nkv;
+        const int j = copies[c], pj = par[j], own = owner[j], n = used(pj);
+        const uint32_t total = (n & ((1 << a.c.page_log) - 1)) * units;
+        if (total == 0) continue;
+        const int from = paged_entry(a.c, g0 + pj, n >> a.c.page_log), dst = paged_entry(a.c, g0 + own, used(own) >> a.c.page_log);
+        if (from < 0 || dst < 0) continue;
         char *base = ((side & 1) ? a.c.v : a.c.k) + (side >> 1) * a.ls + h * a.c.hs;
         const char *src = base + from * a.c.ps;
         char *to_page = base + dst * a.c.ps;
         for (uint32_t i0 = lane; i0 < total; i0 += 32 * PR_BATCH) {
             int4 v[PR_BATCH];
-            int64_t off[PR_BATCH];
 #pragma unroll
             for (int k = 0; k < PR_BATCH; k++) {
                 const uint32_t i = i0 + 32 * k, t = units == 1 || lg ? i >> lg : i / units;
-                off[k] = t * a.c.ts + (i - t * units) * 16;
-                if (i < total) v[k] = *(const int4 *)(src + off[k]);
+                if (i < total) v[k] = *(const int4 *)(src + t * a.c.ts + (i - t * units) * 16);
             }
 #pragma unroll
-            for (int k = 0; k < PR_BATCH; k++) if (i0 + 32 * k < total) *(int4 *)(to_page + off[k]) = v[k];
+            for (int k = 0; k < PR_BATCH; k++) {
+                const uint32_t i = i0 + 32 * k, t = units == 1 || lg ? i >> lg : i / units;
+                if (i < total) *(int4 *)(to_page + t * a.c.ts + (i - t * units) * 16) = v[k];
+            }
         }
     }
 }
@@ -299,8 +304,9 @@ extern "C" int ncmb_paged_reorder(const NcmbPaged *c, int group, const int *pare
     if (cache_device(who)) return -1;
     a.group = group; a.n_layer = n_layer; a.ls = layer_stride * a.c.es; a.parents = parents; a.table2 = table_dst; a.len2 = len_dst; a.refs = refs;
     ProfScope prof(NCMB_K_ELEM, 0, (double)c->rows * runs * c->page * c->hd * a.c.es);
-    // a run a warp, but no more CTAs than keep the GPU busy: each finds the group's parents first
-    const int64_t most = std::max<int64_t>(1, 32LL * ctx().sm_count / c->rows);
-    LAUNCH_PDL(k_paged_reorder, dim3((unsigned)std::min(most, cdiv(runs, PR_WARPS)), c->rows), PR_THREADS, 0, a);
+    // a run of half of the group a warp, but no more CTAs than keep the GPU busy: each finds the group's parents first
+    const int groups = c->rows / group;
+    const int64_t most = std::max<int64_t>(1, PR_CTAS * (int64_t)ctx().sm_count / groups);
+    LAUNCH_PDL(k_paged_reorder, dim3((unsigned)std::min(most, cdiv(runs * cdiv(group, 2), PR_WARPS)), groups), PR_THREADS, 0, a);
     return 0;
 }

@@ -29,10 +29,10 @@ struct RopeArgs {
 // time, the first of them while the angles are formed.
 template <class E, int V, bool PAIRS>
 __global__ void __launch_bounds__(RO_THREADS) k_rope(const __grid_constant__ NcmbRope r, const __grid_constant__ RopeArgs a) {
-    extern __shared__ float2 cs[];               // [per][dims / 2]
+    extern __shared__ __align__(16) float2 cs[];         // [per][pairs, made even]
     __shared__ int64_t xo[RO_TOKENS], yo[RO_TOKENS];
     __shared__ int place[RO_TOKENS];
-    const int tid = threadIdx.x, pairs = r.dims / 2;
+    const int tid = threadIdx.x, pairs = r.dims / 2, row = (pairs + 1) & ~1;
     const uint32_t n0 = blockIdx.x * (uint32_t)a.per;
     const int here = (int)min((uint32_t)a.per, a.tokens - n0);
     RopeWalk at(tid, RO_THREADS, a.n_head, a.items);
@@ -48,22 +48,19 @@ __global__ void __launch_bounds__(RO_THREADS) k_rope(const __grid_constant__ Ncm
     __syncthreads();
     RopeVec<E, V> p[RO_BATCH], q[RO_BATCH];
     RopeWalk from = at;
-    auto load = [&] {
-        from = at;
-#pragma unroll
-        for (int k = 0; k < RO_BATCH; k++) {
-            if (at.tok < here) {
-                const E *x = (const E *)(a.x + xo[at.tok] + at.h * a.xs[2]);
-                p[k] = *(const RopeVec<E, V> *)(x + it.d0);
-                if (it.d1 >= 0) q[k] = *(const RopeVec<E, V> *)(x + it.d1);
-            }
-            at.next();
+    auto load = [&](int k) {
+        if (at.tok < here) {
+            const E *x = (const E *)(a.x + xo[at.tok] + at.h * a.xs[2]);
+            p[k] = *(const RopeVec<E, V> *)(x + it.d0);
+            if (it.d1 >= 0) q[k] = *(const RopeVec<E, V> *)(x + it.d1);
         }
+        at.next();
     };
-    load();
+#pragma unroll
+    for (int k = 0; k < RO_BATCH; k++) load(k);
     for (int i = tid; i < here * pairs; i += RO_THREADS) {
         const int t = i / pairs;
-        cs[i] = rope_angle(r, i - t * pairs, place[t], a.inverse);
+        cs[t * row + rope_place<V, PAIRS>(i - t * pairs, r.dims)] = rope_angle(r, i - t * pairs, place[t], a.inverse);
     }
     __syncthreads();
     while (from.tok < here) {
@@ -73,14 +70,14 @@ __global__ void __launch_bounds__(RO_THREADS) k_rope(const __grid_constant__ Ncm
                 float f[V], g[V];
                 rope_unpack<E, V>(p[k], f);
                 if (it.d1 >= 0) rope_unpack<E, V>(q[k], g);
-                rope_turn<V, PAIRS>(it, cs + from.tok * pairs, f, g);
+                rope_turn<V, PAIRS>(it, r.dims, cs + from.tok * row, f, g);
                 E *y = (E *)(a.y + yo[from.tok] + from.h * a.ys[2]);
                 rope_store<E, V>(y + it.d0, f);
                 if (it.d1 >= 0) rope_store<E, V>(y + it.d1, g);
             }
             from.next();
+            load(k);
         }
-        load();
     }
 }
 
@@ -89,7 +86,7 @@ template <class E, int V> void run_rope(const NcmbRope &r, RopeArgs &a) {
     // some rounds of the CTA's threads, but CTAs for all SMs
     const int64_t per_token = (int64_t)a.n_head * a.items;
     a.per = (int)std::max<int64_t>(1, std::min<int64_t>({RO_TOKENS, 8 * RO_THREADS / per_token, a.tokens / (4 * ctx().sm_count)}));
-    const size_t smem = (size_t)a.per * (r.dims / 2) * sizeof(float2);
+    const size_t smem = (size_t)a.per * ((r.dims / 2 + 1) & ~1) * sizeof(float2);
     const unsigned grid = (unsigned)cdiv(a.tokens, a.per);
     if (r.layout == NCMB_ROPE_HALVES) LAUNCH_PDL((k_rope<E, V, false>), grid, RO_THREADS, smem, r, a);
     else if constexpr (V >= 2) LAUNCH_PDL((k_rope<E, V, true>), grid, RO_THREADS, smem, r, a);

@@ -105,29 +105,53 @@ struct RopeWalk {
         if (h >= heads) { h -= heads; tok++; }
     }
 };
+// Cosines and sines of a token in shared memory: those that a vector needs are read two pairs (16 bytes) at a time, and vectors side by side by
+// threads side by side, so two pairs of all vectors stand together, then the next two.
+template <int V, bool PAIRS> __device__ __forceinline__ int rope_place(int pair, int dims) {
+    constexpr int W = PAIRS ? V / 2 : V;         // pairs of a vector
+    if constexpr (W < 2) return pair;
+    const int vecs = dims / 2 / W, v = pair / W, i = pair % W;
+    return (i / 2 * vecs + v) * 2 + (i & 1);
+}
 // a, b: the item's vectors; cs: the token's cosines and sines
-template <int V, bool PAIRS> __device__ __forceinline__ void rope_turn(const RopeItem &it, const float2 *cs, float (&a)[V], float (&b)[V]) {
+template <int V, bool PAIRS> __device__ __forceinline__ void rope_turn(const RopeItem &it, int dims, const float2 *cs, float (&a)[V], float (&b)[V]) {
+    constexpr int W = PAIRS ? V / 2 : V;
+    const int vecs = dims / 2 / W;
+    auto factors = [&](int pair, float2 (&f)[W]) {
+        if constexpr (W < 2) f[0] = cs[pair];
+        else {
+            const float4 *p = (const float4 *)cs + pair / W;
+#pragma unroll
+            for (int i = 0; i < W / 2; i++) {
+                const float4 u = p[i * vecs];
+                f[2 * i] = make_float2(u.x, u.y);
+                f[2 * i + 1] = make_float2(u.z, u.w);
+            }
+        }
+    };
     if constexpr (PAIRS) {
         static_assert(V >= 2, "a pair is in one vector");
         auto one = [&](int pair, float (&x)[V]) {
             if (pair < 0) return;
+            float2 f[W];
+            factors(pair, f);
 #pragma unroll
-            for (int i = 0; i < V / 2; i++) {
-                const float2 f = cs[pair + i];
+            for (int i = 0; i < W; i++) {
                 const float p = x[2 * i], q = x[2 * i + 1];
-                x[2 * i] = p * f.x - q * f.y;
-                x[2 * i + 1] = q * f.x + p * f.y;
+                x[2 * i] = p * f[i].x - q * f[i].y;
+                x[2 * i + 1] = q * f[i].x + p * f[i].y;
             }
         };
         one(it.pair0, a);
         one(it.pair1, b);
     } else if (it.pair0 >= 0) {
+        float2 f[W];
+        factors(it.pair0, f);
 #pragma unroll
         for (int i = 0; i < V; i++) {
-            const float2 f = cs[it.pair0 + i];
             const float p = a[i], q = b[i];
-            a[i] = p * f.x - q * f.y;
-            b[i] = q * f.x + p * f.y;
+            a[i] = p * f[i].x - q * f[i].y;
+            b[i] = q * f[i].x + p * f[i].y;
         }
     }
 }

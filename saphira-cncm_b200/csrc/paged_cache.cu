@@ -33,7 +33,7 @@ int paged_check(const char *who, const NcmbPaged *c, PagedDev &d) {
 namespace {
 
 // ---- new tokens ----
-constexpr int PA_THREADS = 256, PA_TOKENS = 32, PA_BATCH = 4, PA_ROWS = 1024;
+constexpr int PA_THREADS = 256, PA_TOKENS = 32, PA_BATCH = 3, PA_ROWS = 1024;
 
 struct AppendArgs {
     PagedDev c;
@@ -58,14 +58,15 @@ __device__ int append_row(const int *s, int rows, int i) {
 
 // A CTA has `per` tokens: where each goes and the cosines and sines of its angles once, in shared memory, then all items of its heads -- queries, keys,
 // values -- PA_BATCH of a thread on their way at a time, the first of them while places and angles are found. QE: type of the activations, KE: of the
-// cache. ROPE: 0 none, 1 halves, 2 pairs.
+// cache. ROPE: 0 none, 1 halves, 2 pairs. Bound by latency of its dependent steps -- starts, length, table, angles -- and DRAM: 16 rows of up to 2001 tokens, 32 over
+// 8 x 128 in bf16, 375 MB: 69 us (5.4 TB/s).
 template <class QE, class KE, int V, int ROPE>
-__global__ void __launch_bounds__(PA_THREADS) k_paged_append(const __grid_constant__ NcmbRope r, const __grid_constant__ AppendArgs a) {
-    extern __shared__ __align__(16) float2 cs[];         // [per][pairs, made even]
+__global__ void __launch_bounds__(PA_THREADS, V * sizeof(QE) == 16 ? 4 : 6) k_paged_append(const __grid_constant__ NcmbRope r, const __grid_constant__ AppendArgs a) {
+    extern __shared__ __align__(16) float2 cs[];         // [per][rope_row(dims)]
     __shared__ int64_t slot[PA_TOKENS];          // bytes from the pool's start; -1: not stored, -2: nobody's
     __shared__ int place[PA_TOKENS];
     __shared__ int starts[PA_ROWS + 1];
-    const int tid = threadIdx.x, pairs = ROPE ? r.dims / 2 : 0, cs_row = (pairs + 1) & ~1, heads = a.H + 2 * a.c.nkv;
+    const int tid = threadIdx.x, pairs = ROPE ? r.dims / 2 : 0, cs_row = ROPE ? rope_row(r.dims) : 0, heads = a.H + 2 * a.c.nkv;
     const int n0 = blockIdx.x * a.per, here = min(a.per, a.tokens - n0);
     const bool near = a.c.rows <= PA_ROWS;
     RopeWalk at(tid, PA_THREADS, heads, a.items);
@@ -140,15 +141,15 @@ __global__ void __launch_bounds__(PA_THREADS) k_paged_append(const __grid_consta
 
 template <class QE, class KE, int V> void run_append(const NcmbRope *r, AppendArgs &a) {
     a.items = rope_items(r, a.c.hd, V);
-    // some rounds of the CTA's threads, but CTAs for all SMs
-    const int64_t per_token = (int64_t)(a.H + 2 * a.c.nkv) * a.items;
-    a.per = (int)std::max<int64_t>(1, std::min<int64_t>({PA_TOKENS, 12 * PA_THREADS / per_token, a.tokens / (4 * ctx().sm_count)}));
-    const size_t smem = r ? (size_t)a.per * ((r->dims / 2 + 1) & ~1) * sizeof(float2) : 0;
+    // four items a thread, and CTAs for all SMs (16 rows of up to 2001 tokens, 32 over 8 x 128 in bf16, 4 / 8 / 12 items a thread: 69 / 76 / 77 us)
+    const int64_t per_token = (int64_t)(a.H + 2 * a.c.nkv) * a.items, rounds = V * sizeof(QE) == 16 ? 4 : 20;
+    a.per = (int)std::max<int64_t>(1, std::min<int64_t>({PA_TOKENS, rounds * PA_THREADS / per_token, a.tokens / (4 * ctx().sm_count)}));
+    const size_t smem = r ? (size_t)a.per * rope_row(r->dims) * sizeof(float2) : 0;
     const unsigned grid = (unsigned)cdiv(a.tokens, a.per);
     static const NcmbRope none = {};
     if (!r) { if constexpr (V * sizeof(QE) == 16) LAUNCH_PDL((k_paged_append<QE, KE, V, 0>), grid, PA_THREADS, smem, none, a); }
     else if (r->layout == NCMB_ROPE_HALVES) LAUNCH_PDL((k_paged_append<QE, KE, V, 1>), grid, PA_THREADS, smem, *r, a);
-    else if constexpr (V >= 2) LAUNCH_PDL((k_paged_append<QE, KE, V, 2>), grid, PA_THREADS, smem, *r, a);
+    else if constexpr (V * sizeof(QE) == 16) LAUNCH_PDL((k_paged_append<QE, KE, V, 2>), grid, PA_THREADS, smem, *r, a);
 }
 template <class QE, class KE> void run_append(const NcmbRope *r, AppendArgs &a) {
     switch (rope_vec(r, sizeof(QE))) {
@@ -172,7 +173,7 @@ struct ReorderArgs {
 
 // CTAs (x, group): each finds out whose row every row of the group continues and whose own pages it takes; the rows' tables are dealt to the
 // CTAs, and of each begun page that is copied every CTA has a share.
-// Bound by the copies: 16 groups of 8 beams, 32 layers of 8 x 128 in bf16, pages of 64: REORDER_US.
+// Bound by the copies: 16 groups of 8 beams, 32 layers of 8 x 128 in bf16, pages of 64: 73 us for 467 MB (6.4 TB/s).
 __global__ void __launch_bounds__(PR_THREADS) k_paged_reorder(const __grid_constant__ ReorderArgs a) {
     __shared__ int heir[NCMB_MAX_GROUP];         // lowest row that continues a row; group: none
     __shared__ int taken[NCMB_MAX_GROUP];        // rows whose own pages are free, ascending

@@ -26,13 +26,13 @@ struct RopeArgs {
 };
 
 // A CTA has `per` tokens: their places in memory and their angles once, in shared memory, then all items of their heads, RO_BATCH of a thread on their way at a
-// time, the first of them while the angles are formed.
+// time, the first of them while the angles are formed. Bound by DRAM: 8 x 4000 tokens of 40 heads of 128 in bf16, 655 MB: 100 us (6.5 TB/s).
 template <class E, int V, bool PAIRS>
-__global__ void __launch_bounds__(RO_THREADS) k_rope(const __grid_constant__ NcmbRope r, const __grid_constant__ RopeArgs a) {
-    extern __shared__ __align__(16) float2 cs[];         // [per][pairs, made even]
+__global__ void __launch_bounds__(RO_THREADS, V * sizeof(E) == 16 ? 4 : 6) k_rope(const __grid_constant__ NcmbRope r, const __grid_constant__ RopeArgs a) {
+    extern __shared__ __align__(16) float2 cs[];         // [per][rope_row(dims)]
     __shared__ int64_t xo[RO_TOKENS], yo[RO_TOKENS];
     __shared__ int place[RO_TOKENS];
-    const int tid = threadIdx.x, pairs = r.dims / 2, row = (pairs + 1) & ~1;
+    const int tid = threadIdx.x, pairs = r.dims / 2, row = rope_row(r.dims);
     const uint32_t n0 = blockIdx.x * (uint32_t)a.per;
     const int here = (int)min((uint32_t)a.per, a.tokens - n0);
     RopeWalk at(tid, RO_THREADS, a.n_head, a.items);
@@ -83,13 +83,14 @@ __global__ void __launch_bounds__(RO_THREADS) k_rope(const __grid_constant__ Ncm
 
 template <class E, int V> void run_rope(const NcmbRope &r, RopeArgs &a) {
     a.items = rope_items(&r, a.hd, V);
-    // some rounds of the CTA's threads, but CTAs for all SMs
-    const int64_t per_token = (int64_t)a.n_head * a.items;
-    a.per = (int)std::max<int64_t>(1, std::min<int64_t>({RO_TOKENS, 8 * RO_THREADS / per_token, a.tokens / (4 * ctx().sm_count)}));
-    const size_t smem = (size_t)a.per * ((r.dims / 2 + 1) & ~1) * sizeof(float2);
+    // A thread's items all on their way at once, and CTAs for all SMs (8 x 4000 tokens of 40 x 128 in bf16, 4 / 8 / 20 items a thread: 100 / 107 / 115 us);
+    // short vectors are paced by instructions, so there the angles are shared by more (dims 50 of it, halves, 4 / 20 items: 293 / 277).
+    const int64_t per_token = (int64_t)a.n_head * a.items, rounds = V * sizeof(E) == 16 ? RO_BATCH : 20;
+    a.per = (int)std::max<int64_t>(1, std::min<int64_t>({RO_TOKENS, rounds * RO_THREADS / per_token, a.tokens / (4 * ctx().sm_count)}));
+    const size_t smem = (size_t)a.per * rope_row(r.dims) * sizeof(float2);
     const unsigned grid = (unsigned)cdiv(a.tokens, a.per);
     if (r.layout == NCMB_ROPE_HALVES) LAUNCH_PDL((k_rope<E, V, false>), grid, RO_THREADS, smem, r, a);
-    else if constexpr (V >= 2) LAUNCH_PDL((k_rope<E, V, true>), grid, RO_THREADS, smem, r, a);
+    else if constexpr (V * sizeof(E) == 16) LAUNCH_PDL((k_rope<E, V, true>), grid, RO_THREADS, smem, r, a);
 }
 
 } // namespace
@@ -146,7 +147,7 @@ extern "C" int ncmb_rope(const NcmbRope *r, const void *x, const int64_t *xs, vo
         a.ys[i] = ys[i] * es;
     }
     if (cache_device(who)) return -1;
-    a.x = (const char *)x; a.y = (char *)y; a.pos = pos; a.tokens = (uint32_t)tokens; a.T = T; a.n_head = n_head; a.hd = x == y ? r->dims : hd; a.inverse = inverse != 0;
+    a.x = (const char *)x; a.y = (char *)y; a.pos = pos; a.tokens = (uint32_t)tokens; a.T = T; a.n_head = n_head; a.hd = x == y ? (r->layout == NCMB_ROPE_PAIRS ? std::min(hd, (r->dims + 7) & ~7) : r->dims) : hd; a.inverse = inverse != 0;
     ProfScope prof(NCMB_K_ELEM, 3.0 * tokens * n_head * hd, 2.0 * tokens * n_head * hd * es);
     switch (rope_vec(r, (int)es)) {
         case 8: run_rope<__nv_bfloat16, 8>(*r, a); break;

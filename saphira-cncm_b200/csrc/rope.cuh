@@ -15,12 +15,10 @@ namespace ncmb {
 // 0 when the plan is one that heads of hd can be rotated by, else -1 with a message
 int rope_check(const char *who, const NcmbRope *r, int hd);
 
-// elements of a vector: 16 bytes, or what the pairs of a plan leave whole
+// elements of a vector: 16 bytes, or what halves that are no whole number of them leave whole
 inline int rope_vec(const NcmbRope *r, int elem_bytes) {
     int v = 16 / elem_bytes;
-    if (!r) return v;
-    const int n = r->layout == NCMB_ROPE_PAIRS ? r->dims : r->dims / 2;
-    while (n % v) v >>= 1;
+    while (r && r->layout == NCMB_ROPE_HALVES && r->dims / 2 % v) v >>= 1;
     return v;
 }
 // items of a head
@@ -28,6 +26,9 @@ inline int rope_items(const NcmbRope *r, int hd, int v) {
     if (!r || r->layout == NCMB_ROPE_PAIRS) return (int)cdiv(hd, 2 * v);
     return r->dims / 2 / v + (int)cdiv(hd - r->dims, 2 * v);
 }
+
+// cosines and sines of a token in shared memory: pairs in whole vectors
+__host__ __device__ inline int rope_row(int dims) { return (dims / 2 + 7) & ~7; }
 
 #ifdef __CUDACC__
 // a vector as it is in memory
@@ -110,13 +111,13 @@ struct RopeWalk {
 template <int V, bool PAIRS> __device__ __forceinline__ int rope_place(int pair, int dims) {
     constexpr int W = PAIRS ? V / 2 : V;         // pairs of a vector
     if constexpr (W < 2) return pair;
-    const int vecs = dims / 2 / W, v = pair / W, i = pair % W;
+    const int vecs = (dims / 2 + W - 1) / W, v = pair / W, i = pair % W;
     return (i / 2 * vecs + v) * 2 + (i & 1);
 }
 // a, b: the item's vectors; cs: the token's cosines and sines
 template <int V, bool PAIRS> __device__ __forceinline__ void rope_turn(const RopeItem &it, int dims, const float2 *cs, float (&a)[V], float (&b)[V]) {
     constexpr int W = PAIRS ? V / 2 : V;
-    const int vecs = dims / 2 / W;
+    const int pairs = dims / 2, vecs = (pairs + W - 1) / W;
     auto factors = [&](int pair, float2 (&f)[W]) {
         if constexpr (W < 2) f[0] = cs[pair];
         else {
@@ -137,6 +138,7 @@ template <int V, bool PAIRS> __device__ __forceinline__ void rope_turn(const Rop
             factors(pair, f);
 #pragma unroll
             for (int i = 0; i < W; i++) {
+                if (pair + i >= pairs) break;            // the last vector's dims beyond
                 const float p = x[2 * i], q = x[2 * i + 1];
                 x[2 * i] = p * f[i].x - q * f[i].y;
                 x[2 * i + 1] = q * f[i].x + p * f[i].y;

@@ -21,12 +21,13 @@ namespace {
 constexpr int BM_THREADS = 256, BM_WARPS = BM_THREADS / 32;
 constexpr int BM_EPT = 32, BM_TILE = BM_THREADS * BM_EPT;        // logits of a thread and a CTA at a time
 constexpr int BM_CHUNK = 8;                                      // logits of a thread whose keys fit the list whatever they are, once they are bounded
-constexpr int BM_JOIN = 4;                                       // candidates of a thread at a time where parts are joined
+constexpr int BM_JOIN = 2;                                       // candidates of a thread at a time where parts are joined
 constexpr int BM_BATCH = 4;                                      // tiles from one meeting of the warps to the next
 constexpr int BM_START = 2, BM_ROUNDS = 4, BM_CTAS = 2;          // BM_CTAS: of an SM; with three, 80 registers a thread leave less to overlap (39 -> 47 us)
 constexpr int BM_FEW = 16;                                       // continuations that most calls want
 constexpr float BM_LOG2E = 1.44269504f;
 
+struct alignas(16) PartSum { double sum; float top, unused; };     // of exponentials against the part's maximum
 struct BeamArgs {
     const char *x;
     int64_t ld;                      // bytes
@@ -36,22 +37,43 @@ struct BeamArgs {
     int eos;
     float *scores_out; int *parents, *tokens, *done_out;
     unsigned long long *keys;        // scratch, [group][slot][beam][part]
-    double2 *sums;                   // scratch, [row][part]: maximum, sum
+    PartSum *sums;                   // scratch, [row][part]
     int *arrived;                    // scratch, [group], zero between calls
 };
 
 struct Wide { unsigned long long hi, lo; };      // score; then beam, logit, word
-__device__ __forceinline__ bool operator>(const Wide &a, const Wide &b) { return a.hi > b.hi || (a.hi == b.hi && a.lo > b.lo); }
+__device__ __forceinline__ bool operator>(const Wide &a, const Wide &b) { return (a.hi > b.hi) | ((a.hi == b.hi) & (a.lo > b.lo)); }       // without branches: many of them are in a row
 __device__ __forceinline__ bool bm_there(unsigned long long k) { return k != 0; }
 __device__ __forceinline__ bool bm_there(const Wide &k) { return k.hi != 0; }
 __device__ __forceinline__ unsigned long long bm_xor(unsigned long long k, int o) { return __shfl_xor_sync(0xffffffffu, k, o); }
 __device__ __forceinline__ Wide bm_xor(const Wide &k, int o) { return Wide{__shfl_xor_sync(0xffffffffu, k.hi, o), __shfl_xor_sync(0xffffffffu, k.lo, o)}; }
 
+// The n-th largest of the maxima of 2 n groups of threads or more (of 2^widest threads at most); no key where fewer than n have one. One copy of the code for
+// whoever wants it: a part's first tile, lists that are cut, the join. Code that runs once is paced by instruction fetches.
+template <class K> __device__ __noinline__ K bm_nth(K best, int n, int widest, K *groups, K *bound) {
+    const int lg = min(widest, __clz(2 * n - 1) - 24), size = 1 << lg;           // BM_THREADS >> lg is 2 n or more
+#pragma unroll 1
+    for (int o = 1; o < size; o <<= 1) { const K other = bm_xor(best, o); if (other > best) best = other; }
+    const int tid = threadIdx.x, G = BM_THREADS >> lg, mine = tid >> lg;
+    __syncthreads();
+    if ((tid & (size - 1)) == 0) groups[mine] = best;
+    if (tid == 0) *bound = K{};
+    __syncthreads();
+    int rank = 0;                        // a group's threads share the comparisons with the others; of equal keys the lower group is first
+#pragma unroll 4
+    for (int j = tid & (size - 1); j < G; j += size) { const K other = groups[j]; rank += (other > best) | ((j < mine) & !(best > other)); }
+#pragma unroll 1
+    for (int o = 1; o < size; o <<= 1) rank += __shfl_xor_sync(0xffffffffu, rank, o);
+    if ((tid & (size - 1)) == 0 && rank == n - 1 && bm_there(best)) *bound = best;
+    __syncthreads();
+    return *bound;
+}
+
 // The n largest keys of tiles of EPT a thread; n up to MOST, BM_FEW or NCMB_MAX_BEAMS: the fewer, the less room the lists take.
 // ROOM: keys that the list holds beside 2 n; 0: what a tile adds at most, once it has a bound.
 template <class K, int EPT, int MOST, int ROOM = 0> struct TopN {
-    static constexpr int WIDEST = MOST <= BM_FEW ? 4 : 8;        // threads of a group
-    static constexpr int REACH = MOST <= BM_FEW ? MOST * WIDEST : BM_THREADS / 2;        // threads whose groups reach a bound, at most: n groups of 2 n or more
+    static constexpr int WIDEST = MOST <= BM_FEW ? 2 : 3;        // threads of a group at most: 4, 8
+    static constexpr int REACH = MOST <= BM_FEW ? MOST << WIDEST : BM_THREADS / 2;        // threads whose groups reach a bound, at most: n groups of 2 n or more
     static constexpr int CAP = (ROOM ? ROOM : REACH * EPT) + 2 * MOST;
     static constexpr int PER = (CAP + BM_THREADS - 1) / BM_THREADS;
     K list[CAP], few[REACH * PER > BM_THREADS / 2 ? REACH * PER : BM_THREADS / 2], groups[BM_THREADS], bound;
@@ -61,24 +83,7 @@ template <class K, int EPT, int MOST, int ROOM = 0> struct TopN {
         if (threadIdx.x == 0) { count = 0; bound = K{}; }
         __syncthreads();
     }
-    // the n-th largest of the maxima of 2 n groups of threads or more; no key where fewer than n have one
-    __device__ K nth(K best, int n) {
-        int size = WIDEST;
-        while (size > 1 && BM_THREADS / size < 2 * n) size >>= 1;
-        for (int o = 1; o < size; o <<= 1) { const K other = bm_xor(best, o); if (other > best) best = other; }
-        const int tid = threadIdx.x, G = BM_THREADS / size;
-        __syncthreads();
-        if (tid % size == 0) groups[tid / size] = best;
-        if (tid == 0) bound = K{};
-        __syncthreads();
-        int rank = 0;                    // a group's threads share the comparisons with the others
-#pragma unroll 4
-        for (int j = tid % size; j < G; j += size) rank += groups[j] > best;
-        for (int o = 1; o < size; o <<= 1) rank += __shfl_xor_sync(0xffffffffu, rank, o);
-        if (tid % size == 0 && rank == n - 1 && bm_there(best)) bound = best;
-        __syncthreads();
-        return bound;
-    }
+    __device__ K nth(K best, int n) { return bm_nth(best, n, WIDEST, groups, &bound); }
     // the list becomes its n largest, in order; returns the n-th, no key where there are fewer
     __device__ K settle(int n) {
         const int tid = threadIdx.x, c = count;
@@ -95,16 +100,17 @@ template <class K, int EPT, int MOST, int ROOM = 0> struct TopN {
         }
         __syncthreads();
         if (c > BM_THREADS / 2) m = n_few;
-        int ways = 8;                    // threads that share a key's comparisons
-        while (ways > 1 && m * ways > BM_THREADS) ways >>= 1;
-        for (int i0 = 0; i0 < m; i0 += BM_THREADS / ways) {
-            const int i = i0 + tid / ways;
+        const int lg = m <= BM_THREADS / 8 ? 3 : m <= BM_THREADS / 4 ? 2 : m <= BM_THREADS / 2 ? 1 : 0, ways = 1 << lg;      // threads that share a key's comparisons
+#pragma unroll 1
+        for (int i0 = 0; i0 < m; i0 += BM_THREADS >> lg) {
+            const int i = i0 + (tid >> lg);
             const K mine = few[min(i, m - 1)];
             int rank = 0;
 #pragma unroll 4
-            for (int j = tid % ways; j < m; j += ways) rank += few[j] > mine;
+            for (int j = tid & (ways - 1); j < m; j += ways) rank += few[j] > mine;
+#pragma unroll 1
             for (int o = 1; o < ways; o <<= 1) rank += __shfl_xor_sync(0xffffffffu, rank, o);
-            if (i < m && tid % ways == 0 && rank < n) list[rank] = mine;
+            if (i < m && (tid & (ways - 1)) == 0 && rank < n) list[rank] = mine;
         }
         if (tid == 0) count = min(n, m);
         __syncthreads();
@@ -174,8 +180,8 @@ __device__ __forceinline__ uint32_t bm_order(float x) {          // larger is la
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 __device__ __forceinline__ float bm_clamp(float x) { return fminf(fmaxf(x, -INFINITY), 3.402823466e38f); }      // a NaN is -infinity
-__device__ __forceinline__ unsigned long long bm_key(float x, int w) {       // of a logit; -0 is 0
-    return (unsigned long long)bm_order(x + 0.f) << 32 | (0xffffffffu - (uint32_t)w);
+__device__ __forceinline__ unsigned long long bm_key(float x, int w) {       // of a logit; -0 is 0. Bits 24 ... 31 are free
+    return (unsigned long long)bm_order(x + 0.f) << 32 | (0xffffffu - (uint32_t)w);
 }
 __device__ __forceinline__ float bm_value(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k); }
 __device__ __forceinline__ unsigned long long bm_order(double x) {
@@ -185,8 +191,21 @@ __device__ __forceinline__ unsigned long long bm_order(double x) {
 __device__ __forceinline__ double bm_value(unsigned long long k) { return __longlong_as_double(k >> 63 ? k ^ 1ull << 63 : ~k); }
 
 // ---- a group's parts, by the last CTA that has one ----
+// log t, t > 0, to 1e-12: t = 2^e m with m about 1, log m = 2 atanh s of s = (m - 1) / (m + 1), |s| <= 0.18, by its series. (The library's function is
+// exact to the last bit, in code that takes 2000 cycles to fetch.)
+__device__ __forceinline__ double bm_log(double t) {
+    const unsigned long long u = __double_as_longlong(t);
+    int e = (int)(u >> 52) - 1023;
+    double m = __longlong_as_double((u & 0xfffffffffffffull) | 1023ull << 52);
+    if (m > 1.4) { m *= 0.5; e++; }
+    const double d = m + 1, q = (double)__fdividef(1.f, (float)d), s0 = (m - 1) * q, s = fma(q, fma(-s0, d, m - 1), s0), z = s * s, zz = z * z;      // a quotient, once corrected
+    const double a = fma(z, 1.0 / 3, 1.0), b = fma(z, 1.0 / 7, 1.0 / 5), c = fma(z, 1.0 / 11, 1.0 / 9), f = fma(z, 1.0 / 15, 1.0 / 13);
+    const double r = fma(zz * zz, fma(zz, f, c), fma(zz, b, a));
+    return fma((double)e, 0.693147180559945309, 2 * s * r);
+}
 template <int MOST> struct JoinShared {
     TopN<Wide, BM_JOIN, MOST, BM_JOIN * BM_THREADS> top;         // a whole tile fits
+    unsigned long long bound;
     double lse[NCMB_MAX_BEAMS], score[NCMB_MAX_BEAMS];
     int over[NCMB_MAX_BEAMS];
 };
@@ -205,55 +224,57 @@ template <int MOST> __device__ __noinline__ void beam_join(const BeamArgs &a, in
     };
     load(0);                                                     // on their way while the sums meet
     for (int k = warp; k < a.beams; k += BM_WARPS) {
-        const double2 *s = a.sums + (row0 + k) * a.parts;
+        const PartSum *s = a.sums + (row0 + k) * a.parts;
         const bool ended = a.done && a.done[row0 + k];
         const float sc = a.scores[row0 + k];
-        double m = -INFINITY, t = 0;
+        float m = -INFINITY;
+        double t = 0;
         if (!ended) {
+#pragma unroll 1
             for (int p = lane; p < a.parts; p += 32) {
-                const double2 x = __ldcg(s + p);                 // maximum, sum
-                const double top = fmax(m, x.x), base = top == -INFINITY ? 0 : top;
-                t = t * bm_exp2((float)(m - base) * BM_LOG2E) + x.y * bm_exp2((float)(x.x - base) * BM_LOG2E);
+                const float4 x = __ldcg((const float4 *)(s + p));
+                const float top = fmaxf(m, x.z), base = top == -INFINITY ? 0.f : top;
+                t = t * bm_exp2((m - base) * BM_LOG2E) + __hiloint2double(__float_as_int(x.y), __float_as_int(x.x)) * bm_exp2((x.z - base) * BM_LOG2E);
                 m = top;
             }
-            double top = m;
-            for (int o = 16; o; o >>= 1) top = fmax(top, __shfl_xor_sync(0xffffffffu, top, o));
-            t *= bm_exp2((float)(m - (top == -INFINITY ? 0 : top)) * BM_LOG2E);
-            for (int o = 16; o; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+            float top = m;
+#pragma unroll 1
+            for (int o = 1; o < min(32, a.parts); o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+            t *= bm_exp2((m - (top == -INFINITY ? 0.f : top)) * BM_LOG2E);
+#pragma unroll 1
+            for (int o = 1; o < min(32, a.parts); o <<= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
             m = top;
         }
         if (lane == 0) {
-            sh.lse[k] = ended || m == -INFINITY ? 0.0 : m + log(t);
+            sh.lse[k] = ended || m == -INFINITY ? 0.0 : m + bm_log(t);
             sh.score[k] = sc == sc ? (double)sc : -INFINITY;
             sh.over[k] = ended;
         }
     }
     sh.top.clear();
-    Wide least = {};
+    unsigned long long least = 0;
     const int limit = min(3 * n + 8, 2 * MOST);                  // fewer are in the list when a tile begins, so the tile fits
 #pragma unroll 1
     for (int i0 = 0; i0 < total; i0 += BM_THREADS * BM_JOIN) {
         Wide key[BM_JOIN];
 #pragma unroll
         for (int e = 0; e < BM_JOIN; e++) {
-            const int i = i0 + e * BM_THREADS + tid, j = i / lists, k = (i - j * lists) / a.parts;
-            uint32_t w = 0xffffffffu - (uint32_t)u[e];
-            float x = bm_value((uint32_t)(u[e] >> 32));
-            bool there = u[e] != 0;
-            if (sh.over[k]) {                                    // its end, then the other words, which have nothing
-                there = i < total && (i - j * lists) % a.parts == 0 && j < min(n, a.V);
-                w = j == 0 ? a.eos : j - 1 + (j - 1 >= a.eos);
-                x = j == 0 ? 0.f : -INFINITY;
-            }
+            const int k = NCMB_MAX_BEAMS - 1 - (int)(u[e] >> 24 & 0x7f);
+            const float x = bm_value((uint32_t)(u[e] >> 32));
             const double sc = x == -INFINITY ? -INFINITY : sh.score[k] + ((double)x - sh.lse[k]) + 0.0;
-            key[e] = there ? Wide{bm_order(sc), (unsigned long long)(NCMB_MAX_BEAMS - 1 - k) << 56 | (unsigned long long)bm_order(x) << 24 | (0xffffffu - w)} : Wide{};
+            key[e] = u[e] ? Wide{bm_order(sc), (u[e] >> 24 & 0x7f) << 56 | u[e] >> 32 << 24 | (u[e] & 0xffffff)} : Wide{};
         }
         load(i0 + BM_THREADS * BM_JOIN);
-        if (!bm_there(least)) sh.top.raise(n, least, [&](int e) { return key[e]; });
+        if (least == 0) {                                        // by the scores alone: those that are equal to the n-th join too
+            unsigned long long most = 0;
+#pragma unroll
+            for (int e = 0; e < BM_JOIN; e++) most = max(most, key[e].hi);
+            least = bm_nth(most, n, sh.top.WIDEST, (unsigned long long *)sh.top.groups, &sh.bound);
+        }
         bool full = false, any = false;
 #pragma unroll
         for (int e = 0; e < BM_JOIN; e++) {
-            if (!bm_there(key[e]) || least > key[e]) continue;
+            if (!bm_there(key[e]) || key[e].hi < least) continue;
             const int at = atomicAdd(&sh.top.count, 1);
             sh.top.list[at] = key[e];
             full |= at >= limit;
@@ -263,7 +284,7 @@ template <int MOST> __device__ __noinline__ void beam_join(const BeamArgs &a, in
         if (slots == n && lists <= BM_THREADS * BM_JOIN && !__syncthreads_or(any)) break;
         if (__syncthreads_or(full)) {
             const Wide nth = sh.top.settle(n);
-            if (nth > least) least = nth;
+            least = max(least, nth.hi);
         }
     }
     sh.top.settle(n);
@@ -295,7 +316,7 @@ template <int VE> __device__ __forceinline__ int bm_place(int e) { return (e / V
 template <class E, bool VEC, int MOST>
 __device__ __noinline__ void beam_again(const E *x0, int t0, int t1, int V, int n, TopN<unsigned long long, BM_CHUNK, MOST> &top, unsigned long long &least) {
     constexpr int VE = VEC ? 16 / (int)sizeof(E) : 1;
-    top.drop(0xffffffffu - t0 * BM_TILE);
+    top.drop(0xffffffu - t0 * BM_TILE);
     for (int t = t0; t < t1; t++)
         for (int e0 = 0; e0 < BM_EPT; e0 += BM_CHUNK)
             top.add(n, least, [&](int e) {
@@ -319,7 +340,14 @@ __global__ void __launch_bounds__(BM_THREADS, BM_CTAS) k_beam_select(const __gri
     const int part = (int)(blockIdx.x - row * a.parts), g = (int)(row / a.beams);
     pdl_wait();
     pdl_launch_dependents();
-    if (!(a.done && a.done[row])) {
+    const int lists = a.beams * a.parts, beam = (int)(row - (int64_t)g * a.beams);
+    auto leave = [&](int i, unsigned long long key) {            // as slot i of the part, with its beam
+        a.keys[((int64_t)g * a.slots + i) * lists + beam * a.parts + part] = key ? key | (unsigned long long)(NCMB_MAX_BEAMS - 1 - beam) << 24 : 0ull;
+    };
+    if (a.done && a.done[row]) {                                 // its end, then the other words, which have nothing
+        for (int i = tid; i < a.slots; i += BM_THREADS)
+            leave(i, part > 0 || i >= min(a.n, a.V) ? 0ull : i == 0 ? bm_key(0.f, a.eos) : bm_key(-INFINITY, i - 1 + (i - 1 >= a.eos)));
+    } else {
         const int t0 = (int)((int64_t)part * a.tiles / a.parts), t1 = (int)((int64_t)(part + 1) * a.tiles / a.parts);
         const E *x0 = (const E *)(a.x + row * a.ld);
         auto place = [&](int e) { return bm_place<VE>(e); };
@@ -460,8 +488,7 @@ __global__ void __launch_bounds__(BM_THREADS, BM_CTAS) k_beam_select(const __gri
         }
         // what may be among the n best, and the part's maximum and sum
         if (sh.top.count > a.slots || a.slots == a.n) sh.top.settle(a.n);
-        const int lists = a.beams * a.parts, list = (int)(row - (int64_t)g * a.beams) * a.parts + part;
-        for (int i = tid; i < a.slots; i += BM_THREADS) a.keys[((int64_t)g * a.slots + i) * lists + list] = i < sh.top.count ? sh.top.list[i] : 0ull;
+        for (int i = tid; i < a.slots; i += BM_THREADS) leave(i, i < sh.top.count ? sh.top.list[i] : 0ull);
         float top = m;
         for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
         if (lane == 0) sh.maxima[warp] = top;
@@ -475,7 +502,7 @@ __global__ void __launch_bounds__(BM_THREADS, BM_CTAS) k_beam_select(const __gri
         if (tid == 0) {
             s = 0;
             for (int w = 0; w < BM_WARPS; w++) s += sh.sums[w];
-            a.sums[row * a.parts + part] = make_double2(top, s);
+            a.sums[row * a.parts + part] = PartSum{s, top, 0.f};
         }
     }
     __threadfence();
@@ -534,10 +561,10 @@ extern "C" int ncmb_beam_select(const void *logits, int64_t ldl, int type, int g
         if (cost < best) { best = cost; a.parts = (int)p; }
     }
     a.slots = (int64_t)beams * a.parts * 2 * n_out <= BM_THREADS * BM_JOIN ? 2 * n_out : n_out;
-    const size_t kb = (size_t)rows * a.parts * a.slots * 8, sb = (size_t)rows * a.parts * sizeof(double2);
+    const size_t kb = (size_t)rows * a.parts * a.slots * 8, sb = (size_t)rows * a.parts * sizeof(PartSum);
     char *scratch = (char *)cache_scratch(who, sb + kb);
     if (!scratch) return -1;
-    a.sums = (double2 *)scratch;
+    a.sums = (PartSum *)scratch;
     a.keys = (unsigned long long *)(scratch + sb);
     if (!(a.arrived = (int *)cache_scratch(who, (size_t)groups * 4, SCRATCH_DONE))) return -1;
     ProfScope prof(NCMB_K_SAMPLE, 4.0 * rows * V, (double)rows * V * es);

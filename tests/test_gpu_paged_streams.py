@@ -14,10 +14,15 @@ F32, BF16 = torch.float32, torch.bfloat16
 
 @pytest.fixture(scope="module")
 def cuda():
-    lib = capi.NcmLib(helpers.CUDA_LIB)
-    yield lib
+    return capi.NcmLib(helpers.CUDA_LIB)
+
+
+@pytest.fixture(autouse=True)
+def default_stream(cuda):
+    """A test leaves the library on the stream that torch's calls are on by default."""
+    yield
     torch.cuda.synchronize()
-    lib.ncmb_set_stream(None)
+    cuda.ncmb_set_stream(None)
 
 
 class Work:

@@ -92,9 +92,17 @@ __device__ __forceinline__ void cm_mma_tf32(float (&c)[4], const uint32_t (&a)[4
     asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ void cm_tf32(float v, uint32_t &hi, uint32_t &lo) {
-    asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(hi) : "f"(v));
-    asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(lo) : "f"(v - __uint_as_float(hi)));
+// Two TF32 terms of v, 22 bits. BITS: v cut off after a TF32's bits, and the rest with half of its own last place added and cut off; four instructions of the
+// integer and fp32 pipes for two conversions, which are slower (paged, fp32 cache, 16 heads over 4 x 64, 32 rows of up to 8000: 86 -> 75 us).
+template <bool BITS = false> __device__ __forceinline__ void cm_tf32(float v, uint32_t &hi, uint32_t &lo) {
+    if constexpr (BITS) {
+        hi = __float_as_uint(v) & 0xffffe000u;
+        const float l = v - __uint_as_float(hi);
+        lo = __float_as_uint(fmaf(l, 0x1p-11f, l)) & 0xffffe000u;
+    } else {
+        asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(hi) : "f"(v));
+        asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(lo) : "f"(v - __uint_as_float(hi)));
+    }
 }
 __device__ __forceinline__ float cm_exp2(float x) {
     float y;
@@ -375,7 +383,7 @@ __global__ void __launch_bounds__(CM_THREADS, CmCfg<KE, QE, HDP, R>::ctas(BLOCKS
                     for (int h = 0; h < 2; h++) {
                         uint32_t hi[4], lo[4];
 #pragma unroll
-                        for (int e = 0; e < 4; e++) cm_tf32(x[4 * h + e], hi[e], lo[e]);
+                        for (int e = 0; e < 4; e++) cm_tf32<PAGED>(x[4 * h + e], hi[e], lo[e]);
                         const int u = (d0 / 4 + h) ^ ((m & 1) << 2);
                         *(uint4 *)(qs + m * ROW + u * 16) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
                         *(uint4 *)(qs + (M + m) * ROW + u * 16) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
@@ -484,8 +492,8 @@ __global__ void __launch_bounds__(CM_THREADS, CmCfg<KE, QE, HDP, R>::ctas(BLOCKS
 #pragma unroll
                         for (int e = 0; e < 2; e++) {
                             uint32_t bh[2], bl[2];
-                            cm_tf32(kv[2 * e], bh[0], bl[0]);
-                            cm_tf32(kv[2 * e + 1], bh[1], bl[1]);
+                            cm_tf32<PAGED>(kv[2 * e], bh[0], bl[0]);
+                            cm_tf32<PAGED>(kv[2 * e + 1], bh[1], bl[1]);
                             if constexpr (!R8) cm_mma_tf32(L[j], al[e], bh[0], bh[1]);
                             cm_mma_tf32(L[j], ah[e], bl[0], bl[1]);
                             cm_mma_tf32(S[j], ah[e], bh[0], bh[1]);
@@ -631,11 +639,11 @@ __global__ void __launch_bounds__(CM_THREADS, CmCfg<KE, QE, HDP, R>::ctas(BLOCKS
 #pragma unroll
                 for (int j = 0; j < NT; j++) {                   // k position c: key 2 c, position c + 4: key 2 c + 1
                     if constexpr (R8) {
-                        cm_tf32(S[j][0], ph[j][0], ph[j][1]);
-                        cm_tf32(S[j][1], ph[j][2], ph[j][3]);
+                        cm_tf32<PAGED>(S[j][0], ph[j][0], ph[j][1]);
+                        cm_tf32<PAGED>(S[j][1], ph[j][2], ph[j][3]);
                     } else {
-                        cm_tf32(S[j][0], ph[j][0], pl[j][0]); cm_tf32(S[j][2], ph[j][1], pl[j][1]);
-                        cm_tf32(S[j][1], ph[j][2], pl[j][2]); cm_tf32(S[j][3], ph[j][3], pl[j][3]);
+                        cm_tf32<PAGED>(S[j][0], ph[j][0], pl[j][0]); cm_tf32<PAGED>(S[j][2], ph[j][1], pl[j][1]);
+                        cm_tf32<PAGED>(S[j][1], ph[j][2], pl[j][2]); cm_tf32<PAGED>(S[j][3], ph[j][3], pl[j][3]);
                     }
                 }
 #pragma unroll
@@ -653,8 +661,8 @@ __global__ void __launch_bounds__(CM_THREADS, CmCfg<KE, QE, HDP, R>::ctas(BLOCKS
 #pragma unroll
                         for (int x = 0; x < 4; x++) {
                             uint32_t bh[2], bl[2];
-                            cm_tf32(va[x], bh[0], bl[0]);
-                            cm_tf32(vv[x], bh[1], bl[1]);
+                            cm_tf32<PAGED>(va[x], bh[0], bl[0]);
+                            cm_tf32<PAGED>(vv[x], bh[1], bl[1]);
                             if constexpr (!R8) cm_mma_tf32(cc[x], pl[j], bh[0], bh[1]);
                             cm_mma_tf32(cc[x], ph[j], bl[0], bl[1]);
                             cm_mma_tf32(cc[x], ph[j], bh[0], bh[1]);

@@ -42,7 +42,8 @@ struct AppendArgs {
     int H;                           // 0: no queries
     const int *start, *pos;
     int tokens, T;                   // T: of every row, where start is null
-    int per, items;                  // tokens a CTA, items a head
+    int per;                         // tokens a CTA
+    RopeShare share;
 };
 
 // the row that token i belongs to, -1 for none: the last b with start[b] <= i. s: start, in shared or global memory
@@ -66,11 +67,11 @@ __global__ void __launch_bounds__(PA_THREADS, V * sizeof(QE) == 16 ? 4 : 6) k_pa
     __shared__ int64_t slot[PA_TOKENS];          // bytes from the pool's start; -1: not stored, -2: nobody's
     __shared__ int place[PA_TOKENS];
     __shared__ int starts[PA_ROWS + 1];
-    const int tid = threadIdx.x, pairs = ROPE ? r.dims / 2 : 0, cs_row = ROPE ? rope_row(r.dims) : 0, heads = a.H + 2 * a.c.nkv;
+    const int tid = threadIdx.x, cs_row = ROPE ? rope_row(r.dims) : 0;
     const int n0 = blockIdx.x * a.per, here = min(a.per, a.tokens - n0);
     const bool near = a.c.rows <= PA_ROWS;
-    RopeWalk at(tid, PA_THREADS, heads, a.items);
-    const RopeItem it = rope_item<V, ROPE != 1>(at.u, a.items, ROPE ? r.dims : 0, a.c.hd);
+    RopeWalk at(tid, a.share);
+    const RopeItem it = rope_item<V, ROPE != 1>(at.u, a.share.items, ROPE ? r.dims : 0, a.c.hd);
     pdl_wait();
     pdl_launch_dependents();
     RopeVec<QE, V> p[PA_BATCH], q[PA_BATCH];
@@ -84,7 +85,7 @@ __global__ void __launch_bounds__(PA_THREADS, V * sizeof(QE) == 16 ? 4 : 6) k_pa
             p[x] = *(const RopeVec<QE, V> *)(f + it.d0);
             if (it.d1 >= 0) q[x] = *(const RopeVec<QE, V> *)(f + it.d1);
         }
-        at.next();
+        at.next(a.share);
     };
 #pragma unroll
     for (int x = 0; x < PA_BATCH; x++) load(x);
@@ -107,10 +108,7 @@ __global__ void __launch_bounds__(PA_THREADS, V * sizeof(QE) == 16 ? 4 : 6) k_pa
     }
     __syncthreads();
     if (ROPE) {
-        for (int i = tid; i < here * pairs; i += PA_THREADS) {
-            const int t = i / pairs;
-            cs[t * cs_row + rope_place<V, ROPE == 2>(i - t * pairs, r.dims)] = rope_angle(r, i - t * pairs, place[t], false);
-        }
+        rope_angles(tid, here, a.share, [&](int t, int i) { cs[t * cs_row + rope_place<V, ROPE == 2>(i, r.dims)] = rope_angle(r, i, place[t], false); });
         __syncthreads();
     }
     while (from.tok < here) {
@@ -133,16 +131,16 @@ __global__ void __launch_bounds__(PA_THREADS, V * sizeof(QE) == 16 ? 4 : 6) k_pa
                     if (it.d1 >= 0) rope_store<KE, V>(y + it.d1, g);
                 }
             }
-            from.next();
+            from.next(a.share);
             load(x);
         }
     }
 }
 
 template <class QE, class KE, int V> void run_append(const NcmbRope *r, AppendArgs &a) {
-    a.items = rope_items(r, a.c.hd, V);
+    a.share = rope_share(r, rope_items(r, a.c.hd, V), a.H + 2 * a.c.nkv, PA_THREADS);
     // four items a thread, and CTAs for all SMs (16 rows of up to 2001 tokens, 32 over 8 x 128 in bf16, 4 / 8 / 12 items a thread: 69 / 76 / 77 us)
-    const int64_t per_token = (int64_t)(a.H + 2 * a.c.nkv) * a.items, rounds = V * sizeof(QE) == 16 ? 4 : 20;
+    const int64_t per_token = (int64_t)(a.H + 2 * a.c.nkv) * a.share.items, rounds = V * sizeof(QE) == 16 ? 4 : 20;
     a.per = (int)std::max<int64_t>(1, std::min<int64_t>({PA_TOKENS, rounds * PA_THREADS / per_token, a.tokens / (4 * ctx().sm_count)}));
     const size_t smem = r ? (size_t)a.per * rope_row(r->dims) * sizeof(float2) : 0;
     const unsigned grid = (unsigned)cdiv(a.tokens, a.per);

@@ -22,7 +22,8 @@ struct RopeArgs {
     const int *pos;
     uint32_t tokens, T;
     int n_head, hd, inverse;         // hd: the dims that are moved, in place those that turn
-    int per, items;                  // tokens a CTA, items a head
+    int per;                         // tokens a CTA
+    RopeShare share;
 };
 
 // A CTA has `per` tokens: their places in memory and their angles once, in shared memory, then all items of their heads, RO_BATCH of a thread on their way at a
@@ -32,11 +33,11 @@ __global__ void __launch_bounds__(RO_THREADS, V * sizeof(E) == 16 ? 4 : 6) k_rop
     extern __shared__ __align__(16) float2 cs[];         // [per][rope_row(dims)]
     __shared__ int64_t xo[RO_TOKENS], yo[RO_TOKENS];
     __shared__ int place[RO_TOKENS];
-    const int tid = threadIdx.x, pairs = r.dims / 2, row = rope_row(r.dims);
+    const int tid = threadIdx.x, row = rope_row(r.dims);
     const uint32_t n0 = blockIdx.x * (uint32_t)a.per;
     const int here = (int)min((uint32_t)a.per, a.tokens - n0);
-    RopeWalk at(tid, RO_THREADS, a.n_head, a.items);
-    const RopeItem it = rope_item<V, PAIRS>(at.u, a.items, r.dims, a.hd);
+    RopeWalk at(tid, a.share);
+    const RopeItem it = rope_item<V, PAIRS>(at.u, a.share.items, r.dims, a.hd);
     pdl_wait();
     pdl_launch_dependents();
     if (tid < here) {
@@ -54,14 +55,11 @@ __global__ void __launch_bounds__(RO_THREADS, V * sizeof(E) == 16 ? 4 : 6) k_rop
             p[k] = *(const RopeVec<E, V> *)(x + it.d0);
             if (it.d1 >= 0) q[k] = *(const RopeVec<E, V> *)(x + it.d1);
         }
-        at.next();
+        at.next(a.share);
     };
 #pragma unroll
     for (int k = 0; k < RO_BATCH; k++) load(k);
-    for (int i = tid; i < here * pairs; i += RO_THREADS) {
-        const int t = i / pairs;
-        cs[t * row + rope_place<V, PAIRS>(i - t * pairs, r.dims)] = rope_angle(r, i - t * pairs, place[t], a.inverse);
-    }
+    rope_angles(tid, here, a.share, [&](int t, int i) { cs[t * row + rope_place<V, PAIRS>(i, r.dims)] = rope_angle(r, i, place[t], a.inverse); });
     __syncthreads();
     while (from.tok < here) {
 #pragma unroll
@@ -75,17 +73,17 @@ __global__ void __launch_bounds__(RO_THREADS, V * sizeof(E) == 16 ? 4 : 6) k_rop
                 rope_store<E, V>(y + it.d0, f);
                 if (it.d1 >= 0) rope_store<E, V>(y + it.d1, g);
             }
-            from.next();
+            from.next(a.share);
             load(k);
         }
     }
 }
 
 template <class E, int V> void run_rope(const NcmbRope &r, RopeArgs &a) {
-    a.items = rope_items(&r, a.hd, V);
+    a.share = rope_share(&r, rope_items(&r, a.hd, V), a.n_head, RO_THREADS);
     // A thread's items all on their way at once, and CTAs for all SMs (8 x 4000 tokens of 40 x 128 in bf16, 4 / 8 / 20 items a thread: 100 / 107 / 115 us);
     // short vectors are paced by instructions, so there the angles are shared by more (dims 50 of it, halves, 4 / 20 items: 293 / 277).
-    const int64_t per_token = (int64_t)a.n_head * a.items, rounds = V * sizeof(E) == 16 ? RO_BATCH : 20;
+    const int64_t per_token = (int64_t)a.n_head * a.share.items, rounds = V * sizeof(E) == 16 ? RO_BATCH : 20;
     a.per = (int)std::max<int64_t>(1, std::min<int64_t>({RO_TOKENS, rounds * RO_THREADS / per_token, a.tokens / (4 * ctx().sm_count)}));
     const size_t smem = (size_t)a.per * rope_row(r.dims) * sizeof(float2);
     const unsigned grid = (unsigned)cdiv(a.tokens, a.per);

@@ -27,6 +27,22 @@ inline int rope_items(const NcmbRope *r, int hd, int v) {
     return r->dims / 2 / v + (int)cdiv(hd - r->dims, 2 * v);
 }
 
+// How a CTA's threads share the items of its tokens' heads and the tokens' angles, by divisions that the host does: a thread has item u of every step-th
+// head, and goes from one to the next, and from one angle to the next, by additions.
+struct RopeShare {
+    int items, heads, step, dtok, dh;            // items a head, heads a token; step: heads that the threads cover at once
+    int pairs, dt, dp;                           // pairs a token; from a thread's angle to its next: tokens and pairs
+    uint32_t by_items, by_heads, by_pairs;       // x / d = x * by >> 16, rounded up: exact for x, d up to 256
+};
+inline RopeShare rope_share(const NcmbRope *r, int items, int heads, int threads) {
+    RopeShare s;
+    s.items = items; s.heads = heads; s.step = threads / items; s.dtok = s.step / heads; s.dh = s.step % heads;
+    s.pairs = r ? r->dims / 2 : 1; s.dt = threads / s.pairs; s.dp = threads % s.pairs;
+    auto by = [](int d) { return (uint32_t)cdiv(65536, d); };
+    s.by_items = by(items); s.by_heads = heads > 256 ? 0 : by(heads); s.by_pairs = by(s.pairs);
+    return s;
+}
+
 // cosines and sines of a token in shared memory: pairs in whole vectors
 __host__ __device__ inline int rope_row(int dims) { return (dims / 2 + 7) & ~7; }
 
@@ -88,24 +104,31 @@ template <int V, bool PAIRS> __device__ __forceinline__ RopeItem rope_item(int u
     it.pair1 = PAIRS && it.d1 >= 0 && it.d1 < dims ? it.d1 / 2 : -1;
     return it;
 }
-// The items of a CTA's tokens: a thread has item u of every step-th head, and walks heads and tokens without a division.
+// The items of a thread
 struct RopeWalk {
     int u, tok, h;                   // tok: beyond the CTA's when there is none left
-    int heads, dtok, dh;
-    __device__ RopeWalk(int tid, int threads, int heads_, int items) : heads(heads_) {
-        const int step = threads / items, p = tid / items;
-        u = tid - p * items;
-        tok = p < step ? p / heads : 1 << 20;
-        h = p < step ? p - tok * heads : 0;
-        dtok = step / heads;
-        dh = step - dtok * heads;
+    __device__ RopeWalk(int tid, const RopeShare &s) {
+        const int p = tid * s.by_items >> 16;
+        u = tid - p * s.items;
+        tok = p < s.step ? p * s.by_heads >> 16 : 1 << 20;       // more than 256 heads: by 0, the first token's
+        h = p < s.step ? p - tok * s.heads : 0;
     }
-    __device__ void next() {
-        tok += dtok;
-        h += dh;
-        if (h >= heads) { h -= heads; tok++; }
+    __device__ void next(const RopeShare &s) {
+        tok += s.dtok;
+        h += s.dh;
+        if (h >= s.heads) { h -= s.heads; tok++; }
     }
 };
+// The tokens' angles, each once: angle(token, pair)
+template <class F> __device__ __forceinline__ void rope_angles(int tid, int here, const RopeShare &s, F angle) {
+    int t = tid * s.by_pairs >> 16, i = tid - t * s.pairs;
+    while (t < here) {
+        angle(t, i);
+        t += s.dt;
+        i += s.dp;
+        if (i >= s.pairs) { i -= s.pairs; t++; }
+    }
+}
 // Cosines and sines of a token in shared memory: those that a vector needs are read two pairs (16 bytes) at a time, and vectors side by side by
 // threads side by side, so two pairs of all vectors stand together, then the next two.
 template <int V, bool PAIRS> __device__ __forceinline__ int rope_place(int pair, int dims) {

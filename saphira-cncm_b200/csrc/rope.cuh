@@ -91,17 +91,16 @@ __device__ __forceinline__ float2 rope_angle(const NcmbRope &r, int i, int pos, 
 // where item u of a head stands, what its vectors are rotated by, if at all
 struct RopeItem {
     int d0, d1;              // dims of its two vectors; d1 < 0: there is no second
-    int pair0, pair1;        // first pairs of their rotation, or -1
+    int pair;                // first pair of the first one's rotation, or -1; PAIRS: of the second, as far behind as it stands
 };
 template <int V, bool PAIRS> __device__ __forceinline__ RopeItem rope_item(int u, int items, int dims, int hd) {
     RopeItem it;
     const int rot = PAIRS ? 0 : dims / 2 / V;
-    if (!PAIRS && u < rot) { it.d0 = u * V; it.d1 = it.d0 + dims / 2; it.pair0 = it.pair1 = it.d0; return it; }
+    if (!PAIRS && u < rot) { it.d0 = u * V; it.d1 = it.d0 + dims / 2; it.pair = it.d0; return it; }
     it.d0 = (PAIRS ? 0 : dims) + (u - rot) * V;
     it.d1 = it.d0 + (items - rot) * V;
     if (it.d1 >= hd) it.d1 = -1;
-    it.pair0 = PAIRS && it.d0 < dims ? it.d0 / 2 : -1;
-    it.pair1 = PAIRS && it.d1 >= 0 && it.d1 < dims ? it.d1 / 2 : -1;
+    it.pair = PAIRS ? it.d0 / 2 : -1;
     return it;
 }
 // The items of a thread
@@ -156,7 +155,7 @@ template <int V, bool PAIRS> __device__ __forceinline__ void rope_turn(const Rop
     if constexpr (PAIRS) {
         static_assert(V >= 2, "a pair is in one vector");
         auto one = [&](int pair, float (&x)[V]) {
-            if (pair < 0) return;
+            if (pair >= pairs) return;
             float2 f[W];
             factors(pair, f);
 #pragma unroll
@@ -167,11 +166,11 @@ template <int V, bool PAIRS> __device__ __forceinline__ void rope_turn(const Rop
                 x[2 * i + 1] = q * f[i].x + p * f[i].y;
             }
         };
-        one(it.pair0, a);
-        one(it.pair1, b);
-    } else if (it.pair0 >= 0) {
+        one(it.pair, a);
+        if (it.d1 >= 0) one(it.d1 / 2, b);
+    } else if (it.pair >= 0) {
         float2 f[W];
-        factors(it.pair0, f);
+        factors(it.pair, f);
 #pragma unroll
         for (int i = 0; i < V; i++) {
             const float p = a[i], q = b[i];

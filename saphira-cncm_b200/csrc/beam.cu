@@ -209,7 +209,8 @@ template <int MOST> struct JoinShared {
     double lse[NCMB_MAX_BEAMS], score[NCMB_MAX_BEAMS];
     int over[NCMB_MAX_BEAMS];
 };
-template <int MOST> __device__ __noinline__ void beam_join(const BeamArgs &a, int g, JoinShared<MOST> &sh) {
+// score, ended: of beam threadIdx.x, read when the kernel began
+template <int MOST> __device__ __noinline__ void beam_join(const BeamArgs &a, int g, float score, bool ended, JoinShared<MOST> &sh) {
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, n = a.n, slots = a.slots;
     const int64_t row0 = (int64_t)g * a.beams;
     const int lists = a.beams * a.parts, total = lists * slots;
@@ -223,13 +224,16 @@ template <int MOST> __device__ __noinline__ void beam_join(const BeamArgs &a, in
         }
     };
     load(0);                                                     // on their way while the sums meet
+    if (tid < a.beams) {
+        sh.score[tid] = score == score ? (double)score : -INFINITY;
+        sh.over[tid] = ended;
+    }
+    __syncthreads();
     for (int k = warp; k < a.beams; k += BM_WARPS) {
         const PartSum *s = a.sums + (row0 + k) * a.parts;
-        const bool ended = a.done && a.done[row0 + k];
-        const float sc = a.scores[row0 + k];
         float m = -INFINITY;
         double t = 0;
-        if (!ended) {
+        if (!sh.over[k]) {
 #pragma unroll 1
             for (int p = lane; p < a.parts; p += 32) {
                 const float4 x = __ldcg((const float4 *)(s + p));
@@ -245,11 +249,7 @@ template <int MOST> __device__ __noinline__ void beam_join(const BeamArgs &a, in
             for (int o = 1; o < min(32, a.parts); o <<= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
             m = top;
         }
-        if (lane == 0) {
-            sh.lse[k] = ended || m == -INFINITY ? 0.0 : m + bm_log(t);
-            sh.score[k] = sc == sc ? (double)sc : -INFINITY;
-            sh.over[k] = ended;
-        }
+        if (lane == 0) sh.lse[k] = m == -INFINITY ? 0.0 : m + bm_log(t);
     }
     sh.top.clear();
     unsigned long long least = 0;
@@ -344,6 +344,9 @@ __global__ void __launch_bounds__(BM_THREADS, BM_CTAS) k_beam_select(const __gri
     auto leave = [&](int i, unsigned long long key) {            // as slot i of the part, with its beam
         a.keys[((int64_t)g * a.slots + i) * lists + beam * a.parts + part] = key ? key | (unsigned long long)(NCMB_MAX_BEAMS - 1 - beam) << 24 : 0ull;
     };
+    const bool mine = tid < a.beams;
+    const float score = mine ? a.scores[(int64_t)g * a.beams + tid] : 0.f;       // for the join, should this CTA do it
+    const bool ended = mine && a.done && a.done[(int64_t)g * a.beams + tid];
     if (a.done && a.done[row]) {                                 // its end, then the other words, which have nothing
         for (int i = tid; i < a.slots; i += BM_THREADS)
             leave(i, part > 0 || i >= min(a.n, a.V) ? 0ull : i == 0 ? bm_key(0.f, a.eos) : bm_key(-INFINITY, i - 1 + (i - 1 >= a.eos)));
@@ -512,7 +515,7 @@ __global__ void __launch_bounds__(BM_THREADS, BM_CTAS) k_beam_select(const __gri
     if (!last) return;
     if (tid == 0) a.arrived[g] = 0;                              // for the next call
     __threadfence();
-    beam_join<MOST>(a, g, *(JoinShared<MOST> *)smem);
+    beam_join<MOST>(a, g, score, ended, *(JoinShared<MOST> *)smem);
 }
 
 template <class E, bool VEC, int MOST> void run_select_of(const BeamArgs &a, unsigned grid) {

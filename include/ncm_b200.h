@@ -560,7 +560,7 @@ int ncmb_paged_append(const NcmbPaged *c, const NcmbRope *r, const void *q, int6
                       const void *k, int64_t ldk, const void *v, int64_t ldv, int act_type, int n_tokens, const int *start, const int *pos);
 /* ncmb_cache_attention over a paged cache, without weights: T new tokens of every row, which already stand in slots len[b] ... len[b] + T - 1 (T = 1: a
  * decode step), attend to the row's tokens and to one another, all before them or by `parents`. max_len: an upper bound of the lengths that the
- * host knows, 0 = capacity. A query that sees nothing gets zeros. */
+ * host knows, 0 = capacity. A query that sees nothing gets zeros. out must not overlap q. */
 int ncmb_paged_attention(const NcmbPaged *c, const void *q, int64_t ldq, void *out, int64_t ldo, int act_type, int n_head, int T,
                          const int *parents, float scale, int max_len);
 /* The n_out best continuations of each group of beams. Row g * beams + k of the logits (fp32 or bf16, rows of ldl elements, V words) is beam k of group g,

@@ -98,7 +98,7 @@ __global__ void __launch_bounds__(PA_THREADS, V * sizeof(QE) == 16 ? 4 : 6) k_pa
         int seq = 0;
         const int len = row >= 0 ? a.c.len[row] : -1;
         if (len >= 0) {
-            const int64_t s = (int64_t)len + (a.start ? n - (near ? starts : a.start)[row] : n % a.T);
+            const int64_t s = len + (a.start ? (int64_t)n - (near ? starts : a.start)[row] : n % a.T);
             seq = (int)min(s, (int64_t)INT_MAX);
             const int page = s < (int64_t)a.c.max_pages << a.c.page_log ? paged_entry(a.c, row, (int)(s >> a.c.page_log)) : -1;
             to = page < 0 ? -1 : page * a.c.ps + (s & ((1 << a.c.page_log) - 1)) * a.c.ts;
@@ -139,7 +139,7 @@ __global__ void __launch_bounds__(PA_THREADS, V * sizeof(QE) == 16 ? 4 : 6) k_pa
 
 template <class QE, class KE, int V> void run_append(const NcmbRope *r, AppendArgs &a) {
     a.share = rope_share(r, rope_items(r, a.c.hd, V), a.H + 2 * a.c.nkv, PA_THREADS);
-    // four items a thread, and CTAs for all SMs (16 rows of up to 2001 tokens, 32 over 8 x 128 in bf16, 4 / 8 / 12 items a thread: 69 / 76 / 77 us)
+    // four items a thread (short vectors: more, which share the angles), and CTAs for all SMs (16 rows of up to 2001 tokens, 32 over 8 x 128 in bf16, 4 / 8 / 12 items a thread: 69 / 76 / 77 us)
     const int64_t per_token = (int64_t)(a.H + 2 * a.c.nkv) * a.share.items, rounds = V * sizeof(QE) == 16 ? 4 : 20;
     a.per = (int)std::max<int64_t>(1, std::min<int64_t>({PA_TOKENS, rounds * PA_THREADS / per_token, a.tokens / (4 * ctx().sm_count)}));
     const size_t smem = r ? (size_t)a.per * rope_row(r->dims) * sizeof(float2) : 0;

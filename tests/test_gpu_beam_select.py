@@ -196,3 +196,23 @@ def test_again_and_captured(cuda):
     finally:
         cuda.ncmb_set_stream(None)
     assert all(np.array_equal(a, o.cpu().numpy()) for a, o in zip(first, outs))
+
+
+@pytest.mark.parametrize("G,K,V", [(1, 1, 1 << 24), (2, 3, 3000001)])
+def test_the_largest_vocabularies(cuda, G, K, V):
+    """Against torch's sums and sorts in 64 bits; rows end inside a tile, and a row is split into as many parts as the GPU holds."""
+    g = torch.Generator(device="cuda").manual_seed(V)
+    x = torch.randn(G * K, V, device="cuda", generator=g)
+    scores = -torch.rand(G, K, device="cuda", generator=g)
+    n = 40
+    out = torch.empty(G, n, device="cuda"), *(torch.empty(G, n, dtype=torch.int32, device="cuda") for _ in range(2))
+    assert cuda.ncmb_beam_select(x.data_ptr(), V, capi.F32, G, K, V, scores.data_ptr(), None, -1, n, *(t.data_ptr() for t in out), None) == 0
+    words = x.sort(dim=1, descending=True, stable=True).indices[:, :n]
+    s = scores.double().view(-1, 1) + x.gather(1, words).double() - torch.logsumexp(x.double(), 1, keepdim=True)
+    want, at = s.view(G, K * n).sort(dim=1, descending=True, stable=True)
+    assert ((out[0].double() - want[:, :n]).abs() <= LSE * 20 + 2.0 ** -22).all()         # as many tiles a part as a row has, at most
+    far = torch.ones(G, n, dtype=torch.bool, device="cuda")                               # from the next: those may not change places
+    gap = (want[:, 1:n + 1] - want[:, :n]).abs() > 40 * LSE if K > 1 else torch.ones(G, n, dtype=torch.bool, device="cuda")
+    if K > 1:
+        far = gap & torch.cat([torch.ones_like(gap[:, :1]), gap[:, :-1]], 1)
+    assert (out[1].long() == at[:, :n] // n)[far].all() and (out[2].long() == words.reshape(G, K * n).gather(1, at[:, :n]))[far].all()

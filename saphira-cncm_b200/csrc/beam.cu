@@ -1,16 +1,20 @@
 // The best continuations of groups of beams over beams and vocabulary (ncmb_beam_select, include/ncm_b200.h).
 //
 // score(k, w) = s_k + x_kw - log sum_w exp x_kw, s_k the beam's score so far; the n best of a group, in order. One pass over the logits: a CTA has a
-// part of a row, in tiles of 16 values a thread; it keeps a running maximum and sum a thread and the part's n largest logits -- within a beam
+// part of a row, in tiles of 32 values a thread; it keeps a running maximum and sum a thread and the part's n largest logits -- within a beam
 // the order is that of its logits, so no more of them can be wanted. The last CTA of a group joins the parts.
 //
 // n largest: of the maxima of 2 n or more groups of threads the n-th largest is a bound that n values reach, and few values more; what
-// reaches it goes to a list in shared memory, as does what beats the bound in later tiles; a list that fills up is cut to its n largest, and the bound is
-// theirs. So a value costs a comparison, and few more. Keys are unique -- value, then lower index -- so equal values are no case of their own, and no order of arrival shows in the result. A bound is reached
-// by at most n groups, so a tile adds at most half of its values to the list, whatever the values are.
+// reaches it goes to a list in shared memory, as does what beats the bound in later tiles; a list that fills up is cut to its n largest, and the
+// bound is theirs. So a value costs a comparison, and few more. Keys are unique -- value, then lower index -- so equal values are no case of
+// their own, and no order of arrival shows in the result. However the values lie, a bound is reached by n groups at most, so a few values a thread
+// at a time always fit the list; tiles of which more beat an older bound than there is room for are gone through once more that way.
 //
-// Rounding: exponentials in fp32 against the thread's maximum, 16 of them summed in fp32, everything after in 64 bits; scores in 64 bits, so that
+// Rounding: exponentials in fp32 against the thread's maximum, 32 of them summed in fp32, everything after in 64 bits; scores in 64 bits, so that
 // their order does not depend on the rounding of a score near 100 (2^-18 in fp32). All rows of a call are split alike: equal rows have equal sums.
+//
+// Bound: with many rows by DRAM and instructions together -- 256 rows of 151936 in fp32: 37 us (4.2 TB/s), of which an SM that has two of them
+// streams 27 at 48 GB/s; in bf16 33, by instructions. With few by latency: 4 rows of 50257, 10 us, half of it the join.
 #include "cache.cuh"
 
 #include <algorithm>

@@ -1,7 +1,7 @@
 """The best continuations of groups of beams (ncmb_beam_select) against a plain selection in 64 bits.
 
-Bound of a score: an exponential is within 2^-22 of itself and its argument's rounding within 2^-23 (x 2^-d d <= 0.54 for the term's weight), 16 of them
-are added in fp32 (6 * 2^-24), the sum is scaled by the maximum's changes, each within 2^-22, at most one a tile of a part's (19 here)
+Bound of a score: an exponential is within 2^-22 of itself and its argument's rounding within 2^-23 (x 2^-d d <= 0.54 for the term's weight), 32 of them
+are added in fp32 (10 * 2^-24), the sum is scaled by the maximum's changes, each within 2^-22, at most one a tile after a part's first (18 here)
 and three where threads, warps and parts meet: log sum exp within 25 * 2^-22 = 6e-6, and half a unit of fp32. Two continuations of
 different beams that are nearer than twice that may change places (equal beams, whose sums are equal, may not)."""
 import numpy as np

@@ -52,10 +52,10 @@ __device__ __forceinline__ bool bm_there(const Wide &k) { return k.hi != 0; }
 __device__ __forceinline__ unsigned long long bm_xor(unsigned long long k, int o) { return __shfl_xor_sync(0xffffffffu, k, o); }
 __device__ __forceinline__ Wide bm_xor(const Wide &k, int o) { return Wide{__shfl_xor_sync(0xffffffffu, k.hi, o), __shfl_xor_sync(0xffffffffu, k.lo, o)}; }
 
-// The n-th largest of the maxima of 2 n groups of threads or more (of 2^widest threads at most); no key where fewer than n have one. One copy of the code for
+// The n-th largest of the maxima of 2 n groups of threads or more (of 8 threads at most); no key where fewer than n have one. One copy of the code for
 // whoever wants it: a part's first tile, lists that are cut, the join. Code that runs once is paced by instruction fetches.
-template <class K> __device__ __noinline__ K bm_nth(K best, int n, int widest, K *groups, K *bound) {
-    const int lg = min(widest, __clz(2 * n - 1) - 24), size = 1 << lg;           // BM_THREADS >> lg is 2 n or more
+template <class K> __device__ __noinline__ K bm_nth(K best, int n, K *groups, K *bound) {
+    const int lg = min(3, __clz(2 * n - 1) - 24), size = 1 << lg;           // BM_THREADS >> lg is 2 n or more
 #pragma unroll 1
     for (int o = 1; o < size; o <<= 1) { const K other = bm_xor(best, o); if (other > best) best = other; }
     const int tid = threadIdx.x, G = BM_THREADS >> lg, mine = tid >> lg;
@@ -76,8 +76,7 @@ template <class K> __device__ __noinline__ K bm_nth(K best, int n, int widest, K
 // The n largest keys of tiles of EPT a thread; n up to MOST, BM_FEW or NCMB_MAX_BEAMS: the fewer, the less room the lists take.
 // ROOM: keys that the list holds beside 2 n; 0: what a tile adds at most, once it has a bound.
 template <class K, int EPT, int MOST, int ROOM = 0> struct TopN {
-    static constexpr int WIDEST = MOST <= BM_FEW ? 2 : 3;        // threads of a group at most: 4, 8
-    static constexpr int REACH = MOST <= BM_FEW ? MOST << WIDEST : BM_THREADS / 2;        // threads whose groups reach a bound, at most: n groups of 2 n or more
+    static constexpr int REACH = BM_THREADS / 2;                 // threads whose groups reach a bound, at most: n groups of 2 n or more
     static constexpr int CAP = (ROOM ? ROOM : REACH * EPT) + 2 * MOST;
     static constexpr int PER = (CAP + BM_THREADS - 1) / BM_THREADS;
     K list[CAP], few[REACH * PER > BM_THREADS / 2 ? REACH * PER : BM_THREADS / 2], groups[BM_THREADS], bound;
@@ -87,7 +86,22 @@ template <class K, int EPT, int MOST, int ROOM = 0> struct TopN {
         if (threadIdx.x == 0) { count = 0; bound = K{}; }
         __syncthreads();
     }
-    __device__ K nth(K best, int n) { return bm_nth(best, n, WIDEST, groups, &bound); }
+    __device__ K nth(K best, int n) { return bm_nth(best, n, groups, &bound); }
+    // use(key, rank) for each of m keys
+    template <class USE> __device__ void ranks(const K *keys, int m, USE use) {
+        const int lg = m <= BM_THREADS / 8 ? 3 : m <= BM_THREADS / 4 ? 2 : m <= BM_THREADS / 2 ? 1 : 0, ways = 1 << lg, tid = threadIdx.x;      // threads that share a key's comparisons
+#pragma unroll 1
+        for (int i0 = 0; i0 < m; i0 += BM_THREADS >> lg) {
+            const int i = i0 + (tid >> lg);
+            const K mine = keys[min(i, m - 1)];
+            int rank = 0;
+#pragma unroll 4
+            for (int j = tid & (ways - 1); j < m; j += ways) rank += keys[j] > mine;
+#pragma unroll 1
+            for (int o = 1; o < ways; o <<= 1) rank += __shfl_xor_sync(0xffffffffu, rank, o);
+            if (i < m && (tid & (ways - 1)) == 0) use(mine, rank);
+        }
+    }
     // the list becomes its n largest, in order; returns the n-th, no key where there are fewer
     __device__ K settle(int n) {
         const int tid = threadIdx.x, c = count;
@@ -104,18 +118,7 @@ template <class K, int EPT, int MOST, int ROOM = 0> struct TopN {
         }
         __syncthreads();
         if (c > BM_THREADS / 2) m = n_few;
-        const int lg = m <= BM_THREADS / 8 ? 3 : m <= BM_THREADS / 4 ? 2 : m <= BM_THREADS / 2 ? 1 : 0, ways = 1 << lg;      // threads that share a key's comparisons
-#pragma unroll 1
-        for (int i0 = 0; i0 < m; i0 += BM_THREADS >> lg) {
-            const int i = i0 + (tid >> lg);
-            const K mine = few[min(i, m - 1)];
-            int rank = 0;
-#pragma unroll 4
-            for (int j = tid & (ways - 1); j < m; j += ways) rank += few[j] > mine;
-#pragma unroll 1
-            for (int o = 1; o < ways; o <<= 1) rank += __shfl_xor_sync(0xffffffffu, rank, o);
-            if (i < m && (tid & (ways - 1)) == 0 && rank < n) list[rank] = mine;
-        }
+        ranks(few, m, [&](const K &key, int rank) { if (rank < n) list[rank] = key; });
         if (tid == 0) count = min(n, m);
         __syncthreads();
         return m >= n ? list[n - 1] : K{};
@@ -273,7 +276,7 @@ template <int MOST> __device__ __noinline__ void beam_join(const BeamArgs &a, in
             unsigned long long most = 0;
 #pragma unroll
             for (int e = 0; e < BM_JOIN; e++) most = max(most, key[e].hi);
-            least = bm_nth(most, n, sh.top.WIDEST, (unsigned long long *)sh.top.groups, &sh.bound);
+            least = bm_nth(most, n, (unsigned long long *)sh.top.groups, &sh.bound);
         }
         bool full = false, any = false;
 #pragma unroll
@@ -291,16 +294,17 @@ template <int MOST> __device__ __noinline__ void beam_join(const BeamArgs &a, in
             least = max(least, nth.hi);
         }
     }
-    sh.top.settle(n);
-    for (int i = tid; i < n; i += BM_THREADS) {
-        const Wide x = sh.top.list[i];
+    // the n best to where their ranks say
+    if (sh.top.count > BM_THREADS / 2) sh.top.settle(n);
+    sh.top.ranks(sh.top.list, sh.top.count, [&](const Wide &x, int rank) {
+        if (rank >= n) return;
         const int k = NCMB_MAX_BEAMS - 1 - (int)(x.lo >> 56), w = 0xffffff - (int)(x.lo & 0xffffffu);
-        const int64_t at = (int64_t)g * n + i;
+        const int64_t at = (int64_t)g * n + rank;
         a.scores_out[at] = (float)bm_value(x.hi);
         a.parents[at] = k;
         a.tokens[at] = w;
         if (a.done_out) a.done_out[at] = sh.over[k] || w == a.eos;
-    }
+    });
 }
 
 // ---- CTA (row, part) ----
@@ -512,13 +516,15 @@ __global__ void __launch_bounds__(BM_THREADS, BM_CTAS) k_beam_select(const __gri
             a.sums[row * a.parts + part] = PartSum{s, top, 0.f};
         }
     }
-    __threadfence();
     __syncthreads();
-    if (tid == 0) last = atomicAdd(&a.arrived[g], 1) == a.beams * a.parts - 1;
+    if (tid == 0) {                                              // what the CTA wrote is there before its arrival counts, and what the others wrote is read after theirs
+        __threadfence();
+        last = atomicAdd(&a.arrived[g], 1) == a.beams * a.parts - 1;
+        __threadfence();
+        if (last) a.arrived[g] = 0;                              // for the next call
+    }
     __syncthreads();
     if (!last) return;
-    if (tid == 0) a.arrived[g] = 0;                              // for the next call
-    __threadfence();
     beam_join<MOST>(a, g, score, ended, *(JoinShared<MOST> *)smem);
 }
 

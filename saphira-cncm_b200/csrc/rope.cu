@@ -29,7 +29,7 @@ struct RopeArgs {
 // A CTA has `per` tokens: their places in memory and their angles once, in shared memory, then all items of their heads, RO_BATCH of a thread on their way at a
 // time, the first of them while the angles are formed. Bound by DRAM: 8 x 4000 tokens of 40 heads of 128 in bf16, 655 MB: 100 us (6.5 TB/s).
 template <class E, int V, bool PAIRS>
-__global__ void __launch_bounds__(RO_THREADS, V * sizeof(E) == 16 ? 4 : 6) k_rope(const __grid_constant__ NcmbRope r, const __grid_constant__ RopeArgs a) {
+__global__ void __launch_bounds__(RO_THREADS, 4) k_rope(const __grid_constant__ NcmbRope r, const __grid_constant__ RopeArgs a) {
     extern __shared__ __align__(16) float2 cs[];         // [per][rope_row(dims)]
     __shared__ int64_t xo[RO_TOKENS], yo[RO_TOKENS];
     __shared__ int place[RO_TOKENS];
@@ -79,16 +79,103 @@ __global__ void __launch_bounds__(RO_THREADS, V * sizeof(E) == 16 ? 4 : 6) k_rop
     }
 }
 
-template <class E, int V> void run_rope(const NcmbRope &r, RopeArgs &a) {
-    a.share = rope_share(&r, rope_items(&r, a.hd, V), a.n_head, RO_THREADS);
-    // A thread's items all on their way at once, and CTAs for all SMs (8 x 4000 tokens of 40 x 128 in bf16, 4 / 8 / 20 items a thread: 100 / 107 / 115 us);
-    // short vectors are paced by instructions, so there the angles are shared by more (dims 50 of it, halves, 4 / 20 items: 293 / 277).
-    const int64_t per_token = (int64_t)a.n_head * a.share.items, rounds = V * sizeof(E) == 16 ? RO_BATCH : 20;
-    a.per = (int)std::max<int64_t>(1, std::min<int64_t>({RO_TOKENS, rounds * RO_THREADS / per_token, a.tokens / (4 * ctx().sm_count)}));
+// Halves that are no whole vectors: an element's partner stands somewhere inside two vectors. The CTA's heads go through shared memory as they are; a
+// thread takes the vector that it loaded, cuts its partners out of the two vectors that hold them -- at the same offset for all threads -- and writes
+// 16 bytes. Cosines stand with every VE-th pair side by side, so that threads side by side read side by side.
+// Bound by instructions: dims 50 of 8 x 4000 x 40 heads of 128 in bf16 183 us (an element at a time 269), dims 6 of 4 x 2000 in fp32 68 (84).
+template <class E>
+__global__ void __launch_bounds__(RO_THREADS, 4) k_rope_any(const __grid_constant__ NcmbRope r, const __grid_constant__ RopeArgs a) {
+    constexpr int VE = 16 / sizeof(E), LOG = sizeof(E) == 4 ? 2 : 3;
+    extern __shared__ __align__(16) char smem[];
+    __shared__ int64_t xo[RO_TOKENS], yo[RO_TOKENS];
+    __shared__ int place[RO_TOKENS];
+    const int tid = threadIdx.x, half = r.dims / 2, row = rope_row(r.dims), stride = (half + VE - 1) >> LOG;
+    uint4 *stage = (uint4 *)smem;                // [token][head][vector], and one more
+    float2 *cs = (float2 *)(stage + a.per * a.share.heads * a.share.items + 1);
+    const uint32_t n0 = blockIdx.x * (uint32_t)a.per;
+    const int here = (int)min((uint32_t)a.per, a.tokens - n0), h0 = blockIdx.y * a.share.heads, heads = min(a.share.heads, a.n_head - h0);
+    RopeWalk at(tid, a.share);
+    pdl_wait();
+    pdl_launch_dependents();
+    if (tid < here) {
+        const uint32_t n = n0 + tid, b = n / a.T, t = n - b * a.T;
+        xo[tid] = b * a.xs[0] + t * a.xs[1] + h0 * a.xs[2];
+        yo[tid] = b * a.ys[0] + t * a.ys[1] + h0 * a.ys[2];
+        place[tid] = a.pos ? a.pos[n] : (int)t;
+    }
+    __syncthreads();
+    const RopeWalk from = at;
+    for (; at.tok < here; at.next(a.share)) {
+        if (at.h >= heads) continue;
+        const uint32_t to = (uint32_t)__cvta_generic_to_shared(stage + (at.tok * a.share.heads + at.h) * a.share.items + at.u);
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(a.x + xo[at.tok] + at.h * a.xs[2] + at.u * 16) : "memory");
+    }
+    rope_angles(tid, here, a.share, [&](int t, int i) { cs[t * row + (i & (VE - 1)) * stride + (i >> LOG)] = rope_angle(r, i, place[t], a.inverse); });
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    __syncthreads();
+    // what a thread's vector needs is the same for all of its heads: where its elements' cosines stand, the sign of their sines, its partners' vectors
+    const int d0 = from.u * VE;
+    const bool low = d0 < half, high = d0 + VE > half && d0 < r.dims;
+    int at_cs[VE];
+    uint32_t first = 0, turns = 0;               // bits: elements of the first half, those that turn
+#pragma unroll
+    for (int e = 0; e < VE; e++) {
+        const int d = d0 + e, i = d < half ? d : d - half;
+        if (d < half) first |= 1u << e;
+        if (d < r.dims) turns |= 1u << e;
+        at_cs[e] = d < r.dims ? (i & (VE - 1)) * stride + (i >> LOG) : 0;
+    }
+    // elements s ... s + VE - 1 of a head (those outside it are not used)
+    auto cut = [&](const uint4 *head, int s, float (&y)[VE]) {
+        const int v = s >> LOG, o = s & (VE - 1), w0 = sizeof(E) == 4 ? o : o >> 1;
+        const uint4 l = head[max(v, 0)], h = head[v + 1];
+        const uint32_t w[8] = {l.x, l.y, l.z, l.w, h.x, h.y, h.z, h.w};
+        uint32_t c[5];
+#pragma unroll
+        for (int i = 0; i < 5; i++) {
+            const uint32_t even = w0 & 2 ? w[i + 2] : w[i], odd = w0 & 2 ? w[min(i + 3, 7)] : w[i + 1];
+            c[i] = w0 & 1 ? odd : even;
+        }
+        if (sizeof(E) == 2) {
+#pragma unroll
+            for (int i = 0; i < 4; i++) c[i] = __funnelshift_r(c[i], c[i + 1], (o & 1) * 16);
+        }
+        rope_unpack<E, VE>(make_uint4(c[0], c[1], c[2], c[3]), y);
+    };
+#pragma unroll 2
+    for (at = from; at.tok < here; at.next(a.share)) {
+        if (at.h >= heads) continue;
+        const uint4 *head = stage + (at.tok * a.share.heads + at.h) * a.share.items;
+        const float2 *f = cs + at.tok * row;
+        float x[VE];
+        rope_unpack<E, VE>(head[at.u], x);
+        if (turns) {
+            float p[VE], q[VE];
+            if (low) cut(head, d0 + half, p);
+            if (high) cut(head, d0 - half, q);
+#pragma unroll
+            for (int e = 0; e < VE; e++) {
+                const float2 c = f[at_cs[e]];
+                const float y = x[e] * c.x + (first >> e & 1 ? -p[e] : q[e]) * c.y;
+                if (turns >> e & 1) x[e] = y;
+            }
+        }
+        rope_store<E, VE>((E *)(a.y + yo[at.tok] + at.h * a.ys[2]) + d0, x);
+    }
+}
+
+template <class E> void run_rope(const NcmbRope &r, RopeArgs &a) {
+    constexpr int V = 16 / sizeof(E);
+    const bool any = rope_vec(&r, sizeof(E)) < V;
+    // a thread's items all on their way at once, and CTAs for all SMs (8 x 4000 tokens of 40 x 128 in bf16, 4 / 8 / 20 items a thread: 100 / 107 / 115 us)
+    const int items = any ? (int)cdiv(a.hd, V) : rope_items(&r, a.hd, V), held = (any ? 2 * RO_BATCH : RO_BATCH) * (RO_THREADS / items), heads = any ? std::min(a.n_head, held) : a.n_head;
+    a.share = rope_share(&r, items, heads, RO_THREADS);
+    a.per = (int)std::max<int64_t>(1, std::min<int64_t>({any ? RO_TOKENS / 2 : RO_TOKENS, held / heads, a.tokens / (4 * ctx().sm_count)}));
     const size_t smem = (size_t)a.per * rope_row(r.dims) * sizeof(float2);
     const unsigned grid = (unsigned)cdiv(a.tokens, a.per);
-    if (r.layout == NCMB_ROPE_HALVES) LAUNCH_PDL((k_rope<E, V, false>), grid, RO_THREADS, smem, r, a);
-    else if constexpr (V * sizeof(E) == 16) LAUNCH_PDL((k_rope<E, V, true>), grid, RO_THREADS, smem, r, a);
+    if (any) LAUNCH_PDL((k_rope_any<E>), dim3(grid, (unsigned)cdiv(a.n_head, heads)), RO_THREADS, smem + ((size_t)a.per * heads * items + 1) * 16, r, a);
+    else if (r.layout == NCMB_ROPE_HALVES) LAUNCH_PDL((k_rope<E, V, false>), grid, RO_THREADS, smem, r, a);
+    else LAUNCH_PDL((k_rope<E, V, true>), grid, RO_THREADS, smem, r, a);
 }
 
 } // namespace
@@ -145,13 +232,9 @@ extern "C" int ncmb_rope(const NcmbRope *r, const void *x, const int64_t *xs, vo
         a.ys[i] = ys[i] * es;
     }
     if (cache_device(who)) return -1;
-    a.x = (const char *)x; a.y = (char *)y; a.pos = pos; a.tokens = (uint32_t)tokens; a.T = T; a.n_head = n_head; a.hd = x == y ? (r->layout == NCMB_ROPE_PAIRS ? std::min(hd, (r->dims + 7) & ~7) : r->dims) : hd; a.inverse = inverse != 0;
+    a.x = (const char *)x; a.y = (char *)y; a.pos = pos; a.tokens = (uint32_t)tokens; a.T = T; a.n_head = n_head; a.hd = x == y ? (r->dims + 7) & ~7 : hd; a.inverse = inverse != 0;
     ProfScope prof(NCMB_K_ELEM, 3.0 * tokens * n_head * hd, 2.0 * tokens * n_head * hd * es);
-    switch (rope_vec(r, (int)es)) {
-        case 8: run_rope<__nv_bfloat16, 8>(*r, a); break;
-        case 4: if (es == 2) run_rope<__nv_bfloat16, 4>(*r, a); else run_rope<float, 4>(*r, a); break;
-        case 2: if (es == 2) run_rope<__nv_bfloat16, 2>(*r, a); else run_rope<float, 2>(*r, a); break;
-        default: if (es == 2) run_rope<__nv_bfloat16, 1>(*r, a); else run_rope<float, 1>(*r, a); break;
-    }
+    if (es == 2) run_rope<__nv_bfloat16>(*r, a);
+    else run_rope<float>(*r, a);
     return 0;
 }

@@ -74,7 +74,10 @@ __device__ __forceinline__ void ct_tma(uint32_t dst, const CUtensorMap *m, int d
 }
 __device__ __forceinline__ void ct_fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
-template <class KE, class QE, int HDP>
+// PAGED: keys through the row's table. Whole tiles of a bf16 cache come by TMA from a map of the pool, a box a page (or the part of one that a tile holds);
+// tiles that end inside, or in which an entry is no page, by cp.async, and all of an fp32 cache's through registers, an entry a key. The warps of the
+// softmax look at the entries themselves: which keys are not there.
+template <class KE, class QE, int HDP, bool PAGED = false>
 __global__ void __launch_bounds__(CtCfg<KE, QE, HDP>::THREADS, 1) k_cache_attention_tc(const __grid_constant__ CmArgs a, const __grid_constant__ CUtensorMap mk,
                                                                                         const __grid_constant__ CUtensorMap mv, int *err) {
     using F = CtCfg<KE, QE, HDP>;
@@ -156,6 +159,15 @@ __global__ void __launch_bounds__(CtCfg<KE, QE, HDP>::THREADS, 1) k_cache_attent
     };
     Unit u;
     uint32_t it = 0, un = 0, items = 0;                              // tiles, units, stages (two a tile) so far
+    const int piece_log = PAGED ? min(a.page_log, 7) : 7, pieces = KT >> piece_log;      // of a tile: keys that stand in one page
+    // paged: the entry of the page that holds the row's slot pos, -1 where it is none
+    auto entry = [&](int pos) {
+        const int i = pos >> a.page_log;
+        const int e = i < a.max_pages && a.c.len[u.row] >= 0 ? __ldg(a.table + u.row * a.table_stride + i) : -1;
+        return (unsigned)e < (unsigned)a.n_pages ? e : -1;
+    };
+    auto entries = [&](int t) { return lane < pieces ? entry(t * KT + (lane << piece_log)) : -1; };      // a lane one of tile t's
+    auto missing = [&](int e) { return ~__ballot_sync(0xffffffffu, e >= 0) & ((1u << pieces) - 1); };
 
     if (warp < F::SW) {
         // ================= softmax: row r of the tile, keys 64 hf ... of a key tile, half hf of the dims =================
@@ -239,12 +251,18 @@ __global__ void __launch_bounds__(CtCfg<KE, QE, HDP>::THREADS, 1) k_cache_attent
                     for (int d = 0; d < 32; d++) O[x + d] = fmaf(O[x + d], al_prev, __uint_as_float(o[d]));
                 }
             };
+            int ahead = PAGED ? entries(u.first) : 0;
             for (int t = u.first; t < u.stop; t++, it++) {
+                uint32_t none = 0;                                   // paged: pieces of the tile that no page holds
+                if constexpr (PAGED) {
+                    none = missing(ahead);
+                    ahead = t + 1 < u.stop ? entries(t + 1) : -1;
+                }
                 const uint32_t sb = F::NSB == 2 ? it & 1u : 0u, scol = tl + (uint32_t)F::SCOL + sb * 128u + (uint32_t)hf * 64u;
                 wait(bar_s + 8 * sb, F::NSB == 2 ? (it >> 1) & 1u : it & 1u, 42);
                 tc_fence_after();
                 const int p0 = t * KT + 64 * hf;
-                const bool masked = (t + 1) * KT > u.len;
+                const bool masked = (t + 1) * KT > u.len || none;
                 auto sees = [&](int from) {                          // bit j: the row sees slot from + j
                     uint32_t see = 0xffffffffu;
                     const int rel = from - u.len;                    // node of the first slot
@@ -257,6 +275,10 @@ __global__ void __launch_bounds__(CtCfg<KE, QE, HDP>::THREADS, 1) k_cache_attent
                         see = __funnelshift_r(lo, hi, rel & 31);
                     }
                     if (u.n - from < 32) see &= u.n > from ? (1u << (u.n - from)) - 1 : 0u;
+                    if (PAGED && none) {
+#pragma unroll
+                        for (int x = 0; x < 32; x += 8) if ((none >> ((from - t * KT + x) >> piece_log)) & 1u) see &= ~(0xffu << x);
+                    }
                     return see;
                 };
                 // the maximum, then -- the scores are read again rather than kept: registers -- exponentials
@@ -504,9 +526,13 @@ __global__ void __launch_bounds__(CtCfg<KE, QE, HDP>::THREADS, 1) k_cache_attent
                 }
                 __syncwarp();
             }
-            auto there = [&](int pos) { return pos < u.n && (pos < u.len || ((bits[(pos - u.len) >> 5] >> ((pos - u.len) & 31)) & 1u)); };
+            auto there = [&](int pos) { return pos < u.n && (!PAGED || entry(pos) >= 0) && (pos < u.len || ((bits[(pos - u.len) >> 5] >> ((pos - u.len) & 31)) & 1u)); };
             // stage s of the unit: keys of tile 0, then in turn keys of the next tile and values of this one
             const int count = 2 * (u.stop - u.first);
+            auto place = [&](int pos) -> int64_t {                   // of a key that is there, in bytes
+                if constexpr (PAGED) return entry(pos) * a.ps + (pos & ((1 << a.page_log) - 1)) * a.c.ts;
+                else return pos * a.c.ts;
+            };
             auto tile_of = [&](int s) { return s == 0 ? 0 : s == count - 1 ? (s - 1) / 2 : (s & 1) ? (s + 1) / 2 : (s - 2) / 2; };
             auto is_v = [&](int s) { return s == count - 1 || (s > 0 && !(s & 1)); };
             constexpr int UPR = HDP / 8, RPI = NT / UPR;             // units of 8 dims of a key, keys a step
@@ -518,11 +544,19 @@ __global__ void __launch_bounds__(CtCfg<KE, QE, HDP>::THREADS, 1) k_cache_attent
 #pragma unroll 1
                 for (int s = 0; s < count; s++, it++) {
                     const uint32_t st = it % NST;
+                    const int t = u.first + tile_of(s), e = PAGED ? entries(t) : 0;
                     wait(empty(st), ((it / NST) & 1u) ^ 1u, 47);
                     if ((gone = __any_sync(0xffffffffu, wait.dead))) break;
-                    const int t = u.first + tile_of(s);
                     const uint32_t to = cm_smem(ring + st * F::STAGE);
-                    if ((t + 1) * KT <= u.len) {
+                    if (PAGED && (t + 1) * KT <= u.len && !missing(e)) {
+                        if (lane == 0) { if (warp == F::SW + 1) mbar_expect_tx(full(st), (uint32_t)F::STAGE); else mbar_arrive(full(st)); }
+                        __syncwarp();
+                        if (warp == F::SW + 1 && lane < pieces)
+                            for (int x = 0; x < ATOMS; x++)
+                                ct_tma(to + x * F::KATOM + (lane << piece_log) * 128, is_v(s) ? &mv : &mk, 64 * x, (t * KT + (lane << piece_log)) & ((1 << a.page_log) - 1), u.kvh, e, full(st));
+                        continue;
+                    }
+                    if (!PAGED && (t + 1) * KT <= u.len) {
                         if (pt == 0) {
                             mbar_expect_tx(full(st), (uint32_t)F::STAGE);
                             for (int x = 0; x < ATOMS; x++) ct_tma(to + x * F::KATOM, is_v(s) ? &mv : &mk, 64 * x, t * KT, u.kvh, u.row, full(st));
@@ -535,7 +569,7 @@ __global__ void __launch_bounds__(CtCfg<KE, QE, HDP>::THREADS, 1) k_cache_attent
                     for (int r = lr; r < KT; r += RPI) {
                         const int pos = t * KT + r;
                         const bool ok = in && there(pos);
-                        cm_cp16(mine + r * 128 + (((lu & 7) ^ (r & 7)) * 16), ok ? from + pos * a.c.ts : kb, ok);
+                        cm_cp16(mine + r * 128 + (((lu & 7) ^ (r & 7)) * 16), ok ? from + place(pos) : kb, ok);
                     }
                     asm volatile("cp.async.wait_all;" ::: "memory");
                     ct_fence_async();
@@ -557,10 +591,11 @@ __global__ void __launch_bounds__(CtCfg<KE, QE, HDP>::THREADS, 1) k_cache_attent
 #pragma unroll
                         for (int i = 0; i < N2; i++) {
                             const int rr = lr + i * RPI, pos = (u.first + t) * KT + r0 + rr;
-                            const bool ok = in && rr < KT / 2 && (tail ? there(pos) : true);
+                            const bool ok = in && rr < KT / 2 && (tail || PAGED ? there(pos) : true);
                             const float4 z = make_float4(0.f, 0.f, 0.f, 0.f);
-                            x[2 * i] = ok ? *(const float4 *)(from + pos * a.c.ts) : z;
-                            x[2 * i + 1] = ok ? *(const float4 *)(from + pos * a.c.ts + 16) : z;
+                            const char *at = from + (ok ? place(pos) : 0);
+                            x[2 * i] = ok ? *(const float4 *)at : z;
+                            x[2 * i + 1] = ok ? *(const float4 *)(at + 16) : z;
                         }
                         if (r0 == 0) wait(empty(st), ((s / NST) & 1u) ^ 1u, 47);
 #pragma unroll
@@ -609,19 +644,23 @@ __global__ void __launch_bounds__(CtCfg<KE, QE, HDP>::THREADS, 1) k_cache_attent
     }
 }
 
-// a bf16 cache's keys or values as [row][head][slot][dim], boxes of 64 dims by kt slots (cache_attention.cu)
+// A bf16 cache's keys or values as [rows][head][slots][dim], boxes of 64 dims by kt slots (cache_attention.cu). Of a pool of pages: rows and slots are
+// pages and their slots.
 int ct_map(const char *who, const CacheDev &c, const char *p, int kt, CUtensorMap &m);
 
-template <class KE, class QE, int HDP>
+template <class KE, class QE, int HDP, bool PAGED = false>
 int ct_run_as(const char *who, CmArgs a, int max_keys) {
     using F = CtCfg<KE, QE, HDP>;
     using J = CmCfg<KE, QE, HDP, F::M>;
     a.tiles = (int)cdiv(a.M, F::M);
     CUtensorMap mk = {}, mv = {};
-    if (F::BF && (ct_map(who, a.c, a.c.k, F::KT, mk) || ct_map(who, a.c, a.c.v, F::KT, mv))) return -1;
+    CacheDev box = a.c;
+    if (PAGED) { box.rows = a.n_pages; box.cap = 1 << a.page_log; box.rs = a.ps; }
+    const int high = PAGED ? std::min(F::KT, box.cap) : F::KT;
+    if (F::BF && (ct_map(who, box, a.c.k, high, mk) || ct_map(who, box, a.c.v, high, mv))) return -1;
     static bool set = false;
     if (!set) {
-        CUDA_CHECK(cudaFuncSetAttribute(k_cache_attention_tc<KE, QE, HDP>, cudaFuncAttributeMaxDynamicSharedMemorySize, F::SMEM));
+        CUDA_CHECK(cudaFuncSetAttribute(k_cache_attention_tc<KE, QE, HDP, PAGED>, cudaFuncAttributeMaxDynamicSharedMemorySize, F::SMEM));
         set = true;
     }
     const int rows = a.c.rows;
@@ -643,11 +682,35 @@ int ct_run_as(const char *who, CmArgs a, int max_keys) {
         const int nr = std::min(step, rows - r);
         a.row0 = r;
         a.items = nr;
-        LAUNCH_PDL((k_cache_attention_tc<KE, QE, HDP>), ctas, F::THREADS, F::SMEM, a, mk, mv, tc_err_flag());
+        LAUNCH_PDL((k_cache_attention_tc<KE, QE, HDP, PAGED>), ctas, F::THREADS, F::SMEM, a, mk, mv, tc_err_flag());
         const int64_t joins = nr * row_units * (F::M / (split ? 1 : CM_THREADS / (HDP / 4)));
-        LAUNCH_PDL((k_cache_join<KE, QE, HDP, F::M, false>), (unsigned)(joins + spans / step * nr), CM_THREADS, 0, a, (int)joins, split, cm_wkeys(a.M));
+        LAUNCH_PDL((k_cache_join<KE, QE, HDP, F::M, false, PAGED>), (unsigned)(joins + spans / step * nr), CM_THREADS, 0, a, (int)joins, split, cm_wkeys(a.M));
     }
     return 0;
+}
+
+extern int cache_variant;            // ncmb_set_cache_variant
+// Which tiles: 16 (8) query rows on mma.sync, keys straight from a warp's ring, or 128 rows on tcgen05. By the times that a sweep
+// over 1 - 64 rows of 500 - 30000 tokens, 3 - 64 new tokens and 33 - 448 query rows a kv head gave, in us:
+//   narrow  8 + tiles of 16 rows x (NARROW x keys + 0.013)
+//   wide   14 + WIDE x tiles of 128 rows x (tiles of 128 keys + START), over the SMs
+// e.g. bf16 cache, fp32 queries, 2 x 64, narrow against wide: 1 x 4000 x 112 rows 11 / 17, 16 x 4000 x 56 rows 34 / 38,
+// x 448 rows 153 / 105; 8 x 128: 1 x 500 x 64 rows 11.4 / 24, 16 x 4000 x 64 rows 181 / 148, x 256 rows 667 / 278.
+template <class KE, class QE, int HDP> struct CtCost {
+    static constexpr bool Q32 = sizeof(QE) == 4;
+    static constexpr double NARROW = sizeof(KE) == 4 ? 111e-6 : HDP == 64 ? (Q32 ? 42e-6 : 30e-6) : (Q32 ? 90e-6 : 71e-6);
+    static constexpr double WIDE = sizeof(KE) == 4 ? 4.7 : HDP == 64 ? (Q32 ? 2.9 : 2.05) : (Q32 ? 4.3 : 2.3);
+};
+template <class KE, class QE, int HDP>
+bool takes_wide(const CmArgs &a, int max_keys) {
+    using F = CtCfg<KE, QE, HDP>;
+    using C = CtCost<KE, QE, HDP>;
+    if (a.M <= 16 || cache_variant == 1 || a.M > CT_MOST_ROWS) return false;
+    if (cache_variant == 2) return true;
+    const double heads = (double)a.c.rows * a.c.nkv;
+    const double narrow = 8 + heads * cdiv(a.M, 16) * (C::NARROW * max_keys + 0.013);
+    const double wide = 14 + C::WIDE * ceil(heads * cdiv(a.M, F::M) * (cdiv(max_keys, F::KT) + F::START) / ctx().sm_count);
+    return wide < narrow;
 }
 
 } // namespace ncmb

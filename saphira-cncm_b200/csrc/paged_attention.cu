@@ -1,16 +1,21 @@
 // Attention of a row's new tokens -- a decode step's one, a run, or a tree of drafted ones -- to its pages (ncmb_paged_attention,
-// include/ncm_b200.h): the narrow tiles of cache_mma.cuh with keys and values found through the row's table.
-#include "cache_mma.cuh"
+// include/ncm_b200.h): the tiles of cache_mma.cuh, or of cache_tc.cuh for many query rows, with keys and values found through the row's table.
+#include "cache_tc.cuh"
 #include "paged.cuh"
 
 namespace ncmb {
 namespace {
 
+template <class KE, class QE, int HDP>
+int run_paged_hd(const char *who, const CmArgs &a, int max_keys) {
+    // (as for ncmb_cache_attention: no wide tiles for fp32 caches of more than 64 dims)
+    if constexpr (sizeof(KE) == 2 || HDP == 64) { if (takes_wide<KE, QE, HDP>(a, max_keys)) return ct_run_as<KE, QE, HDP, true>(who, a, max_keys); }
+    auto none = [] {};
+    return a.M <= 8 ? cm_run_as<KE, QE, HDP, 8, false, true>(who, a, max_keys, none) : cm_run_as<KE, QE, HDP, 16, false, true>(who, a, max_keys, none);
+}
 template <class KE, class QE>
 int run_paged(const char *who, const CmArgs &a, int max_keys) {
-    auto none = [] {};
-    if (a.c.hd <= 64) return a.M <= 8 ? cm_run_as<KE, QE, 64, 8, false, true>(who, a, max_keys, none) : cm_run_as<KE, QE, 64, 16, false, true>(who, a, max_keys, none);
-    return a.M <= 8 ? cm_run_as<KE, QE, 128, 8, false, true>(who, a, max_keys, none) : cm_run_as<KE, QE, 128, 16, false, true>(who, a, max_keys, none);
+    return a.c.hd <= 64 ? run_paged_hd<KE, QE, 64>(who, a, max_keys) : run_paged_hd<KE, QE, 128>(who, a, max_keys);
 }
 
 } // namespace

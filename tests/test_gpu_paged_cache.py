@@ -350,3 +350,37 @@ def test_reorder(cuda, dt, layout, groups, group, page, layers, kind):
         assert np.array_equal(d.cpu().numpy(), table)
         if kind == "bad":
             break                                               # rows of other lengths may begin on one another's pages
+
+
+# ------------------------------------------------------------------------------------------- attention of many query rows
+
+@pytest.fixture(params=[1, 2])
+def variant(request, cuda):
+    """Tiles of 16 rows, and of 128 where they take the shape."""
+    cuda.ncmb_set_cache_variant(request.param)
+    yield request.param
+    cuda.ncmb_set_cache_variant(0)
+    assert cuda.ncmb_gemm_tc_check() == 0
+
+
+@pytest.mark.parametrize("kt,qt", TYPES)
+@pytest.mark.parametrize("page", [8, 16, 32, 64, 128, 256, 1024])
+@pytest.mark.parametrize("H,nkv,hd,T,tree", [(8, 2, 64, 9, True), (8, 1, 64, 5, False), (4, 2, 128, 20, True), (6, 2, 72, 40, False)])
+def test_many_query_rows(cuda, variant, kt, qt, page, H, nkv, hd, T, tree):
+    run_attention(cuda, page + T, [0, 1, 127 - T, 128, 129, 700], T, H, nkv, hd, kt, qt, ["token", "head", "gap"][(page + T) % 3], page, tree)
+
+
+@pytest.mark.parametrize("kt,qt", TYPES)
+@pytest.mark.parametrize("page", [8, 32, 256])
+def test_many_query_rows_without_pages(cuda, variant, kt, qt, page):
+    """Entries that are no page in whole tiles, in the last one and at the new tokens; rows of no sequence."""
+    run_attention(cuda, 3, [600, -1, 513, 0, 128, -2 ** 31], 18, 4, 2, 64, kt, qt, "token", page, tree=True,
+                  holes=[(0, 1, -1), (0, 600 // page, 2 ** 31 - 1), (2, 0, 10 ** 6), (2, 300 // page, -3), (3, 0, -5), (4, 0, -1)])
+    run_attention(cuda, 4, [300, 40], 30, 2, 1, 64, kt, qt, "head", page, holes=[(1, 0, -1), (1, 40 // page, -2), (0, 0, -1)])
+
+
+@pytest.mark.parametrize("kt,qt", TYPES)
+@pytest.mark.parametrize("B,n,T,H,nkv,hd,page", [(1, 9000, 16, 32, 8, 64, 16), (7, 2500, 64, 8, 2, 128, 64), (40, 300, 7, 14, 2, 64, 8), (2, 1500, 256, 4, 2, 64, 32)])
+def test_many_query_rows_of_long_rows(cuda, variant, kt, qt, B, n, T, H, nkv, hd, page):
+    """Units cut over CTAs, query rows in several tiles."""
+    run_attention(cuda, B + T, [n] + [(b * 7919) % n for b in range(1, B)], T, H, nkv, hd, kt, qt, "head" if T % 3 else "token", page)

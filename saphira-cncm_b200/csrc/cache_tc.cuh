@@ -526,11 +526,11 @@ __global__ void __launch_bounds__(CtCfg<KE, QE, HDP>::THREADS, 1) k_cache_attent
                 }
                 __syncwarp();
             }
-            auto there = [&](int pos) { return pos < u.n && (!PAGED || entry(pos) >= 0) && (pos < u.len || ((bits[(pos - u.len) >> 5] >> ((pos - u.len) & 31)) & 1u)); };
+            auto there = [&](int pos) { return pos < u.n && (pos < u.len || ((bits[(pos - u.len) >> 5] >> ((pos - u.len) & 31)) & 1u)); };
             // stage s of the unit: keys of tile 0, then in turn keys of the next tile and values of this one
             const int count = 2 * (u.stop - u.first);
-            auto place = [&](int pos) -> int64_t {                   // of a key that is there, in bytes
-                if constexpr (PAGED) return entry(pos) * a.ps + (pos & ((1 << a.page_log) - 1)) * a.c.ts;
+            auto place = [&](int pos, int e) -> int64_t {            // of a key, in bytes; paged: its entry
+                if constexpr (PAGED) return e * a.ps + (pos & ((1 << a.page_log) - 1)) * a.c.ts;
                 else return pos * a.c.ts;
             };
             auto tile_of = [&](int s) { return s == 0 ? 0 : s == count - 1 ? (s - 1) / 2 : (s & 1) ? (s + 1) / 2 : (s - 2) / 2; };
@@ -568,8 +568,9 @@ __global__ void __launch_bounds__(CtCfg<KE, QE, HDP>::THREADS, 1) k_cache_attent
 #pragma unroll 4
                     for (int r = lr; r < KT; r += RPI) {
                         const int pos = t * KT + r;
-                        const bool ok = in && there(pos);
-                        cm_cp16(mine + r * 128 + (((lu & 7) ^ (r & 7)) * 16), ok ? from + place(pos) : kb, ok);
+                        const int in_page = PAGED ? entry(pos) : 0;
+                        const bool ok = in && there(pos) && in_page >= 0;
+                        cm_cp16(mine + r * 128 + (((lu & 7) ^ (r & 7)) * 16), ok ? from + place(pos, in_page) : kb, ok);
                     }
                     asm volatile("cp.async.wait_all;" ::: "memory");
                     ct_fence_async();
@@ -579,8 +580,11 @@ __global__ void __launch_bounds__(CtCfg<KE, QE, HDP>::THREADS, 1) k_cache_attent
             } else {
                 const char *from = (grp ? vb : kb) + lu * 32;
                 const int tiles = u.stop - u.first;
+                int ahead = PAGED ? entries(u.first) : 0;
 #pragma unroll 1
                 for (int t = 0; t < tiles; t++) {
+                    const int e = ahead;
+                    if (PAGED && t + 1 < tiles) ahead = entries(u.first + t + 1);
                     const uint32_t s = it + (grp ? (t + 1 < tiles ? 2 + 2 * t : 2 * tiles - 1) : t ? 2 * t - 1 : 0), st = s % NST;
                     char *to = ring + st * F::STAGE + (lu / 8) * F::KATOM;
                     const bool tail = (u.first + t + 1) * KT > u.len;
@@ -591,9 +595,10 @@ __global__ void __launch_bounds__(CtCfg<KE, QE, HDP>::THREADS, 1) k_cache_attent
 #pragma unroll
                         for (int i = 0; i < N2; i++) {
                             const int rr = lr + i * RPI, pos = (u.first + t) * KT + r0 + rr;
-                            const bool ok = in && rr < KT / 2 && (tail || PAGED ? there(pos) : true);
+                            const int in_page = PAGED ? __shfl_sync(0xffffffffu, e, (r0 + rr) >> piece_log) : 0;     // (rr beyond the half: any lane's)
+                            const bool ok = in && rr < KT / 2 && in_page >= 0 && (tail ? there(pos) : true);
                             const float4 z = make_float4(0.f, 0.f, 0.f, 0.f);
-                            const char *at = from + (ok ? place(pos) : 0);
+                            const char *at = from + (ok ? place(pos, in_page) : 0);
                             x[2 * i] = ok ? *(const float4 *)at : z;
                             x[2 * i + 1] = ok ? *(const float4 *)(at + 16) : z;
                         }

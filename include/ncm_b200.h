@@ -461,7 +461,7 @@ typedef struct {
  * T tokens and the query heads that share the kv head: added to slots [0, len[b]), stored to the T new ones. */
 int ncmb_cache_attention(const NcmbCache *c, const void *q, int64_t ldq, void *out, int64_t ldo, int act_type, int n_head,
                          int T, const int *parents, float scale, int max_len, float *weights);
-/* Diagnostic: which tiles ncmb_cache_attention takes for more than 16 query rows a kv head (T * n_head / n_kv): 0 by size
+/* Diagnostic: which tiles ncmb_cache_attention and ncmb_paged_attention take for more than 16 query rows a kv head (T * n_head / n_kv): 0 by size
  * (default), 1 tiles of 16 rows, 2 tiles of 128 rows where they take the shape. No counterpart in the reference. */
 void ncmb_set_cache_variant(int variant);
 /* Holds every (row, kv head) of a cache to `budget` tokens: kept are the tokens in the text's last min(recent, budget)
@@ -536,7 +536,7 @@ int ncmb_rope(const NcmbRope *r, const void *x, const int64_t *xs, void *y, cons
  * table[b * table_stride + n / page], for n below max_pages * page, its capacity. Rows may share pages (a common beginning, the beams of
  * a group); who writes has pages of its own. An entry outside 0 ... n_pages - 1 is no page: tokens that would stand there are not
  * stored, and nothing sees them. A negative length: the row holds no sequence; nothing is stored for it and its results are zero. The
- * types, head dims and alignments of NcmbCache; rounding, scratch memory, streams and captures as there. */
+ * types, head dims and alignments of NcmbCache; rounding, bounded waits, scratch memory, streams and captures as there. */
 typedef struct {
     void *k, *v;
     int type;                        /* NCMB_F32 or NCMB_BF16 */

@@ -75,8 +75,9 @@ __device__ __forceinline__ void ct_tma(uint32_t dst, const CUtensorMap *m, int d
 __device__ __forceinline__ void ct_fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
 // PAGED: keys through the row's table. Whole tiles of a bf16 cache come by TMA from a map of the pool, a box a page (or the part of one that a tile holds);
-// tiles that end inside, or in which an entry is no page, by cp.async, and all of an fp32 cache's through registers, an entry a key. The warps of the
-// softmax look at the entries themselves: which keys are not there.
+// tiles that end inside, or in which an entry is no page, by cp.async, and all of an fp32 cache's through registers, entries a tile ahead. The warps of the
+// softmax look at the entries themselves: which keys are not there. 16 rows of up to 8000 tokens, 8 new ones, 32 heads over 8 x 128, pages of 64 / 16 / 8: 102 / 104 /
+// 137 us, a contiguous cache 97; fp32, 4 x 8000, 64 new, 16 over 4 x 64: 86 (an entry a key: 148), contiguous 83.
 template <class KE, class QE, int HDP, bool PAGED = false>
 __global__ void __launch_bounds__(CtCfg<KE, QE, HDP>::THREADS, 1) k_cache_attention_tc(const __grid_constant__ CmArgs a, const __grid_constant__ CUtensorMap mk,
                                                                                         const __grid_constant__ CUtensorMap mv, int *err) {

@@ -384,3 +384,56 @@ def test_many_query_rows_without_pages(cuda, variant, kt, qt, page):
 def test_many_query_rows_of_long_rows(cuda, variant, kt, qt, B, n, T, H, nkv, hd, page):
     """Units cut over CTAs, query rows in several tiles."""
     run_attention(cuda, B + T, [n] + [(b * 7919) % n for b in range(1, B)], T, H, nkv, hd, kt, qt, "head" if T % 3 else "token", page)
+
+
+def test_a_call_that_finds_the_error_word_set(cuda):
+    """As for contiguous caches: the call ends, the word is reported, results are not written, the next call is right."""
+    cuda.ncmb_set_cache_variant(2)
+    try:
+        rng = np.random.default_rng(6)
+        pool = Pool(rng, 2, 60, 64, 2, 64, BF16, "token")
+        pool.put(rng, [3040, 57])
+        pool.len.copy_(torch.tensor([3000, 17]))
+        q = torch.randn(2, 40, 14, 64, device="cuda")
+        out = torch.full_like(q, 5.0)
+        assert cuda.ncmb_gemm_tc_check() == 0
+        cuda.ncmb_gemm_tc_raise(47)
+        assert cuda.ncmb_paged_attention(pool.handle(), q.data_ptr(), 14 * 64, out.data_ptr(), 14 * 64, capi.F32, 14, 40, None, 0.0, 0) == 0
+        torch.cuda.synchronize()
+        assert (out == 5.0).all() and cuda.ncmb_gemm_tc_check() == 47
+        run_attention(cuda, 3, [3000, 17], 40, 14, 2, 64, BF16, F32, "token", 64, True)
+        assert cuda.ncmb_gemm_tc_check() == 0
+    finally:
+        cuda.ncmb_set_cache_variant(0)
+
+
+@pytest.mark.parametrize("dt", [F32, BF16])
+def test_a_prompt_in_pieces(cuda, dt):
+    """Appended and attended to in pieces of any sizes, a prompt gives what it gives at once (bf16 products' order aside)."""
+    H, nkv, hd, page, n = 8, 2, 64, 16, 700
+    g = torch.Generator(device="cuda").manual_seed(1)
+    qkv = torch.randn(2, n, H + 2 * nkv, hd, device="cuda", generator=g)
+    r = make_plan(cuda, hd, 0)
+    got = []
+    for pieces in ([256, 256, 188], [1, 7, 100, 255, 16, 16, 200, 105]):
+        pool = Pool(np.random.default_rng(0), 2, n // page + 2, page, nkv, hd, dt, "token")
+        outs, at = [], 0
+        for T in pieces:
+            x = qkv[:, at:at + T].contiguous()
+            ld, w, p = (H + 2 * nkv) * hd, H * hd, x.data_ptr()
+            pool.len.fill_(at)
+            out = torch.empty(2, T, H, hd, device="cuda")
+            assert cuda.ncmb_paged_append(pool.handle(), r, p, ld, p, ld, H, p + w * 4, ld, p + (w + nkv * hd) * 4, ld, capi.F32, 2 * T, None, None) == 0
+            assert cuda.ncmb_paged_attention(pool.handle(), p, ld, out.data_ptr(), w, capi.F32, H, T, None, 0.0, 0) == 0
+            outs.append(out)
+            at += T
+        got.append(torch.cat(outs, 1))
+        k, v = zip(*(pool.row(b, n) for b in range(2)))
+    torch.cuda.synchronize()
+    rot = turned(qkv[:, :, :H].double().cpu().numpy(), np.broadcast_to(np.arange(n), (2, n)), r)[0]
+    ok = np.tril(np.ones((n, n), bool))
+    for b in range(2):
+        for h in range(nkv):
+            want, _, rel = contiguous.attend64(torch.from_numpy(rot[b, :, 4 * h:4 * h + 4]), k[b][:, h], v[b][:, h], ok, hd ** -0.5)
+            for o in got:                                       # queries come rotated in fp32: 2^-21 of a score more
+                contiguous.check(o[b, :, 4 * h:4 * h + 4], want, (rel[..., None] * 1.5 + 2.0 ** -18) * v[b][:, h].abs().max().item(), F32)

@@ -44,6 +44,11 @@ class Work:
         self.so = torch.zeros(12, 4, device="cuda")
         self.po, self.to, self.do = (torch.zeros(12, 4, dtype=torch.int32, device="cuda") for _ in range(3))
         self.t2, self.l2 = torch.zeros_like(self.table), torch.zeros_like(self.len)
+        # the last new tokens of every row once more, 24 at a time: tiles of many query rows
+        self.q2 = r(rows, 24, H, hd)
+        self.out2 = torch.zeros_like(self.q2)
+        self.len2 = (self.len - 23).clamp(min=0)
+        self.c2 = capi.PagedCache.of(self.pool[0, 0], self.pool[1, 0], self.table, self.len2)
         self.plan = capi.Rope()
         assert lib.ncmb_rope_plan(self.plan, hd, 1, 10000.0, 0, 1.0, 0.0, 0.0, 0.0, 1.0) == 0
         torch.cuda.synchronize()
@@ -53,16 +58,17 @@ class Work:
         lib, p, ld, w = self.lib, self.qkv.data_ptr(), (self.H + 2 * self.nkv) * self.hd, self.H * self.hd
         rc = lib.ncmb_paged_append(self.c, self.plan, p, ld, self.q.data_ptr(), w, self.H, p + w * 4, ld, p + (w + self.nkv * self.hd) * 4, ld, capi.F32, 48, None, None)
         rc |= lib.ncmb_paged_attention(self.c, self.q.data_ptr(), w, self.out.data_ptr(), w, capi.F32, self.H, 1, None, 0.0, 0)
+        rc |= lib.ncmb_paged_attention(self.c2, self.q2.data_ptr(), w, self.out2.data_ptr(), w, capi.F32, self.H, 24, None, 0.0, 0)
         rc |= lib.ncmb_beam_select(self.logits.data_ptr(), self.V, capi.F32, 12, 4, self.V, self.scores.data_ptr(), None, 5, 4, self.so.data_ptr(), self.po.data_ptr(), self.to.data_ptr(),
                                    self.do.data_ptr())
         return rc | lib.ncmb_paged_reorder(self.c, 4, self.po.data_ptr(), 2, self.pool.stride(1), self.t2.data_ptr(), self.l2.data_ptr(), None)
 
     def results(self):
-        return [x.clone() for x in (self.pool, self.q, self.out, self.so, self.po, self.to, self.do, self.t2, self.l2)]
+        return [x.clone() for x in (self.pool, self.q, self.out, self.out2, self.so, self.po, self.to, self.do, self.t2, self.l2)]
 
     def clear(self):
         self.pool.copy_(self.pool0)
-        for x in (self.q, self.out, self.so, self.po, self.to, self.do, self.t2, self.l2):
+        for x in (self.q, self.out, self.out2, self.so, self.po, self.to, self.do, self.t2, self.l2):
             x.zero_()
         torch.cuda.synchronize()
 

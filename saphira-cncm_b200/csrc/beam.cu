@@ -198,18 +198,6 @@ __device__ __forceinline__ unsigned long long bm_order(double x) {
 __device__ __forceinline__ double bm_value(unsigned long long k) { return __longlong_as_double(k >> 63 ? k ^ 1ull << 63 : ~k); }
 
 // ---- a group's parts, by the last CTA that has one ----
-// log t, t > 0, to 1e-12: t = 2^e m with m about 1, log m = 2 atanh s of s = (m - 1) / (m + 1), |s| <= 0.18, by its series. (The library's function is
-// exact to the last bit, in code that takes 2000 cycles to fetch.)
-__device__ __forceinline__ double bm_log(double t) {
-    const unsigned long long u = __double_as_longlong(t);
-    int e = (int)(u >> 52) - 1023;
-    double m = __longlong_as_double((u & 0xfffffffffffffull) | 1023ull << 52);
-    if (m > 1.4) { m *= 0.5; e++; }
-    const double d = m + 1, q = (double)__fdividef(1.f, (float)d), s0 = (m - 1) * q, s = fma(q, fma(-s0, d, m - 1), s0), z = s * s, zz = z * z;      // a quotient, once corrected
-    const double a = fma(z, 1.0 / 3, 1.0), b = fma(z, 1.0 / 7, 1.0 / 5), c = fma(z, 1.0 / 11, 1.0 / 9), f = fma(z, 1.0 / 15, 1.0 / 13);
-    const double r = fma(zz * zz, fma(zz, f, c), fma(zz, b, a));
-    return fma((double)e, 0.693147180559945309, 2 * s * r);
-}
 template <int MOST> struct JoinShared {
     TopN<Wide, BM_JOIN, MOST, BM_JOIN * BM_THREADS> top;         // a whole tile fits
     unsigned long long bound;
@@ -256,7 +244,7 @@ template <int MOST> __device__ __noinline__ void beam_join(const BeamArgs &a, in
             for (int o = 1; o < min(32, a.parts); o <<= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
             m = top;
         }
-        if (lane == 0) sh.lse[k] = m == -INFINITY ? 0.0 : m + bm_log(t);
+        if (lane == 0) sh.lse[k] = m == -INFINITY ? 0.0 : m + log(t);
     }
     sh.top.clear();
     unsigned long long least = 0;
@@ -319,8 +307,8 @@ template <class E, int MOST> struct PartShared {
 template <class E, int MOST> constexpr size_t beam_smem() { return std::max(sizeof(PartShared<E, MOST>), sizeof(JoinShared<MOST>)); }
 
 template <int VE> __device__ __forceinline__ int bm_place(int e) { return (e / VE * BM_THREADS + (int)threadIdx.x) * VE + e % VE; }     // of a thread's e-th value in a tile
-// Tiles [t0, t1), of whose keys some found no room in the list: once more, a few values a thread at a time, each time bounded by what these show. Rare: their values lie badly, most of the
-// large ones with few threads, or rise from tile to tile.
+// Tiles [t0, t1), of whose keys some found no room in the list: once more, a few values a thread at a time, each time bounded by what these show.
+// Rare: their values rise from tile to tile, or most of the large ones lie with few threads.
 template <class E, bool VEC, int MOST>
 __device__ __noinline__ void beam_again(const E *x0, int t0, int t1, int V, int n, TopN<unsigned long long, BM_CHUNK, MOST> &top, unsigned long long &least) {
     constexpr int VE = VEC ? 16 / (int)sizeof(E) : 1;

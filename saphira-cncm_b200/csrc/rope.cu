@@ -15,6 +15,7 @@ int rope_check(const char *who, const NcmbRope *r, int hd) {
 namespace {
 
 constexpr int RO_THREADS = 256, RO_TOKENS = 32, RO_BATCH = 4;
+constexpr int RO_SMEM = 48 * 1024 - RO_TOKENS * (8 + 8 + 4);        // what a launch may ask for beside the tokens' places
 
 struct RopeArgs {
     const char *x; char *y;
@@ -170,10 +171,11 @@ template <class E> void run_rope(const NcmbRope &r, RopeArgs &a) {
     // a thread's items all on their way at once, and CTAs for all SMs (8 x 4000 tokens of 40 x 128 in bf16, 4 / 8 / 20 items a thread: 100 / 107 / 115 us)
     const int items = any ? (int)cdiv(a.hd, V) : rope_items(&r, a.hd, V), held = (any ? 2 * RO_BATCH : RO_BATCH) * (RO_THREADS / items), heads = any ? std::min(a.n_head, held) : a.n_head;
     a.share = rope_share(&r, items, heads, RO_THREADS);
-    a.per = (int)std::max<int64_t>(1, std::min<int64_t>({any ? RO_TOKENS / 2 : RO_TOKENS, held / heads, a.tokens / (4 * ctx().sm_count)}));
-    const size_t smem = (size_t)a.per * rope_row(r.dims) * sizeof(float2);
+    const int angles = rope_row(r.dims) * (int)sizeof(float2), staged = any ? heads * items * 16 : 0, spare = any ? 16 : 0;      // bytes a token, and once
+    a.per = (int)std::max<int64_t>(1, std::min<int64_t>({any ? RO_TOKENS / 2 : RO_TOKENS, held / heads, (RO_SMEM - spare) / (angles + staged), a.tokens / (4 * ctx().sm_count)}));
+    const size_t smem = (size_t)a.per * (angles + staged) + spare;
     const unsigned grid = (unsigned)cdiv(a.tokens, a.per);
-    if (any) LAUNCH_PDL((k_rope_any<E>), dim3(grid, (unsigned)cdiv(a.n_head, heads)), RO_THREADS, smem + ((size_t)a.per * heads * items + 1) * 16, r, a);
+    if (any) LAUNCH_PDL((k_rope_any<E>), dim3(grid, (unsigned)cdiv(a.n_head, heads)), RO_THREADS, smem, r, a);
     else if (r.layout == NCMB_ROPE_HALVES) LAUNCH_PDL((k_rope<E, V, false>), grid, RO_THREADS, smem, r, a);
     else LAUNCH_PDL((k_rope<E, V, true>), grid, RO_THREADS, smem, r, a);
 }

@@ -92,13 +92,14 @@ __device__ __forceinline__ void cm_mma_tf32(float (&c)[4], const uint32_t (&a)[4
     asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// Two TF32 terms of v, 22 bits. BITS: v cut off after a TF32's bits, and the rest with half of its own last place added and cut off; four instructions of the
-// integer and fp32 pipes for two conversions, which are slower (paged, fp32 cache, 16 heads over 4 x 64, 32 rows of up to 8000: 86 -> 75 us).
+// Two TF32 terms of v, together within 2^-23 of it. BITS: by the integer and fp32 pipes instead of two conversions, which the paged kernels wait for (fp32, 16 heads
+// over 4 x 64, 32 rows of up to 8000: 79 -> 69 us); contiguous caches (67 us) keep the conversions, and their results. The leading term is rounded as a
+// conversion does, half of its last place added and cut off; the rest is less than 2^12 of v's last places, so a cut after 11 bits loses one of them
+// at most, as rounding would. A NaN that the addition carries into the sign leaves a NaN as the rest.
 template <bool BITS = false> __device__ __forceinline__ void cm_tf32(float v, uint32_t &hi, uint32_t &lo) {
     if constexpr (BITS) {
-        hi = __float_as_uint(v) & 0xffffe000u;
-        const float l = v - __uint_as_float(hi);
-        lo = __float_as_uint(fmaf(l, 0x1p-11f, l)) & 0xffffe000u;
+        hi = (__float_as_uint(v) + 0x1000u) & 0xffffe000u;
+        lo = __float_as_uint(v - __uint_as_float(hi)) & 0xffffe000u;
     } else {
         asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(hi) : "f"(v));
         asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(lo) : "f"(v - __uint_as_float(hi)));

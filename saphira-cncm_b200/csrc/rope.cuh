@@ -1,7 +1,8 @@
 // Rotary positions: what ncmb_rope and ncmb_paged_append share.
 //
 // A pair (x1, x2) at angle a = 2 pi p f, f full turns a position: y1 = m (x1 cos a - x2 sin a), y2 = m (x2 cos a + x1 sin a). p f is formed in 64
-// bits and only its fraction of a turn goes on in fp32: at position 10^6 an fp32 product is off by 0.06 radians.
+// bits and only its fraction of a turn goes on in fp32: at position 10^6 an fp32 product is off by 0.06 radians, the fraction by 2^-26 of a turn at
+// most, 9e-8 radians, less than what the fp32 cosine and sine and the products with them may add (8 units of 2^-24 in all).
 //
 // A thread's item is two vectors of V elements of a head. HALVES: the vectors at i and i + dims / 2, V pairs; PAIRS: the vectors i and i + half of
 // the head's vectors, each of V / 2 pairs; dims that stay: likewise. So threads side by side have vectors side by side. V is 16 bytes where the dims allow it.

@@ -581,7 +581,9 @@ int ncmb_beam_select(const void *logits, int64_t ldl, int type, int groups, int 
  * group; anything else: row j holds no sequence). Full pages are shared. A row's pages from entry len / page on -- the begun one and those in
  * reserve, of which the first has to be there -- are its own: the lowest row that continues a parent keeps the parent's, further ones take
  * those of the group's rows that nobody continues, in order, and get the begun page's tokens copied, in each of n_layer pools, layer_stride
- * elements apart from c->k and c->v, that share the table. So no page has to be found and none is lost but full pages that no row holds any more.
+ * elements apart from c->k and c->v, that share the table. So no page has to be found. Full pages that no row holds any more leave the tables, and where
+ * a row that takes own pages has more full ones than the row that had them, what does not fit its max_pages entries: nothing does while
+ * max_pages is the full pages of a group's longest row and the pages that a row owns. What has left shows in refs alone.
  * table_dst (as c->table, same stride; not c->table) and len_dst (device int[rows], not c->len) receive tables and lengths; entries that have no
  * page become -1. refs: NULL, or device int[n_pages]: to each page's count the change of the number of entries that hold it is added. group up
  * to NCMB_MAX_GROUP and a divisor of rows. */

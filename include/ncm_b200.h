@@ -536,8 +536,9 @@ int ncmb_rope(const NcmbRope *r, const void *x, const int64_t *xs, void *y, cons
  * k[p * page_stride + h * head_stride + s * token_stride + d], of the values likewise with v. Row b's token number n stands in slot n % page of page
  * table[b * table_stride + n / page], for n below max_pages * page, its capacity. Rows may share pages (a common beginning, the beams of
  * a group); who writes has pages of its own. An entry outside 0 ... n_pages - 1 is no page: tokens that would stand there are not
- * stored, and nothing sees them. A negative length: the row holds no sequence; nothing is stored for it and its results are zero. The
- * types, head dims and alignments of NcmbCache; rounding, bounded waits, scratch memory, streams and captures as there. */
+ * stored, and nothing sees them. A negative length: the row holds no sequence; nothing is stored for it, its queries
+ * are not rotated (q_out stays as it was there), and attention gives zeros. The types, head dims and alignments of NcmbCache; rounding, bounded
+ * waits, scratch memory, streams and captures as there. */
 typedef struct {
     void *k, *v;
     int type;                        /* NCMB_F32 or NCMB_BF16 */
@@ -582,8 +583,8 @@ int ncmb_beam_select(const void *logits, int64_t ldl, int type, int groups, int 
  * reserve, of which the first has to be there -- are its own: the lowest row that continues a parent keeps the parent's, further ones take
  * those of the group's rows that nobody continues, in order, and get the begun page's tokens copied, in each of n_layer pools, layer_stride
  * elements apart from c->k and c->v, that share the table. So no page has to be found. Full pages that no row holds any more leave the tables, and where
- * a row that takes own pages has more full ones than the row that had them, what does not fit its max_pages entries: nothing does while
- * max_pages is the full pages of a group's longest row and the pages that a row owns. What has left shows in refs alone.
+ * a row that takes own pages has more full ones than the row that had them, what does not fit its max_pages entries: that is nothing
+ * while max_pages is at least the full pages of the group's longest row and the most pages that a row owns, together. What has left shows in refs alone.
  * table_dst (as c->table, same stride; not c->table) and len_dst (device int[rows], not c->len) receive tables and lengths; entries that have no
  * page become -1. refs: NULL, or device int[n_pages]: to each page's count the change of the number of entries that hold it is added. group up
  * to NCMB_MAX_GROUP and a divisor of rows. */

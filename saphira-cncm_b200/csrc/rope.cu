@@ -192,14 +192,14 @@ extern "C" int ncmb_rope_plan(NcmbRope *r, int dims, int layout, double theta, i
     if (dims < 2 || dims > NCMB_ROPE_MAX || dims % 2) return cache_refuse(who, "%d dims: even, 2 to %d", dims, NCMB_ROPE_MAX);
     if (layout != NCMB_ROPE_HALVES && layout != NCMB_ROPE_PAIRS) return cache_refuse(who, "layout %d of pairs", layout);
     if (scaling < NCMB_ROPE_PLAIN || scaling > NCMB_ROPE_PARTS) return cache_refuse(who, "scaling %d", scaling);
-    if (!(theta > 0 && theta < INFINITY) || !(factor > 0 && factor < INFINITY) || !(fabs(magnitude) < INFINITY)) return cache_refuse(who, "theta %g, factor %g, magnitude %g", theta, factor, magnitude);
+    if (!(theta > 0 && theta < INFINITY) || !(factor > 0 && factor < INFINITY) || !(fabs((float)magnitude) < INFINITY)) return cache_refuse(who, "theta %g, factor %g, magnitude %g", theta, factor, magnitude);
     if (scaling == NCMB_ROPE_PARTS && !(trained > 0 && trained < INFINITY && low < high && fabs(low) < INFINITY && fabs(high) < INFINITY))
         return cache_refuse(who, "a trained context of %g, parts from %g to %g turns", trained, low, high);
     const double two_pi = 6.283185307179586476925;
-    *r = NcmbRope{};
-    r->dims = dims;
-    r->layout = layout;
-    r->magnitude = (float)magnitude;
+    NcmbRope plan = {};
+    plan.dims = dims;
+    plan.layout = layout;
+    plan.magnitude = (float)magnitude;
     if (scaling == NCMB_ROPE_BASE && dims > 2) theta *= pow(factor, dims / (dims - 2.0));
     for (int i = 0; i < dims / 2; i++) {
         double f = pow(theta, -2.0 * i / dims);
@@ -208,8 +208,10 @@ extern "C" int ncmb_rope_plan(NcmbRope *r, int dims, int layout, double theta, i
             const double g = fmin(1.0, fmax(0.0, (trained * f / two_pi - low) / (high - low)));
             f *= g + (1.0 - g) / factor;
         }
-        r->turns[i] = f / two_pi;
+        if (!(f < INFINITY)) return cache_refuse(who, "theta %g, factor %g: pair %d turns without a limit", theta, factor, i);
+        plan.turns[i] = f / two_pi;
     }
+    *r = plan;
     return 0;
 }
 

@@ -68,3 +68,26 @@ def test_what_is_not_a_number_is_not_lost(cuda, bad):
                 assert torch.isnan(out[hit]).all()
             else:
                 assert not torch.isfinite(out[hit]).any()
+
+
+@pytest.mark.parametrize("H", [4, 16])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_scores_are_not_short(cuda, H, hd):
+    """A score whose products are all positive, read off the probability of a key of zeros beside it: exp(-score). The tensor core cuts its accumulator off
+    after each product of eight dims, on the average by half a last place, 2^-24 of what it holds at most; two accumulators take turns, so each is cut n =
+    hd / 16 times, at 1 / n, 2 / n ... of what it comes to: together short by (n + 1) / 2 2^-24 of the score on the average. Everything else (pairs 2^-23,
+    the scaled score 2^-24, an exponential 2^-22 of itself, a fortieth of that of the score) goes either way: 1e-8 of the score for 256 means or more."""
+    rng = np.random.default_rng(hd + H)
+    rows, scale = 64, 40.0 / hd
+    k, v = torch.zeros(rows, 1, 16, hd, device="cuda"), torch.zeros(rows, 1, 16, hd, device="cuda")
+    k[:, 0, 1] = torch.from_numpy(rng.uniform(0.5, 1.5, (rows, hd)).astype(np.float32)).cuda()
+    v[:, 0, 0] = 1.0
+    q = torch.from_numpy(rng.uniform(0.5, 1.5, (rows, H, hd)).astype(np.float32)).cuda()
+    out = torch.empty_like(q)
+    c = capi.PagedCache.of(k, v, torch.arange(rows, dtype=torch.int32, device="cuda")[:, None], torch.ones(rows, dtype=torch.int32, device="cuda"))
+    assert cuda.ncmb_paged_attention(c, q.data_ptr(), H * hd, out.data_ptr(), H * hd, capi.F32, H, 1, None, scale, 0) == 0
+    torch.cuda.synchronize()
+    c2 = float(np.float32(scale) * np.float32(1.44269504))
+    score = (q.double() * k[:, 0, 1].double()[:, None]).sum(-1) * c2
+    short = ((torch.log2(out[..., 0].double()) + torch.log2(1 + torch.exp2(-score)) + score) / score).mean().item()
+    assert -1e-8 <= short <= (hd / 16 + 1) / 2 * 2.0 ** -24 + 1e-8, short / 2.0 ** -24

@@ -502,8 +502,8 @@ int ncmb_block_attention(const NcmbCache *c, const void *q, int64_t ldq, void *o
  * rope_apply above rotates whole heads, halves against one another, by tables of cosines. These calls take a plan instead: which
  * dims of a head are rotated, which of them are a pair, and how far each pair turns from one position to the next. For the pair
  * (x1, x2) of angle a: y1 = magnitude (x1 cos a - x2 sin a), y2 = magnitude (x2 cos a + x1 sin a). Angles are formed in 64 bits: for frequencies of up
- * to a radian a position they are off by |position| 1e-16 turns at most, 1e-9 up to position 10 million and 2e-7 at the ends of 32 bits. The
- * fraction of a turn is rounded to fp32 (2^-26 of a turn), cosines, sines and products are fp32, the result is rounded once. */
+ * to a radian a position they are off by |position| 1e-16 turns at most, 1e-9 up to position 10 million and 2e-7 at the ends of 32 bits. Cosines,
+ * sines and products are fp32, the result is rounded once. */
 enum { NCMB_ROPE_HALVES = 0,             /* dim i and dim i + dims / 2 are a pair */
        NCMB_ROPE_PAIRS = 1 };            /* dims 2 i and 2 i + 1 */
 enum { NCMB_ROPE_PLAIN = 0, NCMB_ROPE_LINEAR = 1, NCMB_ROPE_BASE = 2, NCMB_ROPE_PARTS = 3 };

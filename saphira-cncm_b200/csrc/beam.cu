@@ -10,11 +10,13 @@
 // their own, and no order of arrival shows in the result. However the values lie, a bound is reached by n groups at most, so a few values a thread
 // at a time always fit the list; tiles of which more beat an older bound than there is room for are gone through once more that way.
 //
-// Rounding: exponentials in fp32 against the thread's maximum, 32 of them summed in fp32, everything after in 64 bits; scores in 64 bits, so that
+// Rounding: exponentials in fp32 against the thread's maximum, 32 of them summed in fp32 -- 64 bits from a value on would be several instructions more for
+// each --, everything after in 64 bits: log sum exp within 5e-7 where roundings do not average, 2e-8 where they do. Scores in 64 bits, so that
 // their order does not depend on the rounding of a score near 100 (2^-18 in fp32). All rows of a call are split alike: equal rows have equal sums.
 //
-// Bound: with many rows by DRAM and instructions together -- 256 rows of 151936 in fp32: 37 us (4.2 TB/s), of which an SM that has two of them
-// streams 27 at 48 GB/s; in bf16 33, by instructions. With few by latency: 4 rows of 50257, 9.4 us, 40% of it the join.
+// Bound: with many rows by the SMs that have most of them -- 256 rows of 151936 in fp32: 37 us (4.2 TB/s), of which an SM that has two of them
+// streams 27 at 48 GB/s; in bf16 33: an SM is active in 46 000 of 70 000 cycles on the average and issues in 38% of those, its warps wait for fixed
+// latencies and for one another. With few by latency: 4 rows of 50257, 9.4 us, 40% of it the join.
 #include "cache.cuh"
 
 #include <algorithm>
@@ -27,7 +29,7 @@ constexpr int BM_EPT = 32, BM_TILE = BM_THREADS * BM_EPT;        // logits of a 
 constexpr int BM_CHUNK = 8;                                      // logits of a thread whose keys fit the list whatever they are, once they are bounded
 constexpr int BM_JOIN = 2;                                       // candidates of a thread at a time where parts are joined
 constexpr int BM_BATCH = 4;                                      // tiles from one meeting of the warps to the next
-constexpr int BM_START = 2, BM_ROUNDS = 4, BM_CTAS = 2;          // BM_CTAS: of an SM; with three, 80 registers a thread leave less to overlap (39 -> 47 us)
+constexpr int BM_START = 2, BM_ROUNDS = 4, BM_CTAS = 2;          // BM_CTAS: of an SM; with three, 80 registers a thread leave less to overlap (then 39 -> 47 us)
 constexpr int BM_FEW = 16;                                       // continuations that most calls want
 constexpr float BM_LOG2E = 1.44269504f;
 
@@ -554,7 +556,7 @@ extern "C" int ncmb_beam_select(const void *logits, int64_t ldl, int type, int g
     a.tiles = (int)cdiv(V, BM_TILE);
     a.scores = scores; a.done = done; a.eos = eos; a.scores_out = scores_out; a.parents = parents; a.tokens = tokens; a.done_out = done_out;
     // Parts of a row: as many as fill one to BM_ROUNDS rounds of the CTAs that fit the GPU, whichever takes least where a CTA's start and end take as long as
-    // BM_START tiles (256 rows of 151936 in fp32, 1 / 2 / 3 / 5 parts: 39 / 44 / 49 / 54 us; 32 rows, 4 / 9 parts: 18 / 17; 1 and 9 are taken).
+    // BM_START tiles (256 rows of 151936 in fp32, 1 / 2 / 3 / 5 parts: 37 / 42 / 46 / 53 us, in bf16 33 / 39 / 43 / 50; 32 rows, 4 / 5 / 9 parts: 15.0 / 16.3 / 15.0; 1 and 9 are taken).
     const int64_t resident = BM_CTAS * ctx().sm_count, most = std::max<int64_t>(1, std::min<int64_t>(a.tiles, 65536 / ((int64_t)beams * n_out)));
     int64_t best = INT64_MAX;
     for (int r = 1; r <= BM_ROUNDS; r++) {

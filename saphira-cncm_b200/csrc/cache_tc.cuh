@@ -76,8 +76,8 @@ __device__ __forceinline__ void ct_fence_async() { asm volatile("fence.proxy.asy
 
 // PAGED: keys through the row's table. Whole tiles of a bf16 cache come by TMA from a map of the pool, a box a page (or the part of one that a tile holds);
 // tiles that end inside, or in which an entry is no page, by cp.async, and all of an fp32 cache's through registers, entries a tile ahead. The warps of the
-// softmax look at the entries themselves: which keys are not there. 16 rows of up to 8000 tokens, 8 new ones, 32 heads over 8 x 128, pages of 64 / 16 / 8: 102 / 104 /
-// 137 us, a contiguous cache 97; fp32, 4 x 8000, 64 new, 16 over 4 x 64: 86 (an entry a key: 148), contiguous 83.
+// softmax look at the entries themselves: which keys are not there. 16 rows of up to 8000 tokens, 8 new ones, 32 heads over 8 x 128, pages of 64 / 16 / 8: 101 / 103 /
+// 137 us, a contiguous cache 97; fp32, 4 x 8000, 64 new, 16 over 4 x 64: 88 (an entry a key: 148), contiguous 87.
 template <class KE, class QE, int HDP, bool PAGED = false>
 __global__ void __launch_bounds__(CtCfg<KE, QE, HDP>::THREADS, 1) k_cache_attention_tc(const __grid_constant__ CmArgs a, const __grid_constant__ CUtensorMap mk,
                                                                                         const __grid_constant__ CUtensorMap mv, int *err) {
@@ -702,6 +702,8 @@ extern int cache_variant;            // ncmb_set_cache_variant
 //   wide   14 + WIDE x tiles of 128 rows x (tiles of 128 keys + START), over the SMs
 // e.g. bf16 cache, fp32 queries, 2 x 64, narrow against wide: 1 x 4000 x 112 rows 11 / 17, 16 x 4000 x 56 rows 34 / 38,
 // x 448 rows 153 / 105; 8 x 128: 1 x 500 x 64 rows 11.4 / 24, 16 x 4000 x 64 rows 181 / 148, x 256 rows 667 / 278.
+// Paged caches are chosen for by the same constants, although their narrow tiles of bf16 take up to a third more and wide ones of pages of 8 up to 40%: of 192 calls
+// (1 - 16 rows of 500 - 16000, 5 - 256 new tokens, pages of 8 and 64) 182 are within 6% of the faster kind, the farthest 28.7 for 20.5 us (1 x 4000 x 448 rows, 2 x 64).
 template <class KE, class QE, int HDP> struct CtCost {
     static constexpr bool Q32 = sizeof(QE) == 4;
     static constexpr double NARROW = sizeof(KE) == 4 ? 111e-6 : HDP == 64 ? (Q32 ? 42e-6 : 30e-6) : (Q32 ? 90e-6 : 71e-6);

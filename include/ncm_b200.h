@@ -573,7 +573,8 @@ int ncmb_paged_attention(const NcmbPaged *c, const void *q, int64_t ldq, void *o
  * as -infinity, a logit of +infinity as the largest finite number; what scores -infinity still fills places that nothing else takes.
  * done: NULL, or device int[groups][beams]: a beam with done != 0 has ended: it goes on with the word eos alone, at the score that it has, and its
  * logits are not read. done_out: NULL, or int[groups][n_out]: 1 where the parent was done or the word is eos (eos < 0: no such word, with
- * done NULL). With n_out = beams the outputs of scores and done may be their inputs. All are device arrays.
+ * done NULL). With n_out = beams the outputs of scores and done may be their inputs; else nothing that is written may share
+ * memory with another array. All are device arrays.
  * beams and n_out up to NCMB_MAX_BEAMS, n_out no more than beams * V, V up to 2^24. */
 #define NCMB_MAX_BEAMS 128
 int ncmb_beam_select(const void *logits, int64_t ldl, int type, int groups, int beams, int V, const float *scores, const int *done, int eos,
@@ -585,7 +586,7 @@ int ncmb_beam_select(const void *logits, int64_t ldl, int type, int groups, int 
  * elements apart from c->k and c->v, that share the table. So no page has to be found. Full pages that no row holds any more leave the tables, and where
  * a row that takes own pages has more full ones than the row that had them, what does not fit its max_pages entries: that is nothing
  * while max_pages is at least the full pages of the group's longest row and the most pages that a row owns, together. What has left shows in refs alone.
- * table_dst (as c->table, same stride; not c->table) and len_dst (device int[rows], not c->len) receive tables and lengths; entries that have no
+ * table_dst (as c->table, same stride) and len_dst (device int[rows]), in memory of their own, receive tables and lengths; entries that have no
  * page become -1. refs: NULL, or device int[n_pages]: to each page's count the change of the number of entries that hold it is added. group up
  * to NCMB_MAX_GROUP and a divisor of rows. */
 #define NCMB_MAX_GROUP 256

@@ -17,7 +17,7 @@
 // Bound: with many rows by the SMs that have most of them -- 256 rows of 151936 in fp32: 37 us (4.2 TB/s), of which an SM that has two of them
 // streams 27 at 48 GB/s; in bf16 33: an SM is active in 46 000 of 70 000 cycles on the average and issues in 38% of those, its warps wait for fixed
 // latencies and for one another. With few by latency: 4 rows of 50257, 9.4 us, 40% of it the join.
-#include "cache.cuh"
+#include "paged.cuh"
 
 #include <algorithm>
 
@@ -550,6 +550,15 @@ extern "C" int ncmb_beam_select(const void *logits, int64_t ldl, int type, int g
     if ((uintptr_t)logits % es || ((uintptr_t)scores | (uintptr_t)done | (uintptr_t)scores_out | (uintptr_t)parents | (uintptr_t)tokens | (uintptr_t)done_out) % 4)
         return cache_refuse(who, "arrays have to be aligned to their elements");
     if (rows > 1 << 24) return cache_refuse(who, "%lld rows", (long long)rows);
+    // a group's results are there before other groups have read what they need; in place each group has its own words
+    const size_t gb = (size_t)groups * n_out * 4, ib = (size_t)rows * 4, xb = ((size_t)(rows - 1) * ldl + V) * es;
+    const void *in[2] = {scores, done}, *out[4] = {scores_out, done_out, parents, tokens};
+    for (int i = 0; i < 4; i++) {
+        for (int j = 0; j < 2; j++)
+            if (paged_overlap(out[i], gb, in[j], ib) && !(i == j && out[i] == in[j] && n_out == beams)) return cache_refuse(who, "results in the memory of scores or done, other than in place with as many as there are beams");
+        for (int j = 0; j < i; j++) if (paged_overlap(out[i], gb, out[j], gb)) return cache_refuse(who, "two results in the same memory");
+        if (paged_overlap(out[i], gb, logits, xb)) return cache_refuse(who, "results in the memory of the logits");
+    }
     if (cache_device(who)) return -1;
     BeamArgs a = {};
     a.x = (const char *)logits; a.ld = ldl * es; a.groups = groups; a.beams = beams; a.V = V; a.n = n_out;

@@ -12,6 +12,11 @@ struct PagedDev {
     int64_t table_stride;
     const int *len;
 };
+// whether two arrays share memory; none of no bytes, or that is not there, does
+inline bool paged_overlap(const void *a, size_t na, const void *b, size_t nb) {
+    const uintptr_t x = (uintptr_t)a, y = (uintptr_t)b;
+    return a && b && na && nb && x < y + nb && y < x + na;
+}
 // 0 when the cache's description is one the kernels take (see ncm_b200.h), else -1 with a message
 int paged_check(const char *who, const NcmbPaged *c, PagedDev &d);
 

@@ -297,9 +297,13 @@ extern "C" int ncmb_paged_reorder(const NcmbPaged *c, int group, const int *pare
     if (runs > 1 << 30) return cache_refuse(who, "%d layers of %d kv heads", n_layer, c->n_kv);
     if (c->rows == 0) return 0;
     if (!parents || !table_dst || !len_dst || ((uintptr_t)parents | (uintptr_t)table_dst | (uintptr_t)len_dst | (uintptr_t)refs) % 4) return cache_refuse(who, "parents, table_dst and len_dst: not null, 4-byte aligned");
-    const uintptr_t t0 = (uintptr_t)c->table, t1 = (uintptr_t)table_dst, tb = ((uintptr_t)(c->rows - 1) * c->table_stride + c->max_pages) * 4;
-    const uintptr_t l0 = (uintptr_t)c->len, l1 = (uintptr_t)len_dst, lb = (uintptr_t)c->rows * 4;
-    if ((t0 < t1 + tb && t1 < t0 + tb) || (l0 < l1 + lb && l1 < l0 + lb)) return cache_refuse(who, "new tables and lengths have to stand in memory of their own");
+    // CTAs read what others may have written to already: nothing that is read is written
+    const size_t tb = ((size_t)(c->rows - 1) * c->table_stride + c->max_pages) * 4, lb = (size_t)c->rows * 4;
+    const struct { const void *p; size_t bytes; } in[3] = {{c->table, tb}, {c->len, lb}, {parents, lb}}, out[3] = {{table_dst, tb}, {len_dst, lb}, {refs, (size_t)c->n_pages * 4}};
+    for (int i = 0; i < 3; i++)
+        for (int j = 0; j < 3; j++)
+            if (paged_overlap(out[i].p, out[i].bytes, in[j].p, in[j].bytes) || (j != i && paged_overlap(out[i].p, out[i].bytes, out[j].p, out[j].bytes)))
+                return cache_refuse(who, "new tables, lengths and counts have to stand in memory of their own");
     if (cache_device(who)) return -1;
     a.group = group; a.n_layer = n_layer; a.ls = layer_stride * a.c.es; a.parents = parents; a.table2 = table_dst; a.len2 = len_dst; a.refs = refs;
     ProfScope prof(NCMB_K_ELEM, 0, (double)c->rows * runs * c->page * c->hd * a.c.es);

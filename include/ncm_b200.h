@@ -433,7 +433,7 @@ void   ncmb_lm_nll(NcmbLM *m, const int *ids, int B, int T, const int *lens, dou
  * probabilities of bf16 activations as two (16 bits; the result is rounded to 8); with an fp32 cache queries, keys,
  * probabilities and values as two TF32 terms (22 bits; tiles of 16 rows leave out the product of the smaller ones) or, in
  * wide tiles, as three bf16 terms whose products below 2^-24 are left out. Results of fp32 activations are within 5e-6
- * of the formula's in the 2-norm (1e-7 to 7e-7 measured). An fp32 value beyond 3.39e38 counts as an infinity, and what
+ * of the formula's in the 2-norm (1e-7 to 1e-6 measured). An fp32 value beyond 3.39e38 counts as an infinity, and what
  * attention makes of an infinity that a token sees may be a NaN.
  * Scratch memory belongs to the stream (ncmb_set_stream), is kept for the stream's next call and grows on demand: some
  * MB; with weights also 4 bytes for each query's score of each slot of the capacity, up to 2 GB or what one row needs.

@@ -72,7 +72,7 @@ def test_launches_ask_for_no_more_than_they_may_have(es, halves):
                     per, smem, _ = rope_launch(halves, dims, hd, heads, 10 ** 6, es, in_place=in_place)
                     assert per >= 1 and smem + 32 * 20 <= LAUNCH, (hd, dims, heads, per, smem)
     # the calls that asked for too much
-    assert not halves or rope_launch(True, 250, 256, 4 if es == 2 else 2, 9472, es) == ((15, 15 * 3072 + 16, True))
+    assert not halves or rope_launch(True, 250, 256, 4 if es == 2 else 2, 9472, es) == ((15, 15 * (1024 + 2048) + 16, True))
 
 
 def walk(tid, items, heads, per):
